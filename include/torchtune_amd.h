@@ -36,6 +36,9 @@ extern "C" {
 
 #define TTAMD_BF16 0
 #define TTAMD_F32 1
+/* microscaled formats (ttamd_mx_*) */
+#define TTAMD_MXFP4 4 /* e2m1 elements, two per byte, the earlier one in the low half */
+#define TTAMD_MXFP8 8 /* e4m3 elements */
 
 #define TTAMD_FEW_TOKENS 16 /* most tokens of ttamd_lora_few_fwd_bf16 */
 #define TTAMD_GROUP_MAX 4 /* most members of a group of linears with a common input (ttamd_lora_group_*) */
@@ -784,6 +787,68 @@ int ttamd_swiglu_bwd_bf16(const void* gout, const void* gate, const void* up, vo
  */
 int ttamd_cross_entropy_fwd_bwd_bf16(const void* logits, const int64_t* target, int64_t ignore_index, float grad_scale,
                                      float* loss, void* grad_logits, int64_t rows, int64_t V, void* stream);
+
+
+/* ------------------------------------------------------------------------------------------------
+ * Microscaled (MX) tensors: blocks of 32 consecutive elements of a row with one power-of-two scale
+ * ---------------------------------------------------------------------------------------------- */
+
+/*
+ * x [rows, K] `dtype` -> codes (TTAMD_MXFP4: [rows, K / 2], TTAMD_MXFP8: [rows, K]) and scales [rows, K / 32], K % 32 == 0.
+ * A block's scale is 2^(s - 127) with s = max(floor(log2(max |x|)) - emax + 127, 0), emax 2 (mxfp4) or 8 (mxfp8); its
+ * elements are x / scale rounded to nearest even and saturated (at 6 or 448).  A block that holds an infinity or a NaN has
+ * s = 255 and zero codes, and reads back as NaN.  rows may be 0.  x and codes 16-byte aligned.
+ */
+int ttamd_mx_quantize(const void* x, int dtype, int64_t rows, int64_t K, int format, uint8_t* codes, uint8_t* scales, void* stream);
+/* out [rows, K] `dtype` = code * scale, rounded once. */
+int ttamd_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int format, int64_t rows, int64_t K, int dtype, void* out,
+                        void* stream);
+
+/*
+ * y[M, N] = x^ . W^T (+ bias): x [M, K] bf16 is quantised to activation_format (TTAMD_MXFP8 or TTAMD_MXFP4) on its way in, W
+ * is mxfp4 (w_codes [N, K / 2], w_scales [N, K / 32]).  K % 32 == 0, any M and N; bias bf16 [N] or NULL; y bf16.  fp32 sums,
+ * one rounding.  Pointers 16-byte aligned (bias: 2); workspace: ttamd_mx_linear_workspace_bytes bytes.
+ */
+size_t ttamd_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation_format);
+int ttamd_mx_linear_bf16(const void* x, int activation_format, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
+                         void* y, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+/* Its grad-input, the rounding of x passed straight through: gx[M, K] = gy[M, N] . W.  N % 64 == 0, K % 64 == 0. */
+size_t ttamd_mx_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int ttamd_mx_linear_dx_bf16(const void* gy, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, int64_t M, int64_t N, int64_t K,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * LoRALinear.forward and its backward (torchtune/modules/peft/lora.py:128-147) over frozen mxfp4 weights, for one to
+ * TTAMD_GROUP_MAX linears that read the same input x [M, K] bf16:
+ *   forward:  x^ = mxfp8(x);  h_i = x^ . lora_a_i^T;  y_i = x^ . W_i^T (+ bias_i) + scale_i . h_i . lora_b_i^T
+ *   backward: gh_i = scale_i . gy_i . lora_b_i;  grad_lora_a_i = gh_i^T . x^;  grad_lora_b_i = scale_i . gy_i^T . h_i;
+ *             gx = sum_i gy_i . W_i + gh_i . lora_a_i  (NULL: not wanted)
+ * kept_codes (ttamd_mx_kept_codes_bytes) and kept_scales (ttamd_mx_kept_scales_bytes) are x^, written by the forward and read
+ * by the backward, in a layout of this library's own; h_cat, gh_cat bf16 [M, sum of ranks], the members side by side.
+ * K % 64 == 0, N % 64 == 0, ranks multiples of 8 that add up to at most 64.  Pointers 16-byte aligned (bias: 2).
+ */
+typedef struct ttamd_mx_lora_member {
+  const uint8_t* codes;  /* mxfp4 codes of the weight, [N, K / 2] */
+  const uint8_t* scales; /* [N, K / 32] */
+  const void* lora_a;    /* bf16 [rank, K] */
+  const void* lora_b;    /* bf16 [N, rank] */
+  const void* bias;      /* bf16 [N] or NULL (forward only) */
+  void* y;               /* forward: out, bf16 [M, N].  backward: in, the gradient of that output */
+  void* grad_lora_a;     /* backward: out, bf16 [rank, K] */
+  void* grad_lora_b;     /* backward: out, bf16 [N, rank] */
+  int64_t N;
+  int rank;
+  float scale;           /* alpha / rank */
+} ttamd_mx_lora_member;
+size_t ttamd_mx_kept_codes_bytes(int64_t M, int64_t K);
+size_t ttamd_mx_kept_scales_bytes(int64_t M, int64_t K);
+size_t ttamd_mx_lora_fwd_workspace_bytes(const ttamd_mx_lora_member* members, int n_members, int64_t M, int64_t K);
+int ttamd_mx_lora_fwd_bf16(const void* x, const ttamd_mx_lora_member* members, int n_members, uint8_t* kept_codes, uint8_t* kept_scales,
+                           void* h_cat, int64_t M, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+size_t ttamd_mx_lora_bwd_workspace_bytes(const ttamd_mx_lora_member* members, int n_members, int64_t M, int64_t K);
+int ttamd_mx_lora_bwd_bf16(const uint8_t* kept_codes, const uint8_t* kept_scales, const void* h_cat, const ttamd_mx_lora_member* members,
+                           int n_members, void* gh_cat, void* gx, int64_t M, int64_t K, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

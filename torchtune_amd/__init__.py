@@ -5,6 +5,7 @@ All arithmetic runs in ``lib/libtorchtune_amd.so`` (hand-written HIP, plain C AB
 ``python -m torchtune_amd.build``.
 """
 from .nf4_tensor import NF4Tensor, implements, linear_nf4, to_nf4
+from .mx import MXTensor, linear_mx, lora_linear_mx, to_mx
 from .modules.low_precision import FrozenNF4Linear
 from .modules.peft import DoRALinear, LoRALinear, QATLoRALinear
 from .qat import (
@@ -25,6 +26,10 @@ __all__ = [
     "to_nf4",
     "linear_nf4",
     "implements",
+    "MXTensor",
+    "to_mx",
+    "linear_mx",
+    "lora_linear_mx",
     "FrozenNF4Linear",
     "LoRALinear",
     "DoRALinear",

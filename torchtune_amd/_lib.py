@@ -15,6 +15,8 @@ ABI_VERSION = 1
 
 TTAMD_BF16 = 0
 TTAMD_F32 = 1
+TTAMD_MXFP4 = 4
+TTAMD_MXFP8 = 8
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -195,6 +197,21 @@ SIGNATURES = {
     "ttamd_qkv_rope_repeat_bwd_bf16": (_int, [_c_void_p] * 7 + [_i64] * 5 + [_c_void_p]),
     "ttamd_swiglu_fwd_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "ttamd_cross_entropy_fwd_bwd_bf16": (_int, [_c_void_p, _c_void_p, _i64, _f32, _c_void_p, _c_void_p, _i64, _i64, _c_void_p]),
+    "ttamd_mx_quantize": (_int, [_c_void_p, _int, _i64, _i64, _int, _c_void_p, _c_void_p, _c_void_p]),
+    "ttamd_mx_dequantize": (_int, [_c_void_p, _c_void_p, _int, _i64, _i64, _int, _c_void_p, _c_void_p]),
+    "ttamd_mx_linear_workspace_bytes": (_size, [_i64, _i64, _i64, _int]),
+    "ttamd_mx_linear_bf16": (
+        _int, [_c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_mx_linear_dx_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "ttamd_mx_linear_dx_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_mx_kept_codes_bytes": (_size, [_i64, _i64]),
+    "ttamd_mx_kept_scales_bytes": (_size, [_i64, _i64]),
+    "ttamd_mx_lora_fwd_workspace_bytes": (_size, [_c_void_p, _int, _i64, _i64]),
+    "ttamd_mx_lora_fwd_bf16": (
+        _int, [_c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_mx_lora_bwd_workspace_bytes": (_size, [_c_void_p, _int, _i64, _i64]),
+    "ttamd_mx_lora_bwd_bf16": (
+        _int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
     "ttamd_swiglu_bwd_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 
@@ -215,6 +232,13 @@ class LoraGroupMember(ctypes.Structure):
                 ("quantized_data_t", _c_void_p), ("lora_a", _c_void_p), ("lora_b", _c_void_p), ("bias", _c_void_p),
                 ("y", _c_void_p), ("grad_lora_a", _c_void_p), ("grad_lora_b", _c_void_p), ("N", _i64), ("rank", _int),
                 ("scale", _f32)]
+
+
+class MxLoraMember(ctypes.Structure):
+    """``ttamd_mx_lora_member`` of the header: one adapter linear over an mxfp4 weight."""
+
+    _fields_ = [("codes", _c_void_p), ("scales", _c_void_p), ("lora_a", _c_void_p), ("lora_b", _c_void_p), ("bias", _c_void_p),
+                ("y", _c_void_p), ("grad_lora_a", _c_void_p), ("grad_lora_b", _c_void_p), ("N", _i64), ("rank", _int), ("scale", _f32)]
 
 
 _lock = threading.Lock()

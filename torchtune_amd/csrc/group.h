@@ -113,6 +113,8 @@ bool dense_group_gated_applies(const GroupGemm& d);
 int run_gemm_dense_group_fwd(const void* x, const GroupGemm& d, const void* h_cat, void* workspace, hipStream_t s, void* act = nullptr,
                              const void* tiles = nullptr);
 size_t dense_group_dx_workspace_bytes(const GroupDx& d);
+// the grouped grad-input on the members' weights as stacked forward tiles, whatever made them
+int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles_fwd, hipStream_t s);
 int run_gemm_dense_group_dx(const GroupDx& d, const void* gh_cat, void* gx, void* workspace, hipStream_t s,
                             const void* tiles_fwd = nullptr, bool paired = false);
 

@@ -1372,6 +1372,41 @@ size_t dense_group_dx_workspace_bytes(const GroupDx& d) {
 
 // tiles_fwd != nullptr: no expansion; the launch reads the tiles the forward launch of the same group left in its
 // workspace (the members' weights stacked by rows, or - paired - the gated pair's 128-column alternation).
+int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles_fwd, hipStream_t s) {
+  int64_t n_total = 0;
+  DenseArgs g = {};
+  g.nseg = d.n;
+  g.nout = 1;
+  for (int i = 0; i < d.n; ++i) {
+    TT_REQUIRE(aligned16(d.gy[i]) && d.N[i] % 64 == 0, "dense_dx_on_tiles: gradients must be 16-byte aligned and N (%lld) a multiple of 64", (long long)d.N[i]);
+    if (d.M * d.N[i] * 2 >= (int64_t(1) << 32)) return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: gradient %d too large for 32-bit offsets", i);
+    n_total += d.N[i];
+    g.seg[i].X = d.gy[i];
+    g.seg[i].Kc = (int)d.N[i];
+    if (d.rank[i] > 0) {
+      DenseAdapter& a = g.ad[g.nad++];
+      a.lX = reinterpret_cast<const uint16_t*>(gh_cat) + d.r_off[i];
+      a.lW = d.lora_a[i];
+      a.R = d.rank[i];
+      a.n_begin = 0;
+      a.n_end = (int)d.K;
+      a.lscale = 1.0f;
+    }
+  }
+  TT_REQUIRE(aligned16(tiles_fwd) && aligned16(gx) && d.K % 64 == 0, "dense_dx_on_tiles: tiles and gx must be 16-byte aligned, K (%lld) a multiple of 64", (long long)d.K);
+  if (!(n_total * 2 * 256 < (int64_t(1) << 32) && d.M < (1 << 30) && d.K < (1 << 30)))
+    return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: operands too large for 32-bit offsets");
+  g.out[0].C = reinterpret_cast<uint16_t*>(gx);
+  g.out[0].n_begin = 0;
+  g.out[0].width = (int)d.K;
+  g.Wt = reinterpret_cast<const char*>(tiles_fwd);
+  g.M = (int)d.M; g.Nout = (int)d.K; g.Kc = (int)n_total;
+  g.lw_row_major = 0;
+  g.ldlx = d.r_off[d.n];
+  g.w_tr = 1;
+  return launch_dense(g, s);
+}
+
 int run_gemm_dense_group_dx(const GroupDx& d, const void* gh_cat, void* gx, void* workspace, hipStream_t s, const void* tiles_fwd,
                             bool paired) {
   TT_REQUIRE(d.n >= 1 && d.n <= kGroupMax && dense_group_dx_workspace_bytes(d) > 0, "nf4_group_dx (expanded): shape not served");
