@@ -807,7 +807,8 @@ int ttamd_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int format,
 /*
  * y[M, N] = x^ . W^T (+ bias): x [M, K] bf16 is quantised to activation_format (TTAMD_MXFP8 or TTAMD_MXFP4) on its way in, W
  * is mxfp4 (w_codes [N, K / 2], w_scales [N, K / 32]).  K % 32 == 0, any M and N; bias bf16 [N] or NULL; y bf16.  fp32 sums,
- * one rounding.  Pointers 16-byte aligned (bias: 2); workspace: ttamd_mx_linear_workspace_bytes bytes.
+ * one rounding.  Pointers 16-byte aligned (bias: 2); workspace: ttamd_mx_linear_workspace_bytes bytes
+ * (0, few enough tokens: may be NULL).
  */
 size_t ttamd_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation_format);
 int ttamd_mx_linear_bf16(const void* x, int activation_format, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,

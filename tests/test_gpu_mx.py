@@ -161,3 +161,38 @@ def test_linear_grad_input(m, n, k):
     gx, gb = torch.autograd.grad(y, [xd, bd], gy.cuda())
     _close(gx, gy.double() @ dense, SUMS * (gy.double().abs() @ dense.abs()))
     _close(gb, gy.double().sum((0, 1)), SUMS * gy.double().abs().sum((0, 1)))
+
+
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 32, 47, 48, 49, 64, 65])
+@pytest.mark.parametrize("n,k", [(70, 96), (8200, 1056), (8192 + 16, 4096)])
+def test_linear_few_tokens(m, n, k, act):
+    """Every shape of the kernels for a handful of tokens: one to four tiles of tokens, 16 and 32 outputs per workgroup, and
+    inputs over the whole range."""
+    w, dense = _weight(n, k, 20)
+    x = _special((m, k), 21, torch.float32)
+    x = torch.where(x.abs() > 1e20, x * 1e-20, x).to(BF)  # products stay in range
+    y = linear_mx(x.cuda(), w, activation=act)
+    xq = ox.nearest(x, act)
+    _close(y, xq @ dense.T, (SUMS_FP8 if act == "mxfp8" else SUMS) * (xq.abs() @ dense.abs().T), 1.0)
+
+
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+def test_linear_non_finite_inputs_stay_in_their_row(m, act):
+    """A block of NaN (or with an infinity) makes its token NaN and no other; a NaN block of the weight its output."""
+    w, dense = _weight(96, 256, 22)
+    x = torch.randn(m, 256, generator=_seed(23)).to(BF)
+    x[0, 200] = float("nan")
+    if m > 2:
+        x[2, 3] = -float("inf")
+    w.scales[5, 7] = 255
+    y = linear_mx(x.cuda(), w, activation=act).cpu()
+    bad = torch.zeros(m, 96, dtype=torch.bool)
+    bad[0], bad[:, 5] = True, True
+    if m > 2:
+        bad[2] = True
+    assert torch.equal(torch.isnan(y), bad)
+    xq = ox.nearest(x, act)
+    want = (xq.nan_to_num() @ dense.T)[~bad]
+    _close(y[~bad], want, (SUMS_FP8 if act == "mxfp8" else SUMS) * (xq.nan_to_num().abs() @ dense.abs().T)[~bad])

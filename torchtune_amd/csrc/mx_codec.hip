@@ -30,13 +30,7 @@ struct Bf16x8 {
   mx_u32x4 v;
   __device__ __forceinline__ void load(const void* p, int64_t i) { v = reinterpret_cast<const mx_u32x4*>(p)[i]; }
   __device__ __forceinline__ void clear() { v = mx_u32x4{0, 0, 0, 0}; }
-  __device__ __forceinline__ uint32_t exponent() const {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 m = {0, 0};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[q] & 0x7fff7fffu));
-    return umax(m.x, m.y) >> 7;
-  }
+  __device__ __forceinline__ uint32_t exponent() const { return mx_bf16_exponent(v); }
 };
 struct F32x8 {
   float v[8];
@@ -59,16 +53,10 @@ struct F32x8 {
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
-  v = v > o ? v : o;
-  o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true);           // lanes 2 3 0 1
-  return v > o ? v : o;
-}
 // codes of one piece (zeros for a block of NaN) and the block's scale byte
 template <int FMT, typename V>
 __device__ __forceinline__ mx_u32x2 encode(const V& e, uint32_t& byte) {
-  byte = mx_scale_byte(quad_max(e.exponent()), FMT);
+  byte = mx_scale_byte(mx_quad_max(e.exponent()), FMT);
   const float s = mx_scale_value(byte == 255 ? 127u : byte);
   mx_u32x2 c = {0, 0};
   if constexpr (FMT == TTAMD_MXFP4)
@@ -111,7 +99,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
 #endif
 }
 
-// An input for the products: codes with the row padded to 128 elements by zeros, scales in the products' own layout, and -
+// An input for the products: codes with the row padded to 256 elements by zeros, scales in the products' own layout, and -
 // workgroups past the input's - the weights' scales in that layout (17 / 32 of a byte per element is all there is of a
 // weight, a sixteenth of it scales: their copy costs a launch more than it costs time).
 template <int FMT>
@@ -139,11 +127,11 @@ __global__ __launch_bounds__(256) void mx_quantize_operand_kernel(const void* __
       for (int q = 0; q < 16; ++q)
         if (16 * g + q < nb) d[q >> 2] |= (uint32_t)src[q] << (8 * (q & 3));
     }
-    mx_u32x4 o;
-    o.x = __builtin_amdgcn_perm(d.y, d.x, 0x06040200u);
-    o.y = __builtin_amdgcn_perm(d.w, d.z, 0x06040200u);
-    o.z = __builtin_amdgcn_perm(d.y, d.x, 0x07050301u);
-    o.w = __builtin_amdgcn_perm(d.w, d.z, 0x07050301u);
+    // byte 4 s + q -> byte 4 q + s
+    const uint32_t t0 = __builtin_amdgcn_perm(d.y, d.x, 0x05010400u), t1 = __builtin_amdgcn_perm(d.y, d.x, 0x07030602u);
+    const uint32_t u0 = __builtin_amdgcn_perm(d.w, d.z, 0x05010400u), u1 = __builtin_amdgcn_perm(d.w, d.z, 0x07030602u);
+    const mx_u32x4 o = {__builtin_amdgcn_perm(u0, t0, 0x05040100u), __builtin_amdgcn_perm(u0, t0, 0x07060302u),
+                        __builtin_amdgcn_perm(u1, t1, 0x05040100u), __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
     reinterpret_cast<mx_u32x4*>(w.pieces[which])[(int64_t)g * rows + row] = o;
     return;
   }

@@ -1,15 +1,18 @@
 // Products over microscaled operands: y[M, N] = x^[M, K] . W[N, K]^T (+ s . h . B^T) (+ bias), x^ in mxfp8 or mxfp4, W in
-// mxfp4, on v_mfma_scale_f32_32x32x64_f8f6f4, which multiplies the codes and applies both blocks' scales (fp32 sums).
+// mxfp4, on v_mfma_scale_f32_16x16x128_f8f6f4, which multiplies the codes and applies both blocks' scales (fp32 sums).
 //
-// Operand order of that instruction (lane l: row l % 32, half h = l / 32), found by comparing with products in 64 bits:
-//   fp4: 16 bytes, indices 32 h .. 32 h + 31 of the 64-wide step; fp8: two pieces of 16 bytes, indices 16 h .. and 32 + 16 h ..
-//   scale: the byte of block h of the step, selected from a dword; result: column l % 32 of the second operand, rows
-//   8 (v / 4) + 4 h + v % 4 of the first.
-// The weight is the first operand, so a lane holds four consecutive outputs of one row of y.
+// Operand order of that instruction (lane l: row l % 16, quarter q = l / 16), found by comparing with products in 64 bits:
+//   fp4: 16 bytes, indices 32 q .. 32 q + 31 of the 128-wide step; fp8: two pieces of 16 bytes, indices 16 q .. and 64 + 16 q ..
+//   scale: the lowest byte of a register, that of block q of the step; result: column l % 16 of the second operand, rows
+//   4 q + v of the first.
+// The weight is the first operand, so a lane holds four consecutive outputs of one row of y.  The 16 x 16 x 128 shape and not
+// 32 x 32 x 64: this part is limited by power under matrix load, and loops of nothing but these instructions on random
+// operands run at 4.0 against 3.3 PFLOP/s (fp8 x fp4) and 7.3 against 6.1 (fp4 x fp4).
 //
-// Workgroup: WM x WN waves, a wave computes TM x TN tiles of 32 x 32, k-step 128.  Codes go HBM -> LDS by direct loads of 16
+// Workgroup: WM x WN waves, a wave computes TM x TN tiles of 16 x 16, k-step 128.  Codes go HBM -> LDS by direct loads of 16
 // bytes per lane into a ring of three stages, scales likewise, one 16-byte piece per row and 512 contraction indices, into
-// a ring of two; nothing but LDS reads and matrix instructions is left in the waves.  One barrier per step.
+// a ring of two; nothing but LDS reads and matrix instructions is left in the waves.  One barrier per step.  The kernel is
+// persistent: a workgroup's items follow each other in one pipeline.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,14 +23,15 @@ namespace ttamd {
 namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
+#define TT_INLINE __attribute__((always_inline))
 #define TT_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
 
 struct MxGemmArgs {
-  const uint8_t* xc;   // [M, Kp] or [M, Kp / 2]: codes of the input, rows padded to 128 elements
+  const uint8_t* xc;   // [M, Kp] or [M, Kp / 2]: codes of the input, rows padded to 256 elements
   const uint8_t* xp;   // its scales, [groups][M][16]
   const uint8_t* wc;   // [N, K / 2]
   const uint8_t* wp;   // [groups][N][16]
@@ -41,247 +45,315 @@ struct MxGemmArgs {
   int tiles_m, tiles_n, slices, steps_per_slice;  // steps of 128, a multiple of 4 per slice
 };
 
+constexpr int kCUs = 256;
+
 template <int WM, int WN, int TM, int TN, bool F8>
 struct MxTile {
   static constexpr int kThreads = 64 * WM * WN;
-  static constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
+  static constexpr int BM = 16 * WM * TM, BN = 16 * WN * TN;
   static constexpr int kRowA = F8 ? 128 : 64, kRowW = 64;  // bytes of a row per step
   static constexpr int kA = BM * kRowA, kW = BN * kRowW, kStage = kA + kW;
   static constexpr int kStages = 3;
   static constexpr int kScales = (BM + BN) * 16;
-  static constexpr int kRings = kStages * kStage + 2 * kScales;
+  static constexpr int kLds = kStages * kStage + 2 * kScales;
+  static constexpr int kPerCU = kLds <= 53 * 1024 ? 3 : kLds <= 80 * 1024 ? 2 : 1;  // workgroups that a CU's LDS holds
   static constexpr int kLoadsA = kA / (kThreads * 16), kLoadsW = kW / (kThreads * 16);
   static constexpr int kScaleWaves = (BM + BN) / 64;  // waves' worth of scale pieces
   static constexpr int kLoadsS = (kScaleWaves + WM * WN - 1) / (WM * WN);
-  static constexpr int kPitch = 64 * TN + 16;  // bytes of a row of a wave's output band in LDS
-  static constexpr int kBands = WM * WN * 32 * TM * kPitch;
-  static constexpr int kLds = kRings > kBands ? kRings : kBands;
-  static_assert(kA % (kThreads * 16) == 0 && kW % (kThreads * 16) == 0, "whole loads");
+  static constexpr int kStores = TM * TN / 2;         // of a wave's whole tile
+  static_assert(kA % (kThreads * 16) == 0 && kW % (kThreads * 16) == 0 && (BM + BN) % 64 == 0, "whole loads");
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  static_assert(TN % 2 == 0, "two halves of a step");
 };
 
+// eight outputs of a row; rows of an odd length start anywhere
+struct __attribute__((packed, aligned(2))) MxStore16 {
+  uint32_t d[4];
+};
+
+// f(integral_constant<A>), .. f(integral_constant<B - 1>)
+template <int A, int B, typename F>
+__device__ __forceinline__ void for_range(F&& f) {
+  if constexpr (A < B) {
+    f(std::integral_constant<int, A>{});
+    for_range<A + 1, B>(f);
+  }
+}
+
 template <int WM, int WN, int TM, int TN, bool F8>
-__global__ __launch_bounds__(64 * WM * WN) void mx_gemm_kernel(const MxGemmArgs g) {
+__global__ __launch_bounds__(512) void mx_gemm_kernel(const MxGemmArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using T = MxTile<WM, WN, TM, TN, F8>;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
-
-  // workgroups go to the eight XCDs in turn: each takes a contiguous share of the tiles, in bands of eight row tiles so
-  // that the tiles in flight on one XCD share rows and columns in its L2
-  int tile_m, tile_n, slice;
-  {
-    const int tiles = g.tiles_m * g.tiles_n, total = (int)gridDim.x;
-    int id = (int)blockIdx.x;
-    const int q = total >> 3, rem = total & 7, xcd = id & 7, k = id >> 3;
-    id = xcd * q + (xcd < rem ? xcd : rem) + k;
-    slice = id / tiles;
-    id -= slice * tiles;
-    const int band = 8 * g.tiles_n, b = id / band, in = id - b * band;
-    const int rows = g.tiles_m - 8 * b < 8 ? g.tiles_m - 8 * b : 8;
-    tile_m = 8 * b + in % rows;
-    tile_n = in / rows;
-  }
-  const int m0 = tile_m * T::BM, n0 = tile_n * T::BN;
   const int nk_all = g.Kp >> 7;
-  const int k_begin = slice * g.steps_per_slice;
-  const int k_end = k_begin + g.steps_per_slice < nk_all ? k_begin + g.steps_per_slice : nk_all;
 
-  // ---- sources of the direct loads.  A stage's rows lie in LDS one after the other; the 16-byte pieces of a row are
-  //      permuted by the row (on the address side) so that the 32 rows a wave reads at one piece index spread over the banks
+  // Work items are (slice, tile).  In a round every workgroup takes one; the workgroups of an XCD (they go to the eight XCDs
+  // in turn) take consecutive items, and items walk the tiles in bands of eight row tiles, so that the tiles in flight on
+  // one XCD share rows and columns in its L2.  The last round is spread over the XCDs evenly.
+  const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.slices, grid = (int)gridDim.x;
+  const int xcd = (int)blockIdx.x & 7, place = (int)blockIdx.x >> 3;
+  auto item_of = [&](int round) TT_INLINE {  // -1: none
+    const int begin = round * grid, cnt = total - begin < grid ? total - begin : grid;
+    if (cnt <= 0) return -1;
+    const int q = cnt >> 3, rem = cnt & 7, share = q + (xcd < rem ? 1 : 0);
+    return place < share ? begin + xcd * q + (xcd < rem ? xcd : rem) + place : -1;
+  };
+  struct Item {
+    int m0, n0, k_begin, k_end, slice;
+  };
+  // divisions are worked out in vector registers: their results go back to scalar ones
+  auto uniform = [](int v) TT_INLINE { return __builtin_amdgcn_readfirstlane(v); };
+  auto decode = [&](int id) TT_INLINE {
+    Item w;
+    w.slice = uniform(id / tiles);
+    id -= w.slice * tiles;
+    const int band = 8 * g.tiles_n, b = uniform(id / band), in = id - b * band;
+    const int rows = g.tiles_m - 8 * b < 8 ? g.tiles_m - 8 * b : 8, across = uniform(in / rows);
+    w.m0 = (8 * b + in - across * rows) * T::BM;
+    w.n0 = across * T::BN;
+    w.k_begin = w.slice * g.steps_per_slice;
+    w.k_end = w.k_begin + g.steps_per_slice < nk_all ? w.k_begin + g.steps_per_slice : nk_all;
+    return w;
+  };
+
+  // ---- the requesting side: which step of which item is requested next.  A stage's rows lie in LDS one after the other;
+  //      the 16-byte pieces of a row are permuted by the row (on the address side) so that the rows a wave reads at one
+  //      piece index spread over the banks.  Buffer loads: the uniform part of an address is in scalar registers with the
+  //      number of bytes from there to the operand's end, and what lies past it (rows beyond M or N, a last weight row's
+  //      end, everything behind the last item) is not read.  A weight row that ends inside a step is followed by the next
+  //      row's codes: the input's are zero there.
   const uint32_t lds0 = (uint32_t)(uintptr_t)TT_LDS_PTR(smem);
   const int ldx = F8 ? g.Kp : g.Kp >> 1, ldw = g.K >> 1;
-  const char* const xbase = reinterpret_cast<const char*>(g.xc) + (int64_t)m0 * ldx;
-  const char* const wbase = reinterpret_cast<const char*>(g.wc) + (int64_t)n0 * ldw;
-  uint32_t a_off[T::kLoadsA], w_off[T::kLoadsW], w_over[T::kLoadsW];
-#pragma unroll
-  for (int i = 0; i < T::kLoadsA; ++i) {
-    const int slot = (wave * T::kLoadsA + i) * 64 + lane;  // 16-byte slot of the stage
-    const int row = F8 ? slot >> 3 : slot >> 2;
-    const int piece = F8 ? (slot & 7) ^ ((row >> 1) & 7) : (slot & 3) ^ ((row >> 2) & 3);
-    const int r = m0 + row < g.M ? row : g.M - 1 - m0;
-    a_off[i] = (uint32_t)r * (uint32_t)ldx + 16u * piece;
-  }
-  // the weight's rows are not padded: in a last step that reaches past their end the piece before it is read instead
-  // (the input's codes are zero there)
-#pragma unroll
-  for (int i = 0; i < T::kLoadsW; ++i) {
-    const int slot = (wave * T::kLoadsW + i) * 64 + lane;
-    const int row = slot >> 2, piece = (slot & 3) ^ ((row >> 2) & 3);
-    const int r = n0 + row < g.N ? row : g.N - 1 - n0;
-    w_off[i] = (uint32_t)r * (uint32_t)ldw + 16u * piece;
-    const int end = (nk_all - 1) * 64 + 16 * piece + 16;
-    w_over[i] = end > ldw ? (uint32_t)(end - ldw) : 0u;
-  }
-  // scale pieces: wave w loads rows [64 w, + 64) of the tile's BM input rows and BN weight rows, in rounds of all waves
-  const char* s_src[T::kLoadsS];
-  int64_t s_step[T::kLoadsS];
-  bool s_mine[T::kLoadsS];
-#pragma unroll
-  for (int i = 0; i < T::kLoadsS; ++i) {
-    const int sw = wave + i * WM * WN, row = sw * 64 + lane;
-    s_mine[i] = sw < T::kScaleWaves;
-    if (sw * 64 < T::BM) {
-      const int r = m0 + row < g.M ? m0 + row : g.M - 1;
-      s_src[i] = reinterpret_cast<const char*>(g.xp) + (int64_t)r * 16;
-      s_step[i] = (int64_t)g.M * 16;
+  constexpr int kRowsA = F8 ? 8 : 16;  // rows of an instruction (64 pieces): 128 or 64 bytes each
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  auto dma = [&](uint32_t off, const uint8_t* base, int bytes, uint32_t lds) TT_INLINE {
+    const uint64_t p = (uint64_t)(uintptr_t)base;
+    const v4i srd = {uniform((int)(uint32_t)p), uniform((int)((p >> 32) & 0xffff)), uniform(bytes > 0 ? bytes : 0), 0x00027000};
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(srd), "s"(lds) : "memory", "m0");
+  };
+  // what a lane number is turned into outside the loop over steps is worked out again where it is used: kept, it would take
+  // the registers that the sums need
+  auto fresh = [](int v) TT_INLINE {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  // A lane's offsets from an instruction's first row.  Piece p of a row lies at p ^ (row / 2) % 8 (rows of 128 bytes; odd
+  // instructions: + 4) or p ^ 2 (row / 8) % 2 (64 bytes): a 16-byte read serves lanes 0 - 3, 12 - 15, 20 - 27 and lanes 4 - 11,
+  // 16 - 19, 28 - 31 of each half wave at a time, and with these permutations their pieces fall on different banks
+  const uint32_t w_off = (uint32_t)(lane >> 2) * (uint32_t)ldw + 16u * (uint32_t)((lane & 3) ^ 2 * (lane >> 5));
+  const uint32_t a_off = F8 ? (uint32_t)(lane >> 3) * (uint32_t)ldx + 16u * (uint32_t)((lane & 7) ^ (lane >> 4))
+                            : (uint32_t)(lane >> 2) * (uint32_t)ldx + 16u * (uint32_t)((lane & 3) ^ 2 * (lane >> 5));
+  static_assert(T::kLoadsA % 2 == 0 || !F8, "the parity of an instruction is that of i");
+  int p_round = 0, p_k = 0, p_end = 0, p_stage = 0, p_ring = 0, p_m0 = 0, p_n0 = 0;
+  const uint8_t *p_x = nullptr, *p_w = nullptr;  // the tile's first rows at step p_k,
+  int p_xn = 0, p_wn = 0;                        // and the bytes from there to the operands' ends, as far as a tile reaches
+  bool p_more = false;
+  auto open = [&](int id) TT_INLINE {
+    p_more = id >= 0;
+    const Item w = decode(p_more ? id : 0);
+    p_k = w.k_begin;
+    p_end = w.k_end;
+    p_m0 = w.m0;
+    p_n0 = w.n0;
+    p_x = g.xc + (int64_t)w.m0 * ldx + w.k_begin * T::kRowA;
+    p_w = g.wc + (int64_t)w.n0 * ldw + w.k_begin * T::kRowW;
+    // requests behind the last item read nothing: the number in flight stays what the waits assume
+    p_xn = p_more ? (g.M - w.m0 < T::BM + 1 ? g.M - w.m0 : T::BM + 1) * ldx - w.k_begin * T::kRowA : 0;
+    p_wn = p_more ? (g.N - w.n0 < T::BN + 1 ? g.N - w.n0 : T::BN + 1) * ldw - w.k_begin * T::kRowW : 0;
+  };
+  // load i of the next step's operands
+  auto request = [&](auto i_) TT_INLINE {
+    constexpr int i = decltype(i_)::value;
+    const uint32_t st = lds0 + p_stage * T::kStage;
+    if constexpr (i < T::kLoadsA) {
+      const int q = wave * T::kLoadsA + i;
+      dma(((uint32_t)fresh((int)a_off) ^ (F8 && (i & 1) ? 64u : 0u)) + (uint32_t)(q * kRowsA) * (uint32_t)ldx, p_x, p_xn, st + q * 1024);
     } else {
-      const int r = n0 + row - T::BM < g.N ? n0 + row - T::BM : g.N - 1;
-      s_src[i] = reinterpret_cast<const char*>(g.wp) + (int64_t)r * 16;
-      s_step[i] = (int64_t)g.N * 16;
-    }
-  }
-  auto dma = [&](uint32_t off, const char* base, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
-  };
-  auto issue = [&](int kt, int stage) {  // past the end: the last step again, so that the number of loads in flight is known
-    const bool last = kt >= nk_all - 1;
-    kt = kt < nk_all ? kt : nk_all - 1;
-    const uint32_t sa = lds0 + stage * T::kStage;
-    const char* xb = xbase + (int64_t)kt * T::kRowA;
-    const char* wb = wbase + (int64_t)kt * T::kRowW;
-#pragma unroll
-    for (int i = 0; i < T::kLoadsA; ++i) dma(a_off[i], xb, sa + (wave * T::kLoadsA + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < T::kLoadsW; ++i) {
-      // unsigned wrap-around of the 32-bit offset is avoided: over <= 48 is taken off the piece's own offset
-      dma(last ? w_off[i] + (uint32_t)((kt * T::kRowW)) - w_over[i] : w_off[i], last ? wbase : wb, sa + T::kA + (wave * T::kLoadsW + i) * 1024);
+      const int q = wave * T::kLoadsW + i - T::kLoadsA;
+      dma((uint32_t)fresh((int)w_off) + (uint32_t)(q * 16) * (uint32_t)ldw, p_w, p_wn, st + T::kA + q * 1024);
     }
   };
-  const int groups = (nk_all + 3) >> 2;
-  auto issue_scales = [&](int grp, int ring) {
-    grp = grp < groups ? grp : groups - 1;
+  // on to the step after it; at the first step of a group of four its scales are requested (waves in turn: 64 rows each of
+  // the tile's BM input rows and BN weight rows)
+  auto request_scales = [&]() TT_INLINE {
+    if ((p_k & 3) == 0 && p_more) {
 #pragma unroll
-    for (int i = 0; i < T::kLoadsS; ++i) {
-      if (s_mine[i] || T::kLoadsS == 1) {
-        const uint32_t dst = lds0 + T::kStages * T::kStage + ring * T::kScales + (wave + i * WM * WN) * 1024;
-        if (s_mine[i])
-          asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(s_src[i] + grp * s_step[i]), "s"(dst) : "memory", "m0");
+      for (int i = 0; i < T::kLoadsS; ++i) {
+        const int sw = wave + i * WM * WN;
+        if (sw < T::kScaleWaves) {
+          const bool of_x = sw * 64 < T::BM;
+          const int rows = of_x ? g.M : g.N, first = of_x ? p_m0 + 64 * sw : p_n0 + 64 * sw - T::BM;
+          dma(16u * (uint32_t)fresh(threadIdx.x & 63), (of_x ? g.xp : g.wp) + ((int64_t)(p_k >> 2) * rows + first) * 16,
+              (rows - first < 64 ? rows - first : 64) * 16,
+              lds0 + T::kStages * T::kStage + p_ring * T::kScales + sw * 1024);
+        }
       }
+      p_ring ^= 1;
     }
   };
+  auto advance = [&]() TT_INLINE {
+    p_x += T::kRowA;
+    p_w += T::kRowW;
+    p_xn -= T::kRowA;
+    p_wn -= T::kRowW;
+    p_stage = p_stage == 2 ? 0 : p_stage + 1;
+    if (++p_k == p_end) open(item_of(++p_round));
+  };
 
-  v16f acc[TN][TM];
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[j][i][v] = 0.f;
+  int round = 0, id = item_of(0);
+  if (id < 0) return;
+  Item it = decode(id);
+  open(id);
 
-  // operand reads: piece p of row r of the input at a_rd + 32 i rows, of the weight at w_rd + 32 j rows
-  const int ar = 32 * TM * wm + l31, wr = 32 * TN * wn + l31;
-  int a_rd[4], w_rd[2];
+  v4f acc[TN][TM];
+  auto clear = [&]() TT_INLINE {
 #pragma unroll
-  for (int p = 0; p < 4; ++p)  // F8: pieces 4 c + h and 4 c + 2 + h of sub-step c; fp4: piece 2 c + h
-    a_rd[p] = F8 ? ar * 128 + (((2 * p + half) ^ ((ar >> 1) & 7)) << 4) : ar * 64 + ((((2 * p + half) & 3) ^ ((ar >> 2) & 3)) << 4);
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-  for (int p = 0; p < 2; ++p) w_rd[p] = T::kA + wr * 64 + (((2 * p + half) ^ ((wr >> 2) & 3)) << 4);
-  const int s_rd = T::kStages * T::kStage + 8 * half;
+      for (int i = 0; i < TM; ++i) acc[j][i] = v4f{0.f, 0.f, 0.f, 0.f};
+  };
 
-  mx_u32x2 sx[TM], sw[TN];
-  auto read_scales = [&](int ring) {
+  // operand reads: pieces of rows ar + 16 i of the input and wr + 16 j of the weight (16 rows on, the permutation repeats)
+  const int ar = 16 * TM * wm + r16, wr = 16 * TN * wn + r16;
+  const int a_rd0 = F8 ? ar * 128 + ((quarter ^ ((ar >> 1) & 7)) << 4) : ar * 64 + ((quarter ^ 2 * ((ar >> 3) & 1)) << 4);
+  const int a_rd1 = ar * 128 + (((4 + quarter) ^ ((ar >> 1) & 7)) << 4);
+  const int w_rd = T::kA + wr * 64 + ((quarter ^ 2 * ((wr >> 3) & 1)) << 4);
+  const int s_rd = T::kStages * T::kStage + 4 * quarter;
+
+  // Scales: a dword per tile holds four steps, the current pair's in its low half; it is shifted from pair to pair.
+  // Operands: the input's of a step, each tile's replaced by the next step's as soon as it has been multiplied for the last
+  // time, and the weight's of two half steps (the first and the last TN / 2 of its tiles).
+  constexpr int TH = TN / 2;
+  uint32_t sx[TM], sw[TN];
+  v4i xf[TM][F8 ? 2 : 1], wf[2][TH];
+  auto read_scales = [&](int ring) TT_INLINE {
     const char* p = smem + s_rd + ring * T::kScales;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) sx[i] = *reinterpret_cast<const mx_u32x2*>(p + (ar + 32 * i) * 16);
+    for (int i = 0; i < TM; ++i) sx[i] = *reinterpret_cast<const uint32_t*>(p + (ar + 16 * i) * 16);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sw[j] = *reinterpret_cast<const mx_u32x2*>(p + (T::BM + wr + 32 * j) * 16);
+    for (int j = 0; j < TN; ++j) sw[j] = *reinterpret_cast<const uint32_t*>(p + (T::BM + wr + 16 * j) * 16);
   };
-  auto load4 = [&](const char* p, v8i& v, int at) {
-    const mx_u32x4 q = *reinterpret_cast<const mx_u32x4*>(p);
+  auto shift_scales = [&]() TT_INLINE {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[at + e] = (int)q[e];
+    for (int i = 0; i < TM; ++i) sx[i] >>= 16;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sw[j] >>= 16;
   };
-  // step S of a group of four (S picks the scales' byte)
-  auto step = [&](int stage, auto which) {
-    constexpr int S = decltype(which)::value;
+  auto load4 = [&](const char* p) TT_INLINE { return *reinterpret_cast<const v4i*>(p); };
+  auto read_x = [&](int stage, int i) TT_INLINE {
     const char* st = smem + stage * T::kStage;
+    xf[i][0] = load4(st + a_rd0 + i * 16 * T::kRowA);
+    if constexpr (F8) xf[i][1] = load4(st + a_rd1 + i * 16 * T::kRowA);
+  };
+  auto read_w = [&](int stage, auto half_, int j) TT_INLINE {
+    constexpr int c = decltype(half_)::value;
+    wf[c][j] = load4(smem + stage * T::kStage + w_rd + (TH * c + j) * 16 * 64);
+  };
+  // fp4 operands take four of the eight registers
+  auto wide = [&](v4i lo, v4i hi) TT_INLINE { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); };
+  // after_tile(i): what else the wave does while the matrix cores work, one share after each of the input's tiles
+  auto multiply = [&](auto step_, auto half_, auto after_tile) TT_INLINE {
+    constexpr int S = decltype(step_)::value, c = decltype(half_)::value;
+    __builtin_amdgcn_sched_barrier(0);
+    for_range<0, TM>([&](auto i_) TT_INLINE {
+      constexpr int i = decltype(i_)::value;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      v8i xf[TM] = {}, wf[TN] = {};
+      for (int j = 0; j < TH; ++j)
+        acc[TH * c + j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(wf[c][j], wf[c][j]), wide(xf[i][0], xf[i][F8 ? 1 : 0]),
+                                                                             acc[TH * c + j][i], 4, F8 ? 0 : 4, S, (int)sw[TH * c + j], S, (int)sx[i]);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      after_tile(i_);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    // the products stay in front of what follows: the compiler would sink them behind the next barrier, into the block where
+    // their sums are used next
+#pragma unroll
+    for (int j = 0; j < TH; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(acc[TH * c + j][i]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // ---- what becomes of an item's sums
+  auto finish = [&]() TT_INLINE {
+    const int lane = fresh(threadIdx.x & 63), r16 = lane & 15, quarter = lane >> 4, ar = 16 * TM * wm + r16;
+    if (g.slices > 1) {
+      // fp32 sums of this slice, rounded and finished by the sum of the slices
+      float* out = g.part + (int64_t)it.slice * g.M * g.N;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        if constexpr (F8) {
-          load4(st + a_rd[2 * c] + i * 32 * 128, xf[i], 0);
-          load4(st + a_rd[2 * c + 1] + i * 32 * 128, xf[i], 4);
-        } else {
-          load4(st + a_rd[c] + i * 32 * 64, xf[i], 0);
+        const int row = it.m0 + ar + 16 * i;
+        if (row >= g.M) continue;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int col = it.n0 + 16 * (TN * wn + j) + 4 * quarter;
+          float* p = out + (int64_t)row * g.N + col;
+          if ((g.N & 3) == 0) {
+            if (col < g.N) *reinterpret_cast<v4f*>(p) = acc[j][i];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < g.N) p[e] = acc[j][i][e];
+          }
         }
       }
-#pragma unroll
-      for (int j = 0; j < TN; ++j) load4(st + w_rd[c] + j * 32 * 64, wf[j], 0);
-      constexpr int kDword = S >> 1;
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          // byte 2 (S % 2) + c of the dword: the selects are immediates
-          if (c == 0)
-            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, F8 ? 0 : 4, 2 * (S & 1), sw[j][kDword],
-                                                                       2 * (S & 1), sx[i][kDword]);
-          else
-            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[j][i], 4, F8 ? 0 : 4, 2 * (S & 1) + 1, sw[j][kDword],
-                                                                       2 * (S & 1) + 1, sx[i][kDword]);
-        }
+      return;
     }
-  };
-
-  // ---- pipeline.  Loads of a wave complete in order.  At step t a wave waits until what it requested for step t has
-  //      landed, passes the barrier (everybody's has, and everybody is done with step t - 1), requests step t + 2 into the
-  //      stage of step t - 1, and computes.  Program order: scales 0, stage 0, stage 1; step t: (t % 4 == 0: the next
-  //      group's scales,) stage t + 2.  Newer than stage t at step t's wait are the loads of stage t + 1; scales requested in
-  //      between are waited for with it, three steps before they are read.
-  constexpr int kStageLoads = T::kLoadsA + T::kLoadsW;
-  auto wait_for = [&]() {
-    // lgkmcnt: this wave's reads of step t - 1 are complete before another wave's loads may overwrite them
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStageLoads) : "memory");
-  };
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  using I2 = std::integral_constant<int, 2>;
-  using I3 = std::integral_constant<int, 3>;
-  int stage = 0, ring = 0;
-  auto next = [&]() { stage = stage == 2 ? 0 : stage + 1; };
-  auto two_on = [&]() { return stage == 0 ? 2 : stage - 1; };
-  issue_scales(k_begin >> 2, 0);
-  issue(k_begin, 0);
-  issue(k_begin + 1, 1);
-  for (int t = k_begin; t < k_end; t += 4) {
-    wait_for();
-    issue_scales((t >> 2) + 1, ring ^ 1);
-    issue(t + 2, two_on());
-    read_scales(ring);
-    step(stage, I0{});
-    next();
-    if (t + 1 >= k_end) break;
-    wait_for();
-    issue(t + 3, two_on());
-    step(stage, I1{});
-    next();
-    if (t + 2 >= k_end) break;
-    wait_for();
-    issue(t + 4, two_on());
-    step(stage, I2{});
-    next();
-    if (t + 3 >= k_end) break;
-    wait_for();
-    issue(t + 5, two_on());
-    step(stage, I3{});
-    next();
-    ring ^= 1;
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the requests past the end
-
-  // ---- adapter: s . h . B^T as further contraction steps of 16 ranks, the scale rounded into h's side
-  if (g.rank > 0 && slice == 0) {
-    for (int r0 = 0; r0 < g.rank; r0 += 16) {
-      const int r = r0 + 8 * half;
-      bf16x8_t hx[TM], bw[TN];
+    // Two neighbouring tiles' outputs change places between neighbouring quarters: a lane of quarter q then holds the eight
+    // outputs 8 (q / 2) .. of tile j + q % 2 in its row
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      asm volatile("" ::: "memory");  // one pair of tiles after the other: all of them at once do not fit the registers
+      const int n0 = it.n0 + 16 * (TN * wn + j);
+      float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (g.bias) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // before the exchange: four of each tile
+          const int n = n0 + 16 * (e >> 2) + 4 * quarter + (e & 3);
+          b[e] = n < g.N ? __builtin_bit_cast(float, (uint32_t)g.bias[n] << 16) : 0.f;
+        }
+      }
+      const int col = n0 + 16 * (quarter & 1) + 8 * (quarter >> 1);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        int row = m0 + ar + 32 * i;
+        uint32_t d[4];  // pairs of outputs of tile j in d[0], d[1], of tile j + 1 in d[2], d[3]
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          mx_bf16x2 o;
+          o.x = (__bf16)(acc[j + (e >> 1)][i][2 * (e & 1)] + b[2 * e]);
+          o.y = (__bf16)(acc[j + (e >> 1)][i][2 * (e & 1) + 1] + b[2 * e + 1]);
+          d[e] = __builtin_bit_cast(uint32_t, o);
+        }
+        const auto s0 = __builtin_amdgcn_permlane16_swap(d[0], d[2], false, false);
+        const auto s1 = __builtin_amdgcn_permlane16_swap(d[1], d[3], false, false);
+        MxStore16 o;
+        o.d[0] = s0[0]; o.d[1] = s1[0]; o.d[2] = s0[1]; o.d[3] = s1[1];
+        const int row = it.m0 + ar + 16 * i;
+        uint16_t* y = g.y + (int64_t)row * g.N + col;
+        if (row < g.M && col + 8 <= g.N) {
+          *reinterpret_cast<MxStore16*>(y) = o;
+        } else if (row < g.M) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < g.N) y[e] = (uint16_t)(o.d[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  };
+  // adapter: s . h . B^T as further contraction steps of 32 ranks, the factor rounded into h's side
+  auto adapt = [&]() TT_INLINE {
+    const int lane = fresh(threadIdx.x & 63), r16 = lane & 15, quarter = lane >> 4, ar = 16 * TM * wm + r16, wr = 16 * TN * wn + r16;
+    for (int r0 = 0; r0 < g.rank; r0 += 32) {
+      const int r = r0 + 8 * quarter;
+      bf16x8_t hx[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        int row = it.m0 + ar + 16 * i;
         row = row < g.M ? row : g.M - 1;
         bf16x8_t v = {};
         if (r < g.rank) v = *reinterpret_cast<const bf16x8_t*>(g.h + (int64_t)row * g.ldh + r);
@@ -290,81 +362,92 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_gemm_kernel(const MxGemmArgs 
         hx[i] = v;
       }
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        int row = n0 + wr + 32 * j;
-        row = row < g.N ? row : g.N - 1;
-        bf16x8_t v = {};
-        if (r < g.rank) v = *reinterpret_cast<const bf16x8_t*>(g.lb + (int64_t)row * g.rank + r);
-        bw[j] = v;
-      }
+      for (int c = 0; c < 2; ++c) {
+        asm volatile("" ::: "memory");  // half of the weight's tiles at a time
+        bf16x8_t bw[TH];
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[j], hx[i], acc[j][i], 0, 0, 0);
-    }
-  }
-
-  if (g.slices > 1) {
-    // fp32 sums of this slice, rounded and finished by the sum of the slices
-    float* out = g.part + (int64_t)slice * g.M * g.N;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int row = m0 + ar + 32 * i;
-      if (row >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int col = n0 + 32 * TN * wn + 32 * j + 8 * (v >> 2) + 4 * half + (v & 3);
-          if (col < g.N) out[(int64_t)row * g.N + col] = acc[j][i][v];
+        for (int j = 0; j < TH; ++j) {
+          int row = it.n0 + wr + 16 * (TH * c + j);
+          row = row < g.N ? row : g.N - 1;
+          bf16x8_t v = {};
+          if (r < g.rank) v = *reinterpret_cast<const bf16x8_t*>(g.lb + (int64_t)row * g.rank + r);
+          bw[j] = v;
         }
-    }
-    return;
-  }
-  // ---- the wave's band [32 TM rows][32 TN columns] goes through LDS so that whole row segments are stored
-  __syncthreads();
-  char* band = smem + wave * (32 * TM * T::kPitch);
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
+        for (int j = 0; j < TH; ++j)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int col = n0 + 32 * TN * wn + 32 * j + 8 * q + 4 * half;
-      float b[4] = {0.f, 0.f, 0.f, 0.f};
-      if (g.bias) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < g.N) b[e] = __builtin_bit_cast(float, (uint32_t)g.bias[col + e] << 16);
-      }
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        bf16x4_t o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (__bf16)(acc[j][i][4 * q + e] + b[e]);
-        *reinterpret_cast<bf16x4_t*>(band + (l31 + 32 * i) * T::kPitch + (32 * j + 8 * q + 4 * half) * 2) = o;
+          for (int i = 0; i < TM; ++i) acc[TH * c + j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[j], hx[i], acc[TH * c + j][i], 0, 0, 0);
       }
     }
+  };
+
+  // ---- pipeline over the steps of all of the workgroup's items.  While the matrix cores work on the first half of the
+  //      weight's tiles of step t a wave reads the second half from LDS; then it waits until what it requested for step
+  //      t + 1 has landed, passes the barrier (everybody's has, and everybody's reads of step t are complete), requests step
+  //      t + 3 into the stage of step t, and reads the input and the weight's first half of step t + 1 while the second half
+  //      of step t is multiplied.  An item's outputs are stored while the next one's first steps are on their way.
+  //      Memory operations of a wave complete in order.  Newer than stage t + 1 at step t's wait are the loads of stage
+  //      t + 2 (scales requested in between are waited for with it) and, in the first two steps of an item, the stores of
+  //      the item before: a whole tile's are counted, others are waited for.
+  constexpr int kStageLoads = T::kLoadsA + T::kLoadsW;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  int stage = 0, ring = 0, stored = 0;  // stored: steps for which whole-tile stores may still be in flight
+  for (int t = 0; t < 3; ++t) {
+    request_scales();
+    for_range<0, kStageLoads>(request);
+    advance();
   }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // only this wave reads its band
-  const int col0 = n0 + 32 * TN * wn, row_first = m0 + 32 * TM * wm;
-  if ((g.N & 7) == 0) {
-    constexpr int kPer = 4 * TN;  // 16-byte pieces of a row
-    constexpr int kRows = 64 / kPer;
-#pragma unroll
-    for (int r = 0; r < 32 * TM; r += kRows) {
-      const int rr = r + lane / kPer, c = 8 * (lane % kPer);
-      const mx_u32x4 v = *reinterpret_cast<const mx_u32x4*>(band + rr * T::kPitch + 2 * c);
-      if (row_first + rr < g.M && col0 + c < g.N) *reinterpret_cast<mx_u32x4*>(g.y + (int64_t)(row_first + rr) * g.N + col0 + c) = v;
-    }
-  } else {
-    for (int r = 0; r < 32 * TM; ++r) {
-      if (row_first + r >= g.M) break;
-#pragma unroll
-      for (int c = lane; c < 32 * TN; c += 64) {
-        const uint16_t v = *reinterpret_cast<const uint16_t*>(band + r * T::kPitch + 2 * c);
-        if (col0 + c < g.N) g.y[(int64_t)(row_first + r) * g.N + col0 + c] = v;
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * kStageLoads) : "memory");
+  auto begin_item = [&]() TT_INLINE {
+    read_scales(ring);
+    for_range<0, TM>([&](auto i) TT_INLINE { read_x(stage, i); });
+    for_range<0, TH>([&](auto j) TT_INLINE { read_w(stage, I0{}, j); });
+    clear();
+  };
+  begin_item();
+  auto step = [&](auto step_) TT_INLINE {
+    multiply(step_, I0{}, [&](auto i_) TT_INLINE {  // shares of TH weight tiles
+      constexpr int i = decltype(i_)::value;
+      for_range<TH * i / TM, TH*(i + 1) / TM>([&](auto j) TT_INLINE { read_w(stage, I1{}, j); });
+    });
+    if (stored > 0)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStageLoads + T::kStores) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStageLoads) : "memory");
+    --stored;
+    request_scales();
+    stage = stage == 2 ? 0 : stage + 1;
+    multiply(step_, I1{}, [&](auto i_) TT_INLINE {
+      constexpr int i = decltype(i_)::value;
+      read_x(stage, i);
+      for_range<TH * i / TM, TH*(i + 1) / TM>([&](auto j) TT_INLINE { read_w(stage, I0{}, j); });
+      for_range<kStageLoads * i / TM, kStageLoads*(i + 1) / TM>(request);
+    });
+    advance();
+  };
+  for (;;) {
+    for (int t = it.k_begin;; t += 2) {  // the input's rows are padded to whole pairs of steps by zeros
+      step(I0{});
+      step(I1{});
+      if (t + 2 >= it.k_end) break;
+      if ((t & 2) != 0) {
+        ring ^= 1;
+        read_scales(ring);
+      } else {
+        shift_scales();
       }
     }
+    if (g.rank > 0 && it.slice == 0) adapt();
+    finish();
+    id = item_of(++round);
+    if (id < 0) break;
+    stored = g.slices == 1 && it.m0 + T::BM <= g.M && it.n0 + T::BN <= g.N ? 2 : 0;
+    it = decode(id);
+    ring ^= 1;
+    begin_item();  // once more what the last step has read: held through the end of an item it would take its registers
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #endif
 }
 
@@ -391,11 +474,6 @@ __global__ __launch_bounds__(256) void mx_sum_slices_kernel(const float* __restr
     y[i + e] = __builtin_bit_cast(uint16_t, (__bf16)(s[e] + b));
   }
 }
-
-using TileL8 = MxTile<4, 2, 2, 4, true>;
-using TileL4 = MxTile<4, 2, 2, 4, false>;
-using TileS8 = MxTile<2, 2, 2, 2, true>;
-using TileS4 = MxTile<2, 2, 2, 2, false>;
 
 struct MxPlan {
   bool large;
@@ -427,9 +505,10 @@ int launch_mx(MxGemmArgs& g, hipStream_t s) {
     if (e != hipSuccess) return fail(TTAMD_ELAUNCH, "mx_gemm: cannot reserve %d bytes of LDS: %s", T::kLds, hipGetErrorString(e));
     if (dev >= 0) attr_set[dev] = true;
   }
-  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.slices;
-  if (blocks >= (int64_t(1) << 31)) return fail(TTAMD_EUNSUPPORTED, "mx_gemm: M=%d N=%d are too large for one launch", g.M, g.N);
-  mx_gemm_kernel<WM, WN, TM, TN, F8><<<dim3((unsigned)blocks), dim3(T::kThreads), T::kLds, s>>>(g);
+  const int64_t items = (int64_t)g.tiles_m * g.tiles_n * g.slices;
+  if (items >= (int64_t(1) << 30)) return fail(TTAMD_EUNSUPPORTED, "mx_gemm: M=%d N=%d are too large for one launch", g.M, g.N);
+  const int64_t grid = std::min<int64_t>((items + 7) / 8 * 8, kCUs * T::kPerCU);
+  mx_gemm_kernel<WM, WN, TM, TN, F8><<<dim3((unsigned)grid), dim3(T::kThreads), T::kLds, s>>>(g);
   return check_launch("mx_gemm");
 }
 
@@ -460,9 +539,9 @@ int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, fl
   TT_REQUIRE(p.slices == 1 || part, "mx_gemm: no room for the slices of the contraction");
   int rc;
   if (fmt == TTAMD_MXFP8)
-    rc = p.large ? launch_mx<4, 2, 2, 4, true>(g, s) : launch_mx<2, 2, 2, 2, true>(g, s);
+    rc = p.large ? launch_mx<4, 2, 4, 8, true>(g, s) : launch_mx<2, 2, 4, 4, true>(g, s);
   else
-    rc = p.large ? launch_mx<4, 2, 2, 4, false>(g, s) : launch_mx<2, 2, 2, 2, false>(g, s);
+    rc = p.large ? launch_mx<4, 2, 4, 8, false>(g, s) : launch_mx<2, 2, 4, 4, false>(g, s);
   if (rc || p.slices == 1) return rc;
   const int64_t numel = M * N;
   mx_sum_slices_kernel<<<dim3((unsigned)((numel + 1023) / 1024)), dim3(256), 0, s>>>(part, q.bias, q.y, numel, (int)N, p.slices);
@@ -471,7 +550,7 @@ int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, fl
 
 int check_mx_product(const char* who, int64_t M, int64_t N, int64_t K) {
   TT_REQUIRE(M > 0 && N > 0 && K > 0 && K % kMxBlock == 0, "%s: bad shape M=%lld N=%lld K=%lld (K is a multiple of 32)", who, (long long)M, (long long)N, (long long)K);
-  if (!(M < (1 << 30) && N < (1 << 30) && K < (1 << 23))) return fail(TTAMD_EUNSUPPORTED, "%s: M=%lld N=%lld K=%lld are too large", who, (long long)M, (long long)N, (long long)K);
+  if (!(M < (1 << 30) && N < (1 << 30) && K < (1 << 22))) return fail(TTAMD_EUNSUPPORTED, "%s: M=%lld N=%lld K=%lld are too large", who, (long long)M, (long long)N, (long long)K);
   return TTAMD_OK;
 }
 
@@ -480,7 +559,8 @@ int check_mx_product(const char* who, int64_t M, int64_t N, int64_t K) {
 using namespace ttamd;
 
 extern "C" size_t ttamd_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation_format) {
-  if (M <= 0 || N <= 0 || K <= 0 || K % kMxBlock) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K % kMxBlock || mx_few_quantises(M, K)) return 0;
+  if (mx_few_applies(M)) return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K));
   return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K)) + align256(mx_piece_bytes(N, K)) + mx_gemm_part_bytes(M, N, K);
 }
 
@@ -492,15 +572,20 @@ extern "C" int ttamd_mx_linear_bf16(const void* x, int activation_format, const 
                  (reinterpret_cast<uintptr_t>(bias) & 1u) == 0,
              "mx_linear: pointers must be non-null and 16-byte aligned");
   const size_t need = ttamd_mx_linear_workspace_bytes(M, N, K, activation_format);
-  if (workspace_bytes < need || !workspace || !aligned16(workspace))
+  if (need > 0 && (workspace_bytes < need || !workspace || !aligned16(workspace)))
     return fail(TTAMD_EWORKSPACE, "mx_linear: needs %zu bytes of 16-byte aligned workspace, got %zu", need, workspace_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (mx_few_quantises(M, K)) return run_mx_few(x, nullptr, nullptr, w_codes, w_scales, bias, y, M, N, K, activation_format, s);
   char* w = reinterpret_cast<char*>(workspace);
   MxProduct q = {};
   uint8_t* xc = reinterpret_cast<uint8_t*>(w);
   w += mx_operand_bytes(M, K, activation_format);
   uint8_t* xp = reinterpret_cast<uint8_t*>(w);
   w += align256(mx_piece_bytes(M, K));
+  if (mx_few_applies(M)) {
+    if (int rc = run_mx_quantize_operand(x, M, K, activation_format, xc, xp, nullptr, nullptr, nullptr, 0, s)) return rc;
+    return run_mx_few(nullptr, xc, xp, w_codes, w_scales, bias, y, M, N, K, activation_format, s);
+  }
   uint8_t* wp = reinterpret_cast<uint8_t*>(w);
   w += align256(mx_piece_bytes(N, K));
   if (int rc = run_mx_quantize_operand(x, M, K, activation_format, xc, xp, &w_scales, &N, &wp, 1, s)) return rc;

@@ -31,14 +31,34 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t E, int fmt) {
   return E == 255 ? 255u : (E > em ? E - em : 0u);
 }
 
-// fp8 conversions saturate instead of giving NaN from here to the end of the wave
-__device__ __forceinline__ void mx_saturate_fp8() {
+// fp8 conversions saturate instead of giving NaN from here on.  Switched off again in waves that go on to multiply: the mode
+// also takes the NaN out of what they compute.
+__device__ __forceinline__ void mx_saturate_fp8(bool on = true) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_s_setreg(1 | (23 << 6), 1);  // hwreg(MODE), bit 23: FP16_OVFL
+  __builtin_amdgcn_s_setreg(1 | (23 << 6), on ? 1 : 0);  // hwreg(MODE), bit 23: FP16_OVFL
 #endif
 }
 
+// largest biased exponent of eight bf16
+__device__ __forceinline__ uint32_t mx_bf16_exponent(const mx_u32x4& v) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t mag = v[q] & 0x7fff7fffu;
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, mag));
+  }
+  return (uint32_t)(m.x > m.y ? m.x : m.y) >> 7;
+}
+
 #if defined(__HIP_DEVICE_COMPILE__)
+// the largest of four neighbouring lanes' values
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
+  uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2
+  v = v > o ? v : o;
+  o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true);           // lanes 2 3 0 1
+  return v > o ? v : o;
+}
 __device__ __forceinline__ mx_bf16x2 mx_pair(uint32_t v) { return __builtin_bit_cast(mx_bf16x2, v); }
 // eight elements, as four packed bf16 pairs / as floats, into fp4 (one dword) or fp8 (two)
 __device__ __forceinline__ uint32_t mx_pack4(const mx_u32x4& v, float s) {
@@ -104,14 +124,14 @@ __device__ __forceinline__ void mx_f32_of_fp8(mx_u32x2 c, float s, float (&o)[8]
 // ---------------------------------------------------------------------------------------------------
 // The products' own layout of scales.  Of each row the 16 scale bytes of 512 contraction indices (16 blocks) form one
 // piece, and the pieces of all rows for the same 512 indices lie one after the other: [K / 512 rounded up][rows][16].
-// v_mfma_scale_f32_32x32x64 takes the scale of block 2 c + h of a 64-wide step from lane half h, so byte 8 h + c of a piece
-// holds block 2 c + h: a lane finds the eight scales of its half side by side, and picks one by the instruction's byte
-// select.  Blocks past the end of a row have scale byte 0 (2^-127): whatever codes meet there add less than 2^-149.
+// v_mfma_scale_f32_16x16x128 takes the scale of block q of a 128-wide step from lane quarter q, so byte 4 q + s of a piece
+// holds block 4 s + q: a lane finds the scales of its four steps in one dword.  Blocks past the end of a row have scale byte 0
+// (2^-127), and the input's codes are zero there.
 // ---------------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int64_t mx_groups(int64_t K) { return (K + kMxGroup - 1) / kMxGroup; }
 __host__ __device__ constexpr int64_t mx_piece_bytes(int64_t rows, int64_t K) { return mx_groups(K) * rows * 16; }
-__device__ __forceinline__ int mx_piece_byte(int block_in_group) { return 8 * (block_in_group & 1) + (block_in_group >> 1); }
-__host__ __device__ constexpr int64_t mx_padded_k(int64_t K) { return (K + 127) / 128 * 128; }
+__device__ __forceinline__ int mx_piece_byte(int block_in_group) { return 4 * (block_in_group & 3) + (block_in_group >> 2); }
+__host__ __device__ constexpr int64_t mx_padded_k(int64_t K) { return (K + 255) / 256 * 256; }  // rows of codes: whole pairs of steps
 
 // Internal entry points shared by the translation units
 struct MxProduct {
@@ -127,6 +147,10 @@ struct MxProduct {
 size_t mx_operand_bytes(int64_t M, int64_t K, int fmt);  // codes of an input with padded rows
 size_t mx_gemm_part_bytes(int64_t M, int64_t N, int64_t K);
 int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, float* part, hipStream_t s);
+bool mx_few_applies(int64_t M);     // the product of so few tokens streams the weight (mx_few.hip)
+bool mx_few_quantises(int64_t M, int64_t K);  // and quantises its input by itself
+int run_mx_few(const void* x, const uint8_t* x_codes, const uint8_t* x_pieces, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
+               void* y, int64_t M, int64_t N, int64_t K, int fmt, hipStream_t s);
 int check_mx_product(const char* who, int64_t M, int64_t N, int64_t K);
 int run_mx_quantize_operand(const void* x, int64_t M, int64_t K, int fmt, uint8_t* codes, uint8_t* pieces, const uint8_t* const* w_scales,
                             const int64_t* w_rows, uint8_t* const* w_pieces, int n_weights, hipStream_t s);
