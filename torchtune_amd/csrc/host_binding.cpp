@@ -8,15 +8,7 @@
 // same arguments, and the autograd nodes are C++ ones, so that backward runs without the interpreter too.
 //
 // This extension is the torch side of the C ABI; libtorchtune_amd.so itself stays free of torch types.
-#include <ATen/ATen.h>
-#include <c10/hip/HIPStream.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <pybind11/stl.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include "../../include/torchtune_amd.h"
+#include "host_common.h"
 
 namespace {
 
@@ -24,40 +16,7 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-void check(int rc, const char* what) {
-  if (rc == TTAMD_OK) return;
-  if (rc == TTAMD_EINVAL) TORCH_CHECK_VALUE(false, what, ": ", ttamd_last_error());
-  TORCH_CHECK(false, what, " failed (code ", rc, "): ", ttamd_last_error());
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-
-void need_gpu(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda(), what, ": expected a tensor on an AMD GPU (device 'cuda'), got device '", t.device().str(),
-              "'. torchtune_amd computes only through its HIP kernels.");
-}
-
-// a contiguous bf16 tensor on the GPU
-Tensor bf16(const Tensor& t, const char* what) {
-  need_gpu(t, what);
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, what, ": expected a bfloat16 tensor, got ", t.scalar_type());
-  return t.contiguous();
-}
-
-Tensor scratch(size_t bytes, const Tensor& like) {
-  return at::empty({(int64_t)(bytes > 16 ? bytes : 16)}, like.options().dtype(at::kByte));
-}
-
-size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
-
-// True when the call has to be a node: something is differentiated backward, or carries a forward-mode tangent (the node
-// then raises: none of them has a forward-mode rule, and a plain call would drop the tangent).
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  const bool grad = at::GradMode::is_enabled();
-  for (const Tensor* t : ts)
-    if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
-  return false;
-}
+using namespace ttamd_host;
 
 // A tensor the kernels may read in place of torch's own ops: no forward-mode tangent, no function transform's wrapper, no
 // subclass with a dispatch of its own, and no dispatch mode that would have seen those ops (a FLOP counter, a selective
@@ -812,6 +771,8 @@ Tensor straight_through_linear(const Tensor& x, const Tensor& weight, const Tens
 
 }  // namespace
 
+void bind_mx(py::module_& m);  // host_mx.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // like torch's own ops the calls run without the interpreter's lock: a launch waits where the queue is full
   const py::call_guard<py::gil_scoped_release> unlocked;
@@ -828,4 +789,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fq_per_group", &fq_per_group, unlocked);
   m.def("straight_through", &straight_through, unlocked);
   m.def("straight_through_linear", &straight_through_linear, unlocked);
+  bind_mx(m);
 }

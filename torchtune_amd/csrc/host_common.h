@@ -1,0 +1,52 @@
+// What the translation units of the host extension share: error codes to exceptions, checks, scratch memory.
+#pragma once
+#include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <pybind11/stl.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include "../../include/torchtune_amd.h"
+
+namespace ttamd_host {
+
+using at::Tensor;
+
+inline void check(int rc, const char* what) {
+  if (rc == TTAMD_OK) return;
+  if (rc == TTAMD_EINVAL) TORCH_CHECK_VALUE(false, what, ": ", ttamd_last_error());
+  TORCH_CHECK(false, what, " failed (code ", rc, "): ", ttamd_last_error());
+}
+
+inline void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+inline void need_gpu(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, ": expected a tensor on an AMD GPU (device 'cuda'), got device '", t.device().str(),
+              "'. torchtune_amd computes only through its HIP kernels.");
+}
+
+// a contiguous bf16 tensor on the GPU
+inline Tensor bf16(const Tensor& t, const char* what) {
+  need_gpu(t, what);
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, what, ": expected a bfloat16 tensor, got ", t.scalar_type());
+  return t.contiguous();
+}
+
+inline Tensor scratch(size_t bytes, const Tensor& like) {
+  return at::empty({(int64_t)(bytes > 16 ? bytes : 16)}, like.options().dtype(at::kByte));
+}
+
+inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// True when the call has to be a node: something is differentiated backward, or carries a forward-mode tangent (the node
+// then raises: none of them has a forward-mode rule, and a plain call would drop the tangent).
+inline bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  const bool grad = at::GradMode::is_enabled();
+  for (const Tensor* t : ts)
+    if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
+  return false;
+}
+
+}  // namespace ttamd_host

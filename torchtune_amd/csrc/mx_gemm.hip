@@ -56,7 +56,7 @@ struct MxTile {
   static constexpr int kStages = 3;
   static constexpr int kScales = (BM + BN) * 16;
   static constexpr int kLds = kStages * kStage + 2 * kScales;
-  static constexpr int kPerCU = kLds <= 53 * 1024 ? 3 : kLds <= 80 * 1024 ? 2 : 1;  // workgroups that a CU's LDS holds
+  static constexpr int kPerCU = kLds <= 40 * 1024 ? 4 : kLds <= 53 * 1024 ? 3 : kLds <= 80 * 1024 ? 2 : 1;  // workgroups that a CU's LDS holds
   static constexpr int kLoadsA = kA / (kThreads * 16), kLoadsW = kW / (kThreads * 16);
   static constexpr int kScaleWaves = (BM + BN) / 64;  // waves' worth of scale pieces
   static constexpr int kLoadsS = (kScaleWaves + WM * WN - 1) / (WM * WN);
@@ -475,20 +475,48 @@ __global__ __launch_bounds__(256) void mx_sum_slices_kernel(const float* __restr
   }
 }
 
+// Which tile a product runs on and how often its contraction is cut.  The times, in us, of `waves` work items per CU of
+// `steps` steps each (d + e * waves per step once several share a CU, `alone` for a single one), fitted to 70 shapes of 64 -
+// 3000 rows, 1024 - 14336 outputs and 2048 - 14336 contraction indices on both input formats; the model's choice was
+// the best of all 20 of them in the median and within 11 % of it everywhere.  Both sides of some borders, us, fp8 inputs:
+// 64 x 14336 x 4096 64-wide tiles 13.0, 64 x 128 15.4, 128-wide 21; 333 x 4096 x 4096 64 x 128 15.8, 64-wide 16.5, 128-wide
+// 20.8; 2000 x 4096 x 4096 128-wide 33, 256-wide 46; 3000 x 14336 x 4096 256-wide 138, 128-wide 161; 64 x 4096 x 14336 64-wide
+// in four slices 16.0, in two 22.8, whole 37.
+struct MxShape {
+  int bm, bn;
+  float alone, d, e, item, launch;
+};
+constexpr MxShape kShapes[2][4] = {
+    {{256, 256, 0.76f, 0.f, 0.76f, 7.f, 4.f}, {128, 128, 0.44f, 0.f, 0.315f, 1.2f, 4.5f}, {64, 128, 0.36f, 0.f, 0.225f, 0.6f, 4.f}, {64, 64, 0.28f, 0.08f, 0.13f, 0.4f, 3.5f}},
+    {{256, 256, 1.1f, 0.f, 1.1f, 8.f, 4.f}, {128, 128, 0.53f, 0.f, 0.41f, 1.2f, 4.5f}, {64, 128, 0.385f, 0.f, 0.2625f, 0.6f, 4.f}, {64, 64, 0.29f, 0.165f, 0.122f, 0.4f, 3.5f}}};
+
 struct MxPlan {
-  bool large;
-  int slices, steps_per_slice;
+  int shape, slices, steps_per_slice;
 };
 
-MxPlan plan_mx(int64_t M, int64_t N, int64_t K) {
-  const int64_t steps = mx_padded_k(K) / 128, big = ((M + 255) / 256) * ((N + 255) / 256);
-  if (big >= 192) return MxPlan{true, 1, (int)((steps + 3) / 4 * 4)};
-  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-  const int64_t groups = (steps + 3) / 4;
-  int64_t slices = 512 / tiles;
-  slices = std::max<int64_t>(1, std::min({slices, groups / 2, int64_t(16)}));
-  const int64_t per = (groups + slices - 1) / slices;
-  return MxPlan{false, (int)((groups + per - 1) / per), (int)(4 * per)};
+MxPlan plan_mx(int64_t M, int64_t N, int64_t K, int fmt) {
+  const int64_t steps = mx_padded_k(K) / 128, groups = (steps + 3) / 4;
+  MxPlan best = {0, 1, (int)(4 * groups)};
+  float best_time = 1e30f;
+  for (int shape = 0; shape < 4; ++shape) {
+    const MxShape& t = kShapes[fmt == TTAMD_MXFP8][shape];
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+    for (int64_t slices = 1; slices <= 16 && slices <= groups; slices *= 2) {
+      const int64_t per = (groups + slices - 1) / slices;
+      // partial sums of rows of an odd length are stored element by element; 256 MB of them would not pay anywhere
+      if (slices > 1 && (N % 4 || slices * M * N > (int64_t(1) << 26))) break;
+      if ((groups + per - 1) / per != slices) continue;
+      const float waves = (float)((tiles * slices + kCUs - 1) / kCUs), n = (float)std::min(steps, 4 * per);
+      const float step = waves > 1.f ? std::max(t.alone, t.d + t.e * waves) : t.alone;
+      float time = t.launch + t.item * waves + n * step;
+      if (slices > 1) time += 3.2f + (float)(slices * M * N) * (4.f / 3e6f);
+      if (time < best_time) {
+        best_time = time;
+        best = MxPlan{shape, (int)slices, (int)(4 * per)};
+      }
+    }
+  }
+  return best;
 }
 
 template <int WM, int WN, int TM, int TN, bool F8>
@@ -521,13 +549,25 @@ size_t mx_operand_bytes(int64_t M, int64_t K, int fmt) {
   return align256((size_t)M * (fmt == TTAMD_MXFP4 ? Kp / 2 : Kp));
 }
 
-size_t mx_gemm_part_bytes(int64_t M, int64_t N, int64_t K) {
-  const MxPlan p = plan_mx(M, N, K);
+size_t mx_gemm_part_bytes(int64_t M, int64_t N, int64_t K, int fmt) {
+  const MxPlan p = plan_mx(M, N, K, fmt);
   return p.slices > 1 ? align256((size_t)p.slices * M * N * sizeof(float)) : 0;
 }
 
+namespace {
+template <bool F8>
+int launch_shape(int shape, MxGemmArgs& g, hipStream_t s) {
+  switch (shape) {
+    case 0: return launch_mx<4, 2, 4, 8, F8>(g, s);
+    case 1: return launch_mx<2, 2, 4, 4, F8>(g, s);
+    case 2: return launch_mx<1, 4, 4, 2, F8>(g, s);
+    default: return launch_mx<2, 2, 2, 2, F8>(g, s);
+  }
+}
+}  // namespace
+
 int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, float* part, hipStream_t s) {
-  const MxPlan p = plan_mx(M, N, K);
+  const MxPlan p = plan_mx(M, N, K, fmt);
   MxGemmArgs g = {};
   g.xc = q.x_codes; g.xp = q.x_pieces; g.wc = q.w_codes; g.wp = q.w_pieces;
   g.h = q.h; g.lb = q.lora_b; g.bias = q.bias; g.y = q.y;
@@ -537,11 +577,7 @@ int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, fl
   g.slices = p.slices; g.steps_per_slice = p.steps_per_slice;
   g.part = part;
   TT_REQUIRE(p.slices == 1 || part, "mx_gemm: no room for the slices of the contraction");
-  int rc;
-  if (fmt == TTAMD_MXFP8)
-    rc = p.large ? launch_mx<4, 2, 4, 8, true>(g, s) : launch_mx<2, 2, 4, 4, true>(g, s);
-  else
-    rc = p.large ? launch_mx<4, 2, 4, 8, false>(g, s) : launch_mx<2, 2, 4, 4, false>(g, s);
+  const int rc = fmt == TTAMD_MXFP8 ? launch_shape<true>(p.shape, g, s) : launch_shape<false>(p.shape, g, s);
   if (rc || p.slices == 1) return rc;
   const int64_t numel = M * N;
   mx_sum_slices_kernel<<<dim3((unsigned)((numel + 1023) / 1024)), dim3(256), 0, s>>>(part, q.bias, q.y, numel, (int)N, p.slices);
@@ -560,8 +596,8 @@ using namespace ttamd;
 
 extern "C" size_t ttamd_mx_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation_format) {
   if (M <= 0 || N <= 0 || K <= 0 || K % kMxBlock || mx_few_quantises(M, K)) return 0;
-  if (mx_few_applies(M)) return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K));
-  return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K)) + align256(mx_piece_bytes(N, K)) + mx_gemm_part_bytes(M, N, K);
+  if (mx_few_applies(M, N)) return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K));
+  return mx_operand_bytes(M, K, activation_format) + align256(mx_piece_bytes(M, K)) + align256(mx_piece_bytes(N, K)) + mx_gemm_part_bytes(M, N, K, activation_format);
 }
 
 extern "C" int ttamd_mx_linear_bf16(const void* x, int activation_format, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
@@ -582,7 +618,7 @@ extern "C" int ttamd_mx_linear_bf16(const void* x, int activation_format, const 
   w += mx_operand_bytes(M, K, activation_format);
   uint8_t* xp = reinterpret_cast<uint8_t*>(w);
   w += align256(mx_piece_bytes(M, K));
-  if (mx_few_applies(M)) {
+  if (mx_few_applies(M, N)) {
     if (int rc = run_mx_quantize_operand(x, M, K, activation_format, xc, xp, nullptr, nullptr, nullptr, 0, s)) return rc;
     return run_mx_few(nullptr, xc, xp, w_codes, w_scales, bias, y, M, N, K, activation_format, s);
   }

@@ -80,7 +80,7 @@ FwdSpace fwd_space(const Members& d, void* workspace) {
   size_t part = 0;
   for (int i = 0; i < g.n; ++i) {
     f.pieces[i] = c.take<uint8_t>(mx_piece_bytes(g.N[i], g.K));
-    const size_t p = mx_gemm_part_bytes(g.M, g.N[i], g.K);
+    const size_t p = mx_gemm_part_bytes(g.M, g.N[i], g.K, TTAMD_MXFP8);
     part = p > part ? p : part;
   }
   f.hidden = c.take<float>(group_hidden_ws_bytes(g.M, g.K, g.r_off[g.n]));

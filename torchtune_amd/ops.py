@@ -1444,188 +1444,3 @@ def cross_entropy_fwd_bwd(logits: torch.Tensor, target: torch.Tensor, ignore_ind
                                                   grad.data_ptr(), rows, V, _stream(lg))
     _lib.check(rc, "cross_entropy_fwd_bwd")
     return loss, grad
-
-
-# ---------------------------------------------------------------------------------------------------
-# microscaled tensors
-# ---------------------------------------------------------------------------------------------------
-GROUP_MAX = _lib.GROUP_MAX
-_MX_CODE = {"mxfp4": _lib.TTAMD_MXFP4, "mxfp8": _lib.TTAMD_MXFP8}
-
-
-def mx_quantize(x: torch.Tensor, format: str) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``x [..., K]`` -> (codes uint8 [..., K / 2] (mxfp4) or [..., K] (mxfp8), scales uint8 [..., K / 32])"""
-    code = _code(x.dtype, "mx_quantize")
-    if x.dim() == 0 or x.shape[-1] % 32 or x.shape[-1] == 0:
-        raise ValueError(f"mx_quantize: the last dimension must be a positive multiple of 32, got {tuple(x.shape)}")
-    _need_gpu(x, "mx_quantize")
-    x = x.detach().contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone()
-    K = x.shape[-1]
-    rows = x.numel() // K
-    codes = torch.empty(*x.shape[:-1], K // 2 if format == "mxfp4" else K, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
-    lib = _lib.load()
-    with _on_device(x.device):
-        rc = lib.ttamd_mx_quantize(x.data_ptr(), code, rows, K, _MX_CODE[format], codes.data_ptr(), scales.data_ptr(), _stream(x))
-    _lib.check(rc, "mx_quantize")
-    return codes, scales
-
-
-def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, format: str, dtype: torch.dtype) -> torch.Tensor:
-    code = _code(dtype, "mx_dequantize")
-    _need_gpu(codes, "mx_dequantize")
-    codes, scales = _aligned(codes), scales.contiguous()
-    K = 32 * scales.shape[-1]
-    if K == 0 or codes.numel() * (2 if format == "mxfp4" else 1) != scales.numel() * 32 or scales.device != codes.device:
-        raise ValueError(f"mx_dequantize: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit each other")
-    out = torch.empty(*codes.shape[:-1], K, dtype=dtype, device=codes.device)
-    lib = _lib.load()
-    with _on_device(codes.device):
-        rc = lib.ttamd_mx_dequantize(codes.data_ptr(), scales.data_ptr(), _MX_CODE[format], scales.numel() // scales.shape[-1], K, code,
-                                     out.data_ptr(), _stream(codes))
-    _lib.check(rc, "mx_dequantize")
-    return out
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned, a copy only where it is not."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _mx_weight(codes: torch.Tensor, scales: torch.Tensor, what: str):
-    _need_gpu(codes, what)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
-        raise TypeError(f"{what}: codes and scales must be 2-D uint8 tensors")
-    if codes.shape[0] != scales.shape[0] or codes.shape[1] != 16 * scales.shape[1] or scales.device != codes.device:
-        raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit each other as mxfp4")
-    return _aligned(codes), _aligned(scales)
-
-
-def mx_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, activation: str, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y [M, N] = x^ . W^T (+ bias); x [M, K] bf16, W mxfp4 [N, K]"""
-    x = _aligned(_bf16_2d(x, "mx_linear"))
-    codes, scales = _mx_weight(codes, scales, "mx_linear")
-    (M, K), N = x.shape, codes.shape[0]
-    if codes.shape[1] * 2 != K or codes.device != x.device:
-        raise ValueError(f"mx_linear: x is {tuple(x.shape)} on {x.device}, the weight [{N}, {codes.shape[1] * 2}] on {codes.device}")
-    if bias is not None:
-        if bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,) or bias.device != x.device:
-            raise ValueError(f"mx_linear: bias must be bfloat16 [{N}] on {x.device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}")
-        bias = bias.contiguous()
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    if M == 0 or N == 0:
-        return y
-    lib = _lib.load()
-    nbytes = lib.ttamd_mx_linear_workspace_bytes(M, N, K, _MX_CODE[activation])
-    ws = _workspace(nbytes, x.device)
-    with _on_device(x.device):
-        rc = lib.ttamd_mx_linear_bf16(x.data_ptr(), _MX_CODE[activation], codes.data_ptr(), scales.data_ptr(), _ptr(bias), y.data_ptr(),
-                                      M, N, K, ws.data_ptr(), ws.numel(), _stream(x))
-    _lib.check(rc, "mx_linear")
-    return y
-
-
-def mx_linear_dx(gy: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """gx [M, K] = gy [M, N] . W; sides of W multiples of 64"""
-    gy = _aligned(_bf16_2d(gy, "mx_linear_dx"))
-    codes, scales = _mx_weight(codes, scales, "mx_linear_dx")
-    (M, N), K = gy.shape, codes.shape[1] * 2
-    if codes.shape[0] != N or codes.device != gy.device:
-        raise ValueError(f"mx_linear_dx: gy is {tuple(gy.shape)} on {gy.device}, the weight [{codes.shape[0]}, {K}] on {codes.device}")
-    gx = torch.empty(M, K, dtype=torch.bfloat16, device=gy.device)
-    if M == 0:
-        return gx
-    lib = _lib.load()
-    ws = _workspace(lib.ttamd_mx_linear_dx_workspace_bytes(M, N, K), gy.device)
-    with _on_device(gy.device):
-        rc = lib.ttamd_mx_linear_dx_bf16(gy.data_ptr(), codes.data_ptr(), scales.data_ptr(), gx.data_ptr(), M, N, K, ws.data_ptr(),
-                                         ws.numel(), _stream(gy))
-    _lib.check(rc, "mx_linear_dx")
-    return gx
-
-
-class MxMember:
-    """One adapter linear over an mxfp4 weight: codes [N, K / 2], scales [N, K / 32], lora_a [r, K], lora_b [N, r], bias [N] or
-    None, and the factor of its adapter."""
-
-    __slots__ = ("codes", "scales", "lora_a", "lora_b", "bias", "factor")
-
-    def __init__(self, codes, scales, lora_a, lora_b, bias, factor: float):
-        self.codes, self.scales, self.lora_a, self.lora_b, self.bias, self.factor = codes, scales, lora_a, lora_b, bias, factor
-
-
-def _mx_members(what: str, members: Sequence[MxMember], M: int, K: int, device: torch.device, ys: Sequence[torch.Tensor], grads=None):
-    """ctypes array of the members, and what has to stay alive until the call has been made"""
-    if not 1 <= len(members) <= GROUP_MAX:
-        raise ValueError(f"{what}: 1 to {GROUP_MAX} members, got {len(members)}")
-    arr, alive = (_lib.MxLoraMember * len(members))(), []
-    for i, m in enumerate(members):
-        codes, scales = _mx_weight(m.codes, m.scales, what)
-        N, r = codes.shape[0], m.lora_a.shape[0]
-        a, b = _aligned(_bf16_2d(m.lora_a.detach(), what)), _aligned(_bf16_2d(m.lora_b.detach(), what))
-        if codes.shape[1] * 2 != K or tuple(a.shape) != (r, K) or tuple(b.shape) != (N, r) or tuple(ys[i].shape) != (M, N):
-            raise ValueError(f"{what}: member {i}: weight [{N}, {codes.shape[1] * 2}], lora_a {tuple(a.shape)}, lora_b {tuple(b.shape)}, output "
-                             f"{tuple(ys[i].shape)} do not fit an input [{M}, {K}]")
-        bias = m.bias
-        if bias is not None:
-            if bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,):
-                raise ValueError(f"{what}: member {i}: bias must be bfloat16 [{N}], got {tuple(bias.shape)} {bias.dtype}")
-            bias = bias.detach().contiguous()
-        for t in (codes, a, b, bias, ys[i]):
-            if t is not None and t.device != device:
-                raise ValueError(f"{what}: member {i}: a tensor is on {t.device}, the input on {device}")
-        alive += [codes, scales, a, b, bias]
-        arr[i] = _lib.MxLoraMember(codes.data_ptr(), scales.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(bias), ys[i].data_ptr(),
-                                   _ptr(grads[0][i]) if grads else None, _ptr(grads[1][i]) if grads else None, N, r, float(m.factor))
-    return arr, alive
-
-
-def mx_lora_fwd(x: torch.Tensor, members: Sequence[MxMember]):
-    """(outputs [M, N_i], kept codes, kept scales, h_cat [M, sum of ranks]) of adapter linears over the same x [M, K] bf16.
-    Kept codes and scales are the input in mxfp8, in the library's own layout, for :func:`mx_lora_bwd`."""
-    x = _aligned(_bf16_2d(x, "mx_lora_fwd"))
-    M, K = x.shape
-    bf16, dev = torch.bfloat16, x.device
-    ys = [torch.empty(M, m.codes.shape[0], dtype=bf16, device=dev) for m in members]
-    arr, alive = _mx_members("mx_lora_fwd", members, M, K, dev, ys)
-    lib = _lib.load()
-    codes = torch.empty(lib.ttamd_mx_kept_codes_bytes(M, K), dtype=torch.uint8, device=dev)
-    scales = torch.empty(lib.ttamd_mx_kept_scales_bytes(M, K), dtype=torch.uint8, device=dev)
-    h = torch.empty(M, sum(m.lora_a.shape[0] for m in members), dtype=bf16, device=dev)
-    if M:
-        ws = _workspace(lib.ttamd_mx_lora_fwd_workspace_bytes(arr, len(members), M, K), dev)
-        with _on_device(dev):
-            rc = lib.ttamd_mx_lora_fwd_bf16(x.data_ptr(), arr, len(members), codes.data_ptr(), scales.data_ptr(), h.data_ptr(), M, K,
-                                            ws.data_ptr(), ws.numel(), _stream(x))
-        _lib.check(rc, "mx_lora_fwd")
-    return ys, codes, scales, h
-
-
-def mx_lora_bwd(gys: Sequence[torch.Tensor], codes: torch.Tensor, scales: torch.Tensor, h: torch.Tensor, members: Sequence[MxMember],
-                need_gx: bool = True):
-    """(gx [M, K] or None, [grad lora_a], [grad lora_b]) from the outputs' gradients and what :func:`mx_lora_fwd` kept"""
-    gys = [_aligned(_bf16_2d(g, "mx_lora_bwd")) for g in gys]
-    M, K, dev = h.shape[0], members[0].lora_a.shape[1], h.device
-    gas = [torch.empty(*m.lora_a.shape, dtype=torch.bfloat16, device=dev) for m in members]
-    gbs = [torch.empty(*m.lora_b.shape, dtype=torch.bfloat16, device=dev) for m in members]
-    arr, alive = _mx_members("mx_lora_bwd", members, M, K, dev, gys, (gas, gbs))
-    lib = _lib.load()
-    if codes.numel() != lib.ttamd_mx_kept_codes_bytes(M, K) or scales.numel() != lib.ttamd_mx_kept_scales_bytes(M, K):
-        raise ValueError(f"mx_lora_bwd: the kept input does not belong to [{M}, {K}]")
-    if h.shape[1] != sum(m.lora_a.shape[0] for m in members):
-        raise ValueError(f"mx_lora_bwd: h is {tuple(h.shape)}, the members' ranks add up to {sum(m.lora_a.shape[0] for m in members)}")
-    gx = torch.empty(M, K, dtype=torch.bfloat16, device=dev) if need_gx else None
-    if M == 0:
-        for g in (*gas, *gbs):
-            g.zero_()
-        return gx, gas, gbs
-    gh = torch.empty_like(h)
-    ws = _workspace(lib.ttamd_mx_lora_bwd_workspace_bytes(arr, len(members), M, K), dev)
-    with _on_device(dev):
-        rc = lib.ttamd_mx_lora_bwd_bf16(codes.data_ptr(), scales.data_ptr(), h.data_ptr(), arr, len(members), gh.data_ptr(), _ptr(gx), M, K,
-                                        ws.data_ptr(), ws.numel(), _stream(h))
-    _lib.check(rc, "mx_lora_bwd")
-    return gx, gas, gbs
