@@ -149,7 +149,8 @@ def test_lora(m, k, outs, r):
     _close(grads[0], wgx, SUMS * mgx + HALF * ghs, 2 * HALF)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (40, 192, 128), (333, 512, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 64), (1, 64, 128), (20, 192, 128), (32, 4096, 256), (64, 640, 384), (65, 128, 1152), (167, 512, 1024), (700, 4096, 320),
+                                   (1024, 1024, 1024), (1100, 64, 2048)])
 def test_linear_grad_input(m, n, k):
     w, dense = _weight(n, k, 11)
     g = _seed(12)

@@ -579,8 +579,11 @@ int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, fl
   TT_REQUIRE(p.slices == 1 || part, "mx_gemm: no room for the slices of the contraction");
   const int rc = fmt == TTAMD_MXFP8 ? launch_shape<true>(p.shape, g, s) : launch_shape<false>(p.shape, g, s);
   if (rc || p.slices == 1) return rc;
-  const int64_t numel = M * N;
-  mx_sum_slices_kernel<<<dim3((unsigned)((numel + 1023) / 1024)), dim3(256), 0, s>>>(part, q.bias, q.y, numel, (int)N, p.slices);
+  return run_mx_sum_slices(part, q.bias, q.y, M * N, (int)N, p.slices, s);
+}
+
+int run_mx_sum_slices(const float* part, const uint16_t* bias, uint16_t* y, int64_t numel, int N, int slices, hipStream_t s) {
+  mx_sum_slices_kernel<<<dim3((unsigned)((numel + 1023) / 1024)), dim3(256), 0, s>>>(part, bias, y, numel, N, slices);
   return check_launch("mx_sum_slices");
 }
 

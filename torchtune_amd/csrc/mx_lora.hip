@@ -12,6 +12,8 @@
 namespace ttamd {
 namespace {
 
+constexpr int64_t kMaxGradN = int64_t(1) << 23;  // 128 rows of the output's gradient are addressed with 32 bits
+
 struct Members {
   GroupSkinny sk;
   GroupDx dx;
@@ -30,6 +32,7 @@ int decode(const char* who, const ttamd_mx_lora_member* m, int n, int64_t M, int
     TT_REQUIRE(m[i].N > 0 && m[i].N % 64 == 0, "%s: member %d: N (%lld) must be a positive multiple of 64", who, i, (long long)m[i].N);
     TT_REQUIRE(m[i].rank > 0 && m[i].rank % 8 == 0, "%s: member %d: the rank (%d) must be a positive multiple of 8", who, i, m[i].rank);
     if (int rc = check_mx_product(who, M, m[i].N, K)) return rc;
+    if (m[i].N >= kMaxGradN) return fail(TTAMD_EUNSUPPORTED, "%s: member %d: N (%lld) is too large", who, i, (long long)m[i].N);
     TT_REQUIRE(m[i].codes && m[i].scales && m[i].lora_a && m[i].lora_b && m[i].y && aligned16(m[i].codes) && aligned16(m[i].scales) &&
                    aligned16(m[i].lora_a) && aligned16(m[i].lora_b) && aligned16(m[i].y) && (reinterpret_cast<uintptr_t>(m[i].bias) & 1u) == 0,
                "%s: member %d: pointers must be non-null and 16-byte aligned", who, i);
@@ -91,19 +94,35 @@ FwdSpace fwd_space(const Members& d, void* workspace) {
 
 struct BwdSpace {
   uint16_t* x;
-  float* skinny;
+  float *skinny, *part;
   char* tiles;
   size_t bytes;
 };
+int64_t sum_n(const GroupDx& d) {
+  int64_t n = 0;
+  for (int i = 0; i < d.n; ++i) n += d.N[i];
+  return n;
+}
+// gx: on the codes where the fused kernel serves the shape, else on the weights expanded to bf16 tiles
+int run_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* const* scales, const void* gh, void* gx, float* part, char* tiles, hipStream_t s) {
+  if (mx_dx_fused(d.M, sum_n(d), d.K)) return run_mx_dx(d, codes, scales, gh, gx, part, s);
+  int64_t n = 0;
+  for (int i = 0; i < d.n; ++i) {
+    if (int rc = run_mx_expand_tiles(codes[i], scales[i], d.N[i], d.K, tiles + 2 * n * d.K, s)) return rc;
+    n += d.N[i];
+  }
+  return run_dense_dx_on_tiles(d, gh, gx, tiles, s);
+}
 BwdSpace bwd_space(const Members& d, void* workspace) {
   Cut c{reinterpret_cast<char*>(workspace)};
   BwdSpace b = {};
   const GroupSkinny& g = d.sk;
   b.x = c.take<uint16_t>(2 * g.M * g.K);
   b.skinny = c.take<float>(group_lora_bwd_ws_bytes(g));
-  int64_t n = 0;
-  for (int i = 0; i < g.n; ++i) n += g.N[i];
-  b.tiles = c.take<char>(2 * n * g.K);
+  const int64_t n = sum_n(d.dx);
+  const bool fused = mx_dx_fused(g.M, n, g.K);
+  b.part = c.take<float>(fused ? mx_dx_fused_bytes(g.M, n, g.K) : 0);
+  b.tiles = c.take<char>(fused ? 0 : 2 * n * g.K);
   b.bytes = c.used;
   return b;
 }
@@ -168,33 +187,28 @@ extern "C" int ttamd_mx_lora_bwd_bf16(const uint8_t* kept_codes, const uint8_t* 
   uint16_t* gh = reinterpret_cast<uint16_t*>(gh_cat);
   if (int rc = run_mx_dequantize_operand(kept_codes, kept_scales, M, K, b.x, s)) return rc;
   if (int rc = run_group_lora_bwd(b.x, reinterpret_cast<const uint16_t*>(h_cat), d.sk, gh, b.skinny, s, nullptr)) return rc;
-  if (!gx) return TTAMD_OK;
-  int64_t n = 0;
-  for (int i = 0; i < n_members; ++i) {
-    if (int rc = run_mx_expand_tiles(d.codes[i], d.scales[i], d.sk.N[i], K, b.tiles + 2 * n * K, s)) return rc;
-    n += d.sk.N[i];
-  }
-  return run_dense_dx_on_tiles(d.dx, gh, gx, b.tiles, s);
+  return gx ? run_dx(d.dx, d.codes, d.scales, gh, gx, b.part, b.tiles, s) : TTAMD_OK;
 }
 
 // the grad-input of a product without adapters: gx = gy . W
 extern "C" size_t ttamd_mx_linear_dx_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  return M > 0 && N > 0 && K > 0 && N % 64 == 0 && K % 64 == 0 ? align256(2 * (size_t)N * K) : 0;
+  if (!(M > 0 && N > 0 && K > 0 && N % 64 == 0 && K % 64 == 0)) return 0;
+  return mx_dx_fused(M, N, K) ? mx_dx_fused_bytes(M, N, K) : align256(2 * (size_t)N * K);
 }
 extern "C" int ttamd_mx_linear_dx_bf16(const void* gy, const uint8_t* w_codes, const uint8_t* w_scales, void* gx, int64_t M, int64_t N,
                                        int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_mx_product("mx_linear_dx", M, N, K)) return rc;
+  if (N >= kMaxGradN) return fail(TTAMD_EUNSUPPORTED, "mx_linear_dx: N (%lld) is too large", (long long)N);
   TT_REQUIRE(N % 64 == 0 && K % 64 == 0, "mx_linear_dx: N (%lld) and K (%lld) must be multiples of 64", (long long)N, (long long)K);
   TT_REQUIRE(gy && w_codes && w_scales && gx && aligned16(gy) && aligned16(w_codes) && aligned16(gx), "mx_linear_dx: pointers must be non-null and 16-byte aligned");
   const size_t need = ttamd_mx_linear_dx_workspace_bytes(M, N, K);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(TTAMD_EWORKSPACE, "mx_linear_dx: needs %zu bytes of 16-byte aligned workspace, got %zu", need, workspace_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (int rc = run_mx_expand_tiles(w_codes, w_scales, N, K, workspace, s)) return rc;
   GroupDx d = {};
   d.n = 1;
   d.M = M; d.K = K;
   d.N[0] = N;
   d.gy[0] = reinterpret_cast<const uint16_t*>(gy);
-  return run_dense_dx_on_tiles(d, nullptr, gx, workspace, s);
+  return run_dx(d, &w_codes, &w_scales, nullptr, gx, reinterpret_cast<float*>(workspace), reinterpret_cast<char*>(workspace), s);
 }

@@ -151,6 +151,11 @@ bool mx_few_applies(int64_t M, int64_t N);    // the product of so few tokens st
 bool mx_few_quantises(int64_t M, int64_t K);  // and quantises its input by itself
 int run_mx_few(const void* x, const uint8_t* x_codes, const uint8_t* x_pieces, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
                void* y, int64_t M, int64_t N, int64_t K, int fmt, hipStream_t s);
+int run_mx_sum_slices(const float* part, const uint16_t* bias, uint16_t* y, int64_t numel, int N, int slices, hipStream_t s);
+struct GroupDx;
+bool mx_dx_fused(int64_t M, int64_t n_total, int64_t K);  // the grad-input expands the weights on their way through LDS (mx_dx.hip)
+size_t mx_dx_fused_bytes(int64_t M, int64_t n_total, int64_t K);
+int run_mx_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* const* scales, const void* gh_cat, void* gx, float* part, hipStream_t s);
 int check_mx_product(const char* who, int64_t M, int64_t N, int64_t K);
 int run_mx_quantize_operand(const void* x, int64_t M, int64_t K, int fmt, uint8_t* codes, uint8_t* pieces, const uint8_t* const* w_scales,
                             const int64_t* w_rows, uint8_t* const* w_pieces, int n_weights, hipStream_t s);
