@@ -117,7 +117,8 @@ def test_linear(m, n, k, act):
 
 @pytest.mark.parametrize("r", [8, 16, 24, 64])
 @pytest.mark.parametrize("m,k,outs", [(1, 64, [64]), (24, 128, [192]), (77, 1024, [256]), (350, 2048, [2048]), (513, 320, [64, 128, 64]),
-                                      (300, 1024, [1024, 256, 256])])
+                                      (300, 1024, [1024, 256, 256]),
+                                      (33, 4160, [64]), (20, 8256, [128]), (2500, 320, [128, 64]), (1030, 64, [8192])])
 def test_lora(m, k, outs, r):
     if len(outs) > 1 and r > 16:
         r = 16

@@ -7,6 +7,12 @@ namespace ttamd {
 
 constexpr int kGroupMax = TTAMD_GROUP_MAX;  // most members of a group
 
+// An input kept for the backward pass in mxfp8: codes [M, ld], scales in pieces ([K / 512][M][16], byte 4 q + s block 4 s + q).
+struct KeptInput {
+  const uint8_t *codes, *pieces;
+  int64_t ld;
+};
+
 // What the rank-r products need to know about a group.  The members' hidden activations lie side by side in one
 // [M, r_off[n]] tensor (member i in columns [r_off[i], r_off[i + 1])), and so do their gradients.
 struct GroupSkinny {
@@ -20,6 +26,7 @@ struct GroupSkinny {
   const uint16_t* gy[kGroupMax];      // [M, N]        (backward)
   uint16_t* ga[kGroupMax];            // [rank, K] out (backward)
   uint16_t* gb[kGroupMax];            // [N, rank] out (backward)
+  KeptInput kept;                     // backward: the input, where it is kept in 8 bits (codes non-null)
 };
 
 // What the fused NF4 GEMMs need to know about a group (forward).
@@ -151,6 +158,7 @@ struct SwigluBwdInputs {
   const uint16_t* gate;  // [M, N]
   const uint16_t* up;    // [M, N]
 };
+// x may be null where the group's input is kept in 8 bits
 int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkinny& g, uint16_t* gh_cat, float* ws, hipStream_t s,
                        const SwigluBwdInputs* sw = nullptr);
 

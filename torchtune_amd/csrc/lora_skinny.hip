@@ -15,8 +15,10 @@
 // it (skinny_tn_gh_kernel).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 #include "common.h"
 #include "group.h"
+#include "mx_math.h"
 #include "nf4_math.h"
 #include "swiglu_math.h"
 
@@ -401,10 +403,29 @@ struct TnBatch {
   TnProblem p[kTnMaxProblems];
   int cg_end[kTnMaxProblems];  // workgroups [cg_end[i - 1], cg_end[i]) along x work on problem i
   int n, M, rows_per_split;
+  KeptInput kept;  // the MX forms: problem 0's X
 };
-
-// RGM: most column groups of G any problem of the batch has (registers and LDS are sized for it)
-template <int RGM>
+// Problem 0's X as it is kept in 8 bits, from row m and column c0 on (a multiple of the workgroup's columns, so that all of them lie
+// within one piece of 512): a lane's 16 elements and, apart, their block's scale byte, at 32-bit offsets from addresses the
+// whole wave shares; and as bf16 to LDS.  (Eight elements a lane, half the bytes to a request, took 94 us instead of 38 for
+// [8192, 14336] and a gy of [8192, 4096].)
+__device__ __forceinline__ u32x4_t kept_codes(const KeptInput& k, int64_t m, int c0, int lane_row, int lane_col) {
+  return *reinterpret_cast<const u32x4_t*>(k.codes + m * k.ld + c0 + ((uint32_t)lane_row * (uint32_t)k.ld + (uint32_t)lane_col));
+}
+__device__ __forceinline__ uint32_t kept_scale(const KeptInput& k, int64_t M, int64_t m, int c0, int lane_row, int lane_col) {
+  return (k.pieces + ((int64_t)(c0 >> 9) * M + m) * 16)[16u * (uint32_t)lane_row + (uint32_t)mx_piece_byte(((c0 & 511) + lane_col) >> 5)];
+}
+__device__ __forceinline__ void kept_expand(const u32x4_t& v, uint32_t byte, char* to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float s = mx_scale_value(byte == 255 ? 127u : byte);
+  mx_u32x4 lo = mx_bf16_of_fp8(mx_u32x2{v.x, v.y}, s), hi = mx_bf16_of_fp8(mx_u32x2{v.z, v.w}, s);
+  if (byte == 255) lo = hi = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+  reinterpret_cast<mx_u32x4*>(to)[0] = lo;
+  reinterpret_cast<mx_u32x4*>(to)[1] = hi;
+#endif
+}
+// MX: problem 0's X is the kept 8-bit input, expanded on its way into LDS
+template <int RGM, bool MX>
 __global__ __launch_bounds__(256) void skinny_tn_kernel(const TnBatch a) {
   constexpr int kTrWaveLds = tn_wave_lds(RGM);
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -451,61 +472,86 @@ __global__ __launch_bounds__(256) void skinny_tn_kernel(const TnBatch a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[q][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  u32x4_t xv[8], gv[RGM];
-  auto fetch = [&](int m) {  // rows m .. m + 31 into registers
+  // all rows of this wave.  One form a branch: tested inside, both forms' addresses are kept across the loop (57 registers spilled)
+  auto sweep = [&](auto kept_form) __attribute__((always_inline)) {
+    constexpr bool kept = decltype(kept_form)::value;
+    u32x4_t xv[8], gv[RGM];
+    uint32_t sv[4] = {};
+    auto fetch = [&](int m) {  // rows m .. m + 31 into registers
+      if constexpr (kept) {  // instruction u (0..3): row 8 u + lane / 8, 16-element chunk lane % 8
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int row = m + 4 * u + g;
-      xv[u] = u32x4_t{0, 0, 0, 0};
-      if (row < m_end && xcol_ok) xv[u] = *reinterpret_cast<const u32x4_t*>(xsrc + (int64_t)row * Kc);
-    }
-    const int grow = m + (lane >> 1);
+        for (int u = 0; u < 4; ++u) {
+          xv[u] = u32x4_t{0, 0, 0, 0};
+          if (m + 8 * u + (lane >> 3) < m_end && c0 + 16 * (lane & 7) < Kc) {
+            xv[u] = kept_codes(a.kept, m + 8 * u, c0, lane >> 3, 16 * (lane & 7));
+            sv[u] = kept_scale(a.kept, M, m + 8 * u, c0, lane >> 3, 16 * (lane & 7));
+          }
+        }
+      } else {
 #pragma unroll
-    for (int q = 0; q < RGM; ++q) {
-      gv[q] = u32x4_t{0, 0, 0, 0};
-      if (grow < m_end && gcol + 16 * q < R) gv[q] = *reinterpret_cast<const u32x4_t*>(G + (int64_t)grow * ldg + gcol + 16 * q);
-    }
-  };
-  int m = m_begin + 32 * wave;
-  if (m < m_end) fetch(m);
-  for (; m < m_end; m += 128) {
-    // the previous step's reads of this region are complete: they were waited for before its MFMAs
-#pragma unroll
-    for (int u = 0; u < 8; ++u) *reinterpret_cast<u32x4_t*>(xdst + 4 * u * kTrPitchX) = xv[u];
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) *reinterpret_cast<u32x4_t*>(gdst + 1024 * q) = gv[q];  // zeros beyond R
-    if (m + 128 < m_end) fetch(m + 128);  // in flight while this step is multiplied
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the copy-in has landed (LDS operations of a wave complete in order)
-    u32x2_t ga[RGM], gb[RGM];
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) {
-      ga[q] = lds_read_tr16(grd, 1024 * q);
-      gb[q] = lds_read_tr16(grd, 1024 * q + 4 * 32);
-    }
-    // a wait that names the registers it releases, so that no use can be scheduled ahead of it
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(ga[q]), "+v"(gb[q]));
-    u32x2_t xa[8], xb[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      xa[e] = lds_read_tr16(xrd, 32 * e);
-      xb[e] = lds_read_tr16(xrd, 32 * e + 4 * kTrPitchX);
-    }
-    // The 16 reads return in order: column group e may go once at most 14 - 2 e younger reads are outstanding.
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(xa[e]), "+v"(xb[e]) : "n"(14 - 2 * e));
-      const u32x4_t xop = {xa[e].x, xa[e].y, xb[e].x, xb[e].y};
+        for (int u = 0; u < 8; ++u) {
+          const int row = m + 4 * u + g;
+          xv[u] = u32x4_t{0, 0, 0, 0};
+          if (row < m_end && xcol_ok) xv[u] = *reinterpret_cast<const u32x4_t*>(xsrc + (int64_t)row * Kc);
+        }
+      }
+      const int grow = m + (lane >> 1);
 #pragma unroll
       for (int q = 0; q < RGM; ++q) {
-        if (q < rg) {
-          const u32x4_t gop = {ga[q].x, ga[q].y, gb[q].x, gb[q].y};
-          acc[q][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, gop),
-                                                             __builtin_bit_cast(bf16x8_t, xop), acc[q][e], 0, 0, 0);
+        gv[q] = u32x4_t{0, 0, 0, 0};
+        if (grow < m_end && gcol + 16 * q < R) gv[q] = *reinterpret_cast<const u32x4_t*>(G + (int64_t)grow * ldg + gcol + 16 * q);
+      }
+    };
+    int m = m_begin + 32 * wave;
+    if (m < m_end) fetch(m);
+    for (; m < m_end; m += 128) {
+      // the previous step's reads of this region are complete: they were waited for before its MFMAs
+      if constexpr (kept) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) kept_expand(xv[u], sv[u], my + (8 * u + (lane >> 3)) * kTrPitchX + 32 * (lane & 7));
+      } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) *reinterpret_cast<u32x4_t*>(xdst + 4 * u * kTrPitchX) = xv[u];
+      }
+#pragma unroll
+      for (int q = 0; q < RGM; ++q) *reinterpret_cast<u32x4_t*>(gdst + 1024 * q) = gv[q];  // zeros beyond R
+      if (m + 128 < m_end) fetch(m + 128);  // in flight while this step is multiplied
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the copy-in has landed (LDS operations of a wave complete in order)
+      u32x2_t ga[RGM], gb[RGM];
+#pragma unroll
+      for (int q = 0; q < RGM; ++q) {
+        ga[q] = lds_read_tr16(grd, 1024 * q);
+        gb[q] = lds_read_tr16(grd, 1024 * q + 4 * 32);
+      }
+      // a wait that names the registers it releases, so that no use can be scheduled ahead of it
+#pragma unroll
+      for (int q = 0; q < RGM; ++q) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(ga[q]), "+v"(gb[q]));
+      u32x2_t xa[8], xb[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xa[e] = lds_read_tr16(xrd, 32 * e);
+        xb[e] = lds_read_tr16(xrd, 32 * e + 4 * kTrPitchX);
+      }
+      // The 16 reads return in order: column group e may go once at most 14 - 2 e younger reads are outstanding.
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(xa[e]), "+v"(xb[e]) : "n"(14 - 2 * e));
+        const u32x4_t xop = {xa[e].x, xa[e].y, xb[e].x, xb[e].y};
+#pragma unroll
+        for (int q = 0; q < RGM; ++q) {
+          if (q < rg) {
+            const u32x4_t gop = {ga[q].x, ga[q].y, gb[q].x, gb[q].y};
+            acc[q][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, gop),
+                                                               __builtin_bit_cast(bf16x8_t, xop), acc[q][e], 0, 0, 0);
+          }
         }
       }
     }
-  }
+  };
+  if (MX && which == 0)
+    sweep(std::integral_constant<bool, MX>{});
+  else
+    sweep(std::false_type{});
   float (*red)[32][64] = reinterpret_cast<float (*)[32][64]>(stage);
   // acc[q][e][v] = sum over this wave's rows of G[.][16 q + 4 g + v] * X[.][c0 + 16 e + i]; one column group of G at a
   // time meets in the staging memory
@@ -563,6 +609,49 @@ struct TnWholeOut {
   float scale[kMaxGroup];
   int r_off[kMaxGroup + 1];
 };
+
+#if defined(__HIP_DEVICE_COMPILE__)
+template <int RGM>
+__device__ __forceinline__ void tn_whole_finish(const f32x4_t (&acc)[RGM][4], const TnBatch& a, const TnWholeOut& o, char* whole, int which, int R, int rg, int Kc,
+                                                int c0, int wave, int lane) {
+  const int g = lane >> 4, i = lane & 15;
+  // acc[q][e][v] = sum over this wave's rows of G[.][16 q + 4 g + v] * X[.][c0 + 16 e + i]; 16 columns of G at a time meet in
+  // the staging memory, and every thread finishes one output of them
+  float (*red)[16][64] = reinterpret_cast<float (*)[16][64]>(whole);
+  for (int q = 0; q < rg; ++q) {
+    __syncthreads();  // the staging regions (or the previous group's sums) are free
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float val = acc[0][e][v];
+#pragma unroll
+        for (int qq = 1; qq < RGM; ++qq) val = q == qq ? acc[qq][e][v] : val;
+        red[wave][v * 4 + e][lane] = val;
+      }
+    __syncthreads();
+    float sums[kTnWholeWaves];
+#pragma unroll
+    for (int w = 0; w < kTnWholeWaves; ++w) sums[w] = red[w][wave][lane];
+#pragma unroll
+    for (int d = 1; d < kTnWholeWaves; d *= 2)
+#pragma unroll
+      for (int w = 0; w < kTnWholeWaves; w += 2 * d) sums[w] += sums[w + d];
+    const float s = sums[0];
+    const int r = 16 * q + 4 * g + (wave >> 2), col = c0 + 16 * (wave & 3) + i;
+    if (r >= R) continue;
+    if (which == 0) {
+      int mem = 0;
+#pragma unroll
+      for (int k = 1; k < kMaxGroup; ++k)
+        if (k < a.n - 1 && r >= o.r_off[k]) mem = k;
+      o.ga[mem][(int64_t)(r - o.r_off[mem]) * Kc + col] = f32_to_bf16_bits(s);
+    } else {
+      o.gb[which - 1][(int64_t)col * R + r] = f32_to_bf16_bits(s * o.scale[which - 1]);
+    }
+  }
+}
+#endif
 
 template <int RGM>
 __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kernel(const TnBatch a, const TnWholeOut o) {
@@ -653,41 +742,125 @@ __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kernel(con
     }
     if (!kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
   }
-  // acc[q][e][v] = sum over this wave's rows of G[.][16 q + 4 g + v] * X[.][c0 + 16 e + i]; 16 columns of G at a time meet in
-  // the staging memory, and every thread finishes one output of them
-  float (*red)[16][64] = reinterpret_cast<float (*)[16][64]>(whole);
-  for (int q = 0; q < rg; ++q) {
-    __syncthreads();  // the staging regions (or the previous group's sums) are free
+  tn_whole_finish<RGM>(acc, a, o, whole, which, R, rg, Kc, c0, wave, lane);
+#endif
+}
+
+// The same with problem 0's X kept in 8 bits.  Every group of ranks is multiplied, G's zeros included: with a branch about each
+// product the compiler let the sums read a product before it had been written (no wait states along the branch).
+template <int RGM>
+__global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kept_kernel(const TnBatch a, const TnWholeOut o) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __attribute__((aligned(16))) char whole[];
+  int which = 0;  // uniform over the workgroup
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+  for (int q = 0; q < kTnMaxProblems - 1; ++q)
+    if (q < a.n - 1 && (int)blockIdx.x >= a.cg_end[q]) which = q + 1;
+  const TnProblem& P = a.p[which];
+  const uint16_t* __restrict__ G = P.G;
+  const uint16_t* __restrict__ X = P.X;
+  const int Kc = P.Kc, M = a.M, R = P.R, ldg = P.ldg;
+  const int rg = (R + 15) >> 4;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, i = lane & 15;
+  const int c0 = ((int)blockIdx.x - (which ? a.cg_end[which - 1] : 0)) * kTnWholeCols;
+
+  char* my = whole + wave * tn_whole_wave_lds(RGM);
+  // copy-in: X piece, instruction u (0..3): row 8 u + lane / 8, 16-byte chunk lane % 8; G as in skinny_tn
+  const uint16_t* xsrc = X + c0 + 8 * (lane & 7);  // Kc is a multiple of 64
+  char* xdst = my + (lane >> 3) * kTnWholePitch + 16 * (lane & 7);
+  const int gcol = 8 * (lane & 1);  // + 16 q;  R % 8 == 0: a lane's 8 columns are all in or all out
+  char* gdst = my + 32 * kTnWholePitch + (lane >> 1) * 32 + 16 * (lane & 1);  // + 1024 q
+  const uint32_t my_lds = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)my);
+  const uint32_t xrd = my_lds + (8 * g + (i >> 2)) * kTnWholePitch + 8 * (i & 3);
+  const uint32_t grd = my_lds + 32 * kTnWholePitch + (8 * g + (i >> 2)) * 32 + 8 * (i & 3);
+
+  f32x4_t acc[RGM][4];
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        float val = acc[0][e][v];
+  for (int q = 0; q < RGM; ++q)
 #pragma unroll
-        for (int qq = 1; qq < RGM; ++qq) val = q == qq ? acc[qq][e][v] : val;
-        red[wave][v * 4 + e][lane] = val;
+    for (int e = 0; e < 4; ++e) acc[q][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // all rows of this wave.  One form a branch: tested inside, both forms' addresses are kept across the loop (57 registers spilled)
+  auto sweep = [&](auto kept_form) __attribute__((always_inline)) {
+    constexpr bool kept = decltype(kept_form)::value;
+    u32x4_t xv[4], gv[RGM];
+    uint32_t sv[2] = {};
+    auto fetch = [&](int m) {  // rows m .. m + 31 into registers
+      if constexpr (kept) {  // instruction u (0, 1): row 16 u + lane / 4, 16-element chunk lane % 4
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          xv[u] = u32x4_t{0, 0, 0, 0};
+          if (m + 16 * u + (lane >> 2) < M) {
+            xv[u] = kept_codes(a.kept, m + 16 * u, c0, lane >> 2, 16 * (lane & 3));
+            sv[u] = kept_scale(a.kept, M, m + 16 * u, c0, lane >> 2, 16 * (lane & 3));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int row = m + 8 * u + (lane >> 3);
+          xv[u] = u32x4_t{0, 0, 0, 0};
+          if (row < M) xv[u] = *reinterpret_cast<const u32x4_t*>(xsrc + (int64_t)row * Kc);
+        }
       }
-    __syncthreads();
-    float sums[kTnWholeWaves];
+      const int grow = m + (lane >> 1);
 #pragma unroll
-    for (int w = 0; w < kTnWholeWaves; ++w) sums[w] = red[w][wave][lane];
+      for (int q = 0; q < RGM; ++q) {
+        gv[q] = u32x4_t{0, 0, 0, 0};
+        if (grow < M && gcol + 16 * q < R) gv[q] = *reinterpret_cast<const u32x4_t*>(G + (int64_t)grow * ldg + gcol + 16 * q);
+      }
+    };
+    // Beyond 48 ranks the next rows are fetched behind the products, not beside them, which would spill 29 registers (4096 x 4096
+    // rank 64 at 1000 tokens 28.7 us so, 22.9)
+    constexpr bool kAhead = RGM < 4;
+    int m = 32 * wave;
+    if (m < M) fetch(m);
+    for (; m < M; m += 32 * kTnWholeWaves) {
+      // the previous step's reads of this region are complete: they were waited for before its MFMAs
+      if constexpr (kept) {
 #pragma unroll
-    for (int d = 1; d < kTnWholeWaves; d *= 2)
+        for (int u = 0; u < 2; ++u) kept_expand(xv[u], sv[u], my + (16 * u + (lane >> 2)) * kTnWholePitch + 32 * (lane & 3));
+      } else {
 #pragma unroll
-      for (int w = 0; w < kTnWholeWaves; w += 2 * d) sums[w] += sums[w + d];
-    const float s = sums[0];
-    const int r = 16 * q + 4 * g + (wave >> 2), col = c0 + 16 * (wave & 3) + i;
-    if (r >= R) continue;
-    if (which == 0) {
-      int mem = 0;
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4_t*>(xdst + 8 * u * kTnWholePitch) = xv[u];
+      }
 #pragma unroll
-      for (int k = 1; k < kMaxGroup; ++k)
-        if (k < a.n - 1 && r >= o.r_off[k]) mem = k;
-      o.ga[mem][(int64_t)(r - o.r_off[mem]) * Kc + col] = f32_to_bf16_bits(s);
-    } else {
-      o.gb[which - 1][(int64_t)col * R + r] = f32_to_bf16_bits(s * o.scale[which - 1]);
+      for (int q = 0; q < RGM; ++q) *reinterpret_cast<u32x4_t*>(gdst + 1024 * q) = gv[q];  // zeros beyond R
+      if (kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the copy-in has landed (LDS operations of a wave complete in order)
+      u32x2_t ga[RGM], gb[RGM], xa[4], xb[4];
+#pragma unroll
+      for (int q = 0; q < RGM; ++q) {
+        ga[q] = lds_read_tr16(grd, 1024 * q);
+        gb[q] = lds_read_tr16(grd, 1024 * q + 4 * 32);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        xa[e] = lds_read_tr16(xrd, 32 * e);
+        xb[e] = lds_read_tr16(xrd, 32 * e + 4 * kTnWholePitch);
+      }
+      // waits that name the registers they release, so that no use can be scheduled ahead of them
+#pragma unroll
+      for (int q = 0; q < RGM; ++q) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(ga[q]), "+v"(gb[q]));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(xa[e]), "+v"(xb[e]));
+        const u32x4_t xop = {xa[e].x, xa[e].y, xb[e].x, xb[e].y};
+#pragma unroll
+        for (int q = 0; q < RGM; ++q) {
+          const u32x4_t gop = {ga[q].x, ga[q].y, gb[q].x, gb[q].y};
+          acc[q][e] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, gop), __builtin_bit_cast(bf16x8_t, xop), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        }
+      }
+      if (!kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
     }
-  }
+  };
+  if (which == 0)
+    sweep(std::true_type{});
+  else
+    sweep(std::false_type{});
+  tn_whole_finish<RGM>(acc, a, o, whole, which, R, rg, Kc, c0, wave, lane);
 #endif
 }
 
@@ -1349,10 +1522,11 @@ int run_tn_batch(TnBatch& b, int n, TnSumBatch& f, int ns, const int* sum_proble
   int rgm = 1;
   for (int i = 0; i < n; ++i) rgm = (b.p[i].R + 15) / 16 > rgm ? (b.p[i].R + 15) / 16 : rgm;
   const dim3 grid((unsigned)groups, (unsigned)pl.splits), block(256);
-  if (rgm == 1) skinny_tn_kernel<1><<<grid, block, 0, s>>>(b);
-  else if (rgm == 2) skinny_tn_kernel<2><<<grid, block, 0, s>>>(b);
-  else if (rgm == 3) skinny_tn_kernel<3><<<grid, block, 0, s>>>(b);
-  else skinny_tn_kernel<4><<<grid, block, 0, s>>>(b);
+  const bool mx = b.kept.codes != nullptr;
+  if (rgm == 1) mx ? skinny_tn_kernel<1, true><<<grid, block, 0, s>>>(b) : skinny_tn_kernel<1, false><<<grid, block, 0, s>>>(b);
+  else if (rgm == 2) mx ? skinny_tn_kernel<2, true><<<grid, block, 0, s>>>(b) : skinny_tn_kernel<2, false><<<grid, block, 0, s>>>(b);
+  else if (rgm == 3) mx ? skinny_tn_kernel<3, true><<<grid, block, 0, s>>>(b) : skinny_tn_kernel<3, false><<<grid, block, 0, s>>>(b);
+  else mx ? skinny_tn_kernel<4, true><<<grid, block, 0, s>>>(b) : skinny_tn_kernel<4, false><<<grid, block, 0, s>>>(b);
   int64_t end = 0;
   for (int i = 0; i < ns; ++i) {
     const TnProblem& P = b.p[sum_problem[i]];
@@ -1387,19 +1561,20 @@ size_t tn_part_bytes(int64_t M, int n, const int64_t* Kc, const int* R) {
 // 4096 87.9 -> 61.9 at 2048); at 3000 4096 x 14336 rank 16 takes 39.1 instead of 38.0 us, at 8192 256 x 1024 25.9 instead of 16.5.
 bool tn_whole_pays(const GroupSkinny& g) { return g.M <= 2048; }
 
-template <int RGM>
+template <int RGM, bool MX>
 int launch_tn_whole(const TnBatch& b, const TnWholeOut& o, hipStream_t s) {
+  const auto kernel = MX ? skinny_tn_whole_kept_kernel<RGM> : skinny_tn_whole_kernel<RGM>;
   constexpr int kLds = kTnWholeWaves * tn_whole_wave_lds(RGM);
   static_assert(kLds >= kTnWholeWaves * 16 * 64 * (int)sizeof(float) && kLds <= 160 * 1024, "the sums fit the staging memory");
   static bool set[64] = {};  // the LDS limit is a per-device attribute of the function (a race only repeats the call)
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = -1;
   if (dev < 0 || !set[dev]) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&skinny_tn_whole_kernel<RGM>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return fail(TTAMD_ELAUNCH, "skinny_tn: cannot reserve %d bytes of LDS: %s", kLds, hipGetErrorString(e));
     if (dev >= 0) set[dev] = true;
   }
-  skinny_tn_whole_kernel<RGM><<<dim3((unsigned)b.cg_end[b.n - 1]), dim3(64 * kTnWholeWaves), kLds, s>>>(b, o);
+  kernel<<<dim3((unsigned)b.cg_end[b.n - 1]), dim3(64 * kTnWholeWaves), kLds, s>>>(b, o);
   return check_launch("skinny_tn");
 }
 
@@ -1422,10 +1597,15 @@ int run_tn_whole(TnBatch& b, const GroupSkinny& g, const uint16_t* h_cat, hipStr
     groups += b.p[i].Kc / kTnWholeCols;
     b.cg_end[i] = (int)groups;
   }
-  return rgm == 1   ? launch_tn_whole<1>(b, o, s)
-         : rgm == 2 ? launch_tn_whole<2>(b, o, s)
-         : rgm == 3 ? launch_tn_whole<3>(b, o, s)
-                    : launch_tn_whole<4>(b, o, s);
+  if (b.kept.codes)
+    return rgm == 1   ? launch_tn_whole<1, true>(b, o, s)
+           : rgm == 2 ? launch_tn_whole<2, true>(b, o, s)
+           : rgm == 3 ? launch_tn_whole<3, true>(b, o, s)
+                      : launch_tn_whole<4, true>(b, o, s);
+  return rgm == 1   ? launch_tn_whole<1, false>(b, o, s)
+         : rgm == 2 ? launch_tn_whole<2, false>(b, o, s)
+         : rgm == 3 ? launch_tn_whole<3, false>(b, o, s)
+                    : launch_tn_whole<4, false>(b, o, s);
 }
 
 // ---- gh and gB from one pass over gy (skinny_tn_gh_kernel) ------------------------------------------------------------
@@ -1606,6 +1786,7 @@ int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkin
     TnBatch t = {};
     t.M = (int)g.M;
     t.p[0] = TnProblem{gh_cat, x, nullptr, (int)g.K, rt, rt};
+    t.kept = g.kept;
     int sum_problem[kTnMaxSums], sum_row0[kTnMaxSums];
     for (int i = 0; i < g.n; ++i) {
       f.p[i] = TnSum{nullptr, g.ga[i], 0, g.rank[i], 1.0f, 0, g.K, 1};
@@ -1632,6 +1813,7 @@ int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkin
   TnBatch t = {};
   t.M = (int)g.M;
   t.p[0] = TnProblem{gh_cat, x, nullptr, (int)g.K, rt, rt};
+  t.kept = g.kept;
   if (tn_whole_pays(g)) return run_tn_whole(t, g, h_cat, s);
   TnSumBatch f = {};
   int sum_problem[kTnMaxSums], sum_row0[kTnMaxSums];

@@ -73,6 +73,40 @@ __device__ __forceinline__ void store_codes(uint8_t* codes, int64_t piece, mx_u3
   else
     reinterpret_cast<mx_u32x2*>(codes)[piece] = c;
 }
+// One workgroup's share of the weights' scales in the product's layout: a thread one piece of 16, a wave four pieces of each of
+// 16 rows, so that it reads 64 bytes of a row and writes 256 bytes of a group.  (A row's pieces one after the other are written
+// `rows` pieces apart, all to the same few channels: with K = 14336 that was most of the launch.)
+__device__ __forceinline__ void lay_out_scales(int blk, int K, const OperandWeights& w) {
+  int which = 0;
+#pragma unroll
+  for (int q = 0; q < kMxWeights - 1; ++q)
+    if (q < w.n - 1 && blk >= w.blk_end[q]) which = q + 1;
+  if (which) blk -= w.blk_end[which - 1];
+  const int nb = K / kMxBlock, groups = (nb + 15) >> 4, quads = (groups + 3) >> 2;
+  const int64_t wave = (int64_t)blk * (blockDim.x >> 6) + (threadIdx.x >> 6), rows = w.rows[which];
+  const int lane = threadIdx.x & 63;
+  const int64_t row = wave / quads * 16 + (lane & 15);
+  const int g = (int)(wave % quads) * 4 + (lane >> 4);
+  if (row >= rows || g >= groups) return;
+  const uint8_t* src = w.scales[which] + row * nb + 16 * g;
+  mx_u32x4 d = {0, 0, 0, 0};
+  if ((nb & 15) == 0) {
+    d = *reinterpret_cast<const mx_u32x4*>(src);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {  // no load within a branch, or they wait for each other
+      const int left = nb - 16 * g;
+      const uint32_t byte = src[q < left ? q : left - 1];
+      d[q >> 2] |= (q < left ? byte : 0u) << (8 * (q & 3));
+    }
+  }
+  // byte 4 s + q -> byte 4 q + s
+  const uint32_t t0 = __builtin_amdgcn_perm(d.y, d.x, 0x05010400u), t1 = __builtin_amdgcn_perm(d.y, d.x, 0x07030602u);
+  const uint32_t u0 = __builtin_amdgcn_perm(d.w, d.z, 0x05010400u), u1 = __builtin_amdgcn_perm(d.w, d.z, 0x07030602u);
+  const mx_u32x4 o = {__builtin_amdgcn_perm(u0, t0, 0x05040100u), __builtin_amdgcn_perm(u0, t0, 0x07060302u),
+                      __builtin_amdgcn_perm(u1, t1, 0x05040100u), __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
+  reinterpret_cast<mx_u32x4*>(w.pieces[which])[(int64_t)g * rows + row] = o;
+}
 #endif
 
 template <typename V, int FMT>
@@ -107,34 +141,7 @@ __global__ __launch_bounds__(256) void mx_quantize_operand_kernel(const void* __
                                                                   uint8_t* __restrict__ codes, uint8_t* __restrict__ xp,
                                                                   int x_blocks, const OperandWeights w) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  if ((int)blockIdx.x >= x_blocks) {
-    int blk = (int)blockIdx.x - x_blocks, which = 0;
-#pragma unroll
-    for (int q = 0; q < kMxWeights - 1; ++q)
-      if (q < w.n - 1 && blk >= w.blk_end[q]) which = q + 1;
-    if (which) blk -= w.blk_end[which - 1];
-    const int nb = K / kMxBlock, groups = (nb + 15) >> 4;
-    const int64_t i = (int64_t)blk * 256 + threadIdx.x, rows = w.rows[which];
-    const int64_t row = i / groups;
-    const int g = (int)(i - row * groups);
-    if (row >= rows) return;
-    const uint8_t* src = w.scales[which] + row * nb + 16 * g;
-    mx_u32x4 d = {0, 0, 0, 0};
-    if ((nb & 15) == 0) {
-      d = *reinterpret_cast<const mx_u32x4*>(src);
-    } else {
-#pragma unroll
-      for (int q = 0; q < 16; ++q)
-        if (16 * g + q < nb) d[q >> 2] |= (uint32_t)src[q] << (8 * (q & 3));
-    }
-    // byte 4 s + q -> byte 4 q + s
-    const uint32_t t0 = __builtin_amdgcn_perm(d.y, d.x, 0x05010400u), t1 = __builtin_amdgcn_perm(d.y, d.x, 0x07030602u);
-    const uint32_t u0 = __builtin_amdgcn_perm(d.w, d.z, 0x05010400u), u1 = __builtin_amdgcn_perm(d.w, d.z, 0x07030602u);
-    const mx_u32x4 o = {__builtin_amdgcn_perm(u0, t0, 0x05040100u), __builtin_amdgcn_perm(u0, t0, 0x07060302u),
-                        __builtin_amdgcn_perm(u1, t1, 0x05040100u), __builtin_amdgcn_perm(u1, t1, 0x07060302u)};
-    reinterpret_cast<mx_u32x4*>(w.pieces[which])[(int64_t)g * rows + row] = o;
-    return;
-  }
+  if ((int)blockIdx.x >= x_blocks) return lay_out_scales((int)blockIdx.x - x_blocks, K, w);
   mx_saturate_fp8();
   const uint32_t per_row = (uint32_t)Kp >> 3, real = (uint32_t)K >> 3;
   const int64_t c0 = (int64_t)blockIdx.x * (256 * kChunks);
@@ -216,25 +223,150 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
 #endif
 }
 
-// The kept 8-bit input (rows padded, scales in pieces) as bf16 [M, K].
-__global__ __launch_bounds__(256) void mx_dequantize_operand_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ xp,
-                                                                    int64_t M, int K, int Kp, void* __restrict__ out) {
+// The same for the input of adapter linears, with h = bf16(x^ . A^T) (A the members' rank x K matrices one below the other) from
+// the registers that hold x^.  Workgroup: 16 rows; its 8 waves take the row in turns of 256 elements and add up in LDS, in a
+// fixed order.  Lane l holds row l % 16, elements 8 (l / 16) .. + 7 of each block: the four lanes of a block meet by lane-quarter
+// swaps, and the codes, taken back to bf16, are operands of v_mfma_f32_16x16x32_bf16 as they lie.  (A lane with whole blocks
+// needs no neighbour, but its 16-byte loads lie 64 bytes apart, and the loads of x and A took 1.9 times the time.)
+constexpr int kHiddenWaves = 8, kHiddenTurn = 256;
+struct HiddenMembers {
+  const uint16_t* la[kMxWeights];  // [rank, K]
+  int r_end[kMxWeights];
+  int n;
+};
 #if defined(__HIP_DEVICE_COMPILE__)
-  const uint32_t per_row = (uint32_t)K >> 3;
-  const int64_t c0 = (int64_t)blockIdx.x * (256 * kChunks);
-  const int64_t row0 = c0 / per_row;
-  const uint32_t rem = (uint32_t)(c0 - row0 * per_row) + threadIdx.x;
+// the larger of each half over both sides of a lane swap of a value with itself
+template <typename P>
+__device__ __forceinline__ uint32_t max_u16x2(P swapped) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t a = swapped[0], b = swapped[1];
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+#endif
+// The next turn's x is asked for before this one's codes are stored, its share of A behind the products that read this one's.
+template <int RT>  // groups of 16 ranks
+__global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_quantize_hidden_kernel(const uint16_t* __restrict__ x, int64_t M, int K, int Kp,
+                                                                              uint8_t* __restrict__ codes, uint8_t* __restrict__ xp,
+                                                                              const HiddenMembers a, uint16_t* __restrict__ h,
+                                                                              float* __restrict__ part, int slices, int k_slice, int x_blocks,
+                                                                              const OperandWeights w) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+  if ((int)blockIdx.x >= x_blocks) return lay_out_scales((int)blockIdx.x - x_blocks, K, w);
+  constexpr int kPitch = kHiddenTurn + 32;  // of a row of codes on their way out: its lanes' eight bytes on disjoint banks
+  constexpr int kWaveLds = (16 * kPitch + 1023) / 1024 * 1024;
+  static_assert(kWaveLds >= 1024 * RT, "the sums reuse the memory");
+  __shared__ __attribute__((aligned(16))) char lds[kHiddenWaves * kWaveLds];
+  const int lane = threadIdx.x & 63, r16 = lane & 15, quarter = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t tile = blockIdx.x / slices, row = tile * 16 + r16;
+  const int slice = (int)(blockIdx.x - tile * slices), k_end = (slice + 1) * k_slice < Kp ? (slice + 1) * k_slice : Kp;
+  const bool live = row < M;
+  const int ranks = a.r_end[a.n - 1];
+  const uint16_t* la[RT];  // lane's rank of each group; beyond the last one it computes what nobody stores
 #pragma unroll
-  for (int u = 0; u < kChunks; ++u) {
-    const uint32_t t = rem + 256 * u, r = t / per_row, col = t - r * per_row;
-    const int64_t row = row0 + r;
-    if (row >= M) continue;
-    const uint32_t blk = col >> 2;
-    const mx_u32x2 c = *reinterpret_cast<const mx_u32x2*>(codes + row * Kp + 8 * col);
-    const uint32_t b = xp[((int64_t)(blk >> 4) * M + row) * 16 + mx_piece_byte(blk & 15)];
-    mx_u32x4 o = mx_bf16_of_fp8(c, mx_scale_value(b == 255 ? 127u : b));
-    if (b == 255) o = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-    reinterpret_cast<mx_u32x4*>(out)[row * per_row + col] = o;
+  for (int t = 0; t < RT; ++t) {
+    int r = 16 * t + r16;
+    r = r < ranks ? r : 0;
+    int which = 0;
+#pragma unroll
+    for (int q = 0; q < kMxWeights - 1; ++q)
+      if (q < a.n - 1 && r >= a.r_end[q]) which = q + 1;
+    la[t] = a.la[which] + (int64_t)(r - (which ? a.r_end[which - 1] : 0)) * K;
+  }
+  f32x4 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  mx_u32x4 v[8], b[RT][8];  // of block j this lane's quarter
+  auto load_x = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = mx_u32x4{0, 0, 0, 0};
+      if (live && k0 + 32 * j < K) v[j] = *reinterpret_cast<const mx_u32x4*>(x + row * K + k0 + 32 * j + 8 * quarter);
+    }
+  };
+  auto load_a = [&](int k0) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        b[t][j] = mx_u32x4{0, 0, 0, 0};
+        if (k0 + 32 * j < K) b[t][j] = *reinterpret_cast<const mx_u32x4*>(la[t] + k0 + 32 * j + 8 * quarter);
+      }
+  };
+  char* out = lds + wave * kWaveLds;
+  int k0 = slice * k_slice + kHiddenTurn * wave;
+  if (k0 < k_end) {
+    load_x(k0);
+    load_a(k0);
+  }
+  for (; k0 < k_end; k0 += kHiddenTurn * kHiddenWaves) {
+    const int next = k0 + kHiddenTurn * kHiddenWaves;
+    // conversions saturate between the two settings of the mode; the pins hold them there
+    mx_saturate_fp8();
+    uint32_t byte[8];
+    mx_u32x2 c[8];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      asm volatile("" : "+v"(v[j]), "+v"(v[j + 1]));
+      uint32_t e = mx_bf16_exponent(v[j]) | mx_bf16_exponent(v[j + 1]) << 16;  // of both blocks, met across the lane quarters
+      e = max_u16x2(__builtin_amdgcn_permlane32_swap(e, e, false, false));
+      e = max_u16x2(__builtin_amdgcn_permlane16_swap(e, e, false, false));
+#pragma unroll
+      for (int i = j; i < j + 2; ++i) {
+        byte[i] = mx_scale_byte(i == j ? e & 0xffffu : e >> 16, TTAMD_MXFP8);
+        c[i] = mx_pack8(v[i], mx_scale_value(byte[i] == 255 ? 127u : byte[i]));
+        if (byte[i] == 255) c[i] = mx_u32x2{0, 0};
+        asm volatile("" : "+v"(c[i]));
+      }
+    }
+    mx_saturate_fp8(false);
+    if (next < k_end) load_x(next);
+    // codes by way of LDS (a wave's own, whose accesses go in order), so that they leave as 256 bytes of a row
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *reinterpret_cast<mx_u32x2*>(out + r16 * kPitch + 32 * j + 8 * quarter) = c[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const mx_u32x4 piece = *reinterpret_cast<const mx_u32x4*>(out + (4 * i + quarter) * kPitch + 16 * r16);
+      const int64_t to = tile * 16 + 4 * i + quarter;
+      if (to < M) *reinterpret_cast<mx_u32x4*>(codes + to * Kp + k0 + 16 * r16) = piece;  // Kp is a multiple of 256
+    }
+    if (live) {
+      uint32_t two = byte[0] | byte[4] << 8;  // blocks q and 4 + q lie next to each other in the piece
+#pragma unroll
+      for (int q = 1; q < 4; ++q) two = quarter == q ? byte[q] | byte[4 + q] << 8 : two;
+      *reinterpret_cast<uint16_t*>(xp + ((int64_t)(k0 >> 9) * M + row) * 16 + 4 * quarter + 2 * ((k0 >> 8) & 1)) = (uint16_t)two;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      mx_u32x4 e = mx_bf16_of_fp8(c[j], mx_scale_value(byte[j] == 255 ? 127u : byte[j]));
+      if (byte[j] == 255) e = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e), __builtin_bit_cast(bf16x8, b[t][j]), acc[t], 0, 0, 0);
+    }
+    if (next < k_end) load_a(next);
+  }
+  f32x4 (*sums)[kWaveLds / 1024][64] = reinterpret_cast<f32x4 (*)[kWaveLds / 1024][64]>(lds);
+  __syncthreads();  // the codes' places are free
+#pragma unroll
+  for (int t = 0; t < RT; ++t) sums[wave][t][lane] = acc[t];
+  __syncthreads();
+  // lane l's element v of group t: row 4 (l / 16) + v, rank 16 t + l % 16
+  for (int i = threadIdx.x; i < RT * 256; i += 64 * kHiddenWaves) {
+    const int l = i & 63, e = (i >> 6) & 3, t = i >> 8;
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < kHiddenWaves; ++q) s += sums[q][t][l][e];
+    const int64_t to = tile * 16 + 4 * (l >> 4) + e;
+    const int r = 16 * t + (l & 15);
+    if (to >= M || r >= ranks) continue;
+    if (slices > 1)
+      part[(slice * M + to) * ranks + r] = s;
+    else
+      h[to * ranks + r] = __builtin_bit_cast(uint16_t, (__bf16)s);
   }
 #endif
 }
@@ -275,19 +407,27 @@ int check_codec(const char* who, int dtype, int64_t rows, int64_t K, int format)
 
 }  // namespace
 
+namespace {
+// the weights whose scales a launch lays out, `threads` pieces to a workgroup; their workgroups
+int64_t operand_weights(OperandWeights& w, const uint8_t* const* scales, const int64_t* rows, uint8_t* const* pieces, int n, int64_t K, int threads) {
+  w = OperandWeights{};
+  w.n = n;
+  int64_t blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    w.scales[i] = scales[i];
+    w.pieces[i] = pieces[i];
+    w.rows[i] = rows[i];
+    blocks += ((rows[i] + 15) / 16 * ((mx_groups(K) + 3) / 4) * 64 + threads - 1) / threads;
+    w.blk_end[i] = (int)blocks;
+  }
+  return blocks;
+}
+}  // namespace
+
 int run_mx_quantize_operand(const void* x, int64_t M, int64_t K, int fmt, uint8_t* codes, uint8_t* pieces, const uint8_t* const* w_scales,
                             const int64_t* w_rows, uint8_t* const* w_pieces, int n_weights, hipStream_t s) {
-  const int64_t Kp = mx_padded_k(K), xb = blocks_of(M * (Kp / 8));
-  OperandWeights w = {};
-  w.n = n_weights;
-  int64_t wb = 0;
-  for (int i = 0; i < n_weights; ++i) {
-    w.scales[i] = w_scales[i];
-    w.pieces[i] = w_pieces[i];
-    w.rows[i] = w_rows[i];
-    wb += (w_rows[i] * mx_groups(K) + 255) / 256;
-    w.blk_end[i] = (int)wb;
-  }
+  OperandWeights w;
+  const int64_t Kp = mx_padded_k(K), xb = blocks_of(M * (Kp / 8)), wb = operand_weights(w, w_scales, w_rows, w_pieces, n_weights, K, 256);
   if (xb + wb >= (int64_t(1) << 31)) return fail(TTAMD_EUNSUPPORTED, "mx_quantize_operand: M=%lld K=%lld are too large for one launch", (long long)M, (long long)K);
   if (fmt == TTAMD_MXFP4)
     mx_quantize_operand_kernel<TTAMD_MXFP4><<<dim3((unsigned)(xb + wb)), dim3(256), 0, s>>>(x, M, (int)K, (int)Kp, codes, pieces, (int)xb, w);
@@ -296,13 +436,53 @@ int run_mx_quantize_operand(const void* x, int64_t M, int64_t K, int fmt, uint8_
   return check_launch("mx_quantize_operand");
 }
 
-int run_mx_dequantize_operand(const uint8_t* codes, const uint8_t* pieces, int64_t M, int64_t K, void* out, hipStream_t s) {
-  const int64_t blocks = blocks_of(M * (K / 8));
-  if (blocks >= (int64_t(1) << 31)) return fail(TTAMD_EUNSUPPORTED, "mx_dequantize_operand: M=%lld K=%lld are too large for one launch", (long long)M, (long long)K);
-  mx_dequantize_operand_kernel<<<dim3((unsigned)blocks), dim3(256), 0, s>>>(codes, pieces, M, (int)K, (int)mx_padded_k(K), out);
-  return check_launch("mx_dequantize_operand");
+namespace {
+struct HiddenPlan {
+  int slices, k_slice;
+};
+// A workgroup's round (its eight waves a turn each, 2048 elements of 16 rows) takes 1.9 us and 1.7 more per 16 ranks, what a CU
+// takes in of such loads; with few rows the rounds are dealt to several workgroups where that saves more than the launch that
+// adds their sums (5 us).  Measured without and with (us): 350 x 14336 rank 16 30.3 / 11.6, rank 64 66.6 / 17.6; 1500 x 14336
+// rank 16 32.1 / 23.2; 24 x 4096 rank 64 21.8 / 14.5.
+HiddenPlan plan_hidden(int64_t M, int64_t K, int ranks) {
+  const int64_t round = kHiddenTurn * kHiddenWaves, rounds = (mx_padded_k(K) + round - 1) / round, tiles = (M + 15) / 16;
+  HiddenPlan p = {1, (int)(rounds * round)};
+  const int64_t most = 256 / tiles < rounds ? 256 / tiles : rounds;
+  if (most < 2) return p;
+  const int64_t per = (rounds + most - 1) / most;
+  if ((float)(rounds - per) * (1.9f + 1.7f * (float)((ranks + 15) / 16)) > 5.f) p = HiddenPlan{(int)((rounds + per - 1) / per), (int)(per * round)};
+  return p;
 }
-
+}  // namespace
+size_t mx_hidden_part_bytes(int64_t M, int64_t K, int ranks) {
+  const HiddenPlan p = plan_hidden(M, K, ranks);
+  return p.slices > 1 ? (size_t)p.slices * M * ranks * sizeof(float) : 0;
+}
+int run_mx_quantize_hidden(const void* x, int64_t M, int64_t K, uint8_t* codes, uint8_t* pieces, const uint16_t* const* lora_a, const int* r_off, int n,
+                           uint16_t* h_cat, float* part, const uint8_t* const* w_scales, const int64_t* w_rows, uint8_t* const* w_pieces, hipStream_t s) {
+  OperandWeights w;
+  HiddenMembers a = {};
+  a.n = n;
+  for (int i = 0; i < n; ++i) {
+    a.la[i] = lora_a[i];
+    a.r_end[i] = r_off[i + 1];
+  }
+  const HiddenPlan p = plan_hidden(M, K, r_off[n]);
+  TT_REQUIRE(p.slices == 1 || part, "mx_quantize_hidden: no room for the slices of the contraction");
+  const int64_t xb = (M + 15) / 16 * p.slices, wb = operand_weights(w, w_scales, w_rows, w_pieces, n, K, 64 * kHiddenWaves);
+  if (xb + wb >= (int64_t(1) << 31)) return fail(TTAMD_EUNSUPPORTED, "mx_quantize_hidden: M=%lld K=%lld are too large for one launch", (long long)M, (long long)K);
+  const dim3 grid((unsigned)(xb + wb)), block(64 * kHiddenWaves);
+  const uint16_t* in = reinterpret_cast<const uint16_t*>(x);
+  const int Kp = (int)mx_padded_k(K);
+  switch ((r_off[n] + 15) / 16) {
+    case 1: mx_quantize_hidden_kernel<1><<<grid, block, 0, s>>>(in, M, (int)K, Kp, codes, pieces, a, h_cat, part, p.slices, p.k_slice, (int)xb, w); break;
+    case 2: mx_quantize_hidden_kernel<2><<<grid, block, 0, s>>>(in, M, (int)K, Kp, codes, pieces, a, h_cat, part, p.slices, p.k_slice, (int)xb, w); break;
+    case 3: mx_quantize_hidden_kernel<3><<<grid, block, 0, s>>>(in, M, (int)K, Kp, codes, pieces, a, h_cat, part, p.slices, p.k_slice, (int)xb, w); break;
+    default: mx_quantize_hidden_kernel<4><<<grid, block, 0, s>>>(in, M, (int)K, Kp, codes, pieces, a, h_cat, part, p.slices, p.k_slice, (int)xb, w); break;
+  }
+  if (int rc = check_launch("mx_quantize_hidden")) return rc;
+  return p.slices == 1 ? TTAMD_OK : run_mx_sum_slices(part, nullptr, h_cat, M * r_off[n], r_off[n], p.slices, s);
+}
 int run_mx_expand_tiles(const uint8_t* codes, const uint8_t* scales, int64_t N, int64_t K, void* tiles, hipStream_t s) {
   const int64_t nk = K / 32;
   if (N / 16 >= (int64_t(1) << 31) || (nk + 15) / 16 > 65535) return fail(TTAMD_EUNSUPPORTED, "mx_expand_tiles: weight too large");

@@ -70,30 +70,26 @@ struct Cut {  // consecutive stretches of a workspace
 };
 
 struct FwdSpace {
-  uint16_t* x;
   uint8_t* pieces[kGroupMax];
-  float *hidden, *part;
+  float* part;
   size_t bytes;
 };
 FwdSpace fwd_space(const Members& d, void* workspace) {
   Cut c{reinterpret_cast<char*>(workspace)};
   FwdSpace f = {};
   const GroupSkinny& g = d.sk;
-  f.x = c.take<uint16_t>(2 * g.M * g.K);
-  size_t part = 0;
+  size_t part = mx_hidden_part_bytes(g.M, g.K, g.r_off[g.n]);
   for (int i = 0; i < g.n; ++i) {
     f.pieces[i] = c.take<uint8_t>(mx_piece_bytes(g.N[i], g.K));
     const size_t p = mx_gemm_part_bytes(g.M, g.N[i], g.K, TTAMD_MXFP8);
     part = p > part ? p : part;
   }
-  f.hidden = c.take<float>(group_hidden_ws_bytes(g.M, g.K, g.r_off[g.n]));
   f.part = c.take<float>(part);
   f.bytes = c.used;
   return f;
 }
 
 struct BwdSpace {
-  uint16_t* x;
   float *skinny, *part;
   char* tiles;
   size_t bytes;
@@ -117,7 +113,6 @@ BwdSpace bwd_space(const Members& d, void* workspace) {
   Cut c{reinterpret_cast<char*>(workspace)};
   BwdSpace b = {};
   const GroupSkinny& g = d.sk;
-  b.x = c.take<uint16_t>(2 * g.M * g.K);
   b.skinny = c.take<float>(group_lora_bwd_ws_bytes(g));
   const int64_t n = sum_n(d.dx);
   const bool fused = mx_dx_fused(g.M, n, g.K);
@@ -152,9 +147,7 @@ extern "C" int ttamd_mx_lora_fwd_bf16(const void* x, const ttamd_mx_lora_member*
     return fail(TTAMD_EWORKSPACE, "mx_lora_fwd: needs %zu bytes of 16-byte aligned workspace, got %zu", f.bytes, workspace_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   uint16_t* h = reinterpret_cast<uint16_t*>(h_cat);
-  if (int rc = run_mx_quantize_operand(x, M, K, TTAMD_MXFP8, kept_codes, kept_scales, d.scales, d.sk.N, f.pieces, n_members, s)) return rc;
-  if (int rc = run_mx_dequantize_operand(kept_codes, kept_scales, M, K, f.x, s)) return rc;
-  if (int rc = run_group_hidden(f.x, d.sk, h, f.hidden, s)) return rc;
+  if (int rc = run_mx_quantize_hidden(x, M, K, kept_codes, kept_scales, d.sk.lora_a, d.sk.r_off, n_members, h, f.part, d.scales, d.sk.N, f.pieces, s)) return rc;
   for (int i = 0; i < n_members; ++i) {
     MxProduct q = {};
     q.x_codes = kept_codes; q.x_pieces = kept_scales;
@@ -185,8 +178,8 @@ extern "C" int ttamd_mx_lora_bwd_bf16(const uint8_t* kept_codes, const uint8_t* 
     return fail(TTAMD_EWORKSPACE, "mx_lora_bwd: needs %zu bytes of 16-byte aligned workspace, got %zu", b.bytes, workspace_bytes);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   uint16_t* gh = reinterpret_cast<uint16_t*>(gh_cat);
-  if (int rc = run_mx_dequantize_operand(kept_codes, kept_scales, M, K, b.x, s)) return rc;
-  if (int rc = run_group_lora_bwd(b.x, reinterpret_cast<const uint16_t*>(h_cat), d.sk, gh, b.skinny, s, nullptr)) return rc;
+  d.sk.kept = KeptInput{kept_codes, kept_scales, mx_padded_k(K)};
+  if (int rc = run_group_lora_bwd(nullptr, reinterpret_cast<const uint16_t*>(h_cat), d.sk, gh, b.skinny, s, nullptr)) return rc;
   return gx ? run_dx(d.dx, d.codes, d.scales, gh, gx, b.part, b.tiles, s) : TTAMD_OK;
 }
 

@@ -159,7 +159,9 @@ int run_mx_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* cons
 int check_mx_product(const char* who, int64_t M, int64_t N, int64_t K);
 int run_mx_quantize_operand(const void* x, int64_t M, int64_t K, int fmt, uint8_t* codes, uint8_t* pieces, const uint8_t* const* w_scales,
                             const int64_t* w_rows, uint8_t* const* w_pieces, int n_weights, hipStream_t s);
-int run_mx_dequantize_operand(const uint8_t* codes, const uint8_t* pieces, int64_t M, int64_t K, void* out, hipStream_t s);
+size_t mx_hidden_part_bytes(int64_t M, int64_t K, int ranks);
+int run_mx_quantize_hidden(const void* x, int64_t M, int64_t K, uint8_t* codes, uint8_t* pieces, const uint16_t* const* lora_a, const int* r_off, int n,
+                           uint16_t* h_cat, float* part, const uint8_t* const* w_scales, const int64_t* w_rows, uint8_t* const* w_pieces, hipStream_t s);
 int run_mx_expand_tiles(const uint8_t* codes, const uint8_t* scales, int64_t N, int64_t K, void* tiles, hipStream_t s);
 
 }  // namespace ttamd
