@@ -8,7 +8,9 @@
 // v_mfma_f32_16x16x32_bf16.  Workgroup: 8 waves, tile BM x 128, step 64 of the contraction.  gy, codes and scales go HBM ->
 // LDS by direct loads into a ring of five stages; in step t the workgroup expands the weight rows of step t + 1 (a thread
 // one half block) into one of two buffers and multiplies those of step t, read transposed (ds_read_b64_tr_b16).  One barrier
-// per step.  The contraction is cut into slices where the tiles do not fill the chip.
+// per step, and all that a step reads from LDS is asked for right behind it, before the requests for memory: read, request,
+// expand and multiply one after the other took 0.88 us a step of 128 rows instead of 0.73.  The contraction is cut into slices
+// where the tiles do not fill the chip.
 #include "group.h"
 #include "mx_math.h"
 
@@ -86,9 +88,20 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
     seg_begin += g.n[seg] / kStep;
     ++seg;
   }
+  // the member's addresses, read again only where the next member begins: a wait for the argument memory every step otherwise
+  const uint16_t* gy_at;
+  const uint8_t *codes_at, *scales_at;
+  int N, n;  // row length and next column of gy
+  auto enter = [&]() {
+    N = g.n[seg];
+    n = (p_step - seg_begin) * kStep;
+    gy_at = g.gy[seg] + (int64_t)m0 * N;
+    codes_at = g.codes[seg] + c0 / 2;
+    scales_at = g.scales[seg] + c0 / 32;
+  };
+  enter();
   auto request = [&]() {
     const bool more = p_step < s_end;
-    const int n = (p_step - seg_begin) * kStep, N = g.n[seg];
     const uint32_t st = lds0 + p_stage * T::kStage;
     const int rows = g.M - m0 < BM ? g.M - m0 : BM;
     // gy: 8 rows of 128 bytes per instruction, piece p of a row at p ^ (row / 2) % 8
@@ -96,33 +109,39 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
 #pragma unroll
     for (int i = 0; i < T::kLoadsGy; ++i) {
       const int q = wave * T::kLoadsGy + i;  // its parity flips the permutation's upper bit
-      dma16((off ^ ((q & 1) ? 64u : 0u)) + (uint32_t)(q * 8) * (uint32_t)(2 * N), g.gy[seg] + (int64_t)m0 * N + n, more ? rows * 2 * N - 2 * n : 0,
+      dma16((off ^ ((q & 1) ? 64u : 0u)) + (uint32_t)(q * 8) * (uint32_t)(2 * N), gy_at + n, more ? rows * 2 * N - 2 * n : 0,
             st + q * 1024);
     }
     // codes: 8 rows of 64 bytes per wave by its first 32 lanes (the others read nothing, into the next rows' place of the
     // same wave: 16 rows' room); scales: a dword for each of its 8 rows
     const uint32_t c_off = lane < 32 && c0 + 32 * (lane & 3) < g.K ? (uint32_t)(8 * wave + (lane >> 2)) * (uint32_t)(g.K / 2) + 16u * (lane & 3) : 0x7fffffffu;
     if (lane < 32)
-      dma16(c_off, g.codes[seg] + (int64_t)n * (g.K / 2) + c0 / 2, more ? kStep * (g.K / 2) - c0 / 2 : 0, st + T::kGy + wave * 512);
+      dma16(c_off, codes_at + (int64_t)n * (g.K / 2), more ? kStep * (g.K / 2) - c0 / 2 : 0, st + T::kGy + wave * 512);
     const uint32_t s_off = lane < 8 ? (uint32_t)(8 * wave + lane) * (uint32_t)(g.K / 32) : 0x7fffffffu;
-    dma4(s_off, g.scales[seg] + (int64_t)n * (g.K / 32) + c0 / 32, more ? kStep * (g.K / 32) - c0 / 32 : 0, st + T::kGy + T::kCodes + wave * 256);
+    dma4(s_off, scales_at + (int64_t)n * (g.K / 32), more ? kStep * (g.K / 32) - c0 / 32 : 0, st + T::kGy + T::kCodes + wave * 256);
     p_stage = p_stage == kStages - 1 ? 0 : p_stage + 1;
     ++p_step;
-    if (seg + 1 < g.members && p_step >= seg_begin + N / kStep) {
+    n += kStep;
+    if (n >= N && seg + 1 < g.members) {
       seg_begin += N / kStep;
       ++seg;
+      enter();
     }
   };
 
   // ---- expansion: thread t takes 16 elements of row t / 8: half t % 2 of block (t / 2) % 4
   const int e_row = threadIdx.x >> 3, e_part = threadIdx.x & 7;
-  auto expand = [&](int stage, int buffer) {
+  mx_u32x2 e_codes;
+  uint32_t e_byte;
+  auto expand_read = [&](int stage) {
     const char* st = smem + stage * T::kStage + T::kGy;
-    const mx_u32x2 c = *reinterpret_cast<const mx_u32x2*>(st + e_row * 64 + 8 * e_part);
-    const uint32_t b = *reinterpret_cast<const uint8_t*>(st + T::kCodes + (e_row >> 3) * 256 + (e_row & 7) * 4 + (e_part >> 1));
-    const float s = mx_scale_value(b == 255 ? 127u : b);
-    mx_u32x4 lo = mx_bf16_of_fp4(c.x, s), hi = mx_bf16_of_fp4(c.y, s);
-    if (b == 255) lo = hi = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    e_codes = *reinterpret_cast<const mx_u32x2*>(st + e_row * 64 + 8 * e_part);
+    e_byte = *reinterpret_cast<const uint8_t*>(st + T::kCodes + (e_row >> 3) * 256 + (e_row & 7) * 4 + (e_part >> 1));
+  };
+  auto expand_write = [&](int buffer) {
+    const float s = mx_scale_value(e_byte == 255 ? 127u : e_byte);
+    mx_u32x4 lo = mx_bf16_of_fp4(e_codes.x, s), hi = mx_bf16_of_fp4(e_codes.y, s);
+    if (e_byte == 255) lo = hi = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
     char* to = smem + kStages * T::kStage + buffer * T::kExpanded + e_row * kPitch + 32 * e_part;
     *reinterpret_cast<mx_u32x4*>(to) = lo;
     *reinterpret_cast<mx_u32x4*>(to + 16) = hi;
@@ -138,25 +157,24 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
   const int x_rd[2] = {ar * 128 + ((quarter ^ ((ar >> 1) & 7)) << 4), ar * 128 + (((4 + quarter) ^ ((ar >> 1) & 7)) << 4)};
   // a transposing read: lane i of quarter q points at row 8 q + i / 4 (+ 4), columns 4 (i % 4) .. + 3 of a 16-column block
   const int w_rd = kStages * T::kStage + (8 * quarter + (r16 >> 2)) * kPitch + 8 * (r16 & 3) + 2 * 16 * TC * wc;
-  auto multiply = [&](int stage, int buffer) {
+  bf16x8_t xf[2][TM], wf[2][TC];  // operands of both halves of a step
+  auto operands = [&](int stage, int buffer, int h) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8_t xf[TM], wf[TC];
-#pragma unroll
-      for (int j = 0; j < TC; ++j) {
-        const char* p = smem + w_rd + buffer * T::kExpanded + h * 32 * kPitch + j * 32;
-        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 4 * kPitch));
-        const s16x8_t both = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        wf[j] = __builtin_bit_cast(bf16x8_t, both);
-      }
-#pragma unroll
-      for (int i = 0; i < TM; ++i) xf[i] = *reinterpret_cast<const bf16x8_t*>(smem + stage * T::kStage + x_rd[h] + i * 2048);
-#pragma unroll
-      for (int j = 0; j < TC; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j], xf[i], acc[j][i], 0, 0, 0);
+    for (int j = 0; j < TC; ++j) {
+      const char* p = smem + w_rd + buffer * T::kExpanded + h * 32 * kPitch + j * 32;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 4 * kPitch));
+      const s16x8_t both = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      wf[h][j] = __builtin_bit_cast(bf16x8_t, both);
     }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xf[h][i] = *reinterpret_cast<const bf16x8_t*>(smem + stage * T::kStage + x_rd[h] + i * 2048);
+  };
+  auto multiply = [&](int h) {
+#pragma unroll
+    for (int j = 0; j < TC; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[h][j], xf[h][i], acc[j][i], 0, 0, 0);
   };
 
   // ---- pipeline.  At step t a wave waits until what it requested for step t + 1 has landed and its own expansion of step t
@@ -165,14 +183,19 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
   constexpr int kLoads = T::kLoadsGy + 2;
   for (int i = 0; i < kStages - 1; ++i) request();
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * kLoads) : "memory");
-  expand(0, 0);
+  expand_read(0);
+  expand_write(0);
   int stage = 0;
   for (int t = s_begin; t < s_end; ++t) {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
-    request();
     const int next = stage == kStages - 1 ? 0 : stage + 1, buffer = (t - s_begin) & 1;
-    expand(next, buffer ^ 1);  // behind the last step: zeros
-    multiply(stage, buffer);
+    expand_read(next);  // behind the last step: zeros
+    operands(stage, buffer, 0);
+    operands(stage, buffer, 1);
+    request();
+    expand_write(buffer ^ 1);
+    multiply(0);
+    multiply(1);
     stage = next;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -250,11 +273,11 @@ struct MxDxPlan {
 };
 
 // The fused kernel against the dense product on expanded weights, tile height and slices: the least of a fitted time in us
-// (steps of 64; a workgroup fills a CU, so 256 run in one turn).  Fused, a turn's step takes 0.83 us at 64 rows and 0.95 at
+// (steps of 64; a workgroup fills a CU, so 256 run in one turn).  Fused, a turn's step takes 0.60 us at 64 rows and 0.73 at
 // 128 however few CUs have work; slices write and read fp32 partial sums.  The dense product's 256-wide tiles take 0.92 a step
 // on a nearly idle chip and 1.42 on a full one, where power bounds them, and the expansion writes two bytes an element.
-// Measured, fused against both of the others (us): 24 x 2048 -> 2048 12.3 / 37; 350 x 2048 -> 2048 20.8 / 38; 350 x 6144 ->
-// 4096 55 / 103; 1024 x 6144 -> 4096 92 / 105; 1500 x 6144 -> 4096 156 / 106; 512 x 4096 -> 14336 125 / 95.
+// Measured, fused against both of the others (us): 24 x 2048 -> 2048 10.6 / 39; 350 x 2048 -> 2048 17.8 / 38; 350 x 6144 ->
+// 4096 46 / 107; 1024 x 6144 -> 4096 74 / 109; 1024 x 14336 -> 4096 160 / 236; 350 x 4096 -> 14336 92 / 98, but 1024 192 / 118.
 MxDxPlan plan_dx(int64_t M, int64_t n_total, int64_t K) {
   const int64_t steps = n_total / kStep;
   const int64_t dense_tiles = ((M + 255) / 256) * ((K + 255) / 256);
@@ -268,7 +291,7 @@ MxDxPlan plan_dx(int64_t M, int64_t n_total, int64_t K) {
       const int64_t per = (steps + slices - 1) / slices;
       if ((steps + per - 1) / per != slices) continue;
       if (slices > 1 && (per < 3 || slices * M * K > (int64_t(1) << 26))) break;
-      float time = 3.f + (float)((tiles * slices + 255) / 256) * (float)per * (bm == 64 ? 0.83f : 0.95f);
+      float time = 3.f + (float)((tiles * slices + 255) / 256) * (float)per * (bm == 64 ? 0.60f : 0.73f);
       if (slices > 1) time += 3.f + (float)(slices * M * K) * 2e-6f;
       if (time < best) {
         best = time;
