@@ -126,3 +126,23 @@ def test_cpu_tensors_are_refused():
     bf = torch.bfloat16
     with pytest.raises(RuntimeError, match="AMD GPU"):
         lora_linear_mx(torch.zeros(4, 64, dtype=bf), [w], [torch.zeros(8, 64, dtype=bf)], [torch.zeros(64, 8, dtype=bf)], [1.0])
+
+
+def test_module_refusals():
+    from torchtune_amd import FrozenMXLinear, MXLoRALinear, harness
+
+    for args in ((100, 64, 8, 16.0), (64, 96, 8, 16.0), (64, 64, 12, 16.0), (64, 64, 0, 16.0), (64, 64, 72, 16.0)):
+        with pytest.raises(ValueError):
+            MXLoRALinear(*args)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        FrozenMXLinear(48, 64)
+    with pytest.raises(ValueError, match="unknown format"):
+        FrozenMXLinear(64, 64, activation="int8")
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        FrozenMXLinear(64, 64)
+    with pytest.raises(ValueError, match="unknown base"):
+        harness.build_qlora_decoder("tiny", 8, 16.0, base="int4")
+    with torch.device("meta"):
+        m = MXLoRALinear(128, 64, 8, 16.0, use_bias=True)
+    assert tuple(m.weight_codes.shape) == (64, 64) and tuple(m.weight_scales.shape) == (64, 4) and m.adapter_params() == ["lora_a.weight", "lora_b.weight"]
+    assert tuple(m.mx_weight.shape) == (64, 128)

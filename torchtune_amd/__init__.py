@@ -6,8 +6,8 @@ All arithmetic runs in ``lib/libtorchtune_amd.so`` (hand-written HIP, plain C AB
 """
 from .nf4_tensor import NF4Tensor, implements, linear_nf4, to_nf4
 from .mx import MXTensor, linear_mx, lora_linear_mx, to_mx
-from .modules.low_precision import FrozenNF4Linear
-from .modules.peft import DoRALinear, LoRALinear, QATLoRALinear
+from .modules.low_precision import FrozenMXLinear, FrozenNF4Linear
+from .modules.peft import DoRALinear, LoRALinear, MXLoRALinear, QATLoRALinear
 from .qat import (
     FakeQuantizeConfig,
     FakeQuantizedLinear,
@@ -30,6 +30,8 @@ __all__ = [
     "to_mx",
     "linear_mx",
     "lora_linear_mx",
+    "FrozenMXLinear",
+    "MXLoRALinear",
     "FrozenNF4Linear",
     "LoRALinear",
     "DoRALinear",

@@ -109,6 +109,7 @@ struct LinearMXFn : torch::autograd::Function<LinearMXFn> {
                         int64_t activation) {
     ctx->save_for_backward({codes, scales});
     ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["bias"] = bias.has_value();  // an absent one has no edge to ask about
     return linear_forward(x, codes, scales, bias ? *bias : Tensor(), activation);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -127,7 +128,7 @@ struct LinearMXFn : torch::autograd::Function<LinearMXFn> {
               "linear_mx");
       }
     }
-    if (ctx->needs_input_grad(3)) gbias = gy.sum(0);
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) gbias = gy.sum(0);
     return {gx, Tensor(), Tensor(), gbias, Tensor()};
   }
 };
@@ -310,5 +311,8 @@ void bind_mx(py::module_& m) {
   m.def("mx_quantize", &mx_quantize, unlocked);
   m.def("mx_dequantize", &mx_dequantize, unlocked);
   m.def("mx_linear", &mx_linear, unlocked);
-  m.def("mx_lora", &mx_lora);
+  m.def("mx_lora", [](const Tensor& x, const std::vector<double>& factors, const py::args& flat) {
+    const std::vector<Tensor> ys = mx_lora(x, factors, flat);
+    return py::tuple(py::cast(ys));
+  });
 }

@@ -19,7 +19,7 @@ The output projection is a plain frozen bf16 linear, never NF4 (``_component_bui
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 import torch.nn.functional as F
@@ -28,7 +28,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 from torch.utils.checkpoint import checkpoint
 
 from .modules import layer_ops
-from .modules.peft import (LoRALinear, get_adapter_params, lora_feed_forward, lora_linear_group, lora_swiglu_group,
+from .modules.peft import (LoRALinear, MXLoRALinear, get_adapter_params, lora_feed_forward, lora_linear_group, lora_swiglu_group,
                            set_trainable_params)
 from .qat import FakeQuantizedLinear, Int8DynActInt4WeightQATQuantizer, fake_quantized_linear_group, fake_quantized_swiglu_group
 
@@ -151,14 +151,16 @@ def apply_rope(x: torch.Tensor, cache: torch.Tensor) -> torch.Tensor:
     return out.flatten(3).to(x.dtype)
 
 
-def _linear(in_dim: int, out_dim: int, rank: int, alpha: float, quantize_base: bool) -> nn.Module:
+def _linear(in_dim: int, out_dim: int, rank: int, alpha: float, quantize_base: Union[bool, str]) -> nn.Module:
+    if rank > 0 and quantize_base == "mxfp4":
+        return MXLoRALinear(in_dim, out_dim, rank=rank, alpha=alpha)
     if rank > 0:
         return LoRALinear(in_dim, out_dim, rank=rank, alpha=alpha, quantize_base=quantize_base)
     return nn.Linear(in_dim, out_dim, bias=False)
 
 
 class Attention(nn.Module):
-    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: bool):
+    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: Union[bool, str]):
         super().__init__()
         self.n_heads, self.n_kv, self.head_dim = s.n_heads, s.n_kv_heads, s.head_dim
         self.q_proj = _linear(s.dim, s.n_heads * s.head_dim, rank, alpha, quantize_base)
@@ -193,7 +195,7 @@ class Attention(nn.Module):
 
 
 class FeedForward(nn.Module):
-    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: bool):
+    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: Union[bool, str]):
         super().__init__()
         self.w1 = _linear(s.dim, s.hidden, rank, alpha, quantize_base)  # gate
         self.w2 = _linear(s.hidden, s.dim, rank, alpha, quantize_base)  # down
@@ -225,7 +227,7 @@ def _add_norm(x: torch.Tensor, delta: torch.Tensor, norm: RMSNorm):
 
 
 class DecoderLayer(nn.Module):
-    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: bool):
+    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: Union[bool, str]):
         super().__init__()
         self.sa_norm = RMSNorm(s.dim, s.norm_eps)
         self.attn = Attention(s, rank, alpha, quantize_base)
@@ -248,7 +250,7 @@ class Decoder(nn.Module):
     ``loss_chunks`` = 2 (the reference default is 8): with 288 GB of HBM the fp32 logits of half the batch (2 GB for
     8192 tokens) are no burden, and the vocabulary GEMM runs 25 % faster on 4096-row chunks than on 1024-row ones."""
 
-    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: bool, activation_checkpointing: bool = False,
+    def __init__(self, s: LlamaShape, rank: int, alpha: float, quantize_base: Union[bool, str], activation_checkpointing: bool = False,
                  loss_chunks: int = 2):
         super().__init__()
         self.shape = s
@@ -319,17 +321,23 @@ def _init_weights(model: Decoder, seed: int, std: float = 0.02) -> None:
             p.copy_(torch.randn(p.shape, device=dev, dtype=torch.float32, generator=gen) * 0.01)
         else:
             p.copy_((torch.randn(p.shape, device=dev, dtype=torch.float32, generator=gen) * std).to(torch.bfloat16))
+    for m in model.modules():
+        if isinstance(m, MXLoRALinear):
+            m.set_weight((torch.randn(m.out_dim, m.in_dim, device=dev, dtype=torch.float32, generator=gen) * std).to(torch.bfloat16))
 
 
 def build_qlora_decoder(shape: str | LlamaShape, rank: int, alpha: float, device="cuda", seed: int = 0,
-                        activation_checkpointing: bool = False, dtype: torch.dtype = torch.bfloat16) -> Decoder:
-    """QLoRA model: NF4 base + LoRA on all seven projections, everything but the adapters frozen."""
+                        activation_checkpointing: bool = False, dtype: torch.dtype = torch.bfloat16, base: str = "nf4") -> Decoder:
+    """QLoRA model: quantised base (``base``: "nf4" or "mxfp4") + LoRA on all seven projections, everything but the adapters
+    frozen."""
+    if base not in ("nf4", "mxfp4"):
+        raise ValueError(f"build_qlora_decoder: unknown base {base!r} (one of nf4, mxfp4)")
     s = SHAPES[shape] if isinstance(shape, str) else shape
     prev = torch.get_default_dtype()
     torch.set_default_dtype(dtype)
     try:
         with torch.device(device):
-            model = Decoder(s, rank, alpha, quantize_base=True, activation_checkpointing=activation_checkpointing)
+            model = Decoder(s, rank, alpha, quantize_base=True if base == "nf4" else base, activation_checkpointing=activation_checkpointing)
     finally:
         torch.set_default_dtype(prev)
     _init_weights(model, seed)

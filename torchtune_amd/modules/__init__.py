@@ -1,4 +1,4 @@
-from .low_precision import FrozenNF4Linear
-from .peft import LoRALinear, QATLoRALinear
+from .low_precision import FrozenMXLinear, FrozenNF4Linear
+from .peft import LoRALinear, MXLoRALinear, QATLoRALinear
 
-__all__ = ["FrozenNF4Linear", "LoRALinear", "QATLoRALinear"]
+__all__ = ["FrozenMXLinear", "FrozenNF4Linear", "LoRALinear", "MXLoRALinear", "QATLoRALinear"]

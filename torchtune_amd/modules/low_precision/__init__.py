@@ -1,3 +1,4 @@
+from .mx_linear import FrozenMXLinear
 from .nf4_linear import FrozenNF4Linear
 
-__all__ = ["FrozenNF4Linear"]
+__all__ = ["FrozenMXLinear", "FrozenNF4Linear"]

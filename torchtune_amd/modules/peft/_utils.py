@@ -11,6 +11,7 @@ import torch
 from torch import nn
 
 from ... import ops
+from ...mx import MXTensor
 from ...nf4_tensor import NF4Tensor
 
 
@@ -83,6 +84,7 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
     Plain LoRA: ``W += (alpha / rank) * B @ A``.  With a DoRA ``magnitude`` entry the merged weight is
     ``(W + (alpha / rank) * B @ A) * (magnitude / ||W + (alpha / rank) * B @ A||_row)`` and the magnitude is deleted too.
 
+    An mxfp4 base weight (``weight_codes``, ``weight_scales``) is dequantised and becomes a dense ``weight``.
     A base weight that is still an ``NF4Tensor`` on the GPU (a state dict taken without the dequantising hook) is
     dequantised and merged in one pass by the HIP kernel; a dense weight is updated as the reference does.
     ``use_distributed_barriers`` is the reference's fourth parameter (its checkpoint client passes it by keyword,
@@ -98,7 +100,8 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
             raise NotImplementedError(f"{module}: merging MoE experts is not part of this build")
         a = state_dict[f"{module}.lora_a.weight"]
         b = state_dict[f"{module}.lora_b.weight"]
-        w = state_dict[f"{module}.weight"]
+        codes = state_dict.pop(f"{module}.weight_codes", None)  # an mxfp4 base weight: the merged one is dense
+        w = state_dict[f"{module}.weight"] if codes is None else MXTensor(codes, state_dict.pop(f"{module}.weight_scales"))
         magnitude = state_dict.get(f"{module}.magnitude", None)
         fused = (
             isinstance(w, NF4Tensor) and w.is_cuda and w.block_size == 64 and w.dtype == torch.bfloat16
@@ -112,7 +115,7 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
                 wrote_to_host = w.device
             merged = ops.nf4_dequantize_merge(w.quantized_data, w.block_scalers(), N, K, a.to(w.device), b.to(w.device), scale,
                                               out=host)
-        elif magnitude is not None or isinstance(w, NF4Tensor):
+        elif magnitude is not None or isinstance(w, (NF4Tensor, MXTensor)):
             merged = w.to(a.dtype) + scale * b @ a
         else:
             w += scale * b @ a

@@ -18,6 +18,7 @@ import torch
 from ... import _host, nf4_tensor, ops
 from ...nf4_tensor import _check_in_features
 from .lora import LoRALinear, host_weight
+from .mx_lora import mx_group_applies, mx_lora_group
 
 
 # The backward of ``silu(gate) * up`` inside the library call that multiplies its results with the pair's adapters (one pass
@@ -262,6 +263,8 @@ def lora_feed_forward(x: torch.Tensor, gate: torch.nn.Module, up: torch.nn.Modul
 
 def lora_linear_group(x: torch.Tensor, layers: Sequence[torch.nn.Module]) -> Tuple[torch.Tensor, ...]:
     """``tuple(layer(x) for layer in layers)`` for layers that share the input ``x``."""
+    if mx_group_applies(layers):
+        return mx_lora_group(x, layers)
     if not group_applies(x, layers):
         return tuple(layer(x) for layer in layers)
     out = _native_group(x, layers, False)

@@ -112,4 +112,4 @@ def lora_linear_mx(input: torch.Tensor, weights: Sequence[MXTensor], lora_a: Seq
     for w, a, b, bias in zip(weights, lora_a, lora_b, biases):
         _check_weight(w, "lora_linear_mx")
         flat += [w.codes, w.scales, a, b, bias]
-    return tuple(_host.call("mx_lora", input, [float(s) for s in scales], *flat))
+    return _host.call("mx_lora", input, [float(s) for s in scales], *flat)
