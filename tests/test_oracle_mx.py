@@ -146,3 +146,51 @@ def test_module_refusals():
         m = MXLoRALinear(128, 64, 8, 16.0, use_bias=True)
     assert tuple(m.weight_codes.shape) == (64, 64) and tuple(m.weight_scales.shape) == (64, 4) and m.adapter_params() == ["lora_a.weight", "lora_b.weight"]
     assert tuple(m.mx_weight.shape) == (64, 128)
+
+
+def test_c_entries_refuse_before_they_launch():
+    """Addresses that are never read: every call below is turned away by its checks."""
+    import ctypes
+
+    from torchtune_amd import _lib
+
+    lib = _lib.load()
+    EINVAL, EUNSUPPORTED, EWORKSPACE = -1, -2, -3  # the header's codes
+    p, odd, none = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 2), None
+
+    def member(**kw):
+        f = dict(codes=1 << 12, scales=1 << 12, lora_a=1 << 12, lora_b=1 << 12, bias=None, y=1 << 12, grad_lora_a=1 << 12, grad_lora_b=1 << 12,
+                 N=128, rank=8, scale=1.0)
+        f.update(kw)
+        return _lib.MxLoraMember(**f)
+
+    def ptr(*ms):
+        arr = (_lib.MxLoraMember * len(ms))(*ms)
+        return ctypes.cast(arr, ctypes.c_void_p), len(ms)
+
+    fwd = lambda ms, x=p, m=4, k=64, ws=p, n=1 << 40: lib.ttamd_mx_lora_fwd_bf16(x, *ptr(*ms), p, p, p, m, k, ws, n, None)
+    bwd = lambda ms, gx=p, m=4, k=64, ws=p, n=1 << 40: lib.ttamd_mx_lora_bwd_bf16(p, p, p, *ptr(*ms), p, gx, m, k, ws, n, None)
+    lin = lambda x=p, f=8, m=4, n=128, k=64, ws=p, size=1 << 40, w=p, y=p, bias=none: lib.ttamd_mx_linear_bf16(x, f, w, p, bias, y, m, n, k, ws, size, None)
+    dx = lambda m=4, n=128, k=64, ws=p, size=1 << 40, gy=p, s=p: lib.ttamd_mx_linear_dx_bf16(gy, p, s, p, m, n, k, ws, size, None)
+    cases = [
+        (EINVAL, lambda: lib.ttamd_mx_quantize(p, 99, 4, 64, 4, p, p, None)),
+        (EINVAL, lambda: lib.ttamd_mx_quantize(p, _lib.TTAMD_BF16, 4, 48, 4, p, p, None)),
+        (EINVAL, lambda: lib.ttamd_mx_quantize(p, _lib.TTAMD_BF16, 4, 64, 5, p, p, None)),
+        (EINVAL, lambda: lib.ttamd_mx_quantize(odd, _lib.TTAMD_BF16, 4, 64, 4, p, p, None)),
+        (EINVAL, lambda: lib.ttamd_mx_dequantize(p, none, 4, 4, 64, _lib.TTAMD_BF16, p, None)),
+        (EINVAL, lambda: lin(f=5)), (EINVAL, lambda: lin(k=48)), (EINVAL, lambda: lin(m=0)), (EINVAL, lambda: lin(x=odd)), (EINVAL, lambda: lin(y=none)),
+        (EINVAL, lambda: lin(bias=ctypes.c_void_p(4097))), (EUNSUPPORTED, lambda: lin(k=1 << 23)), (EWORKSPACE, lambda: lin(m=400, size=0)),
+        (EWORKSPACE, lambda: lin(m=400, ws=none)), (EWORKSPACE, lambda: lin(m=400, ws=odd)),
+        (EINVAL, lambda: dx(n=96)), (EINVAL, lambda: dx(k=96)), (EINVAL, lambda: dx(gy=odd)), (EINVAL, lambda: dx(s=odd)), (EUNSUPPORTED, lambda: dx(n=1 << 23)),
+        (EWORKSPACE, lambda: dx(m=4096, n=4096, k=4096, size=16)),
+        (EINVAL, lambda: lib.ttamd_mx_lora_fwd_bf16(p, None, 1, p, p, p, 4, 64, p, 1 << 40, None)),
+        (EINVAL, lambda: fwd([member()] * 5)), (EINVAL, lambda: fwd([member()], k=96)), (EINVAL, lambda: fwd([member()], m=0)),
+        (EINVAL, lambda: fwd([member(N=96)])), (EINVAL, lambda: fwd([member(rank=4)])), (EINVAL, lambda: fwd([member(rank=40), member(rank=32)])),
+        (EINVAL, lambda: fwd([member(lora_b=None)])), (EINVAL, lambda: fwd([member(scales=4098)])), (EINVAL, lambda: fwd([member()], x=odd)),
+        (EUNSUPPORTED, lambda: fwd([member(N=1 << 23)])), (EWORKSPACE, lambda: fwd([member()], n=16)), (EWORKSPACE, lambda: fwd([member()], ws=none)),
+        (EINVAL, lambda: bwd([member(grad_lora_a=None)])), (EINVAL, lambda: bwd([member()], gx=odd)), (EWORKSPACE, lambda: bwd([member()], n=16)),
+    ]
+    for i, (want, call) in enumerate(cases):
+        assert call() == want, (i, lib.ttamd_last_error())
+    assert lib.ttamd_mx_linear_workspace_bytes(0, 1, 64, 8) == 0 and lib.ttamd_mx_lora_fwd_workspace_bytes(*ptr(member(rank=4)), 4, 64) == 0
+    assert lib.ttamd_mx_kept_codes_bytes(3, 320) == 3 * 512 and lib.ttamd_mx_kept_scales_bytes(3, 320) == 3 * 16

@@ -193,7 +193,8 @@ extern "C" int ttamd_mx_linear_dx_bf16(const void* gy, const uint8_t* w_codes, c
   if (int rc = check_mx_product("mx_linear_dx", M, N, K)) return rc;
   if (N >= kMaxGradN) return fail(TTAMD_EUNSUPPORTED, "mx_linear_dx: N (%lld) is too large", (long long)N);
   TT_REQUIRE(N % 64 == 0 && K % 64 == 0, "mx_linear_dx: N (%lld) and K (%lld) must be multiples of 64", (long long)N, (long long)K);
-  TT_REQUIRE(gy && w_codes && w_scales && gx && aligned16(gy) && aligned16(w_codes) && aligned16(gx), "mx_linear_dx: pointers must be non-null and 16-byte aligned");
+  TT_REQUIRE(gy && w_codes && w_scales && gx && aligned16(gy) && aligned16(w_codes) && aligned16(w_scales) && aligned16(gx),
+             "mx_linear_dx: pointers must be non-null and 16-byte aligned");
   const size_t need = ttamd_mx_linear_dx_workspace_bytes(M, N, K);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(TTAMD_EWORKSPACE, "mx_linear_dx: needs %zu bytes of 16-byte aligned workspace, got %zu", need, workspace_bytes);
