@@ -148,16 +148,15 @@ extern "C" int ttamd_mx_lora_fwd_bf16(const void* x, const ttamd_mx_lora_member*
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   uint16_t* h = reinterpret_cast<uint16_t*>(h_cat);
   if (int rc = run_mx_quantize_hidden(x, M, K, kept_codes, kept_scales, d.sk.lora_a, d.sk.r_off, n_members, h, f.part, d.scales, d.sk.N, f.pieces, s)) return rc;
+  MxProduct q[kGroupMax] = {};
   for (int i = 0; i < n_members; ++i) {
-    MxProduct q = {};
-    q.x_codes = kept_codes; q.x_pieces = kept_scales;
-    q.w_codes = d.codes[i]; q.w_pieces = f.pieces[i];
-    q.h = h + d.sk.r_off[i]; q.ldh = d.sk.r_off[n_members]; q.rank = d.sk.rank[i]; q.lora_b = d.sk.lora_b[i]; q.lscale = d.sk.scale[i];
-    q.bias = reinterpret_cast<const uint16_t*>(members[i].bias);
-    q.y = reinterpret_cast<uint16_t*>(members[i].y);
-    if (int rc = run_mx_gemm(q, M, d.sk.N[i], K, TTAMD_MXFP8, f.part, s)) return rc;
+    q[i].x_codes = kept_codes; q[i].x_pieces = kept_scales;
+    q[i].w_codes = d.codes[i]; q[i].w_pieces = f.pieces[i];
+    q[i].h = h + d.sk.r_off[i]; q[i].ldh = d.sk.r_off[n_members]; q[i].rank = d.sk.rank[i]; q[i].lora_b = d.sk.lora_b[i]; q[i].lscale = d.sk.scale[i];
+    q[i].bias = reinterpret_cast<const uint16_t*>(members[i].bias);
+    q[i].y = reinterpret_cast<uint16_t*>(members[i].y);
   }
-  return TTAMD_OK;
+  return run_mx_gemm_group(q, n_members, M, d.sk.N, K, f.part, s);
 }
 
 extern "C" size_t ttamd_mx_lora_bwd_workspace_bytes(const ttamd_mx_lora_member* members, int n_members, int64_t M, int64_t K) {

@@ -147,6 +147,7 @@ struct MxProduct {
 size_t mx_operand_bytes(int64_t M, int64_t K, int fmt);  // codes of an input with padded rows
 size_t mx_gemm_part_bytes(int64_t M, int64_t N, int64_t K, int fmt);
 int run_mx_gemm(const MxProduct& q, int64_t M, int64_t N, int64_t K, int fmt, float* part, hipStream_t s);
+int run_mx_gemm_group(const MxProduct* q, int n, int64_t M, const int64_t* N, int64_t K, float* part, hipStream_t s);
 bool mx_few_applies(int64_t M, int64_t N);    // the product of so few tokens streams the weight (mx_few.hip)
 bool mx_few_quantises(int64_t M, int64_t K);  // and quantises its input by itself
 int run_mx_few(const void* x, const uint8_t* x_codes, const uint8_t* x_pieces, const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
