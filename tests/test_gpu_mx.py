@@ -118,7 +118,7 @@ def test_linear(m, n, k, act):
 @pytest.mark.parametrize("r", [8, 16, 24, 64])
 @pytest.mark.parametrize("m,k,outs", [(1, 64, [64]), (24, 128, [192]), (77, 1024, [256]), (350, 2048, [2048]), (513, 320, [64, 128, 64]),
                                       (300, 1024, [1024, 256, 256]),
-                                      (33, 4160, [64]), (20, 8256, [128]), (2500, 320, [128, 64]), (1030, 64, [8192])])
+                                      (33, 4160, [64]), (20, 8256, [128]), (2500, 320, [128, 64]), (1030, 64, [8192]), (1100, 4096, [1024, 512, 512])])
 def test_lora(m, k, outs, r):
     if len(outs) > 1 and r > 16:
         r = 16
@@ -151,7 +151,7 @@ def test_lora(m, k, outs, r):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 64, 64), (1, 64, 128), (20, 192, 128), (32, 4096, 256), (64, 640, 384), (65, 128, 1152), (167, 512, 1024), (700, 4096, 320),
-                                   (1024, 1024, 1024), (1100, 64, 2048)])
+                                   (1024, 1024, 1024), (1100, 64, 2048), (550, 2048, 4096)])
 def test_linear_grad_input(m, n, k):
     w, dense = _weight(n, k, 11)
     g = _seed(12)

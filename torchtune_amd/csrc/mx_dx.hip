@@ -5,12 +5,13 @@
 //
 // A weight's blocks run along K and the contraction runs along N, so the scales cannot be the matrix instruction's: the codes
 // are expanded to bf16 (exactly: two significant bits times a power of two) on their way through LDS and the product runs on
-// v_mfma_f32_16x16x32_bf16.  Workgroup: 8 waves, tile BM x 128, step 64 of the contraction.  gy, codes and scales go HBM ->
-// LDS by direct loads into a ring of five stages; in step t the workgroup expands the weight rows of step t + 1 (a thread
-// one half block) into one of two buffers and multiplies those of step t, read transposed (ds_read_b64_tr_b16).  One barrier
-// per step, and all that a step reads from LDS is asked for right behind it, before the requests for memory: read, request,
-// expand and multiply one after the other took 0.88 us a step of 128 rows instead of 0.73.  The contraction is cut into slices
-// where the tiles do not fill the chip.
+// v_mfma_f32_16x16x32_bf16.  Workgroup: 8 waves, tile BM x 128 (BM 64, 128 or 256: the weight's share of a step is the same),
+// step 64 of the contraction.  gy, codes and scales go HBM -> LDS by direct loads into a ring of five stages (three at 256
+// rows); in step t the workgroup expands the weight rows of step t + 1 (a thread one half block) into one of two buffers and
+// multiplies those of step t, read transposed (ds_read_b64_tr_b16).  One barrier per step, and all that a step reads from LDS
+// is asked for right behind it, before the requests for memory: read, request, expand and multiply one after the other took
+// 0.88 us a step of 128 rows instead of 0.73.  The contraction is cut into slices where the tiles do not fill the chip.  Bound:
+// LDS and the way through it; the products alone would take 0.2 - 0.9 us a step.
 #include "group.h"
 #include "mx_math.h"
 
@@ -38,12 +39,13 @@ struct MxDxArgs {
   int members, M, K, ldgh, steps, tiles_m, tiles_c, slices, steps_per_slice;
 };
 
-constexpr int kStages = 5, kBC = 128, kStep = 64;
+constexpr int kBC = 128, kStep = 64;
 constexpr int kPitch = 2 * kBC + 32;  // four consecutive rows of a transposing read fall on disjoint banks
 template <int BM>
 struct MxDxTile {
   static constexpr int kGy = BM * 128, kCodes = kStep * kBC / 2, kScales = 8 * 256;  // of a stage, in bytes
   static constexpr int kStage = kGy + kCodes + kScales;
+  static constexpr int kStages = BM <= 128 ? 5 : 3;  // what LDS holds
   static constexpr int kExpanded = kStep * kPitch;
   static constexpr int kLds = kStages * kStage + 2 * kExpanded;
   static constexpr int kLoadsGy = kGy / 8192;  // per wave
@@ -55,7 +57,7 @@ template <int BM>
 __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using T = MxDxTile<BM>;
-  constexpr int TC = T::TC, TM = 4;
+  constexpr int TC = T::TC, TM = 4, kStages = T::kStages;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, r16 = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -179,15 +181,15 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
 
   // ---- pipeline.  At step t a wave waits until what it requested for step t + 1 has landed and its own expansion of step t
   //      is in LDS, and passes the barrier: everybody's is, and everybody is done with step t - 1, whose stage takes the
-  //      request of step t + 4.  Newer than stage t + 1 are the loads of stages t + 2 and t + 3.
+  //      request of step t + 4 (five stages).  Newer than stage t + 1 are the loads of stages t + 2 and t + 3.
   constexpr int kLoads = T::kLoadsGy + 2;
   for (int i = 0; i < kStages - 1; ++i) request();
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * kLoads) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kStages - 2) * kLoads) : "memory");
   expand_read(0);
   expand_write(0);
   int stage = 0;
   for (int t = s_begin; t < s_end; ++t) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 3) * kLoads) : "memory");
     const int next = stage == kStages - 1 ? 0 : stage + 1, buffer = (t - s_begin) & 1;
     expand_read(next);  // behind the last step: zeros
     operands(stage, buffer, 0);
@@ -273,11 +275,12 @@ struct MxDxPlan {
 };
 
 // The fused kernel against the dense product on expanded weights, tile height and slices: the least of a fitted time in us
-// (steps of 64; a workgroup fills a CU, so 256 run in one turn).  Fused, a turn's step takes 0.60 us at 64 rows and 0.73 at
-// 128 however few CUs have work; slices write and read fp32 partial sums.  The dense product's 256-wide tiles take 0.92 a step
-// on a nearly idle chip and 1.42 on a full one, where power bounds them, and the expansion writes two bytes an element.
-// Measured, fused against both of the others (us): 24 x 2048 -> 2048 10.6 / 39; 350 x 2048 -> 2048 17.8 / 38; 350 x 6144 ->
-// 4096 46 / 107; 1024 x 6144 -> 4096 74 / 109; 1024 x 14336 -> 4096 160 / 236; 350 x 4096 -> 14336 92 / 98, but 1024 192 / 118.
+// (steps of 64; a workgroup fills a CU, so 256 run in one turn).  Fused, a turn's step takes 0.60 us at 64 rows, 0.73 at 128 and
+// 1.0 at 256, however few CUs have work; slices write and read fp32 partial sums.  The dense product's 256-wide tiles take 0.92
+// a step on a nearly idle chip and 1.42 on a full one, where power bounds them, and the expansion writes two bytes an element.
+// Measured, fused against both of the others (us): 24 x 2048 -> 2048 10.6 / 39; 350 x 2048 -> 2048 17.9 / 38; 350 x 6144 ->
+// 4096 39 / 103; 1024 x 6144 -> 4096 64 / 106; 1500 x 6144 -> 4096 98 / 112; 350 x 14336 -> 4096 70 / 229; 1024 x 14336 -> 4096
+// 127 / 232; 350 x 4096 -> 14336 69 / 93, but 1024 134 / 120.
 MxDxPlan plan_dx(int64_t M, int64_t n_total, int64_t K) {
   const int64_t steps = n_total / kStep;
   const int64_t dense_tiles = ((M + 255) / 256) * ((K + 255) / 256);
@@ -285,13 +288,13 @@ MxDxPlan plan_dx(int64_t M, int64_t n_total, int64_t K) {
   float best = 6.f + (float)((dense_tiles + 255) / 256) * (float)steps * (0.92f + 0.5f * fill * fill) + (float)n_total * (float)K * 4.6e-7f;
   MxDxPlan p = {0, 1, 0, false};
   if (K % 128) return p;  // rows of scales are loaded in dwords
-  for (int bm = 64; bm <= 128; bm *= 2) {
+  for (int bm = 64; bm <= 256; bm *= 2) {
     const int64_t tiles = ((M + bm - 1) / bm) * ((K + kBC - 1) / kBC);
     for (int64_t slices = 1; slices <= 16; slices *= 2) {
       const int64_t per = (steps + slices - 1) / slices;
       if ((steps + per - 1) / per != slices) continue;
       if (slices > 1 && (per < 3 || slices * M * K > (int64_t(1) << 26))) break;
-      float time = 3.f + (float)((tiles * slices + 255) / 256) * (float)per * (bm == 64 ? 0.60f : 0.73f);
+      float time = 3.f + (float)((tiles * slices + 255) / 256) * (float)per * (bm == 64 ? 0.60f : bm == 128 ? 0.73f : 1.0f);
       if (slices > 1) time += 3.f + (float)(slices * M * K) * 2e-6f;
       if (time < best) {
         best = time;
@@ -350,7 +353,7 @@ int run_mx_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* cons
   g.M = (int)d.M; g.K = (int)d.K; g.ldgh = d.r_off[d.n]; g.steps = (int)(n_total / kStep);
   g.slices = p.slices; g.steps_per_slice = p.steps_per_slice;
   TT_REQUIRE(p.slices == 1 || part, "mx_dx: no room for the slices of the contraction");
-  const int rc = p.bm == 64 ? launch_dx<64>(g, s) : launch_dx<128>(g, s);
+  const int rc = p.bm == 64 ? launch_dx<64>(g, s) : p.bm == 128 ? launch_dx<128>(g, s) : launch_dx<256>(g, s);
   return rc || p.slices == 1 ? rc : run_mx_sum_slices(part, nullptr, g.gx, d.M * d.K, (int)d.K, p.slices, s);
 }
 
