@@ -181,13 +181,13 @@ def test_c_entries_refuse_before_they_launch():
         (EINVAL, lambda: lin(f=5)), (EINVAL, lambda: lin(k=48)), (EINVAL, lambda: lin(m=0)), (EINVAL, lambda: lin(x=odd)), (EINVAL, lambda: lin(y=none)),
         (EINVAL, lambda: lin(bias=ctypes.c_void_p(4097))), (EUNSUPPORTED, lambda: lin(k=1 << 23)), (EWORKSPACE, lambda: lin(m=400, size=0)),
         (EWORKSPACE, lambda: lin(m=400, ws=none)), (EWORKSPACE, lambda: lin(m=400, ws=odd)),
-        (EINVAL, lambda: dx(n=96)), (EINVAL, lambda: dx(k=96)), (EINVAL, lambda: dx(gy=odd)), (EINVAL, lambda: dx(s=odd)), (EUNSUPPORTED, lambda: dx(n=1 << 23)),
+        (EINVAL, lambda: dx(n=96)), (EINVAL, lambda: dx(k=96)), (EINVAL, lambda: dx(gy=odd)), (EINVAL, lambda: dx(s=odd)), (EUNSUPPORTED, lambda: dx(n=1 << 23)), (EUNSUPPORTED, lambda: dx(n=1 << 22)),
         (EWORKSPACE, lambda: dx(m=4096, n=4096, k=4096, size=16)),
         (EINVAL, lambda: lib.ttamd_mx_lora_fwd_bf16(p, None, 1, p, p, p, 4, 64, p, 1 << 40, None)),
         (EINVAL, lambda: fwd([member()] * 5)), (EINVAL, lambda: fwd([member()], k=96)), (EINVAL, lambda: fwd([member()], m=0)),
         (EINVAL, lambda: fwd([member(N=96)])), (EINVAL, lambda: fwd([member(rank=4)])), (EINVAL, lambda: fwd([member(rank=40), member(rank=32)])),
         (EINVAL, lambda: fwd([member(lora_b=None)])), (EINVAL, lambda: fwd([member(scales=4098)])), (EINVAL, lambda: fwd([member()], x=odd)),
-        (EUNSUPPORTED, lambda: fwd([member(N=1 << 23)])), (EWORKSPACE, lambda: fwd([member()], n=16)), (EWORKSPACE, lambda: fwd([member()], ws=none)),
+        (EUNSUPPORTED, lambda: fwd([member(N=1 << 22)])), (EWORKSPACE, lambda: fwd([member()], n=16)), (EWORKSPACE, lambda: fwd([member()], ws=none)),
         (EINVAL, lambda: bwd([member(grad_lora_a=None)])), (EINVAL, lambda: bwd([member()], gx=odd)), (EWORKSPACE, lambda: bwd([member()], n=16)),
     ]
     for i, (want, call) in enumerate(cases):

@@ -12,7 +12,7 @@
 namespace ttamd {
 namespace {
 
-constexpr int64_t kMaxGradN = int64_t(1) << 23;  // 128 rows of the output's gradient are addressed with 32 bits
+constexpr int64_t kMaxGradN = int64_t(1) << 22;  // 256 rows of the output's gradient, 512 N bytes, are counted in 32 bits
 
 struct Members {
   GroupSkinny sk;
