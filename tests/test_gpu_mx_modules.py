@@ -110,11 +110,12 @@ def test_dropout_composes_the_same_sum():
     assert torch.equal(y, linear_mx(x, m.mx_weight) + 2.0 * m.lora_b(m.lora_a(dropped)))
 
 
-def test_merged_checkpoint():
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+def test_merged_checkpoint(where):
     m = _layer(128, 64, 8, seed=7)
     x, a, b = _dense(m), m.lora_a.weight.detach(), m.lora_b.weight.detach()
-    merged = get_merged_lora_ckpt({f"l.{k}": v for k, v in m.state_dict().items()}, rank=8, alpha=16.0)
-    assert set(merged) == {"l.weight"}
+    merged = get_merged_lora_ckpt({f"l.{k}": v.to(where) for k, v in m.state_dict().items()}, rank=8, alpha=16.0)
+    assert set(merged) == {"l.weight"} and merged["l.weight"].device.type == where
     delta = 2.0 * (b.double() @ a.double()).cpu()
     # bf16: the product, its factor and the sum are rounded, two of them before the sum
     _within(merged["l.weight"], x + delta, 3 * HALF * delta.abs() + SUMS * 2.0 * (b.double().abs() @ a.double().abs()).cpu())
@@ -370,6 +371,20 @@ def test_saved_tensors_are_the_eight_bit_input():
         layer(x)
     frozen = {t.data_ptr() for t in (layer.weight_codes, layer.weight_scales, layer.lora_a.weight, layer.lora_b.weight)}
     assert sum(t.numel() * t.element_size() for t in kept if t.data_ptr() not in frozen) == 2048 * (1024 + 32 + 2 * 8)
+
+
+def test_transforms_and_second_derivatives_are_refused():
+    """None of them may drop a tangent, a batch or a second derivative without saying so."""
+    layer, x = _layer(64, 64, 8, seed=110), _randn(6, 64, seed=111).requires_grad_()
+    w = layer.mx_weight
+    for f in (layer, lambda t: linear_mx(t, w)):
+        with pytest.raises(RuntimeError, match="differentiated"):
+            torch.autograd.grad(f(x).sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x.detach())
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (x.detach(),), (torch.ones_like(x),))
+        f(x).sum().backward()  # and what is asked for in earnest still works
 
 
 def test_changed_in_place_after_the_forward_pass():

@@ -69,6 +69,11 @@ Tensor mx_dequantize(const Tensor& codes_, const Tensor& scales_, int64_t format
   return out;
 }
 
+// The backward passes are kernels that autograd does not see into.
+void first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward pass cannot be differentiated (create_graph=True)");
+}
+
 // the weight of a product: 2-D mxfp4
 void check_weight(const Tensor& codes, const Tensor& scales, const Tensor& x, const char* what) {
   check_parts(codes, scales, TTAMD_MXFP4, what);
@@ -113,6 +118,7 @@ struct LinearMXFn : torch::autograd::Function<LinearMXFn> {
     return linear_forward(x, codes, scales, bias ? *bias : Tensor(), activation);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order("linear_mx");
     const auto saved = ctx->get_saved_variables();
     const Tensor codes = dense(saved[0]), scales = dense(saved[1]);
     const int64_t N = codes.size(0), K = 2 * codes.size(1);
@@ -219,6 +225,7 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
     return o.ys;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order("lora_linear_mx");
     const auto saved = ctx->get_saved_variables();
     const Tensor &codes = saved[0], &scales = saved[1], &h = saved[2];
     const std::vector<double> factors = ctx->saved_data["factors"].toDoubleVector();

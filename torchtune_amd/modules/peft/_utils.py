@@ -101,7 +101,11 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
         a = state_dict[f"{module}.lora_a.weight"]
         b = state_dict[f"{module}.lora_b.weight"]
         codes = state_dict.pop(f"{module}.weight_codes", None)  # an mxfp4 base weight: the merged one is dense
-        w = state_dict[f"{module}.weight"] if codes is None else MXTensor(codes, state_dict.pop(f"{module}.weight_scales"))
+        if codes is None:
+            w = state_dict[f"{module}.weight"]
+        else:  # read back on the GPU, also out of a state dict that has left it
+            device = codes.device if codes.is_cuda else torch.device("cuda")
+            w = MXTensor(codes.to(device), state_dict.pop(f"{module}.weight_scales").to(device)).to(a.dtype).to(a.device)
         magnitude = state_dict.get(f"{module}.magnitude", None)
         fused = (
             isinstance(w, NF4Tensor) and w.is_cuda and w.block_size == 64 and w.dtype == torch.bfloat16
@@ -115,7 +119,7 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
                 wrote_to_host = w.device
             merged = ops.nf4_dequantize_merge(w.quantized_data, w.block_scalers(), N, K, a.to(w.device), b.to(w.device), scale,
                                               out=host)
-        elif magnitude is not None or isinstance(w, (NF4Tensor, MXTensor)):
+        elif magnitude is not None or codes is not None or isinstance(w, NF4Tensor):
             merged = w.to(a.dtype) + scale * b @ a
         else:
             w += scale * b @ a
