@@ -827,7 +827,8 @@ int ttamd_mx_linear_dx_bf16(const void* gy, const uint8_t* w_codes, const uint8_
  *             gx = sum_i gy_i . W_i + gh_i . lora_a_i  (NULL: not wanted)
  * kept_codes (ttamd_mx_kept_codes_bytes) and kept_scales (ttamd_mx_kept_scales_bytes) are x^, written by the forward and read
  * by the backward, in a layout of this library's own; h_cat, gh_cat bf16 [M, sum of ranks], the members side by side.
- * K % 64 == 0, N % 64 == 0, N < 2^22, ranks multiples of 8 that add up to at most 64.  Pointers 16-byte aligned (bias: 2).
+ * K % 64 == 0, N % 64 == 0, N < 2^22 (their sum 2^23), ranks multiples of 8 that add up to at most 64.  Pointers 16-byte
+ * aligned (bias: 2).
  */
 typedef struct ttamd_mx_lora_member {
   const uint8_t* codes;  /* mxfp4 codes of the weight, [N, K / 2] */

@@ -396,9 +396,10 @@ def test_changed_in_place_after_the_forward_pass():
         y.sum().backward()
 
 
-def test_offsets_beyond_32_bits():
-    """More than 2^31 elements of input: the last tokens against the same tokens by themselves."""
-    m, k, n, tail = 131072 + 77, 16448, 64, 45
+@pytest.mark.parametrize("k,n", [(16448, 64), (64, 16448)])
+def test_offsets_beyond_32_bits(k, n):
+    """More than 2^31 elements of input, or of output: the last tokens against the same tokens by themselves."""
+    m, tail = 131072 + 77, 45
     if torch.cuda.mem_get_info()[0] < 64 << 30:
         pytest.skip("needs 64 GiB of free device memory")
     layer = _layer(k, n, 8, seed=100)

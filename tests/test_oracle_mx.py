@@ -187,7 +187,7 @@ def test_c_entries_refuse_before_they_launch():
         (EINVAL, lambda: fwd([member()] * 5)), (EINVAL, lambda: fwd([member()], k=96)), (EINVAL, lambda: fwd([member()], m=0)),
         (EINVAL, lambda: fwd([member(N=96)])), (EINVAL, lambda: fwd([member(rank=4)])), (EINVAL, lambda: fwd([member(rank=40), member(rank=32)])),
         (EINVAL, lambda: fwd([member(lora_b=None)])), (EINVAL, lambda: fwd([member(scales=4098)])), (EINVAL, lambda: fwd([member()], x=odd)),
-        (EUNSUPPORTED, lambda: fwd([member(N=1 << 22)])), (EWORKSPACE, lambda: fwd([member()], n=16)), (EWORKSPACE, lambda: fwd([member()], ws=none)),
+        (EUNSUPPORTED, lambda: fwd([member(N=1 << 22)])), (EUNSUPPORTED, lambda: fwd([member(N=(1 << 22) - 64)] * 3)), (EWORKSPACE, lambda: fwd([member()], n=16)), (EWORKSPACE, lambda: fwd([member()], ws=none)),
         (EINVAL, lambda: bwd([member(grad_lora_a=None)])), (EINVAL, lambda: bwd([member()], gx=odd)), (EWORKSPACE, lambda: bwd([member()], n=16)),
     ]
     for i, (want, call) in enumerate(cases):

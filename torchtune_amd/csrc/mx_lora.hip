@@ -52,6 +52,9 @@ int decode(const char* who, const ttamd_mx_lora_member* m, int n, int64_t M, int
     r += m[i].rank;
   }
   TT_REQUIRE(r <= 64, "%s: the members' ranks add up to %d, at most 64 are supported", who, r);
+  int64_t n_total = 0;
+  for (int i = 0; i < n; ++i) n_total += m[i].N;
+  if (n_total >= 2 * kMaxGradN) return fail(TTAMD_EUNSUPPORTED, "%s: the members' outputs (%lld) are too many for one grad-input", who, (long long)n_total);
   d.sk.r_off[n] = d.dx.r_off[n] = r;
   return TTAMD_OK;
 }
@@ -107,7 +110,17 @@ int run_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* const* 
     if (int rc = run_mx_expand_tiles(codes[i], scales[i], d.N[i], d.K, tiles + 2 * n * d.K, s)) return rc;
     n += d.N[i];
   }
-  return run_dense_dx_on_tiles(d, gh, gx, tiles, s);
+  // the dense launch addresses a gradient with 32 bits: longer batches go in stretches of rows
+  int64_t widest = 0;
+  for (int i = 0; i < d.n; ++i) widest = d.N[i] > widest ? d.N[i] : widest;
+  const int64_t rows = ((int64_t(1) << 32) - 1) / (2 * widest) / 256 * 256;
+  for (int64_t r = 0; r < d.M; r += rows) {
+    GroupDx part = d;
+    part.M = d.M - r < rows ? d.M - r : rows;
+    for (int i = 0; i < d.n; ++i) part.gy[i] = d.gy[i] + r * d.N[i];
+    if (int rc = run_dense_dx_on_tiles(part, reinterpret_cast<const uint16_t*>(gh) + r * d.r_off[d.n], reinterpret_cast<uint16_t*>(gx) + r * d.K, tiles, s)) return rc;
+  }
+  return TTAMD_OK;
 }
 BwdSpace bwd_space(const Members& d, void* workspace) {
   Cut c{reinterpret_cast<char*>(workspace)};

@@ -1370,8 +1370,7 @@ size_t dense_group_dx_workspace_bytes(const GroupDx& d) {
   return (size_t)d.K * (size_t)n_total * 2;
 }
 
-// tiles_fwd != nullptr: no expansion; the launch reads the tiles the forward launch of the same group left in its
-// workspace (the members' weights stacked by rows, or - paired - the gated pair's 128-column alternation).
+// The grouped grad-input on weights that lie there as forward tiles, the members' stacked by rows.
 int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles_fwd, hipStream_t s) {
   int64_t n_total = 0;
   DenseArgs g = {};
@@ -1407,6 +1406,8 @@ int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const 
   return launch_dense(g, s);
 }
 
+// tiles_fwd != nullptr: no expansion; the launch reads the tiles the forward launch of the same group left in its
+// workspace (the members' weights stacked by rows, or - paired - the gated pair's 128-column alternation).
 int run_gemm_dense_group_dx(const GroupDx& d, const void* gh_cat, void* gx, void* workspace, hipStream_t s, const void* tiles_fwd,
                             bool paired) {
   TT_REQUIRE(d.n >= 1 && d.n <= kGroupMax && dense_group_dx_workspace_bytes(d) > 0, "nf4_group_dx (expanded): shape not served");
