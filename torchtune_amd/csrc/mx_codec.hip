@@ -1,5 +1,5 @@
 // Microscaled tensors: a bf16 / fp32 tensor into blocks of 32 with a shared power-of-two scale (mxfp4, mxfp8) and back.
-// (torchtune trains over such weights through torchao's MX prototypes; the format is the OCP one, scales rounded down.)
+// (The format is the OCP one, scales rounded down.)
 //
 //     e = max(floor(log2(max |v|)) - emax, -127),  code = RNE(v / 2^e) saturated,  value = code * 2^e
 //
