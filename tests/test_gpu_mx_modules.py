@@ -298,6 +298,9 @@ def test_trace():
     a, b = two(x)
     assert torch.equal(a, b) and tuple(a.shape) == tuple(one.shape)
     assert torch.equal(two(y)[0], lora_linear_group(y, [layer, layer])[0])
+    xr, gy = y.clone().requires_grad_(), _randn(20, 128, seed=66)
+    for f, g in ((traced, lambda t: linear_mx(t, w)), (lambda t: two(t)[1], lambda t: lora_linear_group(t, [layer, layer])[1])):
+        assert torch.equal(torch.autograd.grad(f(xr), [xr], gy)[0], torch.autograd.grad(g(xr), [xr], gy)[0])
 
 
 # ---- views, alignment, edges ------------------------------------------------------------------------
