@@ -342,6 +342,15 @@ def test_no_tokens():
     assert tuple(gx.shape) == (2, 0, 64)
 
 
+def test_no_outputs():
+    w = MXTensor(torch.zeros(0, 64, dtype=torch.uint8, device=DEV), torch.zeros(0, 4, dtype=torch.uint8, device=DEV))
+    x = _randn(5, 128, seed=77).requires_grad_()
+    y = linear_mx(x, w)
+    gx, = torch.autograd.grad(y, [x], torch.zeros_like(y))
+    assert tuple(y.shape) == (5, 0) and tuple(gx.shape) == (5, 128) and not gx.any()
+    assert tuple(w.to().shape) == (0, 128)
+
+
 def test_only_the_gradients_that_are_asked_for():
     layer, x, gy = _layer(128, 64, 8, seed=74, bias=True), _randn(30, 128, seed=75), _randn(30, 64, seed=76)
     every = torch.autograd.grad(layer(x.clone().requires_grad_()), [layer.lora_a.weight, layer.lora_b.weight, layer.bias], gy)

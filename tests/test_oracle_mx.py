@@ -87,6 +87,8 @@ def test_refusals_come_before_the_device_is_asked_for():
         linear_mx(x, _weight(128, 64, "mxfp8"))
     with pytest.raises(RuntimeError, match="shapes cannot be multiplied"):
         linear_mx(torch.zeros(4, 96, dtype=bf), w)
+    with pytest.raises(ValueError, match="inputs"):
+        linear_mx(torch.zeros(4, 0, dtype=bf), _weight(0, 0))
     with pytest.raises(ValueError):
         linear_mx(x, w, activation="int8")
     with pytest.raises(ValueError):

@@ -77,7 +77,7 @@ void first_order(const char* what) {
 // the weight of a product: 2-D mxfp4
 void check_weight(const Tensor& codes, const Tensor& scales, const Tensor& x, const char* what) {
   check_parts(codes, scales, TTAMD_MXFP4, what);
-  TORCH_CHECK_VALUE(codes.dim() == 2, what, ": the weight must have two dimensions, got codes ", codes.sizes());
+  TORCH_CHECK_VALUE(codes.dim() == 2 && codes.size(1) > 0, what, ": the weight must have two dimensions and inputs, got codes ", codes.sizes());
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, what, ": expected a bfloat16 input, got ", x.scalar_type());
   TORCH_CHECK(x.dim() > 0 && x.size(-1) == 2 * codes.size(1), what, ": mat1 and mat2 shapes cannot be multiplied (", x.sizes(), " and ",
               2 * codes.size(1), "x", codes.size(0), ")");
@@ -97,10 +97,9 @@ Tensor linear_forward(const Tensor& x_, const Tensor& codes_, const Tensor& scal
   need_gpu(x_, "linear_mx");
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = dense(x_), codes = dense(codes_), scales = dense(scales_), bias = bias_.defined() ? bias_.contiguous() : bias_;
-  const int64_t K = x.size(-1), N = codes.size(0), M = K ? x.numel() / K : 0;
+  const int64_t K = x.size(-1), N = codes.size(0), M = x.numel() / K;
   Tensor y = at::empty(resized(x, N), x.options());
   if (y.numel() == 0) return y;
-  TORCH_CHECK_VALUE(K > 0, "linear_mx: the last dimension is empty");
   const size_t bytes = ttamd_mx_linear_workspace_bytes(M, N, K, (int)activation);
   const Tensor ws = bytes ? scratch(bytes, x) : Tensor();
   check(ttamd_mx_linear_bf16(x.data_ptr(), (int)activation, (const uint8_t*)codes.data_ptr(), (const uint8_t*)scales.data_ptr(), ptr(bias), y.data_ptr(),
@@ -124,12 +123,14 @@ struct LinearMXFn : torch::autograd::Function<LinearMXFn> {
     const int64_t N = codes.size(0), K = 2 * codes.size(1);
     const c10::DeviceGuard guard(codes.device());
     Tensor gx, gbias;
-    const Tensor gy = dense(g[0]).reshape({-1, N});
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t M = c10::multiply_integers(shape) / K;
+    const Tensor gy = dense(g[0]).reshape({M, N});
     if (ctx->needs_input_grad(0)) {
-      gx = at::empty(ctx->saved_data["shape"].toIntVector(), gy.options());
-      if (gx.numel()) {
-        const Tensor ws = scratch(ttamd_mx_linear_dx_workspace_bytes(gy.size(0), N, K), gy);
-        check(ttamd_mx_linear_dx_bf16(gy.data_ptr(), (const uint8_t*)codes.data_ptr(), (const uint8_t*)scales.data_ptr(), gx.data_ptr(), gy.size(0), N, K,
+      gx = gy.numel() ? at::empty(shape, gy.options()) : at::zeros(shape, gy.options());
+      if (gy.numel()) {
+        const Tensor ws = scratch(ttamd_mx_linear_dx_workspace_bytes(M, N, K), gy);
+        check(ttamd_mx_linear_dx_bf16(gy.data_ptr(), (const uint8_t*)codes.data_ptr(), (const uint8_t*)scales.data_ptr(), gx.data_ptr(), M, N, K,
                                       ws.data_ptr(), ws.numel(), stream_of(gy)),
               "linear_mx");
       }
