@@ -63,14 +63,15 @@ def test_frozen_linear(act, bias):
     assert torch.equal(other(x), y)
 
 
-def test_a_dense_checkpoint_is_quantised_while_it_is_loaded():
-    w = _randn(128, 64, seed=2)
+@pytest.mark.parametrize("dtype", [BF, torch.float32, torch.float16])
+def test_a_dense_checkpoint_is_quantised_while_it_is_loaded(dtype):
+    w = _randn(128, 64, seed=2).to(dtype)
     outer = nn.Sequential(_layer(64, 128), nn.Identity())
     state = {"0.weight": w, "0.lora_a.weight": outer[0].lora_a.weight.detach().clone(), "0.lora_b.weight": outer[0].lora_b.weight.detach().clone()}
     keys = set(state)
     outer.load_state_dict(state)
     assert set(state) == keys  # the caller's dictionary stays as it was
-    want = to_mx(w)
+    want = to_mx(w.float())
     assert torch.equal(outer[0].weight_codes, want.codes) and torch.equal(outer[0].weight_scales, want.scales)
     with pytest.raises(RuntimeError, match="size mismatch"):
         outer.load_state_dict({**state, "0.weight": w[:64]})

@@ -14,6 +14,11 @@ from torch import nn
 from ...mx import BLOCK, MXTensor, linear_mx, to_mx
 
 
+def _pack(dense: torch.Tensor) -> MXTensor:
+    """``dense`` as mxfp4, a float16 or float64 tensor by way of float32."""
+    return to_mx(dense if dense.dtype in (torch.bfloat16, torch.float32) else dense.float(), "mxfp4")
+
+
 class MXWeight(nn.Module):
     """Base of the modules over a frozen mxfp4 weight: its buffers, quantisation and loading."""
 
@@ -24,7 +29,7 @@ class MXWeight(nn.Module):
         if dense.device.type == "meta":
             codes, scales = (torch.empty(n, k // d, dtype=torch.uint8, device="meta") for d in (2, BLOCK))
         else:
-            packed = to_mx(dense.detach(), "mxfp4")
+            packed = _pack(dense.detach())
             codes, scales = packed.codes, packed.scales
         self.register_buffer("weight_codes", codes)
         self.register_buffer("weight_scales", scales)
@@ -39,7 +44,7 @@ class MXWeight(nn.Module):
         n, half = self.weight_codes.shape
         if tuple(dense.shape) != (n, 2 * half):
             raise ValueError(f"{type(self).__name__}: expected a weight of {n} x {2 * half}, got {tuple(dense.shape)}")
-        packed = to_mx(dense.to(self.weight_codes.device), "mxfp4")
+        packed = _pack(dense.to(self.weight_codes.device))
         self.weight_codes.copy_(packed.codes)
         self.weight_scales.copy_(packed.scales)
 
@@ -55,7 +60,7 @@ class MXWeight(nn.Module):
                               f"shape in current model is {tuple(self.mx_weight.shape)}.")
             state_dict[prefix + "weight_codes"], state_dict[prefix + "weight_scales"] = self.weight_codes, self.weight_scales
         else:
-            packed = to_mx(dense.detach().to(self.weight_codes.device), "mxfp4")
+            packed = _pack(dense.detach().to(self.weight_codes.device))
             state_dict[prefix + "weight_codes"], state_dict[prefix + "weight_scales"] = packed.codes, packed.scales
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
