@@ -245,8 +245,10 @@ __device__ __forceinline__ uint32_t max_u16x2(P swapped) {
 #endif
 // The next turn's x is asked for before this one's codes are stored, its share of A behind the products that read this one's,
 // and codes leave by way of LDS as 256 bytes of a row: 109 -> 89 us at 8192 x 14336 rank 16 with x in the caches (4.0 TB/s).
+// Up to 16 ranks half of A's share at a time leaves registers for two workgroups on a CU (8192 x 2048 17.2 -> 13.6 us, 8192 x 4096
+// 28.2 -> 25.0, at 14336 level); with 32 they spill (8192 x 4096 34.9 -> 36.4).
 template <int RT>  // groups of 16 ranks
-__global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_quantize_hidden_kernel(const uint16_t* __restrict__ x, int64_t M, int K, int Kp,
+__global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 4 : 2, RT == 1 ? 4 : 2))) void mx_quantize_hidden_kernel(const uint16_t* __restrict__ x, int64_t M, int K, int Kp,
                                                                               uint8_t* __restrict__ codes, uint8_t* __restrict__ xp,
                                                                               const HiddenMembers a, uint16_t* __restrict__ h,
                                                                               float* __restrict__ part, int slices, int k_slice, int x_blocks,
@@ -280,7 +282,8 @@ __global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  mx_u32x4 v[8], b[RT][8];  // of block j this lane's quarter
+  constexpr int kAhead = RT == 1 ? 4 : 8;  // blocks whose share of A is in registers
+  mx_u32x4 v[8], b[RT][kAhead];  // of block j this lane's quarter
   auto load_x = [&](int k0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kAhead; ++j) {
         b[t][j] = mx_u32x4{0, 0, 0, 0};
         if (k0 + 32 * j < K) b[t][j] = *reinterpret_cast<const mx_u32x4*>(la[t] + k0 + 32 * j + 8 * quarter);
       }
@@ -346,7 +349,8 @@ __global__ __launch_bounds__(64 * kHiddenWaves) __attribute__((amdgpu_waves_per_
       if (byte[j] == 255) e = mx_u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e), __builtin_bit_cast(bf16x8, b[t][j]), acc[t], 0, 0, 0);
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, e), __builtin_bit_cast(bf16x8, b[t][j % kAhead]), acc[t], 0, 0, 0);
+      if (kAhead < 8 && j == kAhead - 1) load_a(k0 + 32 * kAhead);
     }
     if (next < k_end) load_a(next);
   }
