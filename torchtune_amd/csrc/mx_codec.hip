@@ -226,8 +226,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* __res
 // the registers that hold x^.  Workgroup: 16 rows; its 8 waves take the row in turns of 256 elements and add up in LDS, in a
 // fixed order.  Lane l holds row l % 16, elements 8 (l / 16) .. + 7 of each block: the four lanes of a block meet by lane-quarter
 // swaps, and the codes, taken back to bf16, are operands of v_mfma_f32_16x16x32_bf16 as they lie.  (A lane with whole blocks
-// needs no neighbour, but its 16-byte loads lie 64 bytes apart: 137 us instead of 132 at 8192 x 14336, rank 16.)  Bound: what a
-// CU takes in, x once and A once per 16 rows, some 40 GB/s.
+// needs no neighbour, but its 16-byte loads lie 64 bytes apart: 137 us instead of 132 at 8192 x 14336, rank 16.)  Bound: HBM,
+// beside some 600 vector instructions a turn and A, which every 16 rows read again from L2: 103 us at that size behind other work.
 constexpr int kHiddenWaves = 8, kHiddenTurn = 256;
 struct HiddenMembers {
   const uint16_t* la[kMxWeights];  // [rank, K]
