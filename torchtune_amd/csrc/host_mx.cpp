@@ -172,9 +172,16 @@ void fill(ttamd_mx_lora_member& e, const MxMember& m, const Tensor& y) {
   e.scale = (float)m.scale;
 }
 
+// What the backward pass reads, in one piece of memory: the input's codes and scales, and h [M, ranks].
+struct Kept {
+  size_t scales, h, bytes;  // offsets
+  Kept(int64_t M, int64_t K, int64_t ranks)
+      : scales(align256(ttamd_mx_kept_codes_bytes(M, K))), h(scales + align256(ttamd_mx_kept_scales_bytes(M, K))), bytes(h + 2 * M * ranks) {}
+};
+
 struct LoraOut {
   std::vector<Tensor> ys;
-  Tensor codes, scales, h;
+  Tensor kept;
 };
 
 LoraOut lora_forward(const Tensor& x_, const std::vector<MxMember>& given) {
@@ -195,13 +202,12 @@ LoraOut lora_forward(const Tensor& x_, const std::vector<MxMember>& given) {
     fill(arr[i], m, o.ys[i]);
     ranks += m.a.size(0);
   }
-  const auto u8 = x.options().dtype(at::kByte);
-  o.codes = at::empty({(int64_t)ttamd_mx_kept_codes_bytes(M, K)}, u8);
-  o.scales = at::empty({(int64_t)ttamd_mx_kept_scales_bytes(M, K)}, u8);
-  o.h = at::empty({M, ranks}, x.options());
+  const Kept at(M, K, ranks);
+  o.kept = at::empty({(int64_t)at.bytes}, x.options().dtype(at::kByte));
   if (M == 0) return o;
+  uint8_t* kept = (uint8_t*)o.kept.data_ptr();
   const Tensor ws = scratch(ttamd_mx_lora_fwd_workspace_bytes(arr, n, M, K), x);
-  check(ttamd_mx_lora_fwd_bf16(x.data_ptr(), arr, n, (uint8_t*)o.codes.data_ptr(), (uint8_t*)o.scales.data_ptr(), o.h.data_ptr(), M, K, ws.data_ptr(),
+  check(ttamd_mx_lora_fwd_bf16(x.data_ptr(), arr, n, kept, kept + at.scales, kept + at.h, M, K, ws.data_ptr(),
                                ws.numel(), stream_of(x)),
         "lora_linear_mx");
   return o;
@@ -211,7 +217,7 @@ LoraOut lora_forward(const Tensor& x_, const std::vector<MxMember>& given) {
 struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, at::TensorList /*inputs*/, const std::vector<MxMember>& ms) {
     LoraOut o = lora_forward(x, ms);
-    variable_list save = {o.codes, o.scales, o.h};
+    variable_list save = {o.kept};
     std::vector<double> factors;
     std::vector<int64_t> bias;
     for (const MxMember& m : ms) {
@@ -228,22 +234,24 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order("lora_linear_mx");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &codes = saved[0], &scales = saved[1], &h = saved[2];
+    const Tensor& kept = saved[0];
     const std::vector<double> factors = ctx->saved_data["factors"].toDoubleVector();
     const std::vector<int64_t> bias = ctx->saved_data["bias"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
     const int n = (int)factors.size();
-    const c10::DeviceGuard guard(h.device());
-    const int64_t M = h.size(0), K = shape.back();
+    const c10::DeviceGuard guard(kept.device());
+    const int64_t K = shape.back(), M = c10::multiply_integers(shape) / K;
+    int64_t ranks = 0;
     std::vector<Tensor> gys(n), ga(n), gb(n);
     std::vector<MxMember> ms(n);
     ttamd_mx_lora_member arr[TTAMD_GROUP_MAX];
     for (int i = 0; i < n; ++i) {
       MxMember& m = ms[i];
-      m.codes = dense(saved[3 + 4 * i]);
-      m.scales = dense(saved[4 + 4 * i]);
-      m.a = dense(saved[5 + 4 * i]);
-      m.b = dense(saved[6 + 4 * i]);
+      m.codes = dense(saved[1 + 4 * i]);
+      m.scales = dense(saved[2 + 4 * i]);
+      m.a = dense(saved[3 + 4 * i]);
+      m.b = dense(saved[4 + 4 * i]);
       m.scale = factors[i];
+      ranks += m.a.size(0);
       gys[i] = dense(g[i]).reshape({M, m.codes.size(0)});
       ga[i] = M ? at::empty_like(m.a) : at::zeros_like(m.a);
       gb[i] = M ? at::empty_like(m.b) : at::zeros_like(m.b);
@@ -253,11 +261,13 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
     }
     const bool need_x = ctx->needs_input_grad(0);
     Tensor gx;
-    if (need_x) gx = at::empty(shape, h.options());
+    if (need_x) gx = at::empty(shape, gys[0].options());
     if (M) {
-      const Tensor gh = at::empty_like(h), ws = scratch(ttamd_mx_lora_bwd_workspace_bytes(arr, n, M, K), h);
-      check(ttamd_mx_lora_bwd_bf16((const uint8_t*)codes.data_ptr(), (const uint8_t*)scales.data_ptr(), h.data_ptr(), arr, n, gh.data_ptr(), ptr(gx), M, K,
-                                   ws.data_ptr(), ws.numel(), stream_of(h)),
+      const Kept at(M, K, ranks);
+      const uint8_t* k = (const uint8_t*)kept.data_ptr();
+      const size_t bytes = ttamd_mx_lora_bwd_workspace_bytes(arr, n, M, K), gh = align256(bytes);  // the gradient of h behind the workspace
+      const Tensor ws = scratch(gh + 2 * M * ranks, kept);
+      check(ttamd_mx_lora_bwd_bf16(k, k + at.scales, k + at.h, arr, n, (uint8_t*)ws.data_ptr() + gh, ptr(gx), M, K, ws.data_ptr(), bytes, stream_of(kept)),
             "lora_linear_mx");
     }
     variable_list out = {gx};
