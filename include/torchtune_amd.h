@@ -788,6 +788,14 @@ int ttamd_swiglu_bwd_bf16(const void* gout, const void* gate, const void* up, vo
 int ttamd_cross_entropy_fwd_bwd_bf16(const void* logits, const int64_t* target, int64_t ignore_index, float grad_scale,
                                      float* loss, void* grad_logits, int64_t rows, int64_t V, void* stream);
 
+/*
+ * out [N] = sum over the rows of x [M, N], bf16, fp32 sums, one rounding: the gradient of a linear's bias from that of its
+ * output.  The order of the sums depends on M and N only.  x 16-byte aligned; M may be 0 (zeros); workspace:
+ * ttamd_column_sum_workspace_bytes bytes (0: may be NULL).  Unlike a library reduction it clears no memory, so that a recorded
+ * call is the same on every replay.
+ */
+size_t ttamd_column_sum_workspace_bytes(int64_t M, int64_t N);
+int ttamd_column_sum_bf16(const void* x, void* out, int64_t M, int64_t N, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Microscaled (MX) tensors: blocks of 32 consecutive elements of a row with one power-of-two scale

@@ -1,0 +1,115 @@
+"""The gradient of a bias, the sum over the rows of its output's gradient: over sizes, against 64 bits, and recorded into a graph."""
+import ctypes
+
+import pytest
+import torch
+
+from torchtune_amd import MXLoRALinear, MXTensor, _lib, linear_mx, to_mx
+
+BF = torch.bfloat16
+DEV = "cuda"
+
+
+def _randn(*shape, seed, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(BF).to(DEV)
+
+
+def _sum(x):
+    lib = _lib.load()
+    m, n = x.shape
+    out = torch.full((n + 8,), 7.0, dtype=BF, device=DEV)
+    need = lib.ttamd_column_sum_workspace_bytes(m, n)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    assert lib.ttamd_column_sum_bf16(x.data_ptr(), out.data_ptr(), m, n, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    assert bool((out[n:] == 7.0).all())
+    return out[:n]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 7, 8, 64, 65, 127, 128, 136, 1000, 4096, 4104])
+@pytest.mark.parametrize("m", [0, 1, 3, 17, 63, 64, 127, 300, 1999, 8192])
+def test_column_sum(m, n):
+    x = _randn(m, n, seed=m + n)
+    # a half step, and fp32 sums whose chains are shorter than 2^7: a thread's rows, its column's threads and the stretches
+    exact = x.double().sum(0)
+    lost = 2.0 ** -17 * x.double().abs().sum(0)
+    got = _sum(x)
+    assert bool(((got.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 1.01 * lost).all())
+    assert torch.equal(got, _sum(x))
+
+
+@pytest.mark.gpu
+def test_column_sum_keeps_columns_apart_and_counts_every_row():
+    """Whole numbers, so that every sum is exact; a row or a column taken twice or not at all changes one."""
+    for m, n in ((1, 9), (200, 200), (1000, 129), (4099, 264)):
+        x = (torch.arange(m, device=DEV).view(-1, 1) % 3 + torch.arange(n, device=DEV) % 5).to(BF)
+        want = x.double().sum(0)
+        assert torch.equal(_sum(x), want.to(BF))
+    x = _randn(500, 72, seed=1)
+    x[3, 5], x[499, 71] = float("nan"), float("inf")
+    got = _sum(x)
+    assert torch.isnan(got).nonzero().flatten().tolist() == [5] and torch.isinf(got).nonzero().flatten().tolist() == [71]
+
+
+@pytest.mark.gpu
+def test_bias_gradient_beyond_32_bits():
+    m, n = 131072 + 77, 16449
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GiB of free device memory")
+    gy = torch.zeros(m, n, dtype=BF, device=DEV)
+    gy[::1000] = 1.0
+    gy[-5:] = 2.0
+    assert bool((_sum(gy) == float(len(range(0, m, 1000)) + 10)).all())
+
+
+def _weight(n, k):
+    return to_mx(_randn(n, k, seed=2, scale=0.05))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(30, 64), (300, 129), (2100, 1000), (8192, 4096), (20000, 8256)])
+def test_bias_gradients_of_a_recorded_step(m, n):
+    """Replayed on other gradients, with eager calls between the replays: every replay gives what the call gives."""
+    w, bias = _weight(n, 64), _randn(n, seed=3).requires_grad_()
+    x, gy = _randn(m, 64, seed=4), _randn(m, n, seed=5)
+    layer = None
+    if n % 64 == 0:
+        with torch.device(DEV):
+            layer = MXLoRALinear(64, n, 8, 16.0, use_bias=True).to(BF)
+
+    def run():
+        grads = list(torch.autograd.grad(linear_mx(x, w, bias), [bias], gy))
+        if layer is not None:
+            grads += torch.autograd.grad(layer(x), [layer.bias, layer.lora_b.weight], gy)
+        return grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = run()
+    for turn in range(4):
+        gy.copy_(_randn(m, n, seed=10 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in recorded]
+        exact = gy.double().sum(0)
+        assert bool(((got[0].double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 2.0 ** -16 * gy.double().abs().sum(0)).all()), turn
+        for a, b in zip(got, run()):
+            assert torch.equal(a, b), turn
+
+
+def test_column_sum_refusals():
+    """Addresses that are never read: every call below is turned away by its checks."""
+    lib = _lib.load()
+    p, odd = ctypes.c_void_p(1 << 12), ctypes.c_void_p((1 << 12) + 2)
+    call = lambda x=p, out=p, m=400, n=64, ws=p, size=1 << 40: lib.ttamd_column_sum_bf16(x, out, m, n, ws, size, None)
+    need = lib.ttamd_column_sum_workspace_bytes(400, 64)
+    assert need > 0 and lib.ttamd_column_sum_workspace_bytes(3, 64) == 0 and lib.ttamd_column_sum_workspace_bytes(0, 64) == 0
+    for want, got in ((-1, call(x=odd)), (-1, call(x=None)), (-1, call(out=None)), (-1, call(out=ctypes.c_void_p(4097))), (-1, call(m=-1)), (-2, call(n=1 << 29)),
+                      (-3, call(size=need - 1)), (-3, call(ws=None)), (-3, call(ws=odd)), (0, call(n=0))):
+        assert got == want, lib.ttamd_last_error()

@@ -212,6 +212,8 @@ SIGNATURES = {
     "ttamd_mx_lora_bwd_workspace_bytes": (_size, [_c_void_p, _int, _i64, _i64]),
     "ttamd_mx_lora_bwd_bf16": (
         _int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_column_sum_workspace_bytes": (_size, [_i64, _i64]),
+    "ttamd_column_sum_bf16": (_int, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
     "ttamd_swiglu_bwd_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 

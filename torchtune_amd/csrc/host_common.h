@@ -40,6 +40,17 @@ inline Tensor scratch(size_t bytes, const Tensor& like) {
 
 inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
+// The gradient of a bias: the sum over the rows of gy [M, N], contiguous bf16 on the current device.  (torch's own sum clears
+// counters by a memset where it cuts the rows, and a recorded one has given wrong sums on replays after the first.)
+inline Tensor column_sum(const Tensor& gy) {
+  const int64_t M = gy.size(0), N = gy.size(1);
+  Tensor out = at::empty({N}, gy.options());
+  const size_t bytes = ttamd_column_sum_workspace_bytes(M, N);
+  const Tensor ws = bytes ? scratch(bytes, gy) : Tensor();
+  check(ttamd_column_sum_bf16(gy.data_ptr(), out.data_ptr(), M, N, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(gy)), "column_sum");
+  return out;
+}
+
 // True when the call has to be a node: something is differentiated backward, or carries a forward-mode tangent (the node
 // then raises: none of them has a forward-mode rule, and a plain call would drop the tangent).
 inline bool wants_grad(std::initializer_list<const Tensor*> ts) {

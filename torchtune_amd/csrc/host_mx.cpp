@@ -135,7 +135,7 @@ struct LinearMXFn : torch::autograd::Function<LinearMXFn> {
               "linear_mx");
       }
     }
-    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) gbias = gy.sum(0);
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) gbias = column_sum(gy);
     return {gx, Tensor(), Tensor(), gbias, Tensor()};
   }
 };
@@ -274,7 +274,7 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
     for (int i = 0; i < n; ++i) {
       out.push_back(ga[i]);
       out.push_back(gb[i]);
-      if (bias[i]) out.push_back(gys[i].sum(0));
+      if (bias[i]) out.push_back(column_sum(gys[i]));
     }
     out.push_back(Tensor());
     return out;
