@@ -832,7 +832,7 @@ int ttamd_mx_linear_dx_bf16(const void* gy, const uint8_t* w_codes, const uint8_
  * TTAMD_GROUP_MAX linears that read the same input x [M, K] bf16:
  *   forward:  x^ = mxfp8(x);  h_i = x^ . lora_a_i^T;  y_i = x^ . W_i^T (+ bias_i) + scale_i . h_i . lora_b_i^T
  *   backward: gh_i = scale_i . gy_i . lora_b_i;  grad_lora_a_i = gh_i^T . x^;  grad_lora_b_i = scale_i . gy_i^T . h_i;
- *             gx = sum_i gy_i . W_i + gh_i . lora_a_i  (NULL: not wanted)
+ *             gx = sum_i gy_i . W_i + gh_i . lora_a_i  (NULL: not wanted; the adapters' gradients NULL for all members: likewise)
  * kept_codes (ttamd_mx_kept_codes_bytes) and kept_scales (ttamd_mx_kept_scales_bytes) are x^, written by the forward and read
  * by the backward, in a layout of this library's own; h_cat, gh_cat bf16 [M, sum of ranks], the members side by side.
  * K % 64 == 0, N % 64 == 0, N < 2^22 (their sum 2^23), ranks multiples of 8 that add up to at most 64.  Pointers 16-byte

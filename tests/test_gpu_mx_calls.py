@@ -1,0 +1,84 @@
+"""Calls of the microscaled linears that their documentation allows: which gradients a backward pass forms, ranks of groups,
+checkpoints, every code with every scale.  Bounds as in ``test_gpu_mx.py``."""
+import pytest
+import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from oracle import mx_oracle as ox
+from torchtune_amd import MXLoRALinear, MXTensor, lora_linear_mx
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+DEV = "cuda"
+HALF, SUMS, SUMS_FP8 = 2.0 ** -8, 2.0 ** -16, 7 * 2.0 ** -13
+
+
+def _gen(n):
+    return torch.Generator().manual_seed(n)
+
+
+def _randn(*shape, seed, scale=1.0):
+    return (torch.randn(*shape, generator=_gen(seed)) * scale).to(BF).to(DEV)
+
+
+def _layer(k, n, r=8, seed=0, bias=False):
+    with torch.device(DEV):
+        m = MXLoRALinear(k, n, r, 2.0 * r, use_bias=bias).to(BF)
+    with torch.no_grad():
+        m.set_weight(_randn(n, k, seed=seed, scale=0.05))
+        m.lora_a.weight.copy_(_randn(r, k, seed=seed + 1, scale=k ** -0.5))
+        m.lora_b.weight.copy_(_randn(n, r, seed=seed + 2, scale=0.05))
+        if bias:
+            m.bias.copy_(_randn(n, seed=seed + 3))
+    return m
+
+
+class _Allocations(TorchDispatchMode):
+    """sizes of the tensors that a pass allocates"""
+
+    def __init__(self):
+        super().__init__()
+        self.sizes = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if func.overloadpacket.__name__.startswith(("empty", "sum")):
+            self.sizes.append(tuple(out.shape))
+        return out
+
+
+@pytest.mark.parametrize("m,n", [(30, 64), (1100, 8192), (2500, 192)])
+def test_gradients_that_nobody_asks_for_are_not_formed(m, n):
+    """A frozen bias, the usual one, costs no pass over the output's gradient, frozen adapters none for theirs; what is
+    formed has the same bits."""
+    layer, x, gy = _layer(128, n, 8, seed=1, bias=True), _randn(m, 128, seed=2).requires_grad_(), _randn(m, n, seed=3)
+    a, b, bias = layer.lora_a.weight, layer.lora_b.weight, layer.bias
+    every = dict(zip("xabc", torch.autograd.grad(layer(x), [x, a, b, bias], gy)))
+    shapes = dict(a=tuple(a.shape), b=tuple(b.shape), c=tuple(bias.shape))
+    for want in ("x", "ab", "xab", "c", "xc", "a", "xb"):
+        for name, p in zip("xabc", (x, a, b, bias)):
+            p.requires_grad_(name in want)
+        y = layer(x)
+        with _Allocations() as seen:
+            got = torch.autograd.grad(y, [p for name, p in zip("xabc", (x, a, b, bias)) if name in want], gy)
+        for name, g in zip([c for c in "xabc" if c in want], got):
+            assert torch.equal(g, every[name]), (want, name)
+        assert (shapes["c"] in seen.sizes) == ("c" in want), (want, seen.sizes)
+        assert (shapes["a"] in seen.sizes) == (shapes["b"] in seen.sizes) == ("a" in want or "b" in want), (want, seen.sizes)
+
+
+def test_bias_gradients_of_a_group_go_to_their_members():
+    """Some members with a bias, some of those frozen."""
+    layers = [_layer(64, n, 8, seed=10 * i, bias=i != 1) for i, n in enumerate((64, 128, 192, 64))]
+    layers[2].bias.requires_grad_(False)
+    x, gys = _randn(200, 64, seed=5), [_randn(200, l.out_dim, seed=6 + i) for i, l in enumerate(layers)]
+    ys = lora_linear_mx(x, [l.mx_weight for l in layers], [l.lora_a.weight for l in layers], [l.lora_b.weight for l in layers], [2.0] * 4,
+                        [l.bias for l in layers])
+    torch.autograd.backward(ys, gys)
+    for i, (l, g) in enumerate(zip(layers, gys)):
+        if i in (0, 3):
+            want = g.double().sum(0)
+            assert bool(((l.bias.grad.double() - want).abs() <= HALF * want.abs() + SUMS * g.double().abs().sum(0)).all())
+        else:
+            assert l.bias is None or l.bias.grad is None
+        assert l.lora_a.weight.grad is not None and l.lora_b.weight.grad is not None

@@ -196,3 +196,23 @@ def test_c_entries_refuse_before_they_launch():
         assert call() == want, (i, lib.ttamd_last_error())
     assert lib.ttamd_mx_linear_workspace_bytes(0, 1, 64, 8) == 0 and lib.ttamd_mx_lora_fwd_workspace_bytes(*ptr(member(rank=4)), 4, 64) == 0
     assert lib.ttamd_mx_kept_codes_bytes(3, 320) == 3 * 512 and lib.ttamd_mx_kept_scales_bytes(3, 320) == 3 * 16
+
+
+def test_backward_entry_refuses_adapter_gradients_that_are_null_for_some():
+    """All of them null: not wanted.  One of them: a mistake, of whichever member."""
+    import ctypes
+
+    from torchtune_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(1 << 12)
+
+    def bwd(size, *grads):
+        arr = (_lib.MxLoraMember * len(grads))(*(_lib.MxLoraMember(codes=1 << 12, scales=1 << 12, lora_a=1 << 12, lora_b=1 << 12, y=1 << 12, grad_lora_a=a,
+                                                                    grad_lora_b=b, N=128, rank=8, scale=1.0) for a, b in grads))
+        return lib.ttamd_mx_lora_bwd_bf16(p, p, p, ctypes.cast(arr, ctypes.c_void_p), len(grads), p, p, 4, 64, p, size, None)
+
+    q = 1 << 12
+    for grads in (((None, q),), ((q, None),), ((q, q), (None, None)), ((None, None), (q, q)), ((q, q), (q, None)), ((q + 2, q),)):
+        assert bwd(1 << 40, *grads) == -1, grads
+    for grads in (((None, None),), ((None, None), (None, None))):
+        assert bwd(0, *grads) == -3 and b"workspace" in lib.ttamd_last_error()  # past the members' checks

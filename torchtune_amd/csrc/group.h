@@ -158,7 +158,7 @@ struct SwigluBwdInputs {
   const uint16_t* gate;  // [M, N]
   const uint16_t* up;    // [M, N]
 };
-// x may be null where the group's input is kept in 8 bits
+// x may be null where the group's input is kept in 8 bits; ga and gb all null: the adapters' gradients are not wanted
 int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkinny& g, uint16_t* gh_cat, float* ws, hipStream_t s,
                        const SwigluBwdInputs* sw = nullptr);
 

@@ -244,6 +244,15 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
     std::vector<Tensor> gys(n), ga(n), gb(n);
     std::vector<MxMember> ms(n);
     ttamd_mx_lora_member arr[TTAMD_GROUP_MAX];
+    // what is wanted: x's gradient, any adapter's, and which of the biases'
+    const bool need_x = ctx->needs_input_grad(0);
+    bool need_ab = false, need_bias[TTAMD_GROUP_MAX] = {};
+    size_t edge = 1;
+    for (int i = 0; i < n; ++i) {
+      need_ab = need_ab || ctx->needs_input_grad(edge) || ctx->needs_input_grad(edge + 1);
+      edge += 2;
+      if (bias[i]) need_bias[i] = ctx->needs_input_grad(edge++);
+    }
     for (int i = 0; i < n; ++i) {
       MxMember& m = ms[i];
       m.codes = dense(saved[1 + 4 * i]);
@@ -253,16 +262,16 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
       m.scale = factors[i];
       ranks += m.a.size(0);
       gys[i] = dense(g[i]).reshape({M, m.codes.size(0)});
+      fill(arr[i], m, gys[i]);
+      if (!need_ab) continue;
       ga[i] = M ? at::empty_like(m.a) : at::zeros_like(m.a);
       gb[i] = M ? at::empty_like(m.b) : at::zeros_like(m.b);
-      fill(arr[i], m, gys[i]);
       arr[i].grad_lora_a = ga[i].data_ptr();
       arr[i].grad_lora_b = gb[i].data_ptr();
     }
-    const bool need_x = ctx->needs_input_grad(0);
     Tensor gx;
     if (need_x) gx = at::empty(shape, gys[0].options());
-    if (M) {
+    if (M && (need_x || need_ab)) {
       const Kept at(M, K, ranks);
       const uint8_t* k = (const uint8_t*)kept.data_ptr();
       const size_t bytes = ttamd_mx_lora_bwd_workspace_bytes(arr, n, M, K), gh = align256(bytes);  // the gradient of h behind the workspace
@@ -274,7 +283,7 @@ struct LoraMXFn : torch::autograd::Function<LoraMXFn> {
     for (int i = 0; i < n; ++i) {
       out.push_back(ga[i]);
       out.push_back(gb[i]);
-      if (bias[i]) out.push_back(column_sum(gys[i]));
+      if (bias[i]) out.push_back(need_bias[i] ? column_sum(gys[i]) : Tensor());
     }
     out.push_back(Tensor());
     return out;

@@ -1727,6 +1727,7 @@ size_t group_lora_bwd_ws_bytes(const GroupSkinny& g) {
 int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkinny& g, uint16_t* gh_cat, float* ws, hipStream_t s,
                        const SwigluBwdInputs* sw) {
   const int rt = g.r_off[g.n];
+  const bool adapters = g.ga[0] != nullptr;  // else gh alone, to the same bits: the input's gradient needs it
   // the pair's gradients from the pass that reads them (swiglu_bwd_tn_gh_kernel) where that pass exists
   const bool sw_fused = sw && tn_gh_pair(g) && tn_gh_applies(g);
   if (sw) {
@@ -1783,6 +1784,7 @@ int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkin
     }
     sum_partials_kernel<<<dim3((unsigned)((g.M * 16 + 255) / 256), (unsigned)g.n), dim3(256), 0, s>>>(sums);
     if (int rc = check_launch("skinny_tn_gh")) return rc;
+    if (!adapters) return TTAMD_OK;
     TnBatch t = {};
     t.M = (int)g.M;
     t.p[0] = TnProblem{gh_cat, x, nullptr, (int)g.K, rt, rt};
@@ -1810,6 +1812,7 @@ int run_group_lora_bwd(const uint16_t* x, const uint16_t* h_cat, const GroupSkin
     }
     if (int rc = run_nt_batch(b, g.n, true, ws, s)) return rc;
   }
+  if (!adapters) return TTAMD_OK;
   TnBatch t = {};
   t.M = (int)g.M;
   t.p[0] = TnProblem{gh_cat, x, nullptr, (int)g.K, rt, rt};

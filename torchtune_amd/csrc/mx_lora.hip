@@ -28,6 +28,8 @@ int decode(const char* who, const ttamd_mx_lora_member* m, int n, int64_t M, int
   d.sk.M = d.dx.M = M;
   d.sk.K = d.dx.K = K;
   int r = 0;
+  bool adapters = false;  // none of their gradients wanted: all of the pointers are null
+  for (int i = 0; i < n; ++i) adapters = adapters || m[i].grad_lora_a || m[i].grad_lora_b;
   for (int i = 0; i < n; ++i) {
     TT_REQUIRE(m[i].N > 0 && m[i].N % 64 == 0, "%s: member %d: N (%lld) must be a positive multiple of 64", who, i, (long long)m[i].N);
     TT_REQUIRE(m[i].rank > 0 && m[i].rank % 8 == 0, "%s: member %d: the rank (%d) must be a positive multiple of 8", who, i, m[i].rank);
@@ -36,8 +38,8 @@ int decode(const char* who, const ttamd_mx_lora_member* m, int n, int64_t M, int
     TT_REQUIRE(m[i].codes && m[i].scales && m[i].lora_a && m[i].lora_b && m[i].y && aligned16(m[i].codes) && aligned16(m[i].scales) &&
                    aligned16(m[i].lora_a) && aligned16(m[i].lora_b) && aligned16(m[i].y) && (reinterpret_cast<uintptr_t>(m[i].bias) & 1u) == 0,
                "%s: member %d: pointers must be non-null and 16-byte aligned", who, i);
-    TT_REQUIRE(!backward || (m[i].grad_lora_a && m[i].grad_lora_b && aligned16(m[i].grad_lora_a) && aligned16(m[i].grad_lora_b)),
-               "%s: member %d: the adapter gradients must be non-null and 16-byte aligned", who, i);
+    TT_REQUIRE(!backward || !adapters || (m[i].grad_lora_a && m[i].grad_lora_b && aligned16(m[i].grad_lora_a) && aligned16(m[i].grad_lora_b)),
+               "%s: member %d: the adapter gradients must be non-null (or null for all members) and 16-byte aligned", who, i);
     d.codes[i] = m[i].codes;
     d.scales[i] = m[i].scales;
     d.sk.N[i] = d.dx.N[i] = m[i].N;
