@@ -4,8 +4,7 @@ import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from oracle import mx_oracle as ox
-from torchtune_amd import MXLoRALinear, MXTensor, lora_linear_mx
+from torchtune_amd import FrozenMXLinear, MXLoRALinear, linear_mx, lora_linear_mx, to_mx
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -82,3 +81,36 @@ def test_bias_gradients_of_a_group_go_to_their_members():
         else:
             assert l.bias is None or l.bias.grad is None
         assert l.lora_a.weight.grad is not None and l.lora_b.weight.grad is not None
+
+
+# ---- checkpoints -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_a_module_on_the_meta_device_takes_a_dense_checkpoint(where, dtype):
+    """Built without memory and given its tensors by ``assign=True``, as large checkpoints are loaded."""
+    full = _layer(128, 64, 8, seed=20, bias=True)
+    state = {"weight": _randn(64, 128, seed=21).to(dtype).to(where), "bias": full.bias.detach().to(where),
+             "lora_a.weight": full.lora_a.weight.detach().to(where), "lora_b.weight": full.lora_b.weight.detach().to(where)}
+    with torch.device("meta"):
+        layer, frozen = MXLoRALinear(128, 64, 8, 16.0, use_bias=True), FrozenMXLinear(128, 64, bias=True)
+    layer.load_state_dict(state, assign=True)
+    frozen.load_state_dict({"weight": state["weight"], "bias": state["bias"]}, assign=True)
+    assert set(state) == {"weight", "bias", "lora_a.weight", "lora_b.weight"}
+    want = to_mx(state["weight"].float().to(DEV))
+    for m in (layer, frozen):
+        assert m.weight_codes.device.type == where and torch.equal(m.weight_codes.to(DEV), want.codes) and torch.equal(m.weight_scales.to(DEV), want.scales)
+    x = _randn(20, 128, seed=22)
+    full.load_state_dict(state)
+    assert torch.equal(layer.to(DEV)(x), full(x)) and torch.equal(frozen.to(DEV)(x), linear_mx(x, want, full.bias))
+    with torch.device("meta"):
+        again = MXLoRALinear(128, 64, 8, 16.0, use_bias=True)
+    again.load_state_dict(full.state_dict(), assign=True)  # and its own form
+    assert torch.equal(again(x), full(x))
+
+
+def test_a_meta_module_loads_a_meta_checkpoint():
+    with torch.device("meta"):
+        m = MXLoRALinear(128, 64, 8, 16.0)
+        state = {"weight": torch.empty(64, 128), "lora_a.weight": torch.empty(8, 128), "lora_b.weight": torch.empty(64, 8)}
+    m.load_state_dict(state, assign=True)
+    assert m.weight_codes.device.type == "meta" and tuple(m.mx_weight.shape) == (64, 128)

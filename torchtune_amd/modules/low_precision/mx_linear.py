@@ -48,6 +48,18 @@ class MXWeight(nn.Module):
         self.weight_codes.copy_(packed.codes)
         self.weight_scales.copy_(packed.scales)
 
+    def _quantise_for_loading(self, dense: torch.Tensor):
+        """Codes and scales of a checkpoint's dense weight, on the module's device.  A module on the meta device has none to
+        offer: its weight stays where the checkpoint's lies (``load_state_dict(..., assign=True)`` puts it there)."""
+        here = self.weight_codes.device
+        if here.type != "meta":
+            packed = _pack(dense.to(here))
+            return packed.codes, packed.scales
+        if dense.device.type == "meta":
+            return self.weight_codes, self.weight_scales
+        packed = _pack(dense if dense.is_cuda else dense.to("cuda"))
+        return packed.codes.to(dense.device), packed.scales.to(dense.device)
+
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         dense = state_dict.get(prefix + "weight")
         if dense is None:
@@ -60,8 +72,8 @@ class MXWeight(nn.Module):
                               f"shape in current model is {tuple(self.mx_weight.shape)}.")
             state_dict[prefix + "weight_codes"], state_dict[prefix + "weight_scales"] = self.weight_codes, self.weight_scales
         else:
-            packed = _pack(dense.detach().to(self.weight_codes.device))
-            state_dict[prefix + "weight_codes"], state_dict[prefix + "weight_scales"] = packed.codes, packed.scales
+            codes, scales = self._quantise_for_loading(dense.detach())
+            state_dict[prefix + "weight_codes"], state_dict[prefix + "weight_scales"] = codes, scales
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
 
