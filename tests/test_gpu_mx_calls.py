@@ -4,7 +4,8 @@ import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from torchtune_amd import FrozenMXLinear, MXLoRALinear, linear_mx, lora_linear_mx, to_mx
+from torchtune_amd import FrozenMXLinear, MXLoRALinear, MXTensor, linear_mx, lora_linear_mx, to_mx
+from torchtune_amd.modules.peft import get_merged_lora_ckpt
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -114,3 +115,29 @@ def test_a_meta_module_loads_a_meta_checkpoint():
         state = {"weight": torch.empty(64, 128), "lora_a.weight": torch.empty(8, 128), "lora_b.weight": torch.empty(64, 8)}
     m.load_state_dict(state, assign=True)
     assert m.weight_codes.device.type == "meta" and tuple(m.mx_weight.shape) == (64, 128)
+
+
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+@pytest.mark.parametrize("dtype,half", [(torch.float16, 2.0 ** -11), (torch.float32, 2.0 ** -24), (torch.float64, 2.0 ** -53)])
+def test_merging_adapters_of_other_types(dtype, half, where):
+    """The merged weight has the adapters' type, whatever it is; what is merged is the weight's value."""
+    m = _layer(128, 64, 8, seed=30)
+    w = MXTensor(m.weight_codes, m.weight_scales).to(torch.float32).double().cpu()
+    a, b = m.lora_a.weight.detach().to(dtype), m.lora_b.weight.detach().to(dtype)
+    state = {"l.weight_codes": m.weight_codes, "l.weight_scales": m.weight_scales, "l.lora_a.weight": a, "l.lora_b.weight": b}
+    merged = get_merged_lora_ckpt({k: v.to(where) for k, v in state.items()}, rank=8, alpha=16.0)
+    assert set(merged) == {"l.weight"} and merged["l.weight"].dtype == dtype and merged["l.weight"].device.type == where
+    scaled, a = 2.0 * b.double().cpu(), a.double().cpu()
+    # w is exact (fp16: values from 2^-14 on, fewer bits below, a half step 2^-25); eight products with their sums and the last sum are rounded
+    lost = 9 * half * (scaled.abs() @ a.abs()) + (2.0 ** -25 if dtype == torch.float16 else 0.0) * 3
+    err = (merged["l.weight"].double().cpu() - (w + scaled @ a)).abs()
+    assert bool((err <= half * (w + scaled @ a).abs() + 1.01 * lost).all())
+
+
+def test_merging_leaves_what_it_cannot_merge():
+    m = _layer(128, 64, 8, seed=31)
+    state = {f"l.{k}": v for k, v in m.state_dict().items() if k != "weight_scales"}
+    keys = set(state)
+    with pytest.raises(KeyError):
+        get_merged_lora_ckpt(state, rank=8, alpha=16.0)
+    assert set(state) == keys

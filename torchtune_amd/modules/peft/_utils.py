@@ -100,12 +100,15 @@ def get_merged_lora_ckpt(state_dict: Dict[str, Any], rank: int, alpha: float, us
             raise NotImplementedError(f"{module}: merging MoE experts is not part of this build")
         a = state_dict[f"{module}.lora_a.weight"]
         b = state_dict[f"{module}.lora_b.weight"]
-        codes = state_dict.pop(f"{module}.weight_codes", None)  # an mxfp4 base weight: the merged one is dense
+        codes = state_dict.get(f"{module}.weight_codes", None)  # an mxfp4 base weight: the merged one is dense
         if codes is None:
             w = state_dict[f"{module}.weight"]
         else:  # read back on the GPU, also out of a state dict that has left it
             device = codes.device if codes.is_cuda else torch.device("cuda")
-            w = MXTensor(codes.to(device), state_dict.pop(f"{module}.weight_scales").to(device)).to(a.dtype).to(a.device)
+            w = MXTensor(codes.to(device), state_dict[f"{module}.weight_scales"].to(device))
+            w = w.to(a.dtype if a.dtype == torch.bfloat16 else torch.float32).to(device=a.device, dtype=a.dtype)
+            # what cannot be read back stays in the dictionary
+            del state_dict[f"{module}.weight_codes"], state_dict[f"{module}.weight_scales"]
         magnitude = state_dict.get(f"{module}.magnitude", None)
         fused = (
             isinstance(w, NF4Tensor) and w.is_cuda and w.block_size == 64 and w.dtype == torch.bfloat16
