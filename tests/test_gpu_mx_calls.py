@@ -141,3 +141,37 @@ def test_merging_leaves_what_it_cannot_merge():
     with pytest.raises(KeyError):
         get_merged_lora_ckpt(state, rank=8, alpha=16.0)
     assert set(state) == keys
+
+
+# ---- precision -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("factor", [0.75, 1.7, 0.1, 16.0 / 24.0, -3.3])
+@pytest.mark.parametrize("m,outs", [(1, [64]), (40, [1024]), (333, [4096]), (700, [1024, 64]), (2600, [4096]), (2600, [4096, 1024])])
+def test_the_factor_of_an_adapter_adds_no_rounding(m, outs, factor):
+    """Inputs with a single one, a zero weight and one rank in use: h is an element of lora_a, exactly, and an output factor * h *
+    an element of lora_b.  It is rounded once; the factor is held in fp32 (2^-24) and its product with h in 16 bits (2^-17)."""
+    k, r = 128, 64 // len(outs)
+    g = _gen(40)
+    x, at = torch.zeros(m, k), torch.randint(0, k, (m,), generator=g)
+    x[torch.arange(m), at] = 1.0
+    w = [MXTensor(torch.zeros(n, k // 2, dtype=torch.uint8, device=DEV), torch.full((n, k // 32), 127, dtype=torch.uint8, device=DEV)) for n in outs]
+    a, b = [torch.zeros(r, k) for _ in outs], [torch.randn(n, r, generator=g) for n in outs]
+    for t in a:
+        t[r - 3] = torch.randn(k, generator=g)
+    a, b = [t.to(BF) for t in a], [t.to(BF) for t in b]
+    ys = lora_linear_mx(x.to(BF).to(DEV), w, [t.to(DEV) for t in a], [t.to(DEV) for t in b], [factor] * len(outs))
+    for y, a, b in zip(ys, a, b):
+        want = factor * a[r - 3, at].double().view(-1, 1) * b[:, r - 3].double()
+        err = (y.double().cpu() - want).abs()
+        assert bool((err <= (HALF + 2.0 ** -16) * want.abs()).all())
+
+
+def test_adapters_with_infinite_activations():
+    """What is infinite stays infinite, of either sign, and does not become a NaN on the way."""
+    k = 64
+    w = MXTensor(torch.zeros(64, k // 2, dtype=torch.uint8, device=DEV), torch.full((64, k // 32), 127, dtype=torch.uint8, device=DEV))
+    x = torch.zeros(30, k)
+    x[:, 3] = 2.0 ** 100
+    a, b = torch.zeros(8, k), torch.zeros(64, 8)
+    a[1, 3], b[:, 1] = 2.0 ** 27, torch.where(torch.arange(64) % 2 == 0, 1.0, -1.0)
+    y, = lora_linear_mx(x.to(BF).to(DEV), [w], [a.to(BF).to(DEV)], [b.to(BF).to(DEV)], [8.0])  # h is 2^127, its product is not finite
+    assert bool(torch.isinf(y).all()) and bool((torch.signbit(y) == (torch.arange(64, device=DEV) % 2 == 1)).all())

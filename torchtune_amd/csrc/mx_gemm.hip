@@ -366,14 +366,15 @@ __global__ __launch_bounds__(512) void mx_gemm_kernel(const MxGemmArgs g) {
       }
     }
   };
-  // adapter: s . h . B^T as further contraction steps of 32 ranks, the factor rounded into h's side
+  // adapter: s . h . B^T as further contraction steps of 32 ranks.  s . h goes in as the sum of two bf16 numbers, 16 bits of it:
+  // rounded to one it is a second rounding of h (no error for a factor that is a power of two, up to half a step for others)
   auto adapt = [&]() TT_INLINE {
     const int lane = fresh(threadIdx.x & 63), r16 = lane & 15, quarter = lane >> 4, ar = 16 * TM * wm + r16, wr = 16 * TN * wn + r16;
     const MxGemmMember& w = g.m[GROUP ? it.mem : 0];
     const int rank = w.rank, N = w.N;
     for (int r0 = 0; r0 < rank; r0 += 32) {
       const int r = r0 + 8 * quarter;
-      bf16x8_t hx[TM];
+      bf16x8_t hx[TM], hx_low[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         int row = it.m0 + ar + 16 * i;
@@ -381,8 +382,11 @@ __global__ __launch_bounds__(512) void mx_gemm_kernel(const MxGemmArgs g) {
         bf16x8_t v = {};
         if (r < rank) v = *reinterpret_cast<const bf16x8_t*>(w.h + (int64_t)row * g.ldh + r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (__bf16)((float)v[e] * w.lscale);
-        hx[i] = v;
+        for (int e = 0; e < 8; ++e) {
+          const float f = (float)v[e] * w.lscale;
+          hx[i][e] = (__bf16)f;
+          hx_low[i][e] = (__bf16)(__builtin_fabsf(f) < 0x1p127f ? f - (float)hx[i][e] : 0.f);  // infinities stay what they are
+        }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -399,7 +403,10 @@ __global__ __launch_bounds__(512) void mx_gemm_kernel(const MxGemmArgs g) {
 #pragma unroll
         for (int j = 0; j < TH; ++j)
 #pragma unroll
-          for (int i = 0; i < TM; ++i) acc[TH * c + j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[j], hx[i], acc[TH * c + j][i], 0, 0, 0);
+          for (int i = 0; i < TM; ++i) {
+            acc[TH * c + j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[j], hx[i], acc[TH * c + j][i], 0, 0, 0);
+            acc[TH * c + j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bw[j], hx_low[i], acc[TH * c + j][i], 0, 0, 0);
+          }
       }
     }
   };
