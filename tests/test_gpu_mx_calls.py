@@ -175,3 +175,21 @@ def test_adapters_with_infinite_activations():
     a[1, 3], b[:, 1] = 2.0 ** 27, torch.where(torch.arange(64) % 2 == 0, 1.0, -1.0)
     y, = lora_linear_mx(x.to(BF).to(DEV), [w], [a.to(BF).to(DEV)], [b.to(BF).to(DEV)], [8.0])  # h is 2^127, its product is not finite
     assert bool(torch.isinf(y).all()) and bool((torch.signbit(y) == (torch.arange(64, device=DEV) % 2 == 1)).all())
+
+
+@pytest.mark.parametrize("m", [1, 16, 64, 300, 2000])
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+def test_what_a_large_product_leaves_of_small_ones(act, m):
+    """Each token has a large value, a small one and the large one's negative: what is left is the small one, where the sums keep
+    it.  In another eight of the contraction fp32 keeps 2^-23 of it; among the eight neighbours of an mxfp8 input 2^-13."""
+    k = 512
+    w = to_mx(torch.ones(64, k, device=DEV))
+    for near, steps in ((False, range(1, 24)), (True, range(1, 14))):
+        if near and act == "mxfp4":
+            continue  # one block: its elements span less than that
+        for at in ((1, 2, 5, 7) if near else (32, 40, 64, 127, 128, 300)):
+            for e in steps:
+                x = torch.zeros(m, k)
+                x[:, 0], x[:, at], x[:, 256] = 256.0, 256.0 * 2.0 ** -e, -256.0
+                y = linear_mx(x.to(BF).to(DEV), w, activation=act)
+                assert bool((y == 256.0 * 2.0 ** -e).all()), (near, at, e)
