@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
+from oracle import mx_oracle as ox
 from torchtune_amd import FrozenMXLinear, MXLoRALinear, MXTensor, linear_mx, lora_linear_mx, to_mx
 from torchtune_amd.modules.peft import get_merged_lora_ckpt
 
@@ -193,3 +194,17 @@ def test_what_a_large_product_leaves_of_small_ones(act, m):
                 x[:, 0], x[:, at], x[:, 256] = 256.0, 256.0 * 2.0 ** -e, -256.0
                 y = linear_mx(x.to(BF).to(DEV), w, activation=act)
                 assert bool((y == 256.0 * 2.0 ** -e).all()), (near, at, e)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_every_code_with_every_scale_reads_back_rounded_once(fmt, dtype):
+    """Down to the products that are subnormal and up to those that are infinite, to the bit; the scale 255 is NaN whatever the code."""
+    n = 16 if fmt == "mxfp4" else 256
+    codes = torch.arange(n, dtype=torch.uint8)
+    codes = torch.where(codes % 128 == 127, 0, codes) if fmt == "mxfp8" else codes.repeat(2)  # e4m3's NaN comes out of no quantiser
+    codes = codes.to(torch.uint8).expand(256, -1).contiguous()
+    scales = torch.arange(256, dtype=torch.uint8).view(-1, 1).expand(-1, codes.shape[1] // 32).contiguous()
+    got = MXTensor(ox.pack(codes, fmt).to(DEV), scales.to(DEV), format=fmt).to(dtype).cpu()
+    want = ox.values(codes, scales, fmt).to(dtype)
+    assert bool(torch.isnan(got[255]).all()) and torch.equal(got[:255], want[:255]) and torch.equal(torch.signbit(got[:255]), torch.signbit(want[:255]))

@@ -92,7 +92,7 @@ __device__ __forceinline__ mx_u32x2 mx_pack8(const float (&v)[8], float s) {
   return mx_u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
-// the four bf16 pairs of one dword of fp4 codes / two dwords of fp8 codes (exact above bf16's subnormals)
+// the four bf16 pairs of one dword of fp4 codes / two dwords of fp8 codes: exact, or among bf16's subnormals rounded once
 __device__ __forceinline__ mx_u32x4 mx_bf16_of_fp4(uint32_t c, float s) {
   mx_u32x4 o;
   o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));
