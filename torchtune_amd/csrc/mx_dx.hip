@@ -72,7 +72,7 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
   const int s_begin = slice * g.steps_per_slice;
   const int s_end = s_begin + g.steps_per_slice < g.steps ? s_begin + g.steps_per_slice : g.steps;
 
-  // ---- requests.  Buffer loads: rows beyond M, columns beyond K and steps beyond the slice read zeros (a scale of zero is
+  // ---- requests.  Buffer loads: rows beyond M and steps beyond the slice read zeros (a scale of zero is
   //      2^-127, and gy's rows are zero with it)
   const uint32_t lds0 = (uint32_t)(uintptr_t)TT_LDS_PTR(smem);
   auto dma16 = [&](uint32_t off, const void* base, int bytes, uint32_t lds) {
@@ -114,9 +114,8 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
       dma16((off ^ ((q & 1) ? 64u : 0u)) + (uint32_t)(q * 8) * (uint32_t)(2 * N), gy_at + n, more ? rows * 2 * N - 2 * n : 0,
             st + q * 1024);
     }
-    // codes: 8 rows of 64 bytes per wave by its first 32 lanes (the others read nothing, into the next rows' place of the
-    // same wave: 16 rows' room); scales: a dword for each of its 8 rows
-    const uint32_t c_off = lane < 32 && c0 + 32 * (lane & 3) < g.K ? (uint32_t)(8 * wave + (lane >> 2)) * (uint32_t)(g.K / 2) + 16u * (lane & 3) : 0x7fffffffu;
+    // codes: 8 rows of 64 bytes per wave by its first 32 lanes; scales: a dword for each of its 8 rows (K is a multiple of kBC)
+    const uint32_t c_off = (uint32_t)(8 * wave + (lane >> 2)) * (uint32_t)(g.K / 2) + 16u * (lane & 3);
     if (lane < 32)
       dma16(c_off, codes_at + (int64_t)n * (g.K / 2), more ? kStep * (g.K / 2) - c0 / 2 : 0, st + T::kGy + wave * 512);
     const uint32_t s_off = lane < 8 ? (uint32_t)(8 * wave + lane) * (uint32_t)(g.K / 32) : 0x7fffffffu;
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
     int which = 0, first = 0;
     while (which + 1 < g.members && r >= g.rank_end[which]) first = g.rank_end[which++];
     mx_u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    if (r < g.ldgh && c0 + 16 * part < g.K) {
+    if (r < g.ldgh) {
       const mx_u32x4* p = reinterpret_cast<const mx_u32x4*>(g.la[which] + (int64_t)(r - first) * g.K + c0 + 16 * part);
       lo = p[0];
       hi = p[1];
@@ -252,7 +251,7 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
 #pragma unroll
       for (int j = 0; j < TC; ++j) {
         const int c = c0 + 16 * (TC * wc + j) + 4 * quarter;
-        if (c < g.K) *reinterpret_cast<v4f*>(g.part + ((int64_t)slice * g.M + row) * g.K + c) = acc[j][i];
+        *reinterpret_cast<v4f*>(g.part + ((int64_t)slice * g.M + row) * g.K + c) = acc[j][i];
       }
     } else {
 #pragma unroll
@@ -262,7 +261,7 @@ __global__ __launch_bounds__(512) void mx_dx_kernel(const MxDxArgs g) {
         bf16x4_t o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (__bf16)acc[j][i][e];
-        if (c < g.K) *reinterpret_cast<bf16x4_t*>(g.gx + (int64_t)row * g.K + c) = o;
+        *reinterpret_cast<bf16x4_t*>(g.gx + (int64_t)row * g.K + c) = o;
       }
     }
   }
@@ -287,9 +286,9 @@ MxDxPlan plan_dx(int64_t M, int64_t n_total, int64_t K) {
   const float fill = dense_tiles < 256 ? (float)dense_tiles / 256.f : 1.f;
   float best = 6.f + (float)((dense_tiles + 255) / 256) * (float)steps * (0.92f + 0.5f * fill * fill) + (float)n_total * (float)K * 4.6e-7f;
   MxDxPlan p = {0, 1, 0, false};
-  if (K % 128) return p;  // rows of scales are loaded in dwords
+  if (K % kBC) return p;  // whole column tiles, whose rows of scales are dwords
   for (int bm = 64; bm <= 256; bm *= 2) {
-    const int64_t tiles = ((M + bm - 1) / bm) * ((K + kBC - 1) / kBC);
+    const int64_t tiles = ((M + bm - 1) / bm) * (K / kBC);
     for (int64_t slices = 1; slices <= 16; slices *= 2) {
       const int64_t per = (steps + slices - 1) / slices;
       if ((steps + per - 1) / per != slices) continue;
@@ -317,7 +316,7 @@ int launch_dx(MxDxArgs& g, hipStream_t s) {
     if (dev >= 0) attr_set[dev] = true;
   }
   g.tiles_m = (g.M + BM - 1) / BM;
-  g.tiles_c = (g.K + kBC - 1) / kBC;
+  g.tiles_c = g.K / kBC;
   mx_dx_kernel<BM><<<dim3((unsigned)(g.tiles_m * g.tiles_c * g.slices)), dim3(512), T::kLds, s>>>(g);
   return check_launch("mx_dx");
 }
@@ -347,6 +346,7 @@ int run_mx_dx(const GroupDx& d, const uint8_t* const* codes, const uint8_t* cons
     n_total += d.N[i];
   }
   const MxDxPlan p = plan_dx(d.M, n_total, d.K);
+  TT_REQUIRE(p.fused && d.K % kBC == 0, "mx_dx: K (%lld) is taken in whole column tiles of %d", (long long)d.K, kBC);
   g.gh = reinterpret_cast<const uint16_t*>(gh_cat);
   g.gx = reinterpret_cast<uint16_t*>(gx);
   g.part = part;
