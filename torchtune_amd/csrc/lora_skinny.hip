@@ -653,7 +653,11 @@ __device__ __forceinline__ void tn_whole_finish(const f32x4_t (&acc)[RGM][4], co
 }
 #endif
 
-template <int RGM>
+// MX: problem 0's X is the kept 8-bit input.  Every group of ranks that the launch has registers for is multiplied, a narrower
+// problem's zeros included: with a branch about each product the compiler leaves the far side of some without the wait states
+// that the sum's addition needs, in one instantiation or the other as the code around it changes (adapter backward of q, k, v of 4096, 1024 and
+// 1024 outputs, rank 16, 1500 tokens 25.4 us with and without; 4096 x 4096 rank 64 at 1000 21.2).
+template <int RGM, bool MX>
 __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kernel(const TnBatch a, const TnWholeOut o) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(16))) char whole[];
@@ -686,102 +690,7 @@ __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kernel(con
   for (int q = 0; q < RGM; ++q)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[q][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  u32x4_t xv[4], gv[RGM];
-  auto fetch = [&](int m) {  // rows m .. m + 31 into registers
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = m + 8 * u + (lane >> 3);
-      xv[u] = u32x4_t{0, 0, 0, 0};
-      if (row < M) xv[u] = *reinterpret_cast<const u32x4_t*>(xsrc + (int64_t)row * Kc);
-    }
-    const int grow = m + (lane >> 1);
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) {
-      gv[q] = u32x4_t{0, 0, 0, 0};
-      if (grow < M && gcol + 16 * q < R) gv[q] = *reinterpret_cast<const u32x4_t*>(G + (int64_t)grow * ldg + gcol + 16 * q);
-    }
-  };
-  // Beyond 48 ranks the next rows are fetched behind the products, not beside them, which would spill 29 registers (4096 x 4096
-  // rank 64 at 1000 tokens 28.7 us so, 22.9)
-  constexpr bool kAhead = RGM < 4;
-  int m = 32 * wave;
-  if (m < M) fetch(m);
-  for (; m < M; m += 32 * kTnWholeWaves) {
-    // the previous step's reads of this region are complete: they were waited for before its MFMAs
-#pragma unroll
-    for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4_t*>(xdst + 8 * u * kTnWholePitch) = xv[u];
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) *reinterpret_cast<u32x4_t*>(gdst + 1024 * q) = gv[q];  // zeros beyond R
-    if (kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the copy-in has landed (LDS operations of a wave complete in order)
-    u32x2_t ga[RGM], gb[RGM], xa[4], xb[4];
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) {
-      ga[q] = lds_read_tr16(grd, 1024 * q);
-      gb[q] = lds_read_tr16(grd, 1024 * q + 4 * 32);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      xa[e] = lds_read_tr16(xrd, 32 * e);
-      xb[e] = lds_read_tr16(xrd, 32 * e + 4 * kTnWholePitch);
-    }
-    // waits that name the registers they release, so that no use can be scheduled ahead of them
-#pragma unroll
-    for (int q = 0; q < RGM; ++q) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(ga[q]), "+v"(gb[q]));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(xa[e]), "+v"(xb[e]));
-      const u32x4_t xop = {xa[e].x, xa[e].y, xb[e].x, xb[e].y};
-#pragma unroll
-      for (int q = 0; q < RGM; ++q) {
-        if (q < rg) {
-          const u32x4_t gop = {ga[q].x, ga[q].y, gb[q].x, gb[q].y};
-          acc[q][e] += __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, gop), __builtin_bit_cast(bf16x8_t, xop), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        }
-      }
-    }
-    if (!kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
-  }
-  tn_whole_finish<RGM>(acc, a, o, whole, which, R, rg, Kc, c0, wave, lane);
-#endif
-}
-
-// The same with problem 0's X kept in 8 bits.  Every group of ranks is multiplied, G's zeros included: with a branch about each
-// product the compiler let the sums read a product before it had been written (no wait states along the branch).
-template <int RGM>
-__global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kept_kernel(const TnBatch a, const TnWholeOut o) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  extern __shared__ __attribute__((aligned(16))) char whole[];
-  int which = 0;  // uniform over the workgroup
-#pragma unroll
-  for (int q = 0; q < kTnMaxProblems - 1; ++q)
-    if (q < a.n - 1 && (int)blockIdx.x >= a.cg_end[q]) which = q + 1;
-  const TnProblem& P = a.p[which];
-  const uint16_t* __restrict__ G = P.G;
-  const uint16_t* __restrict__ X = P.X;
-  const int Kc = P.Kc, M = a.M, R = P.R, ldg = P.ldg;
-  const int rg = (R + 15) >> 4;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, i = lane & 15;
-  const int c0 = ((int)blockIdx.x - (which ? a.cg_end[which - 1] : 0)) * kTnWholeCols;
-
-  char* my = whole + wave * tn_whole_wave_lds(RGM);
-  // copy-in: X piece, instruction u (0..3): row 8 u + lane / 8, 16-byte chunk lane % 8; G as in skinny_tn
-  const uint16_t* xsrc = X + c0 + 8 * (lane & 7);  // Kc is a multiple of 64
-  char* xdst = my + (lane >> 3) * kTnWholePitch + 16 * (lane & 7);
-  const int gcol = 8 * (lane & 1);  // + 16 q;  R % 8 == 0: a lane's 8 columns are all in or all out
-  char* gdst = my + 32 * kTnWholePitch + (lane >> 1) * 32 + 16 * (lane & 1);  // + 1024 q
-  const uint32_t my_lds = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) void*)my);
-  const uint32_t xrd = my_lds + (8 * g + (i >> 2)) * kTnWholePitch + 8 * (i & 3);
-  const uint32_t grd = my_lds + 32 * kTnWholePitch + (8 * g + (i >> 2)) * 32 + 8 * (i & 3);
-
-  f32x4_t acc[RGM][4];
-#pragma unroll
-  for (int q = 0; q < RGM; ++q)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[q][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // all rows of this wave.  One form a branch: tested inside, both forms' addresses are kept across the loop (57 registers spilled)
+  // all rows of this wave, one form of X a branch
   auto sweep = [&](auto kept_form) __attribute__((always_inline)) {
     constexpr bool kept = decltype(kept_form)::value;
     u32x4_t xv[4], gv[RGM];
@@ -811,8 +720,8 @@ __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kept_kerne
         if (grow < M && gcol + 16 * q < R) gv[q] = *reinterpret_cast<const u32x4_t*>(G + (int64_t)grow * ldg + gcol + 16 * q);
       }
     };
-    // Beyond 48 ranks the next rows are fetched behind the products, not beside them, which would spill 29 registers (4096 x 4096
-    // rank 64 at 1000 tokens 28.7 us so, 22.9)
+    // Beyond 48 ranks the next rows are fetched behind the products, not beside them, which would spill 55 registers (94 where X is
+    // kept in 8 bits)
     constexpr bool kAhead = RGM < 4;
     int m = 32 * wave;
     if (m < M) fetch(m);
@@ -856,8 +765,8 @@ __global__ __launch_bounds__(64 * kTnWholeWaves) void skinny_tn_whole_kept_kerne
       if (!kAhead && m + 32 * kTnWholeWaves < M) fetch(m + 32 * kTnWholeWaves);
     }
   };
-  if (which == 0)
-    sweep(std::true_type{});
+  if (MX && which == 0)
+    sweep(std::integral_constant<bool, MX>{});
   else
     sweep(std::false_type{});
   tn_whole_finish<RGM>(acc, a, o, whole, which, R, rg, Kc, c0, wave, lane);
@@ -1563,7 +1472,7 @@ bool tn_whole_pays(const GroupSkinny& g) { return g.M <= 2048; }
 
 template <int RGM, bool MX>
 int launch_tn_whole(const TnBatch& b, const TnWholeOut& o, hipStream_t s) {
-  const auto kernel = MX ? skinny_tn_whole_kept_kernel<RGM> : skinny_tn_whole_kernel<RGM>;
+  const auto kernel = skinny_tn_whole_kernel<RGM, MX>;
   constexpr int kLds = kTnWholeWaves * tn_whole_wave_lds(RGM);
   static_assert(kLds >= kTnWholeWaves * 16 * 64 * (int)sizeof(float) && kLds <= 160 * 1024, "the sums fit the staging memory");
   static bool set[64] = {};  // the LDS limit is a per-device attribute of the function (a race only repeats the call)
