@@ -1370,15 +1370,15 @@ size_t dense_group_dx_workspace_bytes(const GroupDx& d) {
   return (size_t)d.K * (size_t)n_total * 2;
 }
 
-// The grouped grad-input on weights that lie there as forward tiles, the members' stacked by rows.
-int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles_fwd, hipStream_t s) {
-  int64_t n_total = 0;
+namespace {
+// What every grouped grad-input hands to its launch, whatever its weights: the members' gradients side by side as the contraction,
+// their adapters, and gx.
+DenseArgs group_dx_args(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles) {
   DenseArgs g = {};
   g.nseg = d.n;
   g.nout = 1;
+  int64_t n_total = 0;
   for (int i = 0; i < d.n; ++i) {
-    TT_REQUIRE(aligned16(d.gy[i]) && d.N[i] % 64 == 0, "dense_dx_on_tiles: gradients must be 16-byte aligned and N (%lld) a multiple of 64", (long long)d.N[i]);
-    if (d.M * d.N[i] * 2 >= (int64_t(1) << 32)) return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: gradient %d too large for 32-bit offsets", i);
     n_total += d.N[i];
     g.seg[i].X = d.gy[i];
     g.seg[i].Kc = (int)d.N[i];
@@ -1392,16 +1392,29 @@ int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const 
       a.lscale = 1.0f;
     }
   }
-  TT_REQUIRE(aligned16(tiles_fwd) && aligned16(gx) && d.K % 64 == 0, "dense_dx_on_tiles: tiles and gx must be 16-byte aligned, K (%lld) a multiple of 64", (long long)d.K);
-  if (!(n_total * 2 * 256 < (int64_t(1) << 32) && d.M < (1 << 30) && d.K < (1 << 30)))
-    return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: operands too large for 32-bit offsets");
   g.out[0].C = reinterpret_cast<uint16_t*>(gx);
   g.out[0].n_begin = 0;
   g.out[0].width = (int)d.K;
-  g.Wt = reinterpret_cast<const char*>(tiles_fwd);
+  g.Wt = reinterpret_cast<const char*>(tiles);
   g.M = (int)d.M; g.Nout = (int)d.K; g.Kc = (int)n_total;
   g.lw_row_major = 0;
   g.ldlx = d.r_off[d.n];
+  return g;
+}
+}  // namespace
+
+// The grouped grad-input on weights that lie there as forward tiles, the members' stacked by rows.
+int run_dense_dx_on_tiles(const GroupDx& d, const void* gh_cat, void* gx, const void* tiles_fwd, hipStream_t s) {
+  int64_t n_total = 0;
+  for (int i = 0; i < d.n; ++i) {
+    TT_REQUIRE(aligned16(d.gy[i]) && d.N[i] % 64 == 0, "dense_dx_on_tiles: gradients must be 16-byte aligned and N (%lld) a multiple of 64", (long long)d.N[i]);
+    if (d.M * d.N[i] * 2 >= (int64_t(1) << 32)) return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: gradient %d too large for 32-bit offsets", i);
+    n_total += d.N[i];
+  }
+  TT_REQUIRE(aligned16(tiles_fwd) && aligned16(gx) && d.K % 64 == 0, "dense_dx_on_tiles: tiles and gx must be 16-byte aligned, K (%lld) a multiple of 64", (long long)d.K);
+  if (!(n_total * 2 * 256 < (int64_t(1) << 32) && d.M < (1 << 30) && d.K < (1 << 30)))
+    return fail(TTAMD_EUNSUPPORTED, "dense_dx_on_tiles: operands too large for 32-bit offsets");
+  DenseArgs g = group_dx_args(d, gh_cat, gx, tiles_fwd);
   g.w_tr = 1;
   return launch_dense(g, s);
 }
@@ -1414,9 +1427,6 @@ int run_gemm_dense_group_dx(const GroupDx& d, const void* gh_cat, void* gx, void
   TT_REQUIRE(tiles_fwd ? aligned16(tiles_fwd) : aligned16(workspace), "nf4_group_dx (expanded): workspace / tiles must be 16-byte aligned");
   int64_t n_total = 0;
   for (int i = 0; i < d.n; ++i) n_total += d.N[i];
-  DenseArgs g = {};
-  g.nseg = d.n;
-  g.nout = 1;
   int64_t t_off = 0;
   // one expansion launch for the members when all of them come with, or all without, the transposed copies
   ExpandGroup eg = {};
@@ -1432,29 +1442,12 @@ int run_gemm_dense_group_dx(const GroupDx& d, const void* gh_cat, void* gx, void
       if (int rc = launch_expand(tr ? 1 : 3, eg.m[i].codes, eg.m[i].scal, d.K, d.N[i], n_total >> 5, t_off, reinterpret_cast<char*>(workspace), s))
         return rc;
     t_off += d.N[i] >> 5;
-    g.seg[i].X = d.gy[i];
-    g.seg[i].Kc = (int)d.N[i];
-    if (d.rank[i] > 0) {
-      DenseAdapter& a = g.ad[g.nad++];
-      a.lX = reinterpret_cast<const uint16_t*>(gh_cat) + d.r_off[i];
-      a.lW = d.lora_a[i];
-      a.R = d.rank[i];
-      a.n_begin = 0;
-      a.n_end = (int)d.K;
-      a.lscale = 1.0f;
-    }
   }
   if (one_launch && !tiles_fwd) {
     eg.n = d.n;
     if (int rc = launch_expand_group(d.codes_t[0] ? 1 : 3, eg, n_total >> 5, s)) return rc;
   }
-  g.out[0].C = reinterpret_cast<uint16_t*>(gx);
-  g.out[0].n_begin = 0;
-  g.out[0].width = (int)d.K;
-  g.Wt = reinterpret_cast<const char*>(tiles_fwd ? tiles_fwd : workspace);
-  g.M = (int)d.M; g.Nout = (int)d.K; g.Kc = (int)n_total;
-  g.lw_row_major = 0;
-  g.ldlx = d.r_off[d.n];
+  DenseArgs g = group_dx_args(d, gh_cat, gx, tiles_fwd ? tiles_fwd : workspace);
   g.w_tr = tiles_fwd ? 1 : 0;
   g.w_paired = tiles_fwd && paired ? 1 : 0;
   return launch_dense(g, s);
