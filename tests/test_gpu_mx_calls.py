@@ -208,3 +208,60 @@ def test_every_code_with_every_scale_reads_back_rounded_once(fmt, dtype):
     got = MXTensor(ox.pack(codes, fmt).to(DEV), scales.to(DEV), format=fmt).to(dtype).cpu()
     want = ox.values(codes, scales, fmt).to(dtype)
     assert bool(torch.isnan(got[255]).all()) and torch.equal(got[:255], want[:255]) and torch.equal(torch.signbit(got[:255]), torch.signbit(want[:255]))
+
+
+# ---- groups of many ranks, a handful of tokens ------------------------------------------------------
+@pytest.mark.parametrize("m,k,outs,ranks", [
+    (300, 320, [64, 192], [8, 16]), (300, 1024, [256, 64], [24, 16]), (70, 320, [128, 64, 64], [8, 24, 16]), (700, 512, [64, 128, 64, 64], [16, 16, 16, 16]),
+    (2500, 320, [64, 192], [8, 16]), (2500, 1024, [256, 64], [24, 16]), (2100, 320, [128, 64, 64], [8, 24, 16]), (2300, 512, [64, 128, 64, 64], [16, 16, 16, 16]),
+    (2200, 256, [320, 64], [40, 24]), (2100, 128, [8192, 8256], [16, 8]), (1030, 192, [8192, 8192, 8256], [16, 16, 16])])
+def test_groups_with_ranks_of_their_own(m, k, outs, ranks):
+    """24 to 64 ranks together, equal and not, on both sides of 2048 tokens, and wide outputs."""
+    g = _gen(50)
+    x = torch.randn(m, k, generator=g).to(BF)
+    a = [((torch.rand(r, k, generator=g) * 2 - 1) / k ** 0.5).to(BF) for r in ranks]
+    b = [(torch.randn(n, r, generator=g) * 0.05).to(BF) for n, r in zip(outs, ranks)]
+    gy = [torch.randn(m, n, generator=g).to(BF) for n in outs]
+    factors = [1.7, 0.75, 2.0, 0.3][:len(outs)]
+    w, dense = [], []
+    for n in outs:
+        codes, scales = ox.quantize(torch.randn(n, k, generator=g) * 0.02, "mxfp4")
+        w.append(MXTensor(ox.pack(codes, "mxfp4").to(DEV), scales.to(DEV)))
+        dense.append(ox.values(codes, scales, "mxfp4"))
+    xd, ad, bd = x.to(DEV).requires_grad_(), [t.to(DEV).requires_grad_() for t in a], [t.to(DEV).requires_grad_() for t in b]
+    ys = lora_linear_mx(xd, w, ad, bd, factors)
+    grads = torch.autograd.grad(ys, [xd, *ad, *bd], [t.to(DEV) for t in gy])
+    xq = ox.nearest(x, "mxfp8")
+    wy, wgx, wga, wgb = ox.lora(xq, dense, a, b, factors, gy)
+    my, mgx, mga, mgb = ox.lora(xq.abs(), [d.abs() for d in dense], [t.abs() for t in a], [t.abs() for t in b], factors, [t.abs() for t in gy])
+    ghs = 0.0
+    for i, s in enumerate(factors):
+        h = (xq @ a[i].double().T).abs()
+        gh = (s * (gy[i].double() @ b[i].double())).abs()
+        ghs = ghs + gh @ a[i].double().abs()
+        # h and gh are rounded to bf16, half a step of every term they enter; the norm: that and the result's own rounding
+        for got, want, lost in ((ys[i].detach(), wy[i], SUMS_FP8 * my[i] + HALF * s * (h @ b[i].double().abs().T)),
+                                (grads[1 + i], wga[i], SUMS * mga[i] + HALF * (gh.T @ xq.abs())),
+                                (grads[1 + len(outs) + i], wgb[i], SUMS * mgb[i] + HALF * s * (gy[i].double().abs().T @ h))):
+            _near(got, want, lost)
+    _near(grads[0], wgx, SUMS * mgx + HALF * ghs)
+
+
+def _near(got, want, lost):
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= HALF * want.abs() + lost + 1e-38).all())
+    assert err.norm() <= 2 * HALF * want.norm()
+
+
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 40])
+@pytest.mark.parametrize("n,k", [(70, 96), (2048, 8192), (8200, 1056), (8208, 4096)])
+def test_few_tokens_row_by_row(m, n, k, act):
+    """Tokens from 2^-100 to 2^100, each held to its own outputs: a half step of an output is the most that its rounding makes of it,
+    and what the sums of fp8 products lose, at random signs, is 2^-13 of the largest of eight for each product, some 3e-4 of the outputs' norm."""
+    g = _gen(60)
+    codes, scales = ox.quantize(torch.randn(n, k, generator=g) * 0.02, "mxfp4")
+    w, dense = MXTensor(ox.pack(codes, "mxfp4").to(DEV), scales.to(DEV)), ox.values(codes, scales, "mxfp4")
+    x = (torch.randn(m, k, generator=g) * torch.exp2(torch.linspace(-100, 100, m)).view(-1, 1)).to(BF)
+    err = linear_mx(x.to(DEV), w, activation=act).double().cpu() - (want := ox.nearest(x, act) @ dense.T)
+    assert bool((err.norm(dim=1) <= HALF * want.norm(dim=1)).all())
