@@ -3,8 +3,10 @@ import ctypes
 
 import pytest
 import torch
+from torch import nn
 
-from torchtune_amd import MXLoRALinear, MXTensor, _lib, linear_mx, to_mx
+from torchtune_amd import DoRALinear, Int8DynActInt4WeightQATQuantizer, LoRALinear, MXLoRALinear, _lib, linear_mx, to_mx
+from torchtune_amd.modules.peft import lora_linear_group
 
 BF = torch.bfloat16
 DEV = "cuda"
@@ -113,3 +115,60 @@ def test_column_sum_refusals():
     for want, got in ((-1, call(x=odd)), (-1, call(x=None)), (-1, call(out=None)), (-1, call(out=ctypes.c_void_p(4097))), (-1, call(m=-1)), (-2, call(n=1 << 29)),
                       (-3, call(size=need - 1)), (-3, call(ws=None)), (-3, call(ws=odd)), (0, call(n=0))):
         assert got == want, lib.ttamd_last_error()
+
+
+def _layers(kind, k, n):
+    with torch.device(DEV):
+        if kind == "lora":
+            return [LoRALinear(k, n, 8, 16.0, use_bias=True, quantize_base=True)]
+        if kind == "group":
+            return [LoRALinear(k, n, 8, 16.0, use_bias=True, quantize_base=True) for _ in range(2)]
+        if kind == "dora":
+            return [DoRALinear(k, n, 8, 16.0, use_bias=True, quantize_base=True)]
+        layer = nn.Linear(k, n, bias=True)
+    return [Int8DynActInt4WeightQATQuantizer(groupsize=32).prepare(nn.Sequential(layer))[0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,k,m", [(kind, 64, m) for kind in ("lora", "group", "dora") for m in (40, 2048, 8192)] + [("qat", 64, 40), ("qat", 4096, 8192)])
+def test_recorded_bias_gradients_of_the_other_layers(kind, k, m):
+    """Eager calls give torch's sum, recorded ones the library's: both within a half step and fp32 sums of the exact one, on every
+    replay.  (A fake-quantised linear between those sizes is torch's own node, bias gradient included.)"""
+    n = 4096
+    prev = torch.get_default_dtype()
+    torch.set_default_dtype(BF)
+    try:
+        layers = _layers(kind, k, n)
+    finally:
+        torch.set_default_dtype(prev)
+    biases = []
+    for layer in layers:
+        layer.requires_grad_(False)
+        if isinstance(layer, DoRALinear):
+            layer.initialize_dora_magnitude()
+        biases.append(layer.bias.requires_grad_())
+    x, gys = _randn(m, k, seed=1), [_randn(m, n, seed=2 + i) for i in range(len(layers))]
+
+    def run():
+        ys = lora_linear_group(x, layers) if kind == "group" else [layers[0](x)]
+        return torch.autograd.grad(ys, biases, gys)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = run()
+    for turn in range(3):
+        for i, gy in enumerate(gys):
+            gy.copy_(_randn(m, n, seed=20 + 2 * turn + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in recorded]
+        for a, b, gy in zip(got, run(), gys):
+            assert torch.equal(b, gy.sum(0))
+            exact, lost = gy.double().sum(0), 2.0 ** -16 * gy.double().abs().sum(0)
+            assert bool(((a.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + lost).all()), turn

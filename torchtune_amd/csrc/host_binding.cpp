@@ -372,7 +372,7 @@ struct QLoRALinearFn : torch::autograd::Function<QLoRALinearFn> {
                                         ws.data_ptr(), ws.numel(), stream_of(x2)),
             "qlora_linear_bwd");
     }
-    if (has_bias && ctx->needs_input_grad(3)) gbias = gy.sum(0);
+    if (has_bias && ctx->needs_input_grad(3)) gbias = bias_gradient(gy);
     return {gx, ga, gb, gbias, Tensor(), Tensor(), Tensor()};
   }
 };
@@ -548,7 +548,7 @@ struct QLoRAGroupFn : torch::autograd::Function<QLoRAGroupFn> {
       out.push_back(gb[i]);
       at_input += 2;
       if (bias[i]) {
-        out.push_back(ctx->needs_input_grad(at_input) ? gys[i].reshape({-1, n_out[i]}).sum(0) : Tensor());
+        out.push_back(ctx->needs_input_grad(at_input) ? bias_gradient(gys[i].reshape({-1, n_out[i]})) : Tensor());
         ++at_input;
       }
     }
@@ -755,7 +755,7 @@ struct StraightThroughLinearFn : torch::autograd::Function<StraightThroughLinear
     const Tensor gy = bf16(g[0], "straight_through_linear_bwd").view({-1, g[0].size(-1)});
     if (ctx->needs_input_grad(0)) gx = gemm_mid(1, gy, wq, Tensor()).view(shape);
     if (ctx->needs_input_grad(1)) gw = gemm_mid(2, gy, x.contiguous().view({-1, shape.back()}), Tensor());
-    if (need_b) gb = gy.sum(0);
+    if (need_b) gb = bias_gradient(gy);
     return {gx, gw, Tensor(), gb};
   }
 };

@@ -1,6 +1,7 @@
 // What the translation units of the host extension share: error codes to exceptions, checks, scratch memory.
 #pragma once
 #include <ATen/ATen.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -49,6 +50,13 @@ inline Tensor column_sum(const Tensor& gy) {
   const Tensor ws = bytes ? scratch(bytes, gy) : Tensor();
   check(ttamd_column_sum_bf16(gy.data_ptr(), out.data_ptr(), M, N, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(gy)), "column_sum");
   return out;
+}
+
+// The same for the nodes whose bias gradients are torch's sum to the bit: the own sum where the call is being recorded.
+inline Tensor bias_gradient(const Tensor& gy) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return gy.sum(0);
+  const Tensor c = gy.contiguous();
+  return column_sum((reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone());
 }
 
 // True when the call has to be a node: something is differentiated backward, or carries a forward-mode tangent (the node

@@ -58,7 +58,7 @@ class _QDoRALinearFn(torch.autograd.Function):
                 gx = ops.nf4_linear_bwd_dx(gy0, weight.quantized_data, weight.block_scalers(), K, gh, lora_a,
                                            transposed=weight.backward_copy_for(gy0.shape[0], False)).view(ctx.x_shape)
         if ctx.has_bias and need_bias:
-            gbias = gy0.sum(dim=0)
+            gbias = ops.bias_gradient(gy0)
         return gx, None, (ga if need_a else None), (gb if need_b else None), (gmag if need_m else None), gbias, None
 
 

@@ -115,7 +115,7 @@ def _group_backward(ctx, x2, h_cat, weights, las, lbs, gy2, swiglu=None):
     for i in range(n):
         _, need_a, need_b, need_bias = ctx.needs_input_grad[2 + 4 * i:6 + 4 * i]
         out += [None, grads[i][0] if need_a else None, grads[i][1] if need_b else None,
-                gy2[i].sum(dim=0) if (gy2 is not None and ctx.has_bias[i] and need_bias) else None]
+                ops.bias_gradient(gy2[i]) if (gy2 is not None and ctx.has_bias[i] and need_bias) else None]
     return tuple(out)
 
 
@@ -194,7 +194,7 @@ class _QLoRAFeedForwardFn(torch.autograd.Function):
         out = list(_group_backward(ctx, x2, h_cat, weights[:2], las[:2], lbs[:2], [ggate, gup]))
         _, need_a, need_b, need_bias = ctx.needs_input_grad[10:14]
         out += [None, ga2 if need_a else None, gb2 if need_b else None,
-                gy2.sum(dim=0) if (ctx.has_bias[2] and need_bias) else None]
+                ops.bias_gradient(gy2) if (ctx.has_bias[2] and need_bias) else None]
         return tuple(out)
 
 

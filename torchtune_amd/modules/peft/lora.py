@@ -108,7 +108,7 @@ class _QLoRALinearFn(torch.autograd.Function):
             if not need_b:
                 gb = None
         if ctx.has_bias and need_bias:
-            gbias = gy2.sum(dim=0)
+            gbias = ops.bias_gradient(gy2)
         return gx, None, ga, gb, gbias, None
 
 

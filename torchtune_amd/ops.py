@@ -428,6 +428,24 @@ def nf4_linear_bwd_dx(
     return gx if swiglu is None else (gx, gup)
 
 
+def bias_gradient(gy: torch.Tensor) -> torch.Tensor:
+    """``gy.sum(dim=0)`` of a 2-D bf16 gradient.  While the call is recorded into a graph it is the library's own sum: torch's clears
+    counters by a memset where it cuts the rows, and recorded it has given wrong sums on replays after the first."""
+    if not (gy.is_cuda and gy.dtype == torch.bfloat16 and torch.cuda.is_current_stream_capturing()):
+        return gy.sum(dim=0)
+    gy = _bf16_2d(gy, "bias_gradient")
+    if gy.data_ptr() % 16:
+        gy = gy.clone()
+    M, N = gy.shape
+    out = torch.empty(N, dtype=torch.bfloat16, device=gy.device)
+    lib = _lib.load()
+    ws = _workspace(lib.ttamd_column_sum_workspace_bytes(M, N), gy.device)
+    with torch.cuda.device(gy.device):
+        rc = lib.ttamd_column_sum_bf16(gy.data_ptr(), out.data_ptr(), M, N, ws.data_ptr(), ws.numel(), _stream(gy))
+    _lib.check(rc, "bias_gradient")
+    return out
+
+
 def lora_bwd(
     gy: torch.Tensor, x: torch.Tensor, h: torch.Tensor, lora_b: torch.Tensor, scale: float
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

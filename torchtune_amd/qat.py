@@ -316,7 +316,7 @@ class _TiledFakeQuantLinearFn(torch.autograd.Function):
             # shapes against 0.95 - 1.1 for the vendor library's); narrower layers (k / v) stay on the vendor library
             own = ops.gemm_tn_applies(gy2.shape[0], N, K) and (N // 256) * (K // 256) >= TN_GEMM_MIN_TILES
             gw = ops.gemm_tn(gy2, x2) if own else gy2.t().matmul(x2)
-        gb = gy2.sum(dim=0) if (ctx.has_bias and need_b) else None
+        gb = ops.bias_gradient(gy2) if (ctx.has_bias and need_b) else None
         return gx, gw, gb, None
 
 
@@ -416,7 +416,7 @@ class _TiledFakeQuantGroupFn(torch.autograd.Function):
             elif need_w:
                 own = ops.gemm_tn_applies(M, N, K) and (N // 256) * (K // 256) >= TN_GEMM_MIN_TILES
                 gw = ops.gemm_tn(gy2[i], x2) if own else gy2[i].t().matmul(x2)
-            out += [gw, gy2[i].sum(dim=0) if (ctx.has_bias[i] and need_b) else None]
+            out += [gw, ops.bias_gradient(gy2[i]) if (ctx.has_bias[i] and need_b) else None]
         return tuple(out)
 
 
