@@ -1,7 +1,8 @@
 """``MXLoRALinear``: ``LoRALinear`` (``torchtune/modules/peft/lora.py:27-147``) over a frozen mxfp4 weight.
 
 The input is quantised to mxfp8 once; base product and adapter read it, and it is all that is kept of the input for the
-backward pass (8.25 bits per element).  Layers that read the same input share it: ``lora_linear_group``.
+backward pass (8.25 bits per element).  Layers that read the same input share it, as long as their ranks add up to at most 64:
+``lora_linear_group``.  Adapters and bias are bfloat16 in the forward pass (build the layer with that default dtype, or move it there).
 """
 from __future__ import annotations
 
