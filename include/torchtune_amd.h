@@ -789,6 +789,124 @@ int ttamd_cross_entropy_fwd_bwd_bf16(const void* logits, const int64_t* target, 
                                      float* loss, void* grad_logits, int64_t rows, int64_t V, void* stream);
 
 /*
+ * Norms of queries and keys for each head with the rotary embedding in the same pass, forward and backward:
+ *   n = x / sqrt(mean(x^2) + eps) * scale over a head's head_dim elements (scale NULL in both parts: n = x); then the two elements
+ *   of n that frequency i turns, (2 i, 2 i + 1) if interleaved, else (i, head_dim / 2 + i), become
+ *   (a cos - b sin, b cos + a sin) with (cos, sin) = cache[position][i].  fp32 math, one rounding.
+ *   backward: from gy, the gradient of the output, that of x (out) and, summed in a fixed order, that of scale (gscale).
+ * parts[0] are the query heads, parts[1] the key heads; a part of 0 heads is left out.  x and gy may have any strides (in
+ * elements; a head's elements lie together) and begin at any element; out is contiguous [B, S, heads, head_dim].  dtype
+ * TTAMD_BF16 or TTAMD_F32 for all of x, scale, gy, out, gscale.  head_dim a multiple of 16, at most 512.
+ * positions: NULL (token s has position s) or int64 [n_axes, B, S] with strides; section[a] consecutive frequencies follow
+ * axis a (n_axes > 1; they add up to head_dim / 2).  A position outside [0, cache_rows) gives NaN and reads nothing.
+ * workspace (read only if a gscale is given): ttamd_qk_norm_rope_bwd_workspace_bytes(head_dim) bytes.
+ * The reference has no counterpart (separate eager kernels: torchtune/modules/attention.py:234-290).
+ */
+typedef struct ttamd_rope_heads {
+  const void* x;        /* [B, S, heads, head_dim]; backward without scales: not read, may be NULL */
+  const void* scale;    /* [head_dim] or NULL */
+  const void* gy;       /* backward only */
+  void* out;            /* forward: the output; backward: the gradient of x, or NULL */
+  void* gscale;         /* backward: [head_dim] or NULL */
+  int64_t heads;
+  int64_t x_stride[3];  /* of batch, token, head */
+  int64_t gy_stride[3];
+} ttamd_rope_heads;
+typedef struct ttamd_rope_positions {
+  const float* cache; /* [cache_rows, head_dim / 2, 2] cos, sin; 8-byte aligned */
+  int64_t cache_rows;
+  const int64_t* positions;
+  int64_t stride[3]; /* of axis, batch, token */
+  int n_axes;        /* 1 to 4 */
+  int section[4];
+  int interleaved;
+} ttamd_rope_positions;
+int ttamd_qk_norm_rope_fwd(const ttamd_rope_heads* parts, const ttamd_rope_positions* at, int dtype, float eps, int64_t B, int64_t S,
+                           int64_t head_dim, void* stream);
+size_t ttamd_qk_norm_rope_bwd_workspace_bytes(int64_t head_dim);
+int ttamd_qk_norm_rope_bwd(const ttamd_rope_heads* parts, const ttamd_rope_positions* at, int dtype, float eps, int64_t B, int64_t S,
+                           int64_t head_dim, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given tokens, with z = logits / temperature and p = softmax(z) of each row:
+ *   logprobs [rows, n_tokens] = log p[token] (0 for ignore_index, NaN for any other token outside [0, V));
+ *   entropy [rows] = -sum p log p (NULL: not wanted);
+ *   top_logprobs, top_tokens [rows, top]: the largest log probabilities with their tokens, of equal logits the earlier token
+ *   first; top at most 64 and at most V (0: not wanted);
+ *   stats [rows, 4] fp32, kept for the backward (NULL: not wanted).
+ * A row of nothing but -inf has no distribution: log probabilities of -inf, entropy 0, gradients 0.  A row with a NaN or +inf
+ * has NaN throughout (and tokens without meaning).
+ *   backward: grad [rows, V] contiguous, the logits' type, = (sum_t g_t [j = t] - p_j sum g_t - gH p_j (log p_j + H)) / temperature from
+ *   g_logprobs [rows, n_tokens] and g_entropy [rows] (either NULL: zero).  Ignored tokens have no gradient.
+ * logits: TTAMD_BF16 or TTAMD_F32, V neighbouring elements a row, row r at (r / n_inner) * stride_outer +
+ * (r % n_inner) * stride_inner elements; rows may begin at any element.  fp32 sums in an order that depends on the sizes only.
+ * workspace: ttamd_token_logprobs_workspace_bytes bytes (0: may be NULL).
+ * Beside it in the reference: torchtune/rlhf/utils.py (eager log_softmax and gather).
+ */
+typedef struct ttamd_logits {
+  const void* data;
+  int dtype;
+  int64_t rows, V, n_inner, stride_outer, stride_inner;
+} ttamd_logits;
+size_t ttamd_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int top);
+int ttamd_token_logprobs_fwd(const ttamd_logits* logits, const int64_t* tokens, int64_t n_tokens, int64_t ignore_index, float temperature,
+                             float* logprobs, float* entropy, int top, float* top_logprobs, int64_t* top_tokens, float* stats,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int ttamd_token_logprobs_bwd(const ttamd_logits* logits, const int64_t* tokens, int64_t n_tokens, int64_t ignore_index, float temperature,
+                             const float* stats, const float* g_logprobs, const float* g_entropy, void* grad, void* stream);
+
+/*
+ * One AdamW step over many tensors (torch.optim.AdamW's update, as the reference's recipes configure it), fp32 math:
+ *   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2;
+ *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m' / (sqrt(v') / sqrt(1 - beta2^step) + eps)
+ * every product and sum rounded by itself.  Parameters and gradients of `dtype`, any alignment of an element; the moments of
+ * all tensors lie in two buffers, tensor i's from element `offset` (fp32, state_bits 32) on.
+ *
+ * state_bits 8: a moment is one byte, and TTAMD_ADAMW_BLOCK consecutive elements of a tensor share a byte of exponent (the
+ * tensor's blocks from `block` on in the exponent buffers).  With E the block's exponent byte,
+ *   exp_avg:    bits 6..0 of a code c: 0 is 0, else the fp32 number of bits ((c + 8 (E - 15)) << 20); bit 7 is the sign;
+ *   exp_avg_sq: 0 is 0, else the fp32 number of bits ((c + 16 (E - 15)) << 19).
+ * Writing them adds a 16-bit number of the element to the dropped bits (in their highest 16 places, and half of the rest) and
+ * cuts: right on average, where rounding to nearest would hide that exp_avg_sq moves by (1 - beta2) a step.  E is the exponent of
+ * the block's largest result, at least 16; exp_avg below the range is 0, exp_avg_sq the smallest number.  The numbers are the
+ * two halves (exp_avg_sq the high one) of ttamd_adamw_number(key, element) with key = ttamd_adamw_key(seed, step, tensor).
+ * stochastic (bf16 parameters): p' is rounded with the low half instead of to nearest.
+ *
+ * layout: device array of n_all tensors' places; chunk_map: device array, the tensor of each chunk of
+ * TTAMD_ADAMW_CHUNK elements, tensors one after another, each beginning a chunk.  Both depend on the sizes only.  The call covers
+ * tensors first .. first + n - 1 (n at most TTAMD_ADAMW_TENSORS) and their chunks first_chunk .. first_chunk + n_chunks - 1.
+ * params and grads are host arrays of n device pointers.
+ */
+#define TTAMD_ADAMW_BLOCK 128
+#define TTAMD_ADAMW_CHUNK 4096
+#define TTAMD_ADAMW_TENSORS 240
+typedef struct ttamd_adamw_place {
+  int64_t offset, numel, block;
+  uint32_t first_chunk; /* counted over all tensors */
+  uint32_t number;      /* the tensor's own, for the numbers above */
+} ttamd_adamw_place;
+typedef struct ttamd_adamw_states {
+  const ttamd_adamw_place* layout;
+  const uint32_t* chunk_map;
+  void* exp_avg;
+  void* exp_avg_sq;
+  uint8_t* exp_avg_exponent;    /* state_bits 8 */
+  uint8_t* exp_avg_sq_exponent;
+  int state_bits;
+} ttamd_adamw_states;
+typedef struct ttamd_adamw_scalars {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step, seed;
+  int stochastic;
+} ttamd_adamw_scalars;
+uint32_t ttamd_adamw_key(int64_t seed, int64_t step, uint32_t tensor);
+uint32_t ttamd_adamw_number(uint32_t key, int64_t element);
+int ttamd_adamw_step(void* const* params, const void* const* grads, int n, int dtype, const ttamd_adamw_states* states, uint32_t first,
+                     uint32_t first_chunk, uint32_t n_chunks, const ttamd_adamw_scalars* scalars, void* stream);
+/* The 8-bit moments of all chunks as bf16 numbers (nothing is lost), tensor i from element `offset` of both outputs on. */
+int ttamd_adamw_moments_bf16(const ttamd_adamw_states* states, uint32_t n_chunks, void* exp_avg, void* exp_avg_sq, void* stream);
+
+/*
  * out [N] = sum over the rows of x [M, N], bf16, fp32 sums, one rounding: the gradient of a linear's bias from that of its
  * output.  The order of the sums depends on M and N only.  x 16-byte aligned; M may be 0 (zeros); workspace:
  * ttamd_column_sum_workspace_bytes bytes (0: may be NULL).  Unlike a library reduction it clears no memory, so that a recorded

@@ -1,0 +1,425 @@
+"""``training.AdamW`` against the update written out: to the bit where it is a sequence of fp32 operations (the moments, and what 8 bits
+hold of them), and in 64 bits for the parameters.
+
+Tolerances.  A parameter's change is a product of a quotient: five roundings and the scalars' own, less than 16 * 2^-24 of its size; the
+parameter is scaled and rounded to its type: half a step, or with stochastic rounding a whole one."""
+import copy
+import io
+import math
+
+import pytest
+import torch
+
+from torchtune_amd import _lib
+from torchtune_amd.training import AdamW
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+BLOCK = 128
+
+
+def _tensors(shapes, dtype, seed=0, scale=1e-3):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    params = []
+    for shape in shapes:
+        p = torch.nn.Parameter((torch.randn(shape, generator=g, device=DEV) * 0.05).to(dtype))
+        size = torch.exp(torch.randn((), generator=g, device=DEV) * 2)
+        p.grad = (torch.randn(shape, generator=g, device=DEV) * scale * size).to(dtype)
+        params.append(p)
+    return params
+
+
+def _numbers(seed, step, tensor, n):
+    """(for the second moment, for the first and the parameter): a small n through the library's own function"""
+    lib = _lib.load()
+    key = lib.ttamd_adamw_key(seed, step, tensor)
+    r = torch.tensor([lib.ttamd_adamw_number(key, i) for i in range(n)], dtype=torch.int64)
+    return r >> 16, r & 0xFFFF
+
+
+def _padded(x):
+    return torch.cat([x, x.new_zeros(-x.numel() % BLOCK)]).view(-1, BLOCK)
+
+
+def _hold(x, numbers, mantissa):
+    """codes and exponents of fp32 numbers, from the description of the format"""
+    drop = 23 - mantissa
+    size = x.view(torch.int32).to(torch.int64) & 0x7FFFFFFF
+    k = (size.clamp(max=0x7F800000) + numbers * 2 ** (drop - 16) + 2 ** (drop - 17)) >> drop
+    exponent = (_padded(k).amax(-1) >> mantissa).clamp(min=16)
+    c = k - ((exponent - 15) << mantissa).repeat_interleave(BLOCK)[:x.numel()]
+    if mantissa == 3:
+        return torch.where(c < 1, 0, c + 128 * torch.signbit(x)).to(torch.uint8), exponent.to(torch.uint8)
+    return torch.where(size == 0, 0, c.clamp(min=1)).to(torch.uint8), exponent.to(torch.uint8)
+
+
+def _value(code, exponent, mantissa):
+    code, field = code.to(torch.int64), exponent.to(torch.int64).repeat_interleave(BLOCK)[:code.numel()]
+    size = code & (127 if mantissa == 3 else 255)
+    bits = torch.where(size == 0, 0, (size + ((field - 15) << mantissa)) << (23 - mantissa)).to(torch.int32)
+    v = bits.view(torch.float32)
+    return torch.where(code > 127, -v, v) if mantissa == 3 else v
+
+
+class _Reference:
+    """One tensor's step on the CPU, fp32 moments to the bit and the parameter in 64 bits."""
+
+    def __init__(self, p, number, bits, seed, **group):
+        self.n, self.number, self.bits, self.seed, self.group = p.numel(), number, bits, seed, group
+        self.step, self.m, self.v = 0, torch.zeros(self.n), torch.zeros(self.n)
+
+    def take(self, p, g):
+        c = self.group
+        b1, b2 = c["betas"]
+        self.step += 1
+        p, g = p.detach().cpu().reshape(-1).double(), g.cpu().reshape(-1).float()
+        m = self.m * b1 + g * (1 - b1)
+        v = self.v * b2 + (g * g) * (1 - b2)
+        change = c["lr"] / (1 - b1 ** self.step) * m.double() / (v.double().sqrt() / math.sqrt(1 - b2 ** self.step) + c["eps"])
+        self.want, self.size = p * (1 - c["lr"] * c["weight_decay"]) - change, p.abs() + change.abs()
+        if self.bits == 8:
+            high, low = _numbers(self.seed, self.step, self.number, self.n)
+            self.mc, self.vc = _hold(m, low, 3), _hold(v, high, 4)
+            m, v = _value(*self.mc, 3), _value(*self.vc, 4)
+        self.m, self.v = m, v
+
+    def check(self, p, state, whole_step=False):
+        eps = torch.finfo(p.dtype).eps
+        off = (p.detach().cpu().reshape(-1).double() - self.want).abs()
+        bound = self.want.abs() * eps / (1 if whole_step else 2) + 16 * U * self.size
+        assert bool((off <= bound).all()), float((off / bound).max())
+        assert int(state["step"]) == self.step
+        if self.bits == 8:
+            for name, (code, exponent) in (("exp_avg", self.mc), ("exp_avg_sq", self.vc)):
+                assert torch.equal(state[name].cpu().reshape(-1), code), name
+                assert torch.equal(state[name + "_exponent"].cpu(), exponent), name
+        else:
+            assert torch.equal(state["exp_avg"].cpu().reshape(-1), self.m) and torch.equal(state["exp_avg_sq"].cpu().reshape(-1), self.v)
+
+
+SHAPES = [(1,), (7,), (128,), (129,), (16, 256), (4095,), (4097,), (33, 65), (0,), (2, 3, 2048)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("stochastic", [False, True])
+def test_steps_over_many_tensors(dtype, bits, stochastic):
+    params = _tensors(SHAPES, dtype)
+    group = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    opt = AdamW(params, **group, state_bits=bits, stochastic_rounding=stochastic, seed=7)
+    refs = [_Reference(p, i, bits, 7, **group) for i, p in enumerate(params)]
+    for step in range(3):
+        before = [p.detach().clone() for p in params]
+        if step:
+            for p in params:
+                p.grad = torch.randn_like(p) * 1e-3 * 10 ** step
+        opt.step()
+        for p, b, r in zip(params, before, refs):
+            r.take(b, p.grad)
+            r.check(p, opt.state[p], stochastic and dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_one_launch_holds_some_without_gradients(bits):
+    """Groups with their own rates, tensors that join later and so count their own steps, two types."""
+    params = _tensors([(5 + i % 97,) for i in range(500)], torch.float32) + _tensors([(64,), (65,)], torch.bfloat16, 1)
+    gone = [p.grad for p in params]
+    groups = [{"params": params[:300], "lr": 1e-2}, {"params": params[300:], "weight_decay": 0.0}]
+    opt = AdamW(groups, lr=1e-3, betas=(0.8, 0.9), state_bits=bits, seed=3)
+    scalars = [dict(lr=1e-2 if i < 300 else 1e-3, betas=(0.8, 0.9), eps=1e-8, weight_decay=0.01 if i < 300 else 0.0) for i in range(len(params))]
+    refs = [_Reference(p, i, bits, 3, **c) for i, (p, c) in enumerate(zip(params, scalars))]
+    for step in range(3):
+        used = [i for i in range(len(params)) if step == 2 or i % 5 != step]
+        for i, p in enumerate(params):
+            p.grad = gone[i] if i in used else None
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for i, (p, b, r) in enumerate(zip(params, before, refs)):
+            if i in used:
+                r.take(b, p.grad)
+                r.check(p, opt.state[p])
+            else:
+                assert torch.equal(p.detach(), b) and (p in opt.state) == (r.step > 0)
+    m, v = opt.moments()
+    assert torch.equal(m.float().cpu(), torch.cat([r.m for r in refs])) and torch.equal(v.float().cpu(), torch.cat([r.v for r in refs]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_views_and_other_orders_in_memory(dtype, bits):
+    """Parameters at odd places, transposed ones, ones with gaps; gradients that lie differently: the elements' own results."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    base = (torch.randn(4000, generator=g, device=DEV) * 0.1).to(dtype)
+    wide = (torch.randn(40, 50, generator=g, device=DEV) * 0.1).to(dtype)
+    guard = base.clone(), wide.clone()
+    params = [torch.nn.Parameter(t) for t in (base[1:400], base[401:401 + 33 * 9].view(9, 33).t(), wide[:, 3:20], base[1000:3000].view(2, 1000))]
+    grads = [torch.randn(p.shape, generator=g, device=DEV).to(dtype) * 1e-2 for p in params]
+    grads[0] = torch.stack([grads[0], grads[0]], -1)[:, 0]  # with gaps
+    grads[3] = grads[3].t().contiguous().t()
+    for p, x in zip(params, grads):
+        p.grad = x
+    group = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
+    opt = AdamW(params, **group, state_bits=bits, seed=1)
+    flat = [p.t() if i == 1 else p for i, p in enumerate(params)]  # in the order in memory
+    refs = [_Reference(p, i, bits, 1, **group) for i, p in enumerate(params)]
+    for _ in range(2):
+        before = [p.detach().clone() for p in flat]
+        opt.step()
+        for i, (p, b, r) in enumerate(zip(flat, before, refs)):
+            r.take(b, (grads[i].t() if i == 1 else grads[i]).contiguous())
+            state = dict(opt.state[params[i]])
+            assert state["exp_avg"].shape == params[i].shape
+            if i == 1:
+                state["exp_avg"], state["exp_avg_sq"] = state["exp_avg"].t(), state["exp_avg_sq"].t()
+            r.check(p, state)
+    same = torch.ones(4000, dtype=torch.bool, device=DEV)
+    for lo, hi in ((1, 400), (401, 401 + 297), (1000, 3000)):
+        same[lo:hi] = False
+    assert torch.equal(base[same], guard[0][same])
+    assert torch.equal(wide[:, :3], guard[1][:, :3]) and torch.equal(wide[:, 20:], guard[1][:, 20:])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_of_zero_tiny_and_huge_size(bits):
+    n = 8 * BLOCK
+    p = torch.nn.Parameter(torch.randn(n, device=DEV))
+    grad = torch.zeros(n, device=DEV)
+    grad[BLOCK:2 * BLOCK] = torch.logspace(-30, 3, BLOCK, device=DEV)   # a block over many powers
+    grad[2 * BLOCK:3 * BLOCK] = 1e-22                                   # squares below the smallest normal number
+    grad[3 * BLOCK:4 * BLOCK] = 1e18
+    grad[4 * BLOCK] = -5.0
+    grad[5 * BLOCK:6 * BLOCK] = torch.linspace(-1, 1, BLOCK, device=DEV)
+    group = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0)
+    opt, r = AdamW([p], **group, state_bits=bits, seed=9), None
+    r = _Reference(p, 0, bits, 9, **group)
+    for sign in (1, -1, 0.5, 0):
+        p.grad = grad * sign
+        before = p.detach().clone()
+        opt.step()
+        r.take(before, p.grad)
+        r.check(p, opt.state[p])
+    assert torch.equal(p.detach()[:BLOCK].isfinite().cpu(), torch.ones(BLOCK, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_gradient_that_is_not_finite(bits, bad):
+    p = torch.nn.Parameter(torch.randn(4 * BLOCK, device=DEV))
+    opt = AdamW([p], lr=1e-2, state_bits=bits)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    p.grad = torch.randn_like(p)
+    p.grad[BLOCK + 5] = bad
+    opt.step()
+    for _ in range(2):
+        p.grad = torch.randn_like(p)
+        opt.step()
+    here = torch.zeros(4 * BLOCK, dtype=torch.bool, device=DEV)
+    here[BLOCK + 5] = True
+    assert bool(torch.isnan(p.detach()[here]).all()) and bool(torch.isfinite(p.detach()[~here]).all())
+
+
+def test_eight_bits_are_right_on_average():
+    """4096 elements with the same gradient: their held moments scatter around the fp32 ones.  A rounding's standard deviation is
+    at most half a step (2^-4 of the size for exp_avg, 2^-5 for exp_avg_sq), its mean's a 64th of that; four of those are allowed, and the
+    steps before add up: exp_avg remembers 10, exp_avg_sq up to all 200 of them, but in quadrature.  Rounding to nearest would leave exp_avg_sq
+    where a step of 0.1 % is lost, at less than a tenth of its value."""
+    n = 4096
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = AdamW([p], lr=0.0, betas=(0.9, 0.999), weight_decay=0.0, state_bits=8, seed=11)
+    g = 0.37
+    for step in range(1, 201):
+        p.grad = torch.full((n,), g, device=DEV)
+        opt.step()
+    m, v = (x.double() for x in opt.moments())
+    want_m, want_v = g * (1 - 0.9 ** 200), g * g * (1 - 0.999 ** 200)
+    assert abs(float(m.mean()) / want_m - 1) < 4 / 64 * 2 ** -4 * math.sqrt(10)
+    assert abs(float(v.mean()) / want_v - 1) < 4 / 64 * 2 ** -5 * math.sqrt(200)
+    assert float(v.std()) > 0  # the elements' numbers differ
+
+
+def test_stochastic_rounding_keeps_small_updates():
+    """Changes of a hundredth of bf16's step: lost to the nearest, kept on average.  100 steps of the same sign move each of
+    65536 elements by about one step, with a standard deviation of at most sqrt(100) / 2 steps; the mean's is a 256th of it."""
+    n, steps = 65536, 100
+    change = 2.0 ** -8 / 100
+    results = []
+    for stochastic in (False, True):
+        p = torch.nn.Parameter(torch.full((n,), 1.0, device=DEV, dtype=torch.bfloat16))
+        opt = AdamW([p], lr=change, betas=(0.0, 0.0), eps=0.0, weight_decay=0.0, stochastic_rounding=stochastic, seed=5)
+        for _ in range(steps):
+            p.grad = -torch.ones_like(p)
+            opt.step()
+        results.append(p.detach().double())
+    assert bool((results[0] == 1).all())
+    assert abs(float(results[1].mean()) - 1 - steps * change) < 4 * 2 ** -7 * math.sqrt(steps) / 2 / 256
+
+
+def test_runs_repeat_and_seeds_differ():
+    def run(seed):
+        params = _tensors(SHAPES, torch.bfloat16)
+        opt = AdamW(params, lr=1e-2, state_bits=8, stochastic_rounding=True, seed=seed)
+        for _ in range(2):
+            opt.step()
+        return [p.detach().clone() for p in params] + list(opt.moments())
+
+    a, b, c = run(1), run(1), run(2)
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and not all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["state_dict", "file", "pickle", "deepcopy"])
+def test_saved_and_continued(bits, how):
+    def fresh():
+        return _tensors(SHAPES, torch.bfloat16)
+
+    def grads(params, step):
+        g = torch.Generator(device=DEV).manual_seed(step)
+        for p in params:
+            p.grad = (torch.randn(p.shape, generator=g, device=DEV) * 1e-3).to(p.dtype)
+
+    make = lambda params: AdamW([{"params": params[:4], "lr": 1e-3}, {"params": params[4:]}], lr=1e-2, state_bits=bits, stochastic_rounding=True, seed=2)
+    params = fresh()
+    opt = make(params)
+    for step in range(2):
+        grads(params, step)
+        opt.step()
+    if how == "deepcopy":
+        other, again = copy.deepcopy((params, opt))
+    else:
+        other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        again = make(other)
+        saved = opt.state_dict()
+        if how == "file":
+            f = io.BytesIO()
+            torch.save(saved, f)
+            f.seek(0)
+            saved = torch.load(f, weights_only=True)
+        if how == "pickle":
+            f = io.BytesIO()
+            torch.save(opt, f)
+            f.seek(0)
+            saved = torch.load(f, weights_only=False).state_dict()  # written four lines above
+        again.load_state_dict(saved)
+    for step in range(2, 4):
+        for ps, o in ((params, opt), (other, again)):
+            grads(ps, step)
+            o.step()
+    for p, q in zip(params, other):
+        assert torch.equal(p.detach(), q.detach())
+        for name in opt.state[p]:
+            assert torch.equal(opt.state[p][name], again.state[q][name]), name
+            assert opt.state[p][name].dtype == again.state[q][name].dtype
+    assert again.param_groups[0]["lr"] == 1e-3
+
+
+def test_a_state_dict_of_torchs_optimizer():
+    params = _tensors([(33, 7), (100,)], torch.float32)
+    theirs = torch.optim.AdamW(params, lr=1e-2, fused=True)
+    theirs.step()
+    other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    ours = AdamW(other, lr=1.0)
+    ours.load_state_dict(theirs.state_dict())
+    for p, q in zip(params, other):
+        q.grad = p.grad.clone()
+    theirs.step()
+    ours.step()
+    for p, q in zip(params, other):
+        assert float((p - q).detach().abs().max()) < 1e-2 * 64 * U + 2 * U * float(p.detach().abs().max())
+        assert int(ours.state[q]["step"]) == 2
+    with pytest.raises(ValueError, match="expected"):
+        AdamW(other, state_bits=8).load_state_dict(theirs.state_dict())
+
+
+def test_states_of_the_other_width_are_refused_and_nothing_changes():
+    params = _tensors([(300,)], torch.float32)
+    eight, wide = AdamW(params, state_bits=8), AdamW(params, state_bits=32)
+    eight.step()
+    wide.step()
+    kept = wide.state[params[0]]["exp_avg"].clone()
+    with pytest.raises(ValueError, match="bits"):
+        wide.load_state_dict(eight.state_dict())
+    short = wide.state_dict()
+    short["state"] = {0: {**short["state"][0], "exp_avg": torch.zeros(299)}}
+    with pytest.raises(ValueError, match="elements"):
+        wide.load_state_dict(short)
+    assert torch.equal(wide.state[params[0]]["exp_avg"], kept)
+
+
+def test_refusals():
+    p = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    opt = AdamW([p])
+    p.grad = torch.sparse_coo_tensor([[1]], [1.0], (10,), device=DEV)
+    with pytest.raises(RuntimeError, match="dense"):
+        opt.step()
+    half = torch.nn.Parameter(torch.zeros(10, device=DEV, dtype=torch.float16))
+    half.grad = torch.zeros_like(half)
+    with pytest.raises(TypeError, match="not supported"):
+        AdamW([half]).step()
+    q = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    q.grad = torch.ones_like(q)
+    opt = AdamW([q], lr=0.5)
+    opt.step()
+    after = q.detach().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="graph"):
+            opt.step()
+    assert int(opt.state[q]["step"]) == 1 and torch.equal(q.detach(), after)
+    opt.param_groups[0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.step()
+
+
+def test_closures_hooks_schedulers_and_versions():
+    w = torch.nn.Parameter(torch.ones(3, device=DEV))
+    opt = AdamW([w], lr=0.1, weight_decay=0.0)
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda step: 1.0 / (1 + step))
+    seen = []
+    opt.register_step_post_hook(lambda *a: seen.append(1))
+
+    def closure():
+        opt.zero_grad()
+        loss = (w * w).sum()
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure)) == 3.0 and seen == [1]
+    assert float((w.detach() - 0.9).abs().max()) < 1e-6
+    schedule.step()
+    assert opt.param_groups[0]["lr"] == 0.05
+    before = w._version
+    out = (w * w).sum()
+    w.grad = torch.ones_like(w)
+    opt.step()
+    assert w._version > before
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.backward()
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2, device=DEV))]})
+    opt.param_groups[1]["params"][0].grad = torch.ones(2, device=DEV)
+    opt.step()
+    assert len(opt.state) == 2 and int(opt.state[opt.param_groups[1]["params"][0]]["step"]) == 1
+
+
+def test_on_another_stream():
+    """The states made on one stream, steps on another, the optimizer gone while they run."""
+    results = []
+    for streams in (1, 2):
+        params = _tensors([(1 << 20,)] * 4, torch.float32)
+        opt = AdamW(params, lr=1e-2, state_bits=8, seed=4)
+        opt.step()
+        side = torch.cuda.Stream() if streams == 2 else torch.cuda.current_stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(5):
+                opt.step()
+        del opt
+        junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=DEV) for _ in range(8)]
+        torch.cuda.current_stream().wait_stream(side)
+        results.append(torch.cat([p.detach() for p in params]))
+        del junk
+    assert torch.equal(*results)

@@ -1,0 +1,280 @@
+"""``layer_ops.qk_norm_rope`` against a plain implementation in 64 bits: forward, gradients, views, positions, graphs.
+
+Tolerances.  A result is rounded once to its type, half a step: ``eps / 2`` of its size.  Before that, fp32: a row's mean of squares is a
+sum of positive numbers in at most 16 + 5 additions, so that its inverse root is off by at most 12 * 2^-24, the hardware's by
+2^-23 more; scaling, two products and a difference add 5 * 2^-24.  That is less than 32 * 2^-24 of the numbers that enter an
+output, whose sum ``size`` is computed beside it; backward, a second row sum and four more operations: less than 64 * 2^-24.  The
+scales' gradients add at most 512 such terms one after another."""
+import pytest
+import torch
+
+from torchtune_amd.modules import layer_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+def _table(n, d):
+    angle = torch.outer(torch.arange(n, dtype=torch.float64), 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d))
+    return torch.stack([angle.cos(), angle.sin()], -1).float()
+
+
+def _turns(cache, positions, sections, b, s):
+    """cos, sin [b, s, 1, d / 2] in 64 bits"""
+    half = cache.shape[1]
+    if positions is None:
+        positions = torch.arange(s).expand(b, s)
+    axis = torch.zeros(half, dtype=torch.long)
+    if sections:
+        axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections))
+    else:
+        positions = positions.expand(b, s)[None]
+    rows = cache.double()[positions[axis].permute(1, 2, 0), torch.arange(half)]
+    return rows[..., 0][:, :, None], rows[..., 1][:, :, None]
+
+
+def _rotate(x, cos, sin, interleaved):
+    a, b = (x[..., 0::2], x[..., 1::2]) if interleaved else x.chunk(2, -1)
+    u, v = a * cos - b * sin, b * cos + a * sin
+    return torch.stack([u, v], -1).flatten(-2) if interleaved else torch.cat([u, v], -1)
+
+
+def _plain(x, w, gy, cos, sin, eps, interleaved):
+    """out, its size, gx, its size, gw, its size"""
+    x, gy = x.double(), gy.double()
+    r = torch.ones_like(x[..., :1]) if w is None else 1 / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+    scale = torch.ones(x.shape[-1], dtype=torch.float64) if w is None else w.double()
+    n = x * r * scale
+    out, size = _rotate(n, cos, sin, interleaved), _rotate(n.abs(), cos.abs(), -sin.abs(), interleaved).abs() + _rotate(n.abs(), cos.abs(), sin.abs(), interleaved).abs()
+    g = _rotate(gy, cos, -sin, interleaved)
+    g_size = _rotate(gy.abs(), cos.abs(), -sin.abs(), interleaved).abs() + _rotate(gy.abs(), cos.abs(), sin.abs(), interleaved).abs()
+    if w is None:
+        return out, size, g, g_size, None, None
+    gw, gw_size = (g * x * r).sum((0, 1, 2)), (g_size * x.abs() * r).sum((0, 1, 2))
+    gx = r * (g * scale - x * r * r * (g * scale * x).mean(-1, keepdim=True))
+    gx_size = r * (g_size * scale.abs() + x.abs() * r * r * (g_size * scale.abs() * x.abs()).mean(-1, keepdim=True))
+    return out, size, gx, gx_size, gw, gw_size
+
+
+def _near(got, want, size, terms, dtype):
+    bound = want.abs() * torch.finfo(dtype).eps / 2 + size * terms * U
+    off = (got.double().cpu() - want).abs()
+    assert got.dtype == dtype and got.shape == want.shape
+    assert bool((off <= bound).all()), float((off / bound.clamp(min=1e-300)).max())
+
+
+def _inputs(b, s, nh, kv, d, dtype, norm, layout, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=DEV)
+
+    if layout == "joined":
+        whole = (normal(b, s, nh + 2 * kv, d) * 2).to(dtype)
+        q, k = whole[:, :, :nh], whole[:, :, nh:nh + kv]
+    elif layout == "odd":  # heads that begin at any element, tokens inside
+        q = (normal(b * nh * s * d + 3) * 2).to(dtype)[3:].view(b, nh, s, d).transpose(1, 2)
+        k = (normal(b * kv * s * (d + 5)) * 2).to(dtype).view(b, s, kv, d + 5)[..., 5:]
+    else:
+        q, k = (normal(b, s, nh, d) * 2).to(dtype), (normal(b, s, kv, d) * 2).to(dtype)
+    w = [(1 + 0.3 * normal(d)).to(dtype) for _ in range(2)] if norm else [None, None]
+    gy = [normal(b, s, h, d).to(dtype) for h in (nh, kv)]
+    return [q, k], w, gy
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("b,s,nh,kv,d,layout,axes,interleaved,norm", [
+    (1, 1, 32, 8, 128, "plain", 1, False, True),
+    (1, 1, 1, 1, 16, "plain", 0, True, True),
+    (2, 5, 4, 2, 32, "joined", 0, True, True),
+    (3, 7, 3, 1, 48, "odd", 1, False, True),
+    (2, 33, 8, 2, 64, "joined", 3, False, True),
+    (1, 17, 4, 4, 80, "odd", 3, True, True),
+    (2, 9, 5, 3, 112, "plain", 2, False, False),
+    (1, 130, 6, 2, 256, "joined", 4, True, False),
+    (2, 3, 2, 1, 512, "odd", 0, False, True),
+    (1, 700, 40, 8, 128, "joined", 1, True, True),  # workgroups walk several rows
+])
+def test_forward_and_gradients(dtype, b, s, nh, kv, d, layout, axes, interleaved, norm):
+    xs, ws, gys = _inputs(b, s, nh, kv, d, dtype, norm, layout)
+    cache = _table(900, d)
+    sections = {0: None, 1: None, 2: [d // 2 - 3, 3], 3: [d // 8, d // 2 - d // 8 - 5, 5], 4: [1, d // 4, 0, d // 4 - 1]}[axes]
+    positions = None
+    if axes:
+        shape = (b, s) if sections is None else (len(sections), b, s)
+        positions = torch.randint(0, 900, shape, generator=torch.Generator().manual_seed(1))
+    leaves = [x.detach().requires_grad_() for x in xs] + ([w.requires_grad_() for w in ws] if norm else [])
+    place = None if positions is None else positions.to(DEV)
+    outs = layer_ops.qk_norm_rope(*leaves[:2], cache.to(DEV), *leaves[2:], eps=1e-5, positions=place, sections=sections, interleaved=interleaved)
+    grads = torch.autograd.grad(outs, leaves, gys)
+    cos, sin = _turns(cache, positions, sections, b, s)
+    for i in range(2):
+        w = ws[i].detach().cpu() if norm else None
+        out, size, gx, gx_size, gw, gw_size = _plain(xs[i].detach().cpu(), w, gys[i].cpu(), cos, sin, 1e-5, interleaved)
+        assert outs[i].is_contiguous() and grads[i].is_contiguous()
+        _near(outs[i].detach(), out, size, 32, dtype)
+        _near(grads[i], gx, gx_size, 64, dtype)
+        if norm:
+            _near(grads[2 + i], gw, gw_size, 512, dtype)
+    with torch.no_grad():
+        again = layer_ops.qk_norm_rope(*leaves[:2], cache.to(DEV), *leaves[2:], eps=1e-5, positions=place, sections=sections, interleaved=interleaved)
+    assert all(torch.equal(a, o) for a, o in zip(again, outs))
+
+
+def test_gradients_against_differences():
+    """The directional derivative of a weighted sum of the outputs.  In fp32 with a step h = 2^-6, central differences: the third
+    derivative's share is below h^2 times the sum's size, the rounding's 2^-24 of it over h."""
+    xs, ws, gys = _inputs(1, 3, 2, 1, 32, torch.float32, True, "plain")
+    cache, h = _table(8, 32).to(DEV), 2.0 ** -6
+    leaves = [t.detach().requires_grad_() for t in xs + ws]
+
+    def total(ts):
+        outs = layer_ops.qk_norm_rope(*ts[:2], cache, *ts[2:], interleaved=False)
+        return sum((o.double() * g.double()).sum() for o, g in zip(outs, gys))
+
+    grads = torch.autograd.grad(total(leaves), leaves)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    for i, leaf in enumerate(leaves):
+        way = torch.randn(leaf.shape, generator=g, device=DEV)
+        way = way / way.norm()
+        with torch.no_grad():
+            ends = [total([t + sign * h * way if j == i else t for j, t in enumerate(leaves)]) for sign in (1, -1)]
+        size = sum((o.abs().sum() * gy.abs().max()).item() for o, gy in zip(layer_ops.qk_norm_rope(*xs, cache, *[w.detach() for w in ws], interleaved=False), gys))
+        assert abs(float((ends[0] - ends[1]) / (2 * h) - (grads[i] * way).sum())) < (h * h + 64 * U / h) * size
+
+
+def test_positions_broadcast_and_default():
+    (q, k), (w1, w2), _ = _inputs(3, 6, 4, 2, 64, torch.bfloat16, True, "plain")
+    cache = _table(6, 64).to(DEV)
+    want = layer_ops.qk_norm_rope(q, k, cache, w1, w2)
+    for positions in (torch.arange(6, device=DEV), torch.arange(6, device=DEV)[None], torch.arange(6, device=DEV, dtype=torch.int32).expand(3, 6)):
+        got = layer_ops.qk_norm_rope(q, k, cache, w1, w2, positions=positions)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    axes = torch.arange(6, device=DEV).expand(3, 1, 6)  # one place on every axis is the place on one
+    got = layer_ops.qk_norm_rope(q, k, cache, w1, w2, positions=axes, sections=[10, 11, 11])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_position_outside_the_table_gives_nan_there_only():
+    (q, k), (w1, w2), _ = _inputs(1, 5, 2, 2, 32, torch.float32, True, "plain")
+    cache = _table(10, 32).to(DEV)
+    positions = torch.tensor([[0, 9, 10, -1, 2 ** 40]], device=DEV)
+    inside = torch.tensor([True, True, False, False, False], device=DEV)
+    for out in layer_ops.qk_norm_rope(q, k, cache, w1, w2, positions=positions):
+        assert bool(torch.isnan(out[0, ~inside]).all()) and not bool(torch.isnan(out[0, inside]).any())
+    three = torch.stack([positions.clamp(0, 9)] * 2 + [positions])
+    for out in layer_ops.qk_norm_rope(q, k, cache, w1, w2, positions=three, sections=[4, 4, 8], interleaved=True):
+        bad = torch.isnan(out[0])
+        assert bool(bad[~inside][..., 16:].all()) and not bool(bad[..., :16].any()) and not bool(bad[inside].any())
+
+
+def test_parts_of_the_gradient():
+    """Whatever is asked for, and from whichever output, it has the bits it has beside the others."""
+    xs, ws, gys = _inputs(2, 19, 4, 2, 64, torch.bfloat16, True, "joined")
+    cache = _table(19, 64).to(DEV)
+
+    def grads(wanted, outs_used):
+        ts = [t.detach().requires_grad_(i in wanted) for i, t in enumerate(xs + ws)]
+        outs = layer_ops.qk_norm_rope(*ts[:2], cache, *ts[2:])
+        return torch.autograd.grad([outs[i] for i in outs_used], [ts[i] for i in wanted], [gys[i] for i in outs_used], allow_unused=True)
+
+    every = grads([0, 1, 2, 3], [0, 1])
+    for wanted in ([0], [1], [2], [3], [0, 1], [2, 3], [0, 3]):
+        for got, i in zip(grads(wanted, [0, 1]), wanted):
+            assert torch.equal(got, every[i])
+    only_k = grads([0, 1, 2, 3], [1])
+    assert only_k[0] is None and only_k[2] is None and torch.equal(only_k[1], every[1]) and torch.equal(only_k[3], every[3])
+
+
+def test_gradients_of_views_and_expanded_scalars():
+    """What attention and sums hand back: transposed gradients, and one number for all."""
+    xs, ws, _ = _inputs(2, 9, 4, 2, 64, torch.float32, True, "plain")
+    cache = _table(9, 64).to(DEV)
+    leaves = [t.detach().requires_grad_() for t in xs + ws]
+    outs = layer_ops.qk_norm_rope(*leaves[:2], cache, *leaves[2:])
+    gys = [torch.randn(o.transpose(1, 2).shape, device=DEV).transpose(1, 2) for o in outs]
+    assert not gys[0].is_contiguous()
+    a = torch.autograd.grad(outs, leaves, gys, retain_graph=True)
+    b = torch.autograd.grad(outs, leaves, [g.contiguous() for g in gys], retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    a = torch.autograd.grad(outs[0].sum() + outs[1].sum(), leaves, retain_graph=True)
+    b = torch.autograd.grad(outs, leaves, [torch.ones_like(o) for o in outs])
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_rows_of_zeros_and_empty_batches():
+    (q, k), (w1, w2), _ = _inputs(1, 4, 2, 1, 32, torch.bfloat16, True, "plain")
+    cache = _table(4, 32).to(DEV)
+    q = torch.zeros_like(q).requires_grad_()
+    out, _ = layer_ops.qk_norm_rope(q, k, cache, w1, w2)
+    (g,) = torch.autograd.grad(out.sum(), q)
+    assert not bool(out.any()) and bool(torch.isfinite(g).all())
+    e = torch.zeros(0, 4, 2, 32, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    w = w1.detach().clone().requires_grad_()
+    a, b = layer_ops.qk_norm_rope(e, e[:, :, :1], cache, w, w2)
+    assert a.shape == e.shape and b.shape == (0, 4, 1, 32)
+    ge, gw = torch.autograd.grad(a.sum() + b.sum(), [e, w])
+    assert ge.shape == e.shape and not bool(gw.any())
+    a, b = layer_ops.qk_norm_rope(k, k[:, :, :0], cache)
+    assert b.shape == (1, 4, 0, 32) and torch.equal(a, layer_ops.qk_norm_rope(k, k, cache)[0])
+
+
+def test_agrees_with_the_separate_rotation():
+    """Without scales and interleaved it is ``apply_rope``, bit for bit: the same two products and a difference in fp32."""
+    (q, k), _, _ = _inputs(2, 40, 8, 2, 64, torch.bfloat16, False, "plain")
+    cache = _table(40, 64).to(DEV)
+    a, b = layer_ops.qk_norm_rope(q, k, cache)
+    assert torch.equal(a, layer_ops.apply_rope(q, cache)) and torch.equal(b, layer_ops.apply_rope(k, cache))
+
+
+def test_recorded_into_a_graph():
+    xs, ws, gys = _inputs(2, 50, 8, 2, 64, torch.bfloat16, True, "joined")
+    cache, positions = _table(100, 64).to(DEV), torch.randint(0, 100, (2, 50), device=DEV)
+    leaves = [t.detach().clone().requires_grad_() for t in xs + ws]
+
+    def call():
+        outs = layer_ops.qk_norm_rope(*leaves[:2], cache, *leaves[2:], positions=positions)
+        return list(outs) + list(torch.autograd.grad(outs, leaves, gys))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = call()
+    for i in range(4):
+        with torch.no_grad():
+            for t in leaves[:2]:
+                t.copy_(torch.randn_like(t))
+            positions.copy_(torch.randint(0, 100, (2, 50), device=DEV))
+        graph.replay()
+        got = [t.clone() for t in kept]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, call()))
+
+
+def test_second_derivatives_and_tangents_are_refused():
+    (q, k), (w1, w2), _ = _inputs(1, 2, 2, 1, 32, torch.float32, True, "plain")
+    q.requires_grad_()
+    out, _ = layer_ops.qk_norm_rope(q, k, _table(2, 32).to(DEV), w1, w2)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(out.sum(), q, create_graph=True)
+
+
+def test_a_trace_keeps_the_gradients():
+    (q, k), (w1, w2), gys = _inputs(1, 4, 2, 1, 32, torch.float32, True, "plain")
+    cache = _table(4, 32).to(DEV)
+
+    def f(a, b, c, d):
+        return layer_ops.qk_norm_rope(a, b, cache, c, d)
+
+    leaves = [t.detach().requires_grad_() for t in (q, k, w1, w2)]
+    traced = torch.jit.trace(f, leaves, check_trace=False)
+    got, want = traced(*leaves), f(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(torch.autograd.grad(got, leaves, gys), torch.autograd.grad(want, leaves, gys)):
+        assert torch.equal(a, b)

@@ -20,8 +20,10 @@ from .qat import (
     WeightOnlyInt4Linear,
     ZeroPointDomain,
 )
+from .training.optim import AdamW
 
 __all__ = [
+    "AdamW",
     "NF4Tensor",
     "to_nf4",
     "linear_nf4",

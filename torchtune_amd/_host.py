@@ -52,7 +52,9 @@ class _TracedCall(torch.autograd.Function):
                     for a, need in zip(ctx.rest, ctx.needs_input_grad[1:])]
             outs = getattr(load(), ctx.name)(*args)
             need = [a for a, n in zip(args, ctx.needs_input_grad[1:]) if n]
-            got = iter(torch.autograd.grad(outs, need, grads if isinstance(outs, tuple) else grads[0], allow_unused=True))
+            # some outputs are not differentiable (places, what is only reported)
+            pairs = [(o, g) for o, g in zip(outs, grads) if o.requires_grad] if isinstance(outs, tuple) else [(outs, grads[0])]
+            got = iter(torch.autograd.grad([o for o, _ in pairs], need, [g for _, g in pairs], allow_unused=True))
         return (None, *(next(got) if n else None for n in ctx.needs_input_grad[1:]))
 
 

@@ -20,6 +20,7 @@ TTAMD_MXFP8 = 8
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
+_u32 = ctypes.c_uint32
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 _size = ctypes.c_size_t
@@ -214,6 +215,18 @@ SIGNATURES = {
         _int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
     "ttamd_column_sum_workspace_bytes": (_size, [_i64, _i64]),
     "ttamd_column_sum_bf16": (_int, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_qk_norm_rope_fwd": (_int, [_c_void_p, _c_void_p, _int, _f32, _i64, _i64, _i64, _c_void_p]),
+    "ttamd_qk_norm_rope_bwd_workspace_bytes": (_size, [_i64]),
+    "ttamd_qk_norm_rope_bwd": (_int, [_c_void_p, _c_void_p, _int, _f32, _i64, _i64, _i64, _c_void_p, _size, _c_void_p]),
+    "ttamd_token_logprobs_workspace_bytes": (_size, [_i64, _i64, _int]),
+    "ttamd_token_logprobs_fwd": (
+        _int, [_c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "ttamd_token_logprobs_bwd": (
+        _int, [_c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "ttamd_adamw_key": (_u32, [_i64, _i64, _u32]),
+    "ttamd_adamw_number": (_u32, [_u32, _i64]),
+    "ttamd_adamw_step": (_int, [_c_void_p, _c_void_p, _int, _int, _c_void_p, _u32, _u32, _u32, _c_void_p, _c_void_p]),
+    "ttamd_adamw_moments_bf16": (_int, [_c_void_p, _u32, _c_void_p, _c_void_p, _c_void_p]),
     "ttamd_swiglu_bwd_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }
 
@@ -241,6 +254,40 @@ class MxLoraMember(ctypes.Structure):
 
     _fields_ = [("codes", _c_void_p), ("scales", _c_void_p), ("lora_a", _c_void_p), ("lora_b", _c_void_p), ("bias", _c_void_p),
                 ("y", _c_void_p), ("grad_lora_a", _c_void_p), ("grad_lora_b", _c_void_p), ("N", _i64), ("rank", _int), ("scale", _f32)]
+
+
+class RopeHeads(ctypes.Structure):
+    """``ttamd_rope_heads`` of the header: the query heads, or the key heads."""
+
+    _fields_ = [("x", _c_void_p), ("scale", _c_void_p), ("gy", _c_void_p), ("out", _c_void_p), ("gscale", _c_void_p), ("heads", _i64),
+                ("x_stride", _i64 * 3), ("gy_stride", _i64 * 3)]
+
+
+class RopePositions(ctypes.Structure):
+    """``ttamd_rope_positions`` of the header: the table of angles and which of its rows each token follows."""
+
+    _fields_ = [("cache", _c_void_p), ("cache_rows", _i64), ("positions", _c_void_p), ("stride", _i64 * 3), ("n_axes", _int),
+                ("section", _int * 4), ("interleaved", _int)]
+
+
+class Logits(ctypes.Structure):
+    """``ttamd_logits`` of the header: rows of logits at two nested strides."""
+
+    _fields_ = [("data", _c_void_p), ("dtype", _int), ("rows", _i64), ("V", _i64), ("n_inner", _i64), ("stride_outer", _i64), ("stride_inner", _i64)]
+
+
+class AdamWStates(ctypes.Structure):
+    """``ttamd_adamw_states`` of the header: where the moments of many tensors lie."""
+
+    _fields_ = [("layout", _c_void_p), ("chunk_map", _c_void_p), ("exp_avg", _c_void_p), ("exp_avg_sq", _c_void_p),
+                ("exp_avg_exponent", _c_void_p), ("exp_avg_sq_exponent", _c_void_p), ("state_bits", _int)]
+
+
+class AdamWScalars(ctypes.Structure):
+    """``ttamd_adamw_scalars`` of the header."""
+
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("step", _i64), ("seed", _i64), ("stochastic", _int)]
 
 
 _lock = threading.Lock()

@@ -2,7 +2,7 @@
 
 The library is a plain C-ABI shared object (see ``include/torchtune_amd.h``); it links against the HIP
 runtime only, never against torch.  Next to it goes ``torchtune_amd_host.so``, the extension module that makes layer
-calls into it without the interpreter (``csrc/host_binding.cpp``, ``csrc/host_mx.cpp``).  ``python -m torchtune_amd.build`` rebuilds both.
+calls into it without the interpreter (``csrc/host_*.cpp``).  ``python -m torchtune_amd.build`` rebuilds both.
 """
 from __future__ import annotations
 
@@ -19,9 +19,9 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libtorchtune_amd.so"
 HOST_MODULE = "torchtune_amd_host"
-HOST_SOURCES = ["host_binding.cpp", "host_mx.cpp"]
+HOST_SOURCES = ["host_binding.cpp", "host_mx.cpp", "host_post.cpp"]
 HOST_PATH = LIB_DIR / f"{HOST_MODULE}.so"
-SOURCES = ["capi.hip", "nf4_codec.hip", "fake_quant.hip", "int4_linear.hip", "nf4_gemm.hip", "nf4_gemm_rs.hip", "nf4_gemm_mid.hip", "nf4_gemm_dense.hip", "gemm_tn.hip", "gemm_mid.hip", "nf4_small_m.hip", "lora_skinny.hip", "lora_group.hip", "qlora_linear.hip", "nf4_merge.hip", "neighbours.hip", "mx_codec.hip", "mx_gemm.hip", "mx_few.hip", "mx_dx.hip", "mx_lora.hip", "column_sum.hip"]
+SOURCES = ["capi.hip", "nf4_codec.hip", "fake_quant.hip", "int4_linear.hip", "nf4_gemm.hip", "nf4_gemm_rs.hip", "nf4_gemm_mid.hip", "nf4_gemm_dense.hip", "gemm_tn.hip", "gemm_mid.hip", "nf4_small_m.hip", "lora_skinny.hip", "lora_group.hip", "qlora_linear.hip", "nf4_merge.hip", "neighbours.hip", "mx_codec.hip", "mx_gemm.hip", "mx_few.hip", "mx_dx.hip", "mx_lora.hip", "column_sum.hip", "qk_norm_rope.hip", "token_logprobs.hip", "adamw.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -771,7 +771,8 @@ Tensor straight_through_linear(const Tensor& x, const Tensor& weight, const Tens
 
 }  // namespace
 
-void bind_mx(py::module_& m);  // host_mx.cpp
+void bind_mx(py::module_& m);    // host_mx.cpp
+void bind_post(py::module_& m);  // host_post.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // like torch's own ops the calls run without the interpreter's lock: a launch waits where the queue is full
@@ -790,4 +791,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("straight_through", &straight_through, unlocked);
   m.def("straight_through_linear", &straight_through_linear, unlocked);
   bind_mx(m);
+  bind_post(m);
 }

@@ -1,12 +1,15 @@
-"""RMSNorm, rotary embedding, the SwiGLU gate and the chunk cross entropy as single-pass HIP kernels with autograd.
+"""RMSNorm, rotary embedding, the SwiGLU gate, the chunk cross entropy and token log probabilities as single-pass HIP kernels
+with autograd.
 
 These are the memory-bound neighbours of the quantized linears inside a decoder layer.  The reference runs each as
 a chain of eager kernels: ``RMSNorm`` (``torchtune/modules/rms_norm.py:11-41``), ``Llama3ScaledRoPE.forward``
 (``torchtune/models/llama3_1/_position_embeddings.py:128-190``), ``FeedForward.forward``
 (``torchtune/modules/feed_forward.py:50-53``).  Same arguments and results (to floating-point tolerance); bf16
-tensors on the GPU only, anything else raises.
+tensors on the GPU only (``qk_norm_rope`` and ``token_logprobs``: float32 too), anything else raises.
 """
 from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 from torch import nn
@@ -65,6 +68,32 @@ def qkv_rope_repeat(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: to
     kernel per direction: ``apply_rope(q)``, ``repeat_kv(apply_rope(k), rep)``, ``repeat_kv(v, rep)`` with
     ``rep = n_h // n_kv``, bit for bit."""
     return _host.call("qkv_rope_repeat", q, k, v, cache)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cache: torch.Tensor, q_scale: Optional[torch.Tensor] = None,
+                 k_scale: Optional[torch.Tensor] = None, *, eps: float = 1e-6, positions: Optional[torch.Tensor] = None,
+                 sections: Optional[Sequence[int]] = None, interleaved: bool = True):
+    """Norm of every query and key head and its rotation, one pass forward and one backward: the ``q_norm`` / ``k_norm`` and
+    ``pos_embeddings`` of the reference's attention (``torchtune/modules/attention.py:234-290``), in fp32 and rounded once.
+
+    Args:
+        q, k (torch.Tensor): ``[b, s, n_h, h_d]`` and ``[b, s, n_kv, h_d]``, bfloat16 or float32, ``h_d`` a multiple of 16 up to 512.
+            Views of one projection's output are read where they are.
+        cache (torch.Tensor): float32 ``[positions, h_d / 2, 2]``, cosine and sine of every position and frequency
+        q_scale, k_scale (Optional[torch.Tensor]): ``[h_d]``, of the type of ``q``: ``x / sqrt(mean(x^2) + eps) * scale`` per head.
+            Default: no norm
+        eps (float): added to the mean square
+        positions (Optional[torch.Tensor]): row of ``cache`` for each token, ``[b, s]`` or what broadcasts to it; with ``sections``
+            ``[axes, b, s]``.  Default: 0, 1, .. in every sequence.  A position that is not in ``cache`` gives NaN.
+        sections (Optional[Sequence[int]]): with positions of two to four axes (time, height, width): how many consecutive
+            frequencies follow each; they add up to ``h_d / 2``
+        interleaved (bool): frequency ``i`` turns elements ``2 i`` and ``2 i + 1``; else ``i`` and ``h_d / 2 + i``
+
+    Returns:
+        the two outputs, contiguous.  Differentiable once with respect to ``q``, ``k`` and the scales.
+    """
+    return _host.call("qk_norm_rope", q, k, cache, q_scale, k_scale, float(eps), positions, [] if sections is None else [int(n) for n in sections],
+                      bool(interleaved))
 
 
 class _RepeatKVFn(torch.autograd.Function):
@@ -138,3 +167,38 @@ def cross_entropy_sum(logits: torch.Tensor, target: torch.Tensor, ignore_index: 
     (``torchtune/modules/loss/cross_entropy_loss.py:86-112``).  The gradient w.r.t. the logits is produced in the same
     pass (pre-multiplied by ``scale``) and only rescaled by the incoming gradient in backward; call backward once."""
     return _CrossEntropySumFn.apply(logits, target, ignore_index, scale)
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns; ``None`` where it was not asked for."""
+
+    logprobs: torch.Tensor
+    entropy: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+    top_tokens: Optional[torch.Tensor]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, entropy: bool = False, top: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of given tokens under ``softmax(logits / temperature)``, with the entropy and the most likely
+    alternatives: what preference and policy losses and distillation are made of (the reference's ``logits_to_logprobs``,
+    ``torchtune/rlhf/utils.py``, is an eager log softmax and a gather) and what a sampler reports.  The logits are read once
+    forward, and once more backward; no tensor of their size is kept beside them.
+
+    Args:
+        logits (torch.Tensor): ``[.., V]``, bfloat16 or float32; a shifted view such as ``logits[:, :-1]`` is read where it is
+        tokens (torch.Tensor): int64, a token for each row ``[..]`` or several ``[.., n]``; the same one may occur twice
+        temperature (float): between 1e-6 and 1e6. Default: 1
+        entropy (bool): also return ``-sum p log p`` of each row
+        top (int): also return that many largest log probabilities, at most 64, with their tokens; of equal logits the lower
+            token comes first
+        ignore_index (int): a token that stands for none: its log probability is 0 and has no gradient.  Any other token
+            outside the vocabulary gives NaN.
+
+    Returns:
+        :class:`TokenLogprobs`, float32 and int64.  ``logprobs`` and ``entropy`` are differentiable once with respect to the
+        logits, ``top_logprobs`` is not (pass its tokens as ``tokens`` to train on them).  A row of nothing but ``-inf`` has log
+        probabilities of ``-inf``, entropy 0 and no gradient; NaN or ``+inf`` in a row makes all of it NaN.
+    """
+    logprobs, ent, top_logprobs, top_tokens = _host.call("token_logprobs", logits, tokens, float(temperature), bool(entropy), int(top), int(ignore_index))
+    return TokenLogprobs(logprobs, ent if entropy else None, top_logprobs if top else None, top_tokens if top else None)

@@ -1,3 +1,4 @@
 from . import quantization
+from .optim import AdamW
 
-__all__ = ["quantization"]
+__all__ = ["AdamW", "quantization"]

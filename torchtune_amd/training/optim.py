@@ -1,0 +1,149 @@
+"""AdamW as one kernel over all tensors of a group, with moments of 32 or 8 bits.
+
+The reference's recipes configure ``torch.optim.AdamW(fused=True)`` (``recipes/configs/llama3_1/8B_qlora_single_device.yaml:60-64``)
+or, to save memory, an optimizer of a third package with 8-bit states.  :class:`AdamW` stands in for either.
+"""
+from __future__ import annotations
+
+from itertools import chain
+from typing import Dict, Tuple
+
+import torch
+
+from .. import _host
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` (decoupled weight decay) for parameters on the GPU, bfloat16 or float32.
+
+    A step is ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+    ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``, in fp32 whatever the parameters' type, one pass over
+    all of them.  The moments are held in fp32 or, with ``state_bits=8``, in a byte each and two bytes of exponents for 128
+    elements (a quarter of the memory): the first with a sign, 4 bits of exponent and 3 of mantissa, the second with 4 and 4.
+    They are rounded stochastically, since a change of ``1 - b2`` in a step is smaller than what rounding to the nearest would
+    let through; the numbers are a function of ``seed``, the step, the parameter's place and the element's, so that a run can be
+    repeated and continued.  A gradient that is not finite makes its element NaN for good, as in 32 bits; with 8 bits the 127
+    others of its block lose their moments and stand still.
+
+    Args:
+        params: parameters or groups, as for any ``torch.optim.Optimizer``
+        lr (float): learning rate. Default: 1e-3
+        betas (Tuple[float, float]): decay of the moments. Default: (0.9, 0.999)
+        eps (float): added to the denominator. Default: 1e-8
+        weight_decay (float): Default: 1e-2
+        state_bits (int): 32 or 8. Default: 32
+        stochastic_rounding (bool): round bfloat16 parameters stochastically: updates of less than half a step of the format are
+            then kept on average, as they would be with a float32 copy. Default: False
+        seed (int): of the stochastic rounding. Default: 0
+
+    ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
+    first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
+    other tensors in their place.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  A step cannot be recorded into a
+    graph.
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 *, state_bits: int = 32, stochastic_rounding: bool = False, seed: int = 0) -> None:
+        if isinstance(lr, torch.Tensor):
+            raise TypeError("AdamW: lr must be a number, not a tensor")
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"AdamW: lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
+        if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
+            raise ValueError(f"AdamW: betas must be two numbers in [0, 1), got {betas}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
+        self._plans: Dict[int, tuple] = {}
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self._plans = {}
+
+    def _plan(self, index: int):
+        """The group's native side; it takes over the states that are there already."""
+        params = self.param_groups[index]["params"]
+        known = self._plans.get(index)
+        if known is not None and known[1] is params and known[2] == len(params):
+            return known[0]
+        first = sum(len(g["params"]) for g in self.param_groups[:index])
+        plan = _host.load().AdamWGroup(params, first, self.defaults["state_bits"])
+        given = [i for i, p in enumerate(params) if self.state.get(p)]
+        plan.make(given)
+        for i in given:
+            held = self.state[params[i]]
+            self._show(plan, params, i)
+            for name, tensor in self.state[params[i]].items():
+                if name == "step":
+                    tensor.fill_(int(held[name]))
+                else:
+                    tensor.copy_(held[name].reshape(tensor.shape))
+        self._plans[index] = (plan, params, len(params))
+        return plan
+
+    def _show(self, plan, params, i: int) -> None:
+        names = ("step", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
+        self.state[params[i]] = dict(zip(names, plan.state(i)))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step; with ``closure``, which computes the loss again, its value is returned."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        d = self.defaults
+        for index, group in enumerate(self.param_groups):
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW: amsgrad and maximize are not supported")
+            plan, params = self._plan(index), group["params"]
+            beta1, beta2 = group["betas"]
+            for i in plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], d["seed"], d["stochastic_rounding"]):
+                self._show(plan, params, i)
+        return loss
+
+    def moments(self):
+        """``(exp_avg, exp_avg_sq)`` of all parameters that have states, one after another in their order, as two flat tensors of
+        numbers: the fp32 states themselves where they lie that way already, bfloat16 (exact) for 8-bit states."""
+        firsts, seconds = [], []
+        for index in range(len(self.param_groups)):
+            plan = self._plan(index)
+            whole = plan.whole()
+            for m, v in plan.moments() if whole is None else [whole]:
+                firsts.append(m.reshape(-1))
+                seconds.append(v.reshape(-1))
+        if not firsts:
+            raise RuntimeError("AdamW.moments: no parameter has taken a step yet")
+        return (firsts[0], seconds[0]) if len(firsts) == 1 else (torch.cat(firsts), torch.cat(seconds))
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict) -> None:
+        """What :meth:`state_dict` gave, of an optimizer with as many bits."""
+        saved, eight = state_dict["state"], self.defaults["state_bits"] == 8
+        ids = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
+        params = list(chain.from_iterable(g["params"] for g in self.param_groups))
+        if len(ids) == len(params):  # else the base class refuses it
+            for key, p in zip(ids, params):
+                if key in saved:
+                    self._check_saved(saved[key], p, eight)
+        # the states pass the base class by: it would cast them to the parameters' type
+        super().load_state_dict({**state_dict, "state": {}})
+        for key, p in zip(ids, params):
+            if key in saved:
+                self.state[p] = dict(saved[key])
+        self._plans = {}
+        for index in range(len(self.param_groups)):
+            self._plan(index)
+
+    @staticmethod
+    def _check_saved(held, p, eight: bool) -> None:
+        names = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_exponent", "exp_avg_sq_exponent"} if eight else set())
+        if not names <= set(held):
+            raise ValueError(f"AdamW.load_state_dict: a state holds {sorted(held)}, expected {sorted(names)}")
+        blocks = -(-p.numel() // 128)
+        for name in names - {"step"}:
+            t = held[name]
+            if (t.dtype == torch.uint8) != eight:
+                raise ValueError(f"AdamW.load_state_dict: {name} is {t.dtype}, the states of this optimizer have {8 if eight else 32} bits")
+            if t.numel() != (blocks if name.endswith("exponent") else p.numel()):
+                raise ValueError(f"AdamW.load_state_dict: {name} has {t.numel()} elements, the parameter {p.numel()}")
