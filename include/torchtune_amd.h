@@ -872,22 +872,25 @@ int ttamd_token_logprobs_bwd(const ttamd_logits* logits, const int64_t* tokens, 
  * two halves (exp_avg_sq the high one) of ttamd_adamw_number(key, element) with key = ttamd_adamw_key(seed, step, tensor).
  * stochastic (bf16 parameters): p' is rounded with the low half instead of to nearest.
  *
- * layout: device array of n_all tensors' places; chunk_map: device array, the tensor of each chunk of
- * TTAMD_ADAMW_CHUNK elements, tensors one after another, each beginning a chunk.  Both depend on the sizes only.  The call covers
- * tensors first .. first + n - 1 (n at most TTAMD_ADAMW_TENSORS) and their chunks first_chunk .. first_chunk + n_chunks - 1.
- * params and grads are host arrays of n device pointers.
+ * eps counts as at least 1.1e-19, the root of the smallest normal number.
+ *
+ * chunks: device array, a description of each TTAMD_ADAMW_CHUNK consecutive elements of a tensor, tensors one after another, each
+ * beginning a chunk (an empty tensor has none).  It depends on the sizes only.  The call covers tensors first .. first + n - 1
+ * (n at most TTAMD_ADAMW_TENSORS), whose chunks are first_chunk .. first_chunk + n_chunks - 1.  params and grads are host
+ * arrays of n device pointers.
  */
 #define TTAMD_ADAMW_BLOCK 128
 #define TTAMD_ADAMW_CHUNK 4096
 #define TTAMD_ADAMW_TENSORS 240
-typedef struct ttamd_adamw_place {
-  int64_t offset, numel, block;
-  uint32_t first_chunk; /* counted over all tensors */
-  uint32_t number;      /* the tensor's own, for the numbers above */
-} ttamd_adamw_place;
+typedef struct ttamd_adamw_chunk {
+  int64_t start;         /* its first element in the tensor */
+  int64_t numel;         /* of the tensor */
+  int64_t offset, block; /* of the tensor */
+  uint32_t tensor;
+  uint32_t number; /* the tensor's own, for the numbers above */
+} ttamd_adamw_chunk;
 typedef struct ttamd_adamw_states {
-  const ttamd_adamw_place* layout;
-  const uint32_t* chunk_map;
+  const ttamd_adamw_chunk* chunks;
   void* exp_avg;
   void* exp_avg_sq;
   uint8_t* exp_avg_exponent;    /* state_bits 8 */

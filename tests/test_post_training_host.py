@@ -136,7 +136,7 @@ def test_the_c_entries_check_their_arguments():
     assert lib.ttamd_token_logprobs_bwd(ctypes.byref(logits), p, 1, -100, 1.0, None, p, None, p, None) == -1
     assert lib.ttamd_token_logprobs_bwd(ctypes.byref(logits), p, 1, -100, 1.0, p, None, None, p, None) == -1
 
-    states = _lib.AdamWStates(p, p, p, p, None, None, 32)
+    states = _lib.AdamWStates(p, p, p, None, None, 32)
     scalars = _lib.AdamWScalars(1e-3, 0.9, 0.999, 1e-8, 0.01, 1, 0, 0)
     ptrs = (ctypes.c_void_p * 1)(p)
 

@@ -279,7 +279,7 @@ class Logits(ctypes.Structure):
 class AdamWStates(ctypes.Structure):
     """``ttamd_adamw_states`` of the header: where the moments of many tensors lie."""
 
-    _fields_ = [("layout", _c_void_p), ("chunk_map", _c_void_p), ("exp_avg", _c_void_p), ("exp_avg_sq", _c_void_p),
+    _fields_ = [("chunks", _c_void_p), ("exp_avg", _c_void_p), ("exp_avg_sq", _c_void_p),
                 ("exp_avg_exponent", _c_void_p), ("exp_avg_sq_exponent", _c_void_p), ("state_bits", _int)]
 
 

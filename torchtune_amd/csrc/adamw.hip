@@ -8,7 +8,7 @@
 //
 // One launch covers up to 240 tensors: their addresses travel in the kernel's arguments (they may change from step to step),
 // their sizes and places in the state buffers stand in a table on the GPU (they do not).  A workgroup takes 4096 elements of one
-// tensor, which the chunk map names.
+// tensor; all that it has to know of them is one entry of that table.
 //
 // 8 bits: 128 elements, 16 lanes of 8, share an exponent, so that finding it takes four moves within a row of lanes.  A code is
 // the top of the fp32 number itself, exponent and 3 (m) or 4 (v) bits of mantissa, relative to the block's exponent: writing and
@@ -18,7 +18,7 @@
 namespace ttamd {
 namespace {
 
-constexpr int kChunk = TTAMD_ADAMW_CHUNK, kBlock = TTAMD_ADAMW_BLOCK;
+constexpr int kChunk = TTAMD_ADAMW_CHUNK, kBlock = TTAMD_ADAMW_BLOCK, kPieces = kChunk / 2048;  // 2048: eight elements a thread
 
 // two rounds of multiplication and shift over a sequence with the golden ratio's step
 TT_HD uint32_t spread(uint32_t x) {
@@ -41,7 +41,8 @@ struct StepArgs {
   ttamd_adamw_states st;
   Scalars c;
   uint64_t seed_step;  // of the keys, see key_of
-  uint32_t first, first_chunk;
+  uint32_t first;        // tensor of t[0]
+  uint32_t first_chunk;  // of workgroup 0
   struct {
     void* p;
     const void* g;
@@ -68,108 +69,104 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {  // of sixteen lanes
 
 typedef uint32_t u32x2_at1_t __attribute__((ext_vector_type(2), aligned(1)));
 
-// Eight elements from element `at` of n: whole where they are there, one by one at the end.
-template <class T>
+// Eight elements from element `at` of n (n > 0).  FULL: all of them are there; else each for itself, those behind the end from the last one
+// (what they become is never stored).
+template <class T, bool FULL>
 __device__ __forceinline__ void load8(const typename T::elem* p, int64_t at, int64_t n, float (&v)[8]) {
-  if (at + 8 <= n) {
+  if constexpr (FULL) {
     T::unpack(T::load_once(p + at), v);
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = at + i < n ? T::get(p + at + i) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = T::get(p + (at + i < n ? at + i : n - 1));
+  }
 }
-template <class T>
+template <class T, bool FULL>
 __device__ __forceinline__ void store8(typename T::elem* p, int64_t at, int64_t n, const float (&v)[8]) {
-  if (at + 8 <= n) {
+  if constexpr (FULL) {
     T::store(p + at, T::pack(v));
-    return;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < n) T::put(p + at + i, v[i]);
   }
-  for (int i = 0; i < 8; ++i)
-    if (at + i < n) T::put(p + at + i, v[i]);
 }
-__device__ __forceinline__ void load_codes(const uint8_t* p, int64_t at, int64_t n, uint32_t (&c)[2]) {
-  if (at + 8 <= n) {
-    const u32x2_at1_t v = *reinterpret_cast<const u32x2_at1_t*>(p + at);
-    c[0] = v.x;
-    c[1] = v.y;
-    return;
-  }
-  c[0] = c[1] = 0;
-  for (int i = 0; i < 8; ++i)
-    if (at + i < n) c[i >> 2] |= (uint32_t)p[at + i] << (8 * (i & 3));
+template <bool FULL>
+__device__ __forceinline__ u32x2_at1_t load_codes(const uint8_t* p, int64_t at, int64_t n) {
+  if constexpr (FULL) return __builtin_nontemporal_load(reinterpret_cast<const u32x2_at1_t*>(p + at));
+  u32x2_at1_t c = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i >> 2] |= (uint32_t)p[at + i < n ? at + i : n - 1] << (8 * (i & 3));
+  return c;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t at, int64_t n, const uint32_t (&c)[2]) {
-  if (at + 8 <= n) {
-    *reinterpret_cast<u32x2_at1_t*>(p + at) = u32x2_at1_t{c[0], c[1]};
-    return;
+template <bool FULL>
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t at, int64_t n, const u32x2_at1_t& c) {
+  if constexpr (FULL) {
+    __builtin_nontemporal_store(c, reinterpret_cast<u32x2_at1_t*>(p + at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i < n) p[at + i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
   }
-  for (int i = 0; i < 8; ++i)
-    if (at + i < n) p[at + i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
 }
 
 template <bool FIRST>
 struct Code {  // FIRST: a sign and three bits of mantissa; else four
   static constexpr int mantissa = FIRST ? 3 : 4, drop = 23 - mantissa;
-  static __device__ __forceinline__ float value(uint32_t c, uint32_t base) {
-    const uint32_t size = FIRST ? c & 127u : c;
+  // byte i of c
+  static __device__ __forceinline__ float value(uint32_t c, int i, uint32_t base) {
+    const uint32_t high = c << (24 - 8 * i), size = FIRST ? (high >> 24) & 127u : high >> 24;
     const uint32_t bits = size ? (size + base) << drop : 0u;
-    return bits_f32(FIRST ? bits | (c & 128u) << 24 : bits);
+    return bits_f32(FIRST ? (bits & 0x7fffffffu) | (high & 0x80000000u) : bits);
   }
-  // the number's top bits after `r` (16 bits) has decided which way they are rounded
+  // the number's top bits after 16 bits of r (FIRST: the low ones) have decided which way they are rounded
   static __device__ __forceinline__ uint32_t top(float x, uint32_t r) {
-    const uint32_t size = min(f32_bits(x) & 0x7fffffffu, 0x7f800000u);
-    return (size + (r << (drop - 16)) + (1u << (drop - 17))) >> drop;
+    const uint32_t size = min(FIRST ? f32_bits(x) & 0x7fffffffu : f32_bits(x), 0x7f800000u);
+    const uint32_t half = 1u << (drop - 17), more = FIRST ? (r << (drop - 16)) & (0xffffu << (drop - 16)) : (r >> (32 - drop)) & (0xffffu << (drop - 16));
+    return (size + (more | half)) >> drop;
   }
   static __device__ __forceinline__ uint32_t base(uint32_t exponent) { return (exponent - 15u) << mantissa; }
   static __device__ __forceinline__ uint32_t exponent(uint32_t largest_top) { return max(largest_top >> mantissa, 16u); }
   static __device__ __forceinline__ uint32_t code(uint32_t top, float x, uint32_t base) {
     const int c = (int)top - (int)base;
     if (FIRST) return c < 1 ? 0u : (uint32_t)c | ((f32_bits(x) >> 24) & 128u);
-    return f32_bits(x) << 1 == 0u ? 0u : (uint32_t)max(c, 1);
+    return (uint32_t)max(c, (int)min(f32_bits(x), 1u));  // never 0 unless x is: x is not negative
   }
 };
 
-template <class T, bool EIGHT, bool ROUND>
-__global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
+// What a lane does with eight elements, in three parts, so that the loads of several pieces lie before the first use.
+template <class T, bool EIGHT, bool FULL>
+struct Piece {
   typedef typename T::elem E;
-  const uint32_t chunk = a.first_chunk + blockIdx.x, tensor = a.st.chunk_map[chunk];
-  const ttamd_adamw_place place = a.st.layout[tensor];
-  E* p = reinterpret_cast<E*>(a.t[tensor - a.first].p);
-  const E* g = reinterpret_cast<const E*>(a.t[tensor - a.first].g);
-  const int64_t n = place.numel, start = (int64_t)(chunk - place.first_chunk) * kChunk;
-  uint32_t key = 0;
-  if constexpr (EIGHT || ROUND) key = key_of(a.seed_step, place.number);
-#pragma unroll
-  for (int piece = 0; piece < kChunk / 2048; ++piece) {
-    const int64_t at = start + piece * 2048 + 8 * threadIdx.x;
-    const bool any = at < n;  // lanes behind the end stay for the row maxima
-    float pv[8], gv[8], m[8], v[8];
-    load8<T>(p, at, n, pv);
-    load8<T>(g, at, n, gv);
-    const int64_t block = place.block + at / kBlock;
+  float p[8], g[8], m[8], v[8];
+  u32x2_at1_t mc, vc;
+  uint32_t em, ev;
+
+  __device__ __forceinline__ void load(const StepArgs& a, const ttamd_adamw_chunk& c, const E* params, const E* grads, int64_t at) {
+    load8<T, FULL>(params, at, c.numel, p);
+    load8<T, FULL>(grads, at, c.numel, g);
     if constexpr (EIGHT) {
-      uint32_t mc[2], vc[2], em = 16, ev = 16;
-      load_codes(reinterpret_cast<const uint8_t*>(a.st.exp_avg) + place.offset, at, n, mc);
-      load_codes(reinterpret_cast<const uint8_t*>(a.st.exp_avg_sq) + place.offset, at, n, vc);
-      if (any) {
-        em = a.st.exp_avg_exponent[block];
-        ev = a.st.exp_avg_sq_exponent[block];
-      }
+      mc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(a.st.exp_avg) + c.offset, at, c.numel);
+      vc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(a.st.exp_avg_sq) + c.offset, at, c.numel);
+      const int64_t block = c.block + (FULL ? at : min(at, c.numel - 1)) / kBlock;
+      em = a.st.exp_avg_exponent[block];
+      ev = a.st.exp_avg_sq_exponent[block];
+    } else {
+      load8<F32, FULL>(reinterpret_cast<const float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
+      load8<F32, FULL>(reinterpret_cast<const float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
+    }
+  }
+
+  // The moments are the sequence of roundings that the interface describes.  The change of the parameter takes the hardware's root
+  // and reciprocal, an ulp each.
+  template <bool ROUND>
+  __device__ __forceinline__ void step_and_store(const StepArgs& a, const ttamd_adamw_chunk& c, E* params, int64_t at, uint32_t key) {
+    if constexpr (EIGHT) {
       const uint32_t bm = Code<true>::base(em), bv = Code<false>::base(ev);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        m[i] = Code<true>::value((mc[i >> 2] >> (8 * (i & 3))) & 255u, bm);
-        v[i] = Code<false>::value((vc[i >> 2] >> (8 * (i & 3))) & 255u, bv);
+        m[i] = Code<true>::value(mc[i >> 2], i & 3, bm);
+        v[i] = Code<false>::value(vc[i >> 2], i & 3, bv);
       }
-    } else {
-      load8<F32>(reinterpret_cast<const float*>(a.st.exp_avg) + place.offset, at, n, m);
-      load8<F32>(reinterpret_cast<const float*>(a.st.exp_avg_sq) + place.offset, at, n, v);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m[i] = m[i] * a.c.b1 + gv[i] * a.c.c1;
-      v[i] = v[i] * a.c.b2 + (gv[i] * gv[i]) * a.c.c2;
-      pv[i] = pv[i] * a.c.keep - a.c.rate * (m[i] / (__builtin_sqrtf(v[i]) * a.c.root + a.c.eps));
     }
     uint32_t r[8];
     if constexpr (EIGHT || ROUND) {
@@ -177,74 +174,112 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = spread(x0 + i * kStep);
     }
-    if constexpr (ROUND) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t b = f32_bits(pv[i]);
-        // NaN and infinity as they are
-        pv[i] = (b & 0x7f800000u) == 0x7f800000u ? pv[i] : bits_f32((b + (r[i] & 0xffffu)) & 0xffff0000u);
-      }
+    for (int i = 0; i < 8; ++i) {
+      m[i] = m[i] * a.c.b1 + g[i] * a.c.c1;
+      v[i] = v[i] * a.c.b2 + (g[i] * g[i]) * a.c.c2;
+      const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[i]), a.c.root, a.c.eps);
+      p[i] = __builtin_fmaf(m[i] * a.c.rate, -__builtin_amdgcn_rcpf(d), p[i] * a.c.keep);
+      // infinity stays one: its mantissa has no bits to carry from
+      if constexpr (ROUND) p[i] = p[i] != p[i] ? p[i] : bits_f32((f32_bits(p[i]) + (r[i] & 0xffffu)) & 0xffff0000u);
     }
-    store8<T>(p, at, n, pv);
+    store8<T, FULL>(params, at, c.numel, p);
     if constexpr (EIGHT) {
       uint32_t mt[8], vt[8], mm = 0, vm = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        mt[i] = Code<true>::top(m[i], r[i] & 0xffffu);
-        vt[i] = Code<false>::top(v[i], r[i] >> 16);
-        if (at + i < n) {
+        mt[i] = Code<true>::top(m[i], r[i]);
+        vt[i] = Code<false>::top(v[i], r[i]);
+        if (FULL || at + i < c.numel) {
           mm = max(mm, mt[i]);
           vm = max(vm, vt[i]);
         }
       }
-      const uint32_t em = Code<true>::exponent(row_max(mm)), ev = Code<false>::exponent(row_max(vm));
-      const uint32_t bm = Code<true>::base(em), bv = Code<false>::base(ev);
-      uint32_t mc[2] = {0, 0}, vc[2] = {0, 0};
+      const uint32_t em1 = Code<true>::exponent(row_max(mm)), ev1 = Code<false>::exponent(row_max(vm));
+      const uint32_t bm = Code<true>::base(em1), bv = Code<false>::base(ev1);
+      u32x2_at1_t mo = {0, 0}, vo = {0, 0};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        mc[i >> 2] |= Code<true>::code(mt[i], m[i], bm) << (8 * (i & 3));
-        vc[i >> 2] |= Code<false>::code(vt[i], v[i], bv) << (8 * (i & 3));
+        mo[i >> 2] |= Code<true>::code(mt[i], m[i], bm) << (8 * (i & 3));
+        vo[i >> 2] |= Code<false>::code(vt[i], v[i], bv) << (8 * (i & 3));
       }
-      store_codes(reinterpret_cast<uint8_t*>(a.st.exp_avg) + place.offset, at, n, mc);
-      store_codes(reinterpret_cast<uint8_t*>(a.st.exp_avg_sq) + place.offset, at, n, vc);
-      if (any && (threadIdx.x & 15) == 0) {
-        a.st.exp_avg_exponent[block] = (uint8_t)em;
-        a.st.exp_avg_sq_exponent[block] = (uint8_t)ev;
+      store_codes<FULL>(reinterpret_cast<uint8_t*>(a.st.exp_avg) + c.offset, at, c.numel, mo);
+      store_codes<FULL>(reinterpret_cast<uint8_t*>(a.st.exp_avg_sq) + c.offset, at, c.numel, vo);
+      if ((threadIdx.x & 15) == 0 && (FULL || at < c.numel)) {
+        a.st.exp_avg_exponent[c.block + at / kBlock] = (uint8_t)em1;
+        a.st.exp_avg_sq_exponent[c.block + at / kBlock] = (uint8_t)ev1;
       }
     } else {
-      store8<F32>(reinterpret_cast<float*>(a.st.exp_avg) + place.offset, at, n, m);
-      store8<F32>(reinterpret_cast<float*>(a.st.exp_avg_sq) + place.offset, at, n, v);
+      store8<F32, FULL>(reinterpret_cast<float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
+      store8<F32, FULL>(reinterpret_cast<float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
     }
   }
+};
+
+template <class T, bool EIGHT, bool ROUND>
+__global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
+  typedef typename T::elem E;
+  const ttamd_adamw_chunk c = a.st.chunks[a.first_chunk + blockIdx.x];
+  E* p = reinterpret_cast<E*>(a.t[c.tensor - a.first].p);
+  const E* g = reinterpret_cast<const E*>(a.t[c.tensor - a.first].g);
+  uint32_t key = 0;
+  if constexpr (EIGHT || ROUND) key = key_of(a.seed_step, c.number);
+  const int64_t at = c.start + 8 * threadIdx.x;
+  if (c.start + kChunk <= c.numel) {  // uniform
+    Piece<T, EIGHT, true> x[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) x[i].load(a, c, p, g, at + 2048 * i);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) x[i].template step_and_store<ROUND>(a, c, p, at + 2048 * i, key);
+    return;
+  }
+#pragma unroll 1
+  for (int i = 0; i < kPieces; ++i) {
+    const int64_t here = at + 2048 * i, wave = here - 8 * (threadIdx.x & 63);
+    if (wave >= c.numel) return;  // whole waves: the rows' maxima need all their lanes
+    if (wave + 512 <= c.numel) {
+      Piece<T, EIGHT, true> x;
+      x.load(a, c, p, g, here);
+      x.template step_and_store<ROUND>(a, c, p, here, key);
+    } else {
+      Piece<T, EIGHT, false> x;
+      x.load(a, c, p, g, here);
+      x.template step_and_store<ROUND>(a, c, p, here, key);
+    }
+  }
+}
+
+template <bool FULL>
+__device__ __forceinline__ void read_out(const ttamd_adamw_states& st, const ttamd_adamw_chunk& c, int64_t at, uint16_t* exp_avg, uint16_t* exp_avg_sq) {
+  const u32x2_at1_t mc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(st.exp_avg) + c.offset, at, c.numel);
+  const u32x2_at1_t vc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(st.exp_avg_sq) + c.offset, at, c.numel);
+  const int64_t block = c.block + at / kBlock;
+  const uint32_t bm = Code<true>::base(st.exp_avg_exponent[block]), bv = Code<false>::base(st.exp_avg_sq_exponent[block]);
+  float m[8], v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = Code<true>::value(mc[i >> 2], i & 3, bm);
+    v[i] = Code<false>::value(vc[i >> 2], i & 3, bv);
+  }
+  store8<BF16, FULL>(exp_avg + c.offset, at, c.numel, m);
+  store8<BF16, FULL>(exp_avg_sq + c.offset, at, c.numel, v);
 }
 
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ttamd_adamw_states st, uint16_t* __restrict__ exp_avg,
                                                             uint16_t* __restrict__ exp_avg_sq) {
-  const uint32_t chunk = blockIdx.x;
-  const ttamd_adamw_place place = st.layout[st.chunk_map[chunk]];
-  const int64_t n = place.numel, start = (int64_t)(chunk - place.first_chunk) * kChunk;
+  const ttamd_adamw_chunk c = st.chunks[blockIdx.x];
 #pragma unroll
-  for (int piece = 0; piece < kChunk / 2048; ++piece) {
-    const int64_t at = start + piece * 2048 + 8 * threadIdx.x;
-    if (at >= n) continue;
-    const int64_t block = place.block + at / kBlock;
-    uint32_t mc[2], vc[2];
-    load_codes(reinterpret_cast<const uint8_t*>(st.exp_avg) + place.offset, at, n, mc);
-    load_codes(reinterpret_cast<const uint8_t*>(st.exp_avg_sq) + place.offset, at, n, vc);
-    const uint32_t bm = Code<true>::base(st.exp_avg_exponent[block]), bv = Code<false>::base(st.exp_avg_sq_exponent[block]);
-    float m[8], v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m[i] = Code<true>::value((mc[i >> 2] >> (8 * (i & 3))) & 255u, bm);
-      v[i] = Code<false>::value((vc[i >> 2] >> (8 * (i & 3))) & 255u, bv);
-    }
-    store8<BF16>(exp_avg + place.offset, at, n, m);
-    store8<BF16>(exp_avg_sq + place.offset, at, n, v);
+  for (int i = 0; i < kPieces; ++i) {
+    const int64_t at = c.start + 2048 * i + 8 * threadIdx.x;
+    if (at + 8 <= c.numel)
+      read_out<true>(st, c, at, exp_avg, exp_avg_sq);
+    else if (at < c.numel)
+      read_out<false>(st, c, at, exp_avg, exp_avg_sq);
   }
 }
 
 int check_states(const char* who, const ttamd_adamw_states* s) {
-  TT_REQUIRE(s && s->layout && s->chunk_map && s->exp_avg && s->exp_avg_sq, "%s: null pointer argument", who);
+  TT_REQUIRE(s && s->chunks && s->exp_avg && s->exp_avg_sq, "%s: null pointer argument", who);
   TT_REQUIRE(s->state_bits == 32 || s->state_bits == 8, "%s: states of %d bits (8 or 32)", who, s->state_bits);
   TT_REQUIRE(s->state_bits == 32 || (s->exp_avg_exponent && s->exp_avg_sq_exponent), "%s: null pointer argument", who);
   return TTAMD_OK;
@@ -282,7 +317,8 @@ extern "C" int ttamd_adamw_step(void* const* params, const void* const* grads, i
   for (int i = n; i < TTAMD_ADAMW_TENSORS; ++i) a.t[i] = {nullptr, nullptr};
   a.c = {(float)s->beta1, (float)(1 - s->beta1), (float)s->beta2, (float)(1 - s->beta2), (float)(1 - s->lr * s->weight_decay),
          (float)(s->lr / (1 - __builtin_pow(s->beta1, (double)s->step))), (float)(1 / __builtin_sqrt(1 - __builtin_pow(s->beta2, (double)s->step))),
-         (float)s->eps};
+         // the hardware's root takes what lies below the smallest normal number for 0: the roots of those are below this
+         (float)(s->eps > 1.1e-19 ? s->eps : 1.1e-19)};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(n_chunks), block(256);
   const bool eight = states->state_bits == 8;

@@ -347,20 +347,24 @@ void check_param(const Tensor& p) {
 // Parameters of one type on one device with the buffers that hold their moments.
 struct Block {
   std::vector<Tensor> params;
-  std::vector<ttamd_adamw_place> places;
+  struct Place {
+    int64_t offset, numel, block;
+  };
+  std::vector<Place> places;
   std::vector<uint32_t> chunks;  // first chunk of each tensor, and the end
-  Tensor layout, map, exp_avg, exp_avg_sq, exp_avg_exponent, exp_avg_sq_exponent, steps;
+  Tensor table, exp_avg, exp_avg_sq, exp_avg_exponent, exp_avg_sq_exponent, steps;
   int bits;
+  at::ScalarType type;         // of the parameters
   c10::hip::HIPStream stream;  // that the buffers were made on
 
   Block(std::vector<Tensor> ps, const std::vector<int64_t>& numbers, int bits_)
-      : params(std::move(ps)), bits(bits_), stream(c10::hip::getCurrentHIPStream(params[0].get_device())) {
+      : params(std::move(ps)), bits(bits_), type(params[0].scalar_type()), stream(c10::hip::getCurrentHIPStream(params[0].get_device())) {
     const c10::DeviceGuard guard(params[0].device());
     int64_t n = 0, blocks = 0;
     uint64_t chunk = 0;
     for (size_t i = 0; i < params.size(); ++i) {
       const int64_t m = params[i].numel();
-      places.push_back({n, m, blocks, (uint32_t)chunk, (uint32_t)numbers[i]});
+      places.push_back({n, m, blocks});
       chunks.push_back((uint32_t)chunk);
       n += m;
       blocks += (m + TTAMD_ADAMW_BLOCK - 1) / TTAMD_ADAMW_BLOCK;
@@ -376,20 +380,17 @@ struct Block {
       exp_avg_sq_exponent = at::full_like(exp_avg_exponent, 16);
     }
     steps = at::zeros({(int64_t)params.size()}, at::kLong);
-    const auto host = at::TensorOptions(at::kByte);
-    Tensor l = at::empty({(int64_t)(places.size() * sizeof(ttamd_adamw_place))}, host), c = at::empty({(int64_t)(chunk * 4)}, host);
-    memcpy(l.data_ptr(), places.data(), l.numel());
-    uint32_t* to = (uint32_t*)c.data_ptr();
+    const Tensor host = at::empty({(int64_t)(std::max<uint64_t>(chunk, 1) * sizeof(ttamd_adamw_chunk))}, at::kByte);
+    ttamd_adamw_chunk* to = (ttamd_adamw_chunk*)host.data_ptr();
     for (size_t i = 0; i < params.size(); ++i)
-      for (uint32_t j = chunks[i]; j < chunks[i + 1]; ++j) to[j] = (uint32_t)i;
-    layout = l.to(params[0].device());
-    map = c.to(params[0].device());
+      for (uint32_t j = chunks[i]; j < chunks[i + 1]; ++j)
+        to[j] = {(int64_t)(j - chunks[i]) * TTAMD_ADAMW_CHUNK, places[i].numel, places[i].offset, places[i].block, (uint32_t)i, (uint32_t)numbers[i]};
+    table = host.to(params[0].device());
   }
 
   ttamd_adamw_states states() const {
     ttamd_adamw_states s = {};
-    s.layout = (const ttamd_adamw_place*)layout.data_ptr();
-    s.chunk_map = (const uint32_t*)map.data_ptr();
+    s.chunks = (const ttamd_adamw_chunk*)table.data_ptr();
     s.exp_avg = exp_avg.data_ptr();
     s.exp_avg_sq = exp_avg_sq.data_ptr();
     if (bits == 8) {
@@ -403,7 +404,7 @@ struct Block {
   // The buffers outlive what another stream does with them.
   void used_on(const c10::hip::HIPStream& now) const {
     if (now == stream) return;
-    for (const Tensor* t : {&layout, &map, &exp_avg, &exp_avg_sq, &exp_avg_exponent, &exp_avg_sq_exponent})
+    for (const Tensor* t : {&table, &exp_avg, &exp_avg_sq, &exp_avg_exponent, &exp_avg_sq_exponent})
       if (t->defined()) c10::hip::HIPCachingAllocator::recordStream(t->storage().data_ptr(), now);
   }
 
@@ -428,39 +429,33 @@ struct Block {
     return {m, v};
   }
 
-  // as the parameter lies in memory
-  static Tensor laid_out(const Tensor& g, const Tensor& p, bool dense) {
-    if (g.sizes() == p.sizes() && g.strides() == p.strides() && dense) return g;
-    if (!dense || p.is_contiguous()) return g.contiguous();
-    return at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
-  }
-
   void step(const ttamd_adamw_scalars& scalars) {
     const c10::DeviceGuard guard(params[0].device());
     const auto now = c10::hip::getCurrentHIPStream(params[0].get_device());
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, kAdamW,
                 ": a step cannot be recorded into a graph (its count, and with it the bias corrections, would stand still)");
     // everything is checked before anything is changed
-    for (const Tensor& p : params) {
-      const Tensor& g = p.grad();
+    const size_t n = params.size();
+    std::vector<const Tensor*> grads(n);  // null: none
+    for (size_t i = 0; i < n; ++i) {
+      const Tensor &p = params[i], &g = p.grad();
       if (!g.defined()) continue;
+      grads[i] = &g;
       check_param(p);
       TORCH_CHECK(g.layout() == at::kStrided && !g.key_set().has(c10::DispatchKey::Python), kAdamW, ": gradients must be plain dense tensors");
       TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), kAdamW, ": a gradient is ", g.scalar_type(), ", its parameter ", p.scalar_type());
-      TORCH_CHECK(g.device() == p.device() && p.device() == params[0].device(), kAdamW, ": a parameter or its gradient has left ", params[0].device().str());
-    }
-    for (size_t i = 0; i < params.size(); ++i) {
-      TORCH_CHECK(params[i].numel() == places[i].numel && params[i].scalar_type() == params[0].scalar_type(), kAdamW,
+      TORCH_CHECK(g.device() == p.device() && p.device() == exp_avg.device(), kAdamW, ": a parameter or its gradient has left ", exp_avg.device().str());
+      TORCH_CHECK(p.numel() == places[i].numel && g.sizes() == p.sizes() && p.scalar_type() == type, kAdamW,
                   ": a parameter's size or type has changed");
     }
     used_on(now);
     const ttamd_adamw_states s = states();
-    const int dtype = type_code(params[0], kAdamW);
+    const int dtype = type == at::kBFloat16 ? TTAMD_BF16 : TTAMD_F32;
     int64_t* count = steps.data_ptr<int64_t>();
     void* p[TTAMD_ADAMW_TENSORS];
     const void* g[TTAMD_ADAMW_TENSORS];
-    for (size_t first = 0; first < params.size();) {
-      if (!params[first].grad().defined()) {
+    for (size_t first = 0; first < n;) {
+      if (!grads[first]) {
         ++first;
         continue;
       }
@@ -468,18 +463,23 @@ struct Block {
       std::vector<Tensor> hold;
       std::vector<std::pair<Tensor, Tensor>> back;
       size_t end = first;
-      for (; end < params.size() && end - first < TTAMD_ADAMW_TENSORS && params[end].grad().defined() && count[end] == count[first]; ++end) {
-        const Tensor& t = params[end];
+      for (; end < n && end - first < TTAMD_ADAMW_TENSORS && grads[end] && count[end] == count[first]; ++end) {
+        const Tensor &t = params[end], &grad = *grads[end];
         const bool dense = t.is_non_overlapping_and_dense();
-        Tensor at = t.detach();
-        if (!dense) {
-          back.push_back({at, at.contiguous()});
-          at = back.back().second;
+        if (dense) {
+          p[end - first] = t.data_ptr();
+        } else {
+          const Tensor plain = t.detach();
+          back.push_back({plain, plain.contiguous()});
+          p[end - first] = back.back().second.data_ptr();
         }
-        Tensor grad = laid_out(t.grad(), t, dense);
-        p[end - first] = at.data_ptr();
-        g[end - first] = grad.data_ptr();
-        if (!grad.is_same(t.grad())) hold.push_back(std::move(grad));
+        if (dense && grad.strides() == t.strides()) {
+          g[end - first] = grad.data_ptr();
+        } else {
+          // as the parameter lies in memory
+          hold.push_back(!dense || t.is_contiguous() ? grad.contiguous() : at::empty_strided(t.sizes(), t.strides(), grad.options()).copy_(grad));
+          g[end - first] = hold.back().data_ptr();
+        }
         // an empty tensor has no address; nothing reads it
         if (t.numel() == 0) g[end - first] = p[end - first] = exp_avg.data_ptr();
       }
