@@ -10,12 +10,14 @@
 // Everything is computed in fp32 from the inputs and rounded once.  Nothing but the inputs is kept for the backward: the row is
 // read there anyway, and its r costs less than reading one that was kept.
 //
-// Bound: HBM.  A row (one head of one token) belongs to G = 2^ceil(log2(D / 16)) neighbouring lanes, each with 16 of its elements:
-// those that frequencies 8 j .. 8 j + 7 turn, so that a pair never leaves its lane and one piece of the table serves both pairings.
+// Bound: HBM.  A row (one head of one token) belongs to G = 8, 16, 32 or 64 neighbouring lanes, each with eight of its elements,
+// which are whole pairs.
 #include "row_vec.h"
 
 namespace ttamd {
 namespace {
+
+constexpr int kBwdGrid = 1280;  // workgroups of the backward with scale gradients, one more after rounding
 
 struct Part {
   const void* x;
@@ -24,6 +26,8 @@ struct Part {
   void* out;
   int64_t xs[3], gs[3];  // of batch, token, head
   uint32_t heads;
+  uint32_t units;  // pieces of a token's heads
+  uint32_t wgs;    // workgroups
 };
 
 struct RopeArgs {
@@ -35,63 +39,58 @@ struct RopeArgs {
   int end[3];  // first frequencies of the axes 1 .. 3
   int n_axes;
   uint32_t S, tokens;  // tokens = B * S
+  uint32_t some;  // heads in a unit
   int D, lanes, log_group;
-  float eps;
+  float eps, inv_D;
 };
 
-template <bool INTER>
-struct Pairs {  // element of the lane's sixteen
+// A lane's eight elements: 8 j .. 8 j + 7, or four of the head's first half and four of its second, 4 j .. 4 j + 3 and
+// D / 2 + 4 j ..  The latter where a pair is made of both halves, and for fp32, whose lanes then write whole lines together.
+// Pair p of a lane is elements first(p) and second(p) of the eight, and turned by `frequency`.
+template <class T, bool INTER>
+struct Lane {
+  typedef typename T::elem E;
+  static constexpr bool split = !INTER || sizeof(E) == 4;
   static constexpr int first(int p) { return INTER ? 2 * p : p; }
-  static constexpr int second(int p) { return INTER ? 2 * p + 1 : p + 8; }
+  static constexpr int second(int p) { return INTER ? 2 * p + 1 : p + 4; }
+  static __device__ __forceinline__ int element(int j, int e, int D) { return split ? 4 * j + (e & 3) + (e >> 2) * (D >> 1) : 8 * j + e; }
+  static __device__ __forceinline__ int frequency(int j, int p, int D) {
+    return split && INTER ? 2 * j + (p & 1) + (p >> 1) * (D >> 2) : 4 * j + p;
+  }
+  typename T::Raw raw;
+  __device__ __forceinline__ void load(const E* p, int j, int D, bool active) {
+    raw = typename T::Raw{};
+    if (!active) return;
+    if constexpr (split)
+      raw = T::join(T::load4_once(p + 4 * j), T::load4_once(p + 4 * j + (D >> 1)));
+    else
+      raw = T::load_once(p + 8 * j);
+  }
+  __device__ __forceinline__ void unpack(float (&v)[8]) const { T::unpack(raw, v); }
+  static __device__ __forceinline__ void store(E* p, int j, int D, const float (&v)[8]) {
+    const typename T::Raw r = T::pack(v);
+    if constexpr (split) {
+      T::store4(p + 4 * j, T::low(r));
+      T::store4(p + 4 * j + (D >> 1), T::high(r));
+    } else {
+      T::store(p + 8 * j, r);
+    }
+  }
 };
 
-// where a lane's two pieces of eight begin
-template <bool INTER>
-__device__ __forceinline__ int piece(int j, int which, int D) {
-  return INTER ? 16 * j + 8 * which : 8 * j + (D >> 1) * which;
-}
-
-template <class T, bool INTER>
-__device__ __forceinline__ void load16(const typename T::elem* p, int j, int D, bool active, float (&v)[16]) {
-  float a[8], b[8];
-  typename T::Raw ra = {}, rb = {};
-  if (active) {
-    ra = T::load_once(p + piece<INTER>(j, 0, D));
-    rb = T::load_once(p + piece<INTER>(j, 1, D));
-  }
-  T::unpack(ra, a);
-  T::unpack(rb, b);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = a[i];
-    v[8 + i] = b[i];
-  }
-}
-
-template <class T, bool INTER>
-__device__ __forceinline__ void store16(typename T::elem* p, int j, int D, const float (&v)[16]) {
-  float a[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a[i] = v[i];
-    b[i] = v[8 + i];
-  }
-  T::store(p + piece<INTER>(j, 0, D), T::pack(a));
-  T::store(p + piece<INTER>(j, 1, D), T::pack(b));
-}
-
-// cosines and sines of frequencies 8 j .. 8 j + 7 at token (b, s).  A position outside the table gives NaN and reads nothing.
-__device__ __forceinline__ void angles(const RopeArgs& a, uint32_t b, uint32_t s, int j, bool active, float (&cs)[8], float (&sn)[8]) {
+// cosines and sines of a lane's four pairs at token (b, s).  A position outside the table gives NaN and reads nothing.
+template <class L>
+__device__ __forceinline__ void angles(const RopeArgs& a, uint32_t b, uint32_t s, int j, bool active, float (&cs)[4], float (&sn)[4]) {
   const int half = a.D >> 1;
+  const float nan = __builtin_nanf("");
   if (a.n_axes <= 1) {  // uniform
     const int64_t pos = a.pos ? a.pos[b * a.ps[1] + s * a.ps[2]] : (int64_t)s;
     const bool inside = active && (uint64_t)pos < (uint64_t)a.cache_rows;
-    const f32x4_at4_t* c = reinterpret_cast<const f32x4_at4_t*>(a.cache + (pos * half + 8 * j) * 2);
+    const float* c = a.cache + pos * half * 2;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float nan = __builtin_nanf("");
+    for (int q = 0; q < 2; ++q) {
       f32x4_at4_t v = {nan, nan, nan, nan};
-      if (inside) v = c[q];
+      if (inside) v = *reinterpret_cast<const f32x4_at4_t*>(c + 2 * L::frequency(j, 2 * q, a.D));
       cs[2 * q] = v.x;
       sn[2 * q] = v.y;
       cs[2 * q + 1] = v.z;
@@ -103,24 +102,26 @@ __device__ __forceinline__ void angles(const RopeArgs& a, uint32_t b, uint32_t s
 #pragma unroll
   for (int x = 0; x < 4; ++x) pos[x] = x < a.n_axes ? a.pos[x * a.ps[0] + b * a.ps[1] + s * a.ps[2]] : 0;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int i = 8 * j + p;
+  for (int p = 0; p < 4; ++p) {
+    const int i = L::frequency(j, p, a.D);
     const int64_t at = i < a.end[0] ? pos[0] : i < a.end[1] ? pos[1] : i < a.end[2] ? pos[2] : pos[3];
     typedef float f32x2_t __attribute__((ext_vector_type(2)));
-    f32x2_t v = {__builtin_nanf(""), __builtin_nanf("")};
+    f32x2_t v = {nan, nan};
     if (active && (uint64_t)at < (uint64_t)a.cache_rows) v = *reinterpret_cast<const f32x2_t*>(a.cache + (at * half + i) * 2);
     cs[p] = v.x;
     sn[p] = v.y;
   }
 }
 
-// the sum over the 2^log_group lanes of a row, in every one of them
-__device__ __forceinline__ float row_sum(float v, int log_group) {
-  if (log_group > 0) v += row_partner<1>(v);
-  if (log_group > 1) v += row_partner<2>(v);
-  if (log_group > 2) v += row_partner<4>(v);
-  if (log_group > 3) v += row_partner<8>(v);
-  if (log_group > 4) v += __shfl_xor(v, 16, kWave);
+// the sum over the 2^LOG lanes of a row, in every one of them
+template <int LOG>
+__device__ __forceinline__ float row_sum(float v) {
+  v += row_partner<1>(v);
+  v += row_partner<2>(v);
+  v += row_partner<4>(v);
+  if constexpr (LOG > 3) v += row_partner<8>(v);
+  if constexpr (LOG > 4) v += __shfl_xor(v, 16, kWave);
+  if constexpr (LOG > 5) v += __shfl_xor(v, 32, kWave);
   return v;
 }
 
@@ -130,118 +131,151 @@ __device__ __forceinline__ float inverse_root(float v) {
   return sizeof(typename T::elem) == 2 ? __builtin_amdgcn_rsqf(v) : 1.f / __builtin_sqrtf(v);
 }
 
-template <class T, bool NORM, bool INTER>
+// What a group of lanes works on: every units-th head of one token, one after another, so that the angles are read once for them
+// and the next head is on its way while one is worked on.  Neighbouring groups work on neighbouring heads.
+struct Unit {
+  uint32_t token, b, s, head;
+  __device__ __forceinline__ Unit(const RopeArgs& a, const Part& part, uint32_t u) {
+    token = u / part.units;
+    head = u - token * part.units;
+    b = token / a.S;
+    s = token - b * a.S;
+  }
+};
+
+template <class T, int LOG, bool NORM, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_rope_fwd_kernel(const RopeArgs a) {
   typedef typename T::elem E;
-  const uint32_t row = (uint32_t)(((uint64_t)blockIdx.x * 256 + threadIdx.x) >> a.log_group);
-  const uint32_t H = a.part[0].heads + a.part[1].heads;
-  if (row >= a.tokens * H) return;  // the lanes of a row leave together
-  const int j = threadIdx.x & ((1 << a.log_group) - 1);
-  const bool active = j < a.lanes;
-  const uint32_t token = row / H, h = row - token * H, b = token / a.S, s = token - b * a.S;
-  const bool key = h >= a.part[0].heads;
-  const Part& part = a.part[key];
-  const uint32_t head = key ? h - a.part[0].heads : h;
-  float x[16], w[16], cs[8], sn[8];
-  load16<T, INTER>(reinterpret_cast<const E*>(part.x) + b * part.xs[0] + s * part.xs[1] + head * part.xs[2], j, a.D, active, x);
-  angles(a, b, s, j, active, cs, sn);
+  typedef Lane<T, INTER> L;
+  const int j = threadIdx.x & ((1 << LOG) - 1);
+  const bool active = j < a.lanes, key = blockIdx.x >= a.part[0].wgs;
+  const Part& part = a.part[key];  // uniform
+  const uint32_t u = (uint32_t)(((uint64_t)(blockIdx.x - (key ? a.part[0].wgs : 0)) * 256 + threadIdx.x) >> LOG);
+  if (u >= a.tokens * part.units) return;  // the lanes of a group leave together
+  Unit at(a, part, u);
+  const E* x = reinterpret_cast<const E*>(part.x) + at.b * part.xs[0] + at.s * part.xs[1] + at.head * part.xs[2];
+  E* out = reinterpret_cast<E*>(part.out) + ((int64_t)at.token * part.heads + at.head) * a.D;
+  L row;
+  row.load(x, j, a.D, active);
+  float w[8], cs[4], sn[4];
+  angles<L>(a, at.b, at.s, j, active, cs, sn);
   if constexpr (NORM) {
-    load16<T, INTER>(reinterpret_cast<const E*>(part.scale), j, a.D, active, w);
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
-    const float r = inverse_root<T>(row_sum(ss, a.log_group) / (float)a.D + a.eps);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
+    L scale;
+    scale.load(reinterpret_cast<const E*>(part.scale), j, a.D, active);
+    scale.unpack(w);
   }
-  float o[16];
+  const int64_t step = part.units * part.xs[2], out_step = (int64_t)part.units * a.D;
+  for (uint32_t h = at.head; h < part.heads; h += part.units, x += step, out += out_step) {
+    float v[8], o[8];
+    row.unpack(v);
+    if (h + part.units < part.heads) row.load(x + step, j, a.D, active);
+    if constexpr (NORM) {
+      float ss = 0.f;
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const float u = x[Pairs<INTER>::first(p)], v = x[Pairs<INTER>::second(p)];
-    o[Pairs<INTER>::first(p)] = u * cs[p] - v * sn[p];
-    o[Pairs<INTER>::second(p)] = v * cs[p] + u * sn[p];
+      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+      const float r = inverse_root<T>(row_sum<LOG>(ss) * a.inv_D + a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float c = v[L::first(p)], d = v[L::second(p)];
+      o[L::first(p)] = c * cs[p] - d * sn[p];
+      o[L::second(p)] = d * cs[p] + c * sn[p];
+    }
+    if (active) L::store(out, j, a.D, o);
   }
-  if (active) store16<T, INTER>(reinterpret_cast<E*>(part.out) + ((int64_t)token * part.heads + head) * a.D, j, a.D, o);
 }
 
-constexpr int kBwdGrid = 1024;  // workgroups of the backward with scale gradients; each leaves a row of partial sums per part
-
-// GSCALE: a fixed number of workgroups walk the rows, first those of the queries, then those of the keys, and each lane sums the
-// scale gradient of its elements over the rows that it sees; else there is a workgroup for every 256 / G rows.
-template <class T, bool NORM, bool INTER, bool GSCALE>
+// GSCALE: a workgroup walks units of its part with a stride of the part's workgroups, and each lane sums the scale gradient of its
+// elements over all that it sees; else there is a workgroup for every 256 / G units.
+template <class T, int LOG, bool NORM, bool INTER, bool GSCALE>
 __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const RopeArgs a, float* __restrict__ partial) {
   typedef typename T::elem E;
+  typedef Lane<T, INTER> L;
   __shared__ float sums[GSCALE ? 512 : 1];
-  const int G = 1 << a.log_group, j = threadIdx.x & (G - 1);
-  const bool active = j < a.lanes;
-  const uint32_t per_wg = 256u >> a.log_group;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Part& part = a.part[which];
-    float w[16], gs[16];
+  const int G = 1 << LOG, j = threadIdx.x & (G - 1);
+  const bool active = j < a.lanes, key = blockIdx.x >= a.part[0].wgs;
+  const uint32_t per_wg = 256u >> LOG;
+  const Part& part = a.part[key];  // uniform
+  float w[8], gs[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gs[i] = 0.f;
-    if constexpr (NORM) {
-      if (part.heads) load16<T, INTER>(reinterpret_cast<const E*>(part.scale), j, a.D, active, w);
-    }
-    const uint64_t rows = (uint64_t)a.tokens * part.heads;
-    for (uint64_t row0 = (uint64_t)blockIdx.x * per_wg; row0 < rows; row0 += (uint64_t)gridDim.x * per_wg) {
-      const uint32_t row = (uint32_t)row0 + (threadIdx.x >> a.log_group);
-      if (row >= rows) continue;  // the lanes of a row together
-      const uint32_t token = row / part.heads, head = row - token * part.heads, b = token / a.S, s = token - b * a.S;
-      float gy[16], x[16], cs[8], sn[8], g[16];
-      load16<T, INTER>(reinterpret_cast<const E*>(part.gy) + b * part.gs[0] + s * part.gs[1] + head * part.gs[2], j, a.D, active, gy);
-      if constexpr (NORM)
-        load16<T, INTER>(reinterpret_cast<const E*>(part.x) + b * part.xs[0] + s * part.xs[1] + head * part.xs[2], j, a.D, active, x);
-      angles(a, b, s, j, active, cs, sn);
+  for (int i = 0; i < 8; ++i) gs[i] = 0.f;
+  if constexpr (NORM) {
+    L scale;
+    scale.load(reinterpret_cast<const E*>(part.scale), j, a.D, active);
+    scale.unpack(w);
+  }
+  const uint64_t units = (uint64_t)a.tokens * part.units;
+  const int64_t g_step = part.units * part.gs[2], x_step = part.units * part.xs[2], out_step = (int64_t)part.units * a.D;
+  for (uint64_t u = (uint64_t)(blockIdx.x - (key ? a.part[0].wgs : 0)) * per_wg + (threadIdx.x >> LOG); u < units;
+       u += (uint64_t)part.wgs * per_wg) {  // the lanes of a group together
+    const Unit at(a, part, (uint32_t)u);
+    const E* gyp = reinterpret_cast<const E*>(part.gy) + at.b * part.gs[0] + at.s * part.gs[1] + at.head * part.gs[2];
+    const E* xp = reinterpret_cast<const E*>(part.x) + at.b * part.xs[0] + at.s * part.xs[1] + at.head * part.xs[2];
+    E* out = reinterpret_cast<E*>(part.out) + ((int64_t)at.token * part.heads + at.head) * a.D;
+    L gy_row, x_row;
+    gy_row.load(gyp, j, a.D, active);
+    if constexpr (NORM) x_row.load(xp, j, a.D, active);
+    float cs[4], sn[4];
+    angles<L>(a, at.b, at.s, j, active, cs, sn);
+    for (uint32_t h = at.head; h < part.heads; h += part.units, gyp += g_step, xp += x_step, out += out_step) {
+      float gy[8], x[8], g[8];
+      gy_row.unpack(gy);
+      if constexpr (NORM) x_row.unpack(x);
+      if (h + part.units < part.heads) {
+        gy_row.load(gyp + g_step, j, a.D, active);
+        if constexpr (NORM) x_row.load(xp + x_step, j, a.D, active);
+      }
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const float u = gy[Pairs<INTER>::first(p)], v = gy[Pairs<INTER>::second(p)];
-        g[Pairs<INTER>::first(p)] = u * cs[p] + v * sn[p];
-        g[Pairs<INTER>::second(p)] = v * cs[p] - u * sn[p];
+      for (int p = 0; p < 4; ++p) {
+        const float c = gy[L::first(p)], d = gy[L::second(p)];
+        g[L::first(p)] = c * cs[p] + d * sn[p];
+        g[L::second(p)] = d * cs[p] - c * sn[p];
       }
       if constexpr (NORM) {
         float ss = 0.f, dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
-        const float r = inverse_root<T>(row_sum(ss, a.log_group) / (float)a.D + a.eps);
+        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+        const float r = inverse_root<T>(row_sum<LOG>(ss) * a.inv_D + a.eps);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if constexpr (GSCALE) gs[i] += active ? g[i] * x[i] * r : 0.f;  // idle lanes hold NaN angles
+        for (int i = 0; i < 8; ++i) {
+          const float gx = g[i] * x[i];  // an idle lane's angles are NaN; it adds nothing to the row and keeps its sums to itself
+          if constexpr (GSCALE) gs[i] = __builtin_fmaf(gx, r, gs[i]);
           g[i] *= w[i];
-          dot += active ? g[i] * x[i] : 0.f;
+          dot = __builtin_fmaf(gx, w[i], dot);
         }
-        const float c = row_sum(dot, a.log_group) / (float)a.D * r * r;
+        const float c = row_sum<LOG>(active ? dot : 0.f) * a.inv_D * r * r;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = r * (g[i] - x[i] * c);
+        for (int i = 0; i < 8; ++i) g[i] = r * __builtin_fmaf(-c, x[i], g[i]);
       }
-      if (active && part.out) store16<T, INTER>(reinterpret_cast<E*>(part.out) + (int64_t)row * a.D, j, a.D, g);
+      if (active && part.out) L::store(out, j, a.D, g);
     }
-    if constexpr (GSCALE) {
-      // the lanes that hold the same elements meet in LDS, one row of the workgroup after another: a fixed order
-      for (int r = 0; r < (int)per_wg; ++r) {
-        __syncthreads();
-        if ((int)(threadIdx.x >> a.log_group) != r || !active) continue;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float* at = sums + piece<INTER>(j, i >> 3, a.D) + (i & 7);
-          *at = r ? *at + gs[i] : gs[i];
-        }
-      }
+  }
+  if constexpr (GSCALE) {
+    // the lanes that hold the same elements meet in LDS, one group of the workgroup after another: a fixed order
+    for (int r = 0; r < (int)per_wg; ++r) {
       __syncthreads();
-      for (int d = threadIdx.x; d < a.D; d += 256) partial[((int64_t)which * gridDim.x + blockIdx.x) * a.D + d] = sums[d];
+      if ((int)(threadIdx.x >> LOG) != r || !active) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float* at = sums + L::element(j, i, a.D);
+        *at = r ? *at + gs[i] : gs[i];
+      }
     }
+    __syncthreads();
+    for (int d = threadIdx.x; d < a.D; d += 256) partial[(int64_t)blockIdx.x * a.D + d] = sums[d];
   }
 }
 
-// gscale[d] = sum over the workgroups' partial sums, in slices of a fixed order; blockIdx.y is the part
+// gscale[d] = sum over the partial sums of the part's workgroups, in slices of a fixed order; blockIdx.y is the part
 template <class T>
-__global__ __launch_bounds__(1024) void qk_norm_rope_gscale_kernel(const float* __restrict__ partial, int n, int D, void* gq, void* gk) {
+__global__ __launch_bounds__(1024) void qk_norm_rope_gscale_kernel(const float* __restrict__ partial, int nq, int nk, int D, void* gq, void* gk) {
   typedef typename T::elem E;
   __shared__ float red[64][17];
   const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, d = blockIdx.x * 16 + col;  // D % 16 == 0
-  const int per = (n + 63) / 64, lo = slice * per, hi = min(lo + per, n);
-  const float* p = partial + (int64_t)blockIdx.y * n * D + d;
+  const int n = blockIdx.y ? nk : nq, per = (n + 63) / 64, lo = slice * per, hi = min(lo + per, n);
+  const float* p = partial + (int64_t)(blockIdx.y ? nq : 0) * D + d;
   float s = 0.f;
 #pragma unroll 4
   for (int w = lo; w < hi; ++w) s += p[(int64_t)w * D];
@@ -253,6 +287,8 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_gscale_kernel(const float* 
   for (int i = 0; i < 64; ++i) s += red[i][col];
   T::put(out + d, s);
 }
+
+unsigned workgroups(int64_t units, int log_group) { return (unsigned)(((units << log_group) + 255) / 256); }
 
 int prepare(const char* who, RopeArgs& a, const ttamd_rope_heads* parts, const ttamd_rope_positions* at, int dtype, float eps, int64_t B,
             int64_t S, int64_t D, bool backward) {
@@ -303,31 +339,45 @@ int prepare(const char* who, RopeArgs& a, const ttamd_rope_heads* parts, const t
   a.S = (uint32_t)S;
   a.tokens = (uint32_t)(B * S);
   a.D = (int)D;
-  a.lanes = (int)(D / 16);
-  a.log_group = 0;
+  a.lanes = (int)(D / 8);
+  a.log_group = 3;
   while ((1 << a.log_group) < a.lanes) ++a.log_group;
   a.eps = eps;
+  a.inv_D = (float)(1.0 / (double)D);
+  // as many heads in a unit as leave lanes for four waves on every SIMD of the chip
+  a.some = 4;
+  while (a.some > 1 && ((B * S * heads) << a.log_group) < (int64_t)a.some * 4 * 1024 * kWave) a.some >>= 1;
+  for (Part& q : a.part) {
+    q.units = (q.heads + a.some - 1) / a.some;
+    q.wgs = workgroups((int64_t)a.tokens * q.units, a.log_group);
+  }
   return TTAMD_OK;
 }
-
-unsigned workgroups(int64_t rows, int log_group) { return (unsigned)(((rows << log_group) + 255) / 256); }
 
 }  // namespace
 }  // namespace ttamd
 
 using namespace ttamd;
 
-#define TT_ROPE_CALL(T, NORM_, INTER_, LAUNCH)  \
-  if (NORM_) {                                  \
-    if (INTER_) {                               \
-      LAUNCH(T, true, true)                     \
-    } else {                                    \
-      LAUNCH(T, true, false)                    \
-    }                                           \
-  } else if (INTER_) {                          \
-    LAUNCH(T, false, true)                      \
-  } else {                                      \
-    LAUNCH(T, false, false)                     \
+// LAUNCH(type, log of a row's lanes, norm, interleaved) with what the call asks for
+#define TT_ROPE_LANES(T, N, I, LAUNCH) \
+  switch (a.log_group) {               \
+    case 3: LAUNCH(T, 3, N, I); break; \
+    case 4: LAUNCH(T, 4, N, I); break; \
+    case 5: LAUNCH(T, 5, N, I); break; \
+    default: LAUNCH(T, 6, N, I);       \
+  }
+#define TT_ROPE_PAIRS(T, N, LAUNCH)           \
+  if (at->interleaved) {                      \
+    TT_ROPE_LANES(T, N, true, LAUNCH)         \
+  } else {                                    \
+    TT_ROPE_LANES(T, N, false, LAUNCH)        \
+  }
+#define TT_ROPE_CALL(N, LAUNCH)               \
+  if (dtype == TTAMD_BF16) {                  \
+    TT_ROPE_PAIRS(BF16, N, LAUNCH)            \
+  } else {                                    \
+    TT_ROPE_PAIRS(F32, N, LAUNCH)             \
   }
 
 extern "C" int ttamd_qk_norm_rope_fwd(const ttamd_rope_heads* parts, const ttamd_rope_positions* at, int dtype, float eps, int64_t B,
@@ -335,20 +385,20 @@ extern "C" int ttamd_qk_norm_rope_fwd(const ttamd_rope_heads* parts, const ttamd
   RopeArgs a;
   if (int rc = prepare("qk_norm_rope_fwd", a, parts, at, dtype, eps, B, S, head_dim, false)) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid(workgroups((int64_t)a.tokens * (a.part[0].heads + a.part[1].heads), a.log_group)), block(256);
+  const dim3 grid(a.part[0].wgs + a.part[1].wgs), block(256);
   const bool norm = parts[0].scale || parts[1].scale;
-#define TT_LAUNCH(T, N, I) qk_norm_rope_fwd_kernel<T, N, I><<<grid, block, 0, st>>>(a);
-  if (dtype == TTAMD_BF16) {
-    TT_ROPE_CALL(BF16, norm, at->interleaved, TT_LAUNCH)
+#define TT_LAUNCH(T, L, N, I) qk_norm_rope_fwd_kernel<T, L, N, I><<<grid, block, 0, st>>>(a)
+  if (norm) {
+    TT_ROPE_CALL(true, TT_LAUNCH)
   } else {
-    TT_ROPE_CALL(F32, norm, at->interleaved, TT_LAUNCH)
+    TT_ROPE_CALL(false, TT_LAUNCH)
   }
 #undef TT_LAUNCH
   return check_launch("qk_norm_rope_fwd");
 }
 
 extern "C" size_t ttamd_qk_norm_rope_bwd_workspace_bytes(int64_t head_dim) {
-  return head_dim > 0 ? (size_t)kBwdGrid * 2 * (size_t)head_dim * sizeof(float) : 0;
+  return head_dim > 0 ? (size_t)(kBwdGrid + 1) * (size_t)head_dim * sizeof(float) : 0;
 }
 
 extern "C" int ttamd_qk_norm_rope_bwd(const ttamd_rope_heads* parts, const ttamd_rope_positions* at, int dtype, float eps, int64_t B,
@@ -360,29 +410,30 @@ extern "C" int ttamd_qk_norm_rope_bwd(const ttamd_rope_heads* parts, const ttamd
   const bool norm = parts[0].scale || parts[1].scale;
   void* gq = parts[0].heads ? parts[0].gscale : nullptr;
   void* gk = parts[1].heads ? parts[1].gscale : nullptr;
-  const unsigned most = workgroups((int64_t)a.tokens * (a.part[0].heads > a.part[1].heads ? a.part[0].heads : a.part[1].heads), a.log_group);
   if (gq || gk) {
     const size_t need = ttamd_qk_norm_rope_bwd_workspace_bytes(head_dim);
     TT_REQUIRE(workspace && aligned16(workspace), "qk_norm_rope_bwd: the gradients of the scales need a 16-byte aligned workspace");
     if (workspace_bytes < need) return fail(TTAMD_EWORKSPACE, "qk_norm_rope_bwd: workspace has %zu bytes, needs %zu", workspace_bytes, need);
     float* partial = reinterpret_cast<float*>(workspace);
-    const dim3 grid(most < (unsigned)kBwdGrid ? most : (unsigned)kBwdGrid), sum_grid((unsigned)head_dim / 16, 2);
-#define TT_LAUNCH(T, N, I) qk_norm_rope_bwd_kernel<T, true, I, true><<<grid, block, 0, st>>>(a, partial);
-    if (dtype == TTAMD_BF16) {
-      TT_ROPE_CALL(BF16, true, at->interleaved, TT_LAUNCH)
-      qk_norm_rope_gscale_kernel<BF16><<<sum_grid, dim3(1024), 0, st>>>(partial, (int)grid.x, (int)head_dim, gq, gk);
-    } else {
-      TT_ROPE_CALL(F32, true, at->interleaved, TT_LAUNCH)
-      qk_norm_rope_gscale_kernel<F32><<<sum_grid, dim3(1024), 0, st>>>(partial, (int)grid.x, (int)head_dim, gq, gk);
-    }
+    // the parts share the workgroups so that each takes as many rounds
+    const unsigned rounds = (a.part[0].wgs + a.part[1].wgs + kBwdGrid - 1) / kBwdGrid;
+    for (Part& p : a.part) p.wgs = (p.wgs + rounds - 1) / rounds;
+    const int nq = (int)a.part[0].wgs, nk = (int)a.part[1].wgs;
+    const dim3 grid(nq + nk), sum_grid((unsigned)head_dim / 16, 2);
+#define TT_LAUNCH(T, L, N, I) qk_norm_rope_bwd_kernel<T, L, N, I, true><<<grid, block, 0, st>>>(a, partial)
+    TT_ROPE_CALL(true, TT_LAUNCH)
 #undef TT_LAUNCH
+    if (dtype == TTAMD_BF16)
+      qk_norm_rope_gscale_kernel<BF16><<<sum_grid, dim3(1024), 0, st>>>(partial, nq, nk, (int)head_dim, gq, gk);
+    else
+      qk_norm_rope_gscale_kernel<F32><<<sum_grid, dim3(1024), 0, st>>>(partial, nq, nk, (int)head_dim, gq, gk);
   } else {
-    const dim3 grid(most);
-#define TT_LAUNCH(T, N, I) qk_norm_rope_bwd_kernel<T, N, I, false><<<grid, block, 0, st>>>(a, nullptr);
-    if (dtype == TTAMD_BF16) {
-      TT_ROPE_CALL(BF16, norm, at->interleaved, TT_LAUNCH)
+    const dim3 grid(a.part[0].wgs + a.part[1].wgs);
+#define TT_LAUNCH(T, L, N, I) qk_norm_rope_bwd_kernel<T, L, N, I, false><<<grid, block, 0, st>>>(a, nullptr)
+    if (norm) {
+      TT_ROPE_CALL(true, TT_LAUNCH)
     } else {
-      TT_ROPE_CALL(F32, norm, at->interleaved, TT_LAUNCH)
+      TT_ROPE_CALL(false, TT_LAUNCH)
     }
 #undef TT_LAUNCH
   }

@@ -7,6 +7,7 @@
 namespace ttamd {
 
 typedef uint32_t u32x4_at2_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_at2_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f32x4_at4_t __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
@@ -36,6 +37,13 @@ struct BF16 {
     return Raw{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
   }
   static __device__ __forceinline__ void store(elem* p, const Raw& r) { __builtin_nontemporal_store(r, reinterpret_cast<Raw*>(p)); }
+  // four neighbours
+  typedef u32x2_at2_t Raw4;
+  static __device__ __forceinline__ Raw4 load4_once(const elem* p) { return __builtin_nontemporal_load(reinterpret_cast<const Raw4*>(p)); }
+  static __device__ __forceinline__ void store4(elem* p, const Raw4& r) { __builtin_nontemporal_store(r, reinterpret_cast<Raw4*>(p)); }
+  static __device__ __forceinline__ Raw join(const Raw4& a, const Raw4& b) { return Raw{a.x, a.y, b.x, b.y}; }
+  static __device__ __forceinline__ Raw4 low(const Raw& r) { return Raw4{r.x, r.y}; }
+  static __device__ __forceinline__ Raw4 high(const Raw& r) { return Raw4{r.z, r.w}; }
 };
 
 struct F32 {
@@ -68,6 +76,12 @@ struct F32 {
     __builtin_nontemporal_store(r.a, q);
     __builtin_nontemporal_store(r.b, q + 1);
   }
+  typedef f32x4_at4_t Raw4;
+  static __device__ __forceinline__ Raw4 load4_once(const elem* p) { return __builtin_nontemporal_load(reinterpret_cast<const Raw4*>(p)); }
+  static __device__ __forceinline__ void store4(elem* p, const Raw4& r) { __builtin_nontemporal_store(r, reinterpret_cast<Raw4*>(p)); }
+  static __device__ __forceinline__ Raw join(const Raw4& a, const Raw4& b) { return Raw{a, b}; }
+  static __device__ __forceinline__ Raw4 low(const Raw& r) { return r.a; }
+  static __device__ __forceinline__ Raw4 high(const Raw& r) { return r.b; }
 };
 
 // A lane's counterpart in a row of sixteen: inside a quad by one and by two, then mirrored in eight and in sixteen (quad
