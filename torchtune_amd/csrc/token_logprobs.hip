@@ -51,6 +51,7 @@ __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = f32_bits(v != v ? -__builtin_inff() : v + 0.f);  // -0 is 0
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float from_ordered(uint32_t k) { return bits_f32((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ uint64_t candidate(float v, uint32_t at) { return ((uint64_t)ordered(v) << 32) | (0xffffffffu - at); }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -143,18 +144,22 @@ __device__ __forceinline__ void fetch(const typename T::elem* x, uint32_t at, ui
   for (int i = 0; i < 8; ++i) v[i] = at + i < end ? T::get(x + at + i) : -__builtin_inff();
 }
 
-// A lower bound of the k-th largest of n numbers in LDS (their 16 highest bits), by halving; the whole first wave calls it.
-__device__ __forceinline__ uint32_t kth_bound(const uint32_t* keys, int n, int k) {
-  uint32_t bound = 0;
-  for (int bit = 15; bit >= 0; --bit) {
-    const uint32_t trial = bound | (1u << bit);
-    int count = 0;
-    for (int i = threadIdx.x; i < n; i += kWave) count += (keys[i] >> 16) >= trial;
+// A lower bound of the k-th largest of 64 N numbers in LDS (their 16 highest bits), by halving; the whole first wave calls it.
+// The wave counts with its lane masks: no exchange between lanes, no LDS but for the first read.
+template <int N>
+__device__ __forceinline__ uint32_t kth_bound(const uint32_t* keys, int k) {
+  uint32_t mine[N], bound = 0;
 #pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) count += __shfl_xor(count, off, kWave);
+  for (int i = 0; i < N; ++i) mine[i] = keys[threadIdx.x + kWave * i];
+#pragma unroll 1
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+    const uint32_t trial = bound | bit;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(mine[i] >= trial));
     if (count >= k) bound = trial;
   }
-  return bound << 16;
+  return bound;
 }
 
 struct TopScratch {
@@ -188,21 +193,38 @@ __device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, 
   if (threadIdx.x == 0) t.count = 0;
   __syncthreads();
   if (threadIdx.x < kWave) {
-    const uint32_t b = kth_bound(t.keys, NT, k);
+    const uint32_t b = kth_bound<NT / kWave>(t.keys, k);
     if (threadIdx.x == 0) t.bound = b;
   }
   __syncthreads();
   const uint32_t bound = t.bound;
   if (key >= bound) {
-    for (uint32_t at = lo + 8 * threadIdx.x; at < hi; at += 8 * NT) {
-      float v[8];
-      fetch<T>(x, at, hi, v);
+    auto look = [&](const float(&v)[8], uint32_t at) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (at + i >= hi || ordered(v[i]) < bound) continue;
+        if (ordered(v[i]) < bound || at + i >= hi) continue;
         const uint32_t slot = atomicAdd(&t.count, 1u);
         if (slot < kCandidates) t.found[slot] = candidate(v[i], at + i);
       }
+    };
+    // few threads come here, each for itself: what counts is how many of its loads are under way together
+    constexpr int kAhead = 4;
+    uint32_t at = lo + 8 * threadIdx.x;
+    for (; at + 8 * NT * (kAhead - 1) + 8 <= hi; at += 8 * NT * kAhead) {
+      typename T::Raw raw[kAhead];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) raw[q] = T::load(x + at + 8 * NT * q);
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        float v[8];
+        T::unpack(raw[q], v);
+        look(v, at + 8 * NT * q);
+      }
+    }
+    for (; at < hi; at += 8 * NT) {
+      float v[8];
+      fetch<T>(x, at, hi, v);
+      look(v, at);
     }
   }
   __syncthreads();
@@ -242,9 +264,23 @@ __device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, 
   __syncthreads();
 }
 
+// The first given token of a thread with its logit, asked for before the row is read: two reads that depend on each other.
+template <class T>
+struct Given {
+  int64_t token = 0;
+  float x = 0.f;
+  bool valid = false;
+  __device__ __forceinline__ void read(const LogitArgs& a, uint32_t row, const typename T::elem* logits, int i) {
+    if (i >= a.n_tokens) return;
+    token = a.tokens[(int64_t)row * a.n_tokens + i];
+    valid = (uint64_t)token < a.V;  // any other place gives NaN and reads nothing
+    if (valid) x = T::get(logits + token);
+  }
+};
+
 // What is written for a row from its maximum and sums; every thread has them.
 template <class T, int NT, bool ENT>
-__device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem* x, Running r, const TopScratch* t, float (*lds)[3]) {
+__device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem* x, Running r, Given<T> given, const TopScratch* t, float (*lds)[3]) {
   float s, u;
   if (__builtin_fabsf(r.max) < __builtin_inff() && !(r.s > 0.f && r.s < __builtin_inff())) {
     // c x overflows (a row masked with the lowest value of its type): the differences do not.
@@ -288,19 +324,15 @@ __device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem*
   }
   const float none = -__builtin_inff();
   for (int i = threadIdx.x; i < a.n_tokens; i += NT) {
-    const int64_t at = (int64_t)row * a.n_tokens + i, token = a.tokens[at];
-    float lp = 0.f;
-    if (token != a.ignore_index) {
-      const bool valid = (uint64_t)token < a.V;  // any other place gives NaN and reads nothing
-      lp = __builtin_nanf("");
-      if (valid) lp = empty ? none : (T::get(x + token) - m) * a.inv_temp - lse;
-    }
-    a.logprobs[at] = lp;
+    if (i >= NT) given.read(a, row, x, i);
+    float lp = given.valid ? empty ? none : (given.x - m) * a.inv_temp - lse : __builtin_nanf("");
+    if (given.token == a.ignore_index) lp = 0.f;
+    a.logprobs[(int64_t)row * a.n_tokens + i] = lp;
   }
   for (int i = threadIdx.x; i < a.top; i += NT) {
     const uint64_t best = t->best[i];
     const uint32_t place = min(0xffffffffu - (uint32_t)best, a.V - 1);
-    const float v = T::get(x + place);  // as it stands there, a NaN as one
+    const float v = from_ordered((uint32_t)(best >> 32));  // in a row with a NaN, lse is one
     a.top_logprobs[(int64_t)row * a.top + i] = empty ? none : (v - m) * a.inv_temp - lse;
     a.top_tokens[(int64_t)row * a.top + i] = (int64_t)place;
   }
@@ -322,6 +354,8 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const LogitArgs 
   const uint32_t row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
   const E* x = row_of<T>(a, row);
   const uint32_t lo = seg * a.segment, hi = min(lo + a.segment, a.V);
+  Given<T> given;
+  if (a.segments == 1) given.read(a, row, x, threadIdx.x);
   Running r;
   uint32_t at = lo + 8 * threadIdx.x;
   // two pieces of eight at a time: the maximum is moved once for sixteen elements
@@ -341,7 +375,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const LogitArgs 
   meet<NT, ENT>(r, a.c, lds);
   if constexpr (TOP) find_top<T, NT>(top[0], x, lo, hi, mine, a.top);
   if (a.segments == 1) {
-    finish<T, NT, ENT>(a, row, x, r, top, lds);
+    finish<T, NT, ENT>(a, row, x, r, given, top, lds);
     return;
   }
   if (threadIdx.x == 0) {
@@ -364,6 +398,8 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
   const uint32_t row = blockIdx.x;
   const typename T::elem* x = row_of<T>(a, row);
   const float* p = a.part + 4 * (int64_t)row * a.segments;
+  Given<T> given;
+  given.read(a, row, x, threadIdx.x);
   // segment of a lane, summed by the wave; all waves do the same
   Running r;
   const int lane = threadIdx.x & 63;
@@ -382,11 +418,11 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
     const int i = (k + n - 1) / n, need = (k + i - 1) / i;
     const uint64_t* f = a.part_top + (int64_t)row * n * k;
     TopScratch& t = top[0];
-    if ((int)threadIdx.x < n) t.keys[threadIdx.x] = (uint32_t)(f[threadIdx.x * k + i - 1] >> 32);
+    if (threadIdx.x < kSegmentsMax) t.keys[threadIdx.x] = (int)threadIdx.x < n ? (uint32_t)(f[threadIdx.x * k + i - 1] >> 32) : 0u;
     if (threadIdx.x == 0) t.count = 0;
     __syncthreads();
     if (threadIdx.x < kWave) {
-      const uint32_t b = kth_bound(t.keys, n, need);
+      const uint32_t b = kth_bound<kSegmentsMax / kWave>(t.keys, need);
       if (threadIdx.x == 0) t.bound = b;
     }
     __syncthreads();
@@ -410,7 +446,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
       __syncthreads();
     }
   }
-  finish<T, 256, ENT>(a, row, x, r, top, lds);
+  finish<T, 256, ENT>(a, row, x, r, given, top, lds);
 }
 
 constexpr int kBwdThreads = 256, kBwdPieces = 4;  // pieces of eight elements for each thread
@@ -493,7 +529,7 @@ __global__ __launch_bounds__(kBwdThreads) void token_logprobs_bwd_kernel(const G
 
 // How many segments a row is cut into: where the rows alone leave compute units empty, pieces of at least 4096 elements.
 uint32_t segments_of(int64_t rows, int64_t V) {
-  const int64_t want = 512 / rows, most = (V + 4095) / 4096;
+  const int64_t want = 1024 / rows, most = (V + 4095) / 4096;
   const int64_t n = want < most ? want : most;
   return (uint32_t)(n < 1 ? 1 : n > kSegmentsMax ? kSegmentsMax : n);
 }
