@@ -546,6 +546,7 @@ struct AdamWGroup {
 
   // the places of parameters that got their states in this step
   std::vector<int64_t> step(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, bool stochastic) {
+    const at::NoGradGuard no_grad;
     std::vector<int64_t> fresh;
     for (size_t i = 0; i < params.size(); ++i) {
       if (where[i].first >= 0 || !params[i].grad().defined()) continue;

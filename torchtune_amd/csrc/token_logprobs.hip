@@ -54,15 +54,21 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float from_ordered(uint32_t k) { return bits_f32((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ uint64_t candidate(float v, uint32_t at) { return ((uint64_t)ordered(v) << 32) | (0xffffffffu - at); }
 
+// over the wave, in every lane: each row of sixteen by moves of the vector ALU, then one lane of each
+__device__ __forceinline__ float lane_of(float v, int lane) { return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), lane)); }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off, kWave));
-  return v;
+  v = __builtin_fmaxf(v, row_partner<1>(v));
+  v = __builtin_fmaxf(v, row_partner<2>(v));
+  v = __builtin_fmaxf(v, row_partner<4>(v));
+  v = __builtin_fmaxf(v, row_partner<8>(v));
+  return __builtin_fmaxf(__builtin_fmaxf(lane_of(v, 0), lane_of(v, 16)), __builtin_fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 __device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+  v += row_partner<1>(v);
+  v += row_partner<2>(v);
+  v += row_partner<4>(v);
+  v += row_partner<8>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
 // what a thread knows of the elements it has seen: largest x; sums shifted by M = fp32(c max), a finite number
@@ -162,8 +168,10 @@ __device__ __forceinline__ uint32_t kth_bound(const uint32_t* keys, int k) {
   return bound;
 }
 
+constexpr int kRankAhead = 8;
+
 struct TopScratch {
-  uint64_t found[kCandidates];
+  uint64_t found[kCandidates + kRankAhead];
   uint64_t best[kTopMax];
   uint32_t keys[1024];
   uint32_t count, bound;
@@ -174,11 +182,15 @@ struct TopScratch {
 template <int NT>
 __device__ __forceinline__ void rank(TopScratch& t, int n, int k) {
   for (int i = threadIdx.x; i < k; i += NT) t.best[i] = 0;
+  if (threadIdx.x < kRankAhead) t.found[n + threadIdx.x] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t mine = t.found[i];
     int above = 0;
-    for (int q = 0; q < n; ++q) above += t.found[q] > mine;
+    for (int q = 0; q < n; q += kRankAhead) {
+#pragma unroll
+      for (int e = 0; e < kRankAhead; ++e) above += t.found[q + e] > mine;
+    }
     if (above < k) t.best[above] = mine;
   }
   __syncthreads();

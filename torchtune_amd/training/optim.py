@@ -85,7 +85,6 @@ class AdamW(torch.optim.Optimizer):
         names = ("step", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
         self.state[params[i]] = dict(zip(names, plan.state(i)))
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step; with ``closure``, which computes the loss again, its value is returned."""
         loss = None
