@@ -12,8 +12,8 @@
 // Bound: HBM, closely followed by the vector ALU in the forward over bf16: at 6 TB/s a compute unit takes about 5 elements a
 // cycle, which leaves twelve lane operations for each, and exp2 alone takes four.
 //
-// The largest elements come from the same pass: the k-th largest of the threads' maxima is no larger than the k-th largest
-// element, so that only threads whose maximum reaches it (about k of them) look at their elements again; what they find is
+// The largest elements come from the same pass: a number that k maxima of disjoint sets of elements reach is no larger than the k-th
+// largest element, so that only threads whose maximum reaches it (a few more than k) look at their elements again; what they find is
 // ranked by counting.  An element and its place are one 64-bit number (larger value first, of equal values the earlier place), so
 // that the result does not depend on the order in which candidates are found.
 #include "row_vec.h"
@@ -150,13 +150,11 @@ __device__ __forceinline__ void fetch(const typename T::elem* x, uint32_t at, ui
   for (int i = 0; i < 8; ++i) v[i] = at + i < end ? T::get(x + at + i) : -__builtin_inff();
 }
 
-// A lower bound of the k-th largest of 64 N numbers in LDS (their 16 highest bits), by halving; the whole first wave calls it.
-// The wave counts with its lane masks: no exchange between lanes, no LDS but for the first read.
+// A bound that k of the wave's numbers, N a lane, reach (the k-th largest, cut to 16 bits), by halving.  The wave counts with its lane
+// masks.
 template <int N>
-__device__ __forceinline__ uint32_t kth_bound(const uint32_t* keys, int k) {
-  uint32_t mine[N], bound = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) mine[i] = keys[threadIdx.x + kWave * i];
+__device__ __forceinline__ uint32_t kth_bound(const uint32_t (&mine)[N], int k) {
+  uint32_t bound = 0;
 #pragma unroll 1
   for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
     const uint32_t trial = bound | bit;
@@ -197,30 +195,85 @@ __device__ __forceinline__ void rank(TopScratch& t, int n, int k) {
 }
 
 // The k largest elements of [lo, hi) of a row, in t.best.  mine: the largest of the elements this thread has seen, which are
-// the pieces of eight lo + 8 (threadIdx.x + NT i).
+// the pieces of eight lo + 8 (threadIdx.x + NT i); largest: that of all threads.
 template <class T, int NT>
-__device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, uint32_t hi, float mine, int k) {
+__device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, uint32_t hi, float mine, float largest, int k) {
   const uint32_t key = ordered(mine);
-  t.keys[threadIdx.x] = key;
   if (threadIdx.x == 0) t.count = 0;
-  __syncthreads();
-  if (threadIdx.x < kWave) {
-    const uint32_t b = kth_bound<NT / kWave>(t.keys, k);
-    if (threadIdx.x == 0) t.bound = b;
-  }
-  __syncthreads();
-  const uint32_t bound = t.bound;
-  if (key >= bound) {
-    auto look = [&](const float(&v)[8], uint32_t at) {
+  uint32_t bound = ordered(largest);
+  if (k > 1) {
+    // k maxima that reach the bound hold k elements that do.  Of n maxima (of threads, or of the threads of one lane of all waves)
+    // about n ln(n / (n - k)) elements reach it: from 64 maxima 24 for k = 20, but 97 for k = 50 against 56 from 256.
+    constexpr int N = NT / kWave;
+    t.keys[threadIdx.x] = key;
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+      uint32_t maxima[N], group[1] = {0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (ordered(v[i]) < bound || at + i >= hi) continue;
-        const uint32_t slot = atomicAdd(&t.count, 1u);
-        if (slot < kCandidates) t.found[slot] = candidate(v[i], at + i);
+      for (int w = 0; w < N; ++w) {
+        maxima[w] = t.keys[threadIdx.x + kWave * w];
+        group[0] = max(group[0], maxima[w]);
       }
-    };
-    // few threads come here, each for itself: what counts is how many of its loads are under way together
-    constexpr int kAhead = 4;
+      const uint32_t b = k <= 24 ? kth_bound(group, k) : kth_bound(maxima, k);
+      if (threadIdx.x == 0) t.bound = b;
+    }
+    __syncthreads();
+    bound = t.bound;
+  } else {
+    __syncthreads();
+  }
+  const float least = bound <= ordered(-__builtin_inff()) ? -__builtin_inff() : from_ordered(bound);
+  auto look = [&](const float(&v)[8], uint32_t at) {
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, v[i]);
+    if (!(top >= least)) return;
+    uint32_t some = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) some += v[i] >= least && at + i < hi;
+    uint32_t slot = atomicAdd(&t.count, some);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!(v[i] >= least && at + i < hi)) continue;
+      if (slot < kCandidates) t.found[slot] = candidate(v[i], at + i);
+      ++slot;
+    }
+  };
+  // What this costs is the number of times that a wave waits for memory, with four loads under way: each thread that reaches the
+  // bound for itself, or all lanes for one such thread after another, a piece each.
+  constexpr int kAhead = 4;
+  const uint32_t lane = threadIdx.x & 63, pieces = (hi - lo + 8 * NT - 1) / (8 * NT);
+  uint64_t todo = __ballot(key >= bound);
+  if ((uint32_t)__popcll(todo) * ((pieces + 63) / 64) < pieces) {  // uniform
+    while (todo) {
+      uint32_t first[kAhead];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        first[q] = todo ? lo + 8 * ((threadIdx.x & ~63u) + (uint32_t)__builtin_ctzll(todo)) : hi;
+        todo &= todo - 1;
+      }
+      for (uint32_t piece = lane; piece < pieces + lane; piece += kWave) {
+        typename T::Raw raw[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+          const uint32_t at = first[q] + 8 * NT * piece;
+          raw[q] = typename T::Raw{};
+          if (at + 8 <= hi) raw[q] = T::load(x + at);
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+          const uint32_t at = first[q] + 8 * NT * piece;
+          if (at >= hi) continue;
+          float v[8];
+          if (at + 8 <= hi)
+            T::unpack(raw[q], v);
+          else
+            fetch<T>(x, at, hi, v);
+          look(v, at);
+        }
+      }
+    }
+  } else if (key >= bound) {
     uint32_t at = lo + 8 * threadIdx.x;
     for (; at + 8 * NT * (kAhead - 1) + 8 <= hi; at += 8 * NT * kAhead) {
       typename T::Raw raw[kAhead];
@@ -385,7 +438,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const LogitArgs 
   }
   const float mine = r.max;
   meet<NT, ENT>(r, a.c, lds);
-  if constexpr (TOP) find_top<T, NT>(top[0], x, lo, hi, mine, a.top);
+  if constexpr (TOP) find_top<T, NT>(top[0], x, lo, hi, mine, r.max, a.top);
   if (a.segments == 1) {
     finish<T, NT, ENT>(a, row, x, r, given, top, lds);
     return;
@@ -430,17 +483,14 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
     const int i = (k + n - 1) / n, need = (k + i - 1) / i;
     const uint64_t* f = a.part_top + (int64_t)row * n * k;
     TopScratch& t = top[0];
-    if (threadIdx.x < kSegmentsMax) t.keys[threadIdx.x] = (int)threadIdx.x < n ? (uint32_t)(f[threadIdx.x * k + i - 1] >> 32) : 0u;
+    static_assert(kSegmentsMax <= kWave, "a lane for each segment");
     if (threadIdx.x == 0) t.count = 0;
-    __syncthreads();
-    if (threadIdx.x < kWave) {
-      const uint32_t b = kth_bound<kSegmentsMax / kWave>(t.keys, need);
-      if (threadIdx.x == 0) t.bound = b;
-    }
+    const uint32_t reached[1] = {lane < n ? (uint32_t)(f[lane * k + i - 1] >> 32) : 0u};
+    const uint32_t bound = kth_bound(reached, need);  // in every wave
     __syncthreads();
     for (int q = threadIdx.x; q < n * k; q += 256) {
       const uint64_t one = f[q];
-      if (one == 0 || (uint32_t)(one >> 32) < t.bound) continue;
+      if (one == 0 || (uint32_t)(one >> 32) < bound) continue;
       const uint32_t slot = atomicAdd(&t.count, 1u);
       if (slot < kCandidates) t.found[slot] = one;
     }
@@ -581,8 +631,6 @@ int prepare(const char* who, LogitArgs& a, const ttamd_logits* l, const int64_t*
   return TTAMD_OK;
 }
 
-constexpr int kFwdThreads = 512;
-
 template <class T, bool ENT, bool TOP>
 void launch_fwd(const LogitArgs& a, hipStream_t st) {
   const dim3 grid(a.rows * a.segments);
@@ -590,7 +638,12 @@ void launch_fwd(const LogitArgs& a, hipStream_t st) {
     token_logprobs_fwd_kernel<T, 256, ENT, TOP><<<grid, dim3(256), 0, st>>>(a);
     token_logprobs_join_kernel<T, ENT, TOP><<<dim3(a.rows), dim3(256), 0, st>>>(a);
   } else {
-    token_logprobs_fwd_kernel<T, kFwdThreads, ENT, TOP><<<grid, dim3(kFwdThreads), 0, st>>>(a);
+    // A wave for a row of few elements: 8000 x 1024 in 8.3 us (64 threads), 13.5 (256), 25.8 (512).  Above, 256: 1799 x 32064 in 26.2
+    // (31.4 with 64, 27.5 with 512), 2048 x 128256 forward and backward in 258 (263 with 512, 260 with 1024).
+    if (a.V <= 4096)
+      token_logprobs_fwd_kernel<T, 64, ENT, TOP><<<grid, dim3(64), 0, st>>>(a);
+    else
+      token_logprobs_fwd_kernel<T, 256, ENT, TOP><<<grid, dim3(256), 0, st>>>(a);
   }
 }
 
