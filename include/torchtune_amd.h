@@ -841,7 +841,7 @@ int ttamd_qk_norm_rope_bwd(const ttamd_rope_heads* parts, const ttamd_rope_posit
  * logits: TTAMD_BF16 or TTAMD_F32, V neighbouring elements a row, row r at (r / n_inner) * stride_outer +
  * (r % n_inner) * stride_inner elements; rows may begin at any element.  fp32 sums in an order that depends on the sizes only.
  * workspace: ttamd_token_logprobs_workspace_bytes bytes (0: may be NULL).
- * Beside it in the reference: torchtune/rlhf/utils.py (eager log_softmax and gather).
+ * The reference has an eager log softmax and a gather for the first (torchtune/rlhf/).
  */
 typedef struct ttamd_logits {
   const void* data;

@@ -19,7 +19,7 @@ The output projection is a plain frozen bf16 linear, never NF4 (``_component_bui
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -64,6 +64,9 @@ class LlamaShape:
     vocab: int = 128256
     rope_base: float = 500000.0
     norm_eps: float = 1e-5
+    qk_norm: bool = False  # a norm of every query and key head before the rotation
+    rope_sections: Optional[Tuple[int, ...]] = None  # positions of several axes: how many frequencies follow each
+    max_positions: int = 8192  # rows of the table where positions are given
 
     @property
     def head_dim(self) -> int:
@@ -140,11 +143,11 @@ def rope_cache(seq_len: int, head_dim: int, base: float, device) -> torch.Tensor
 
 
 def apply_rope(x: torch.Tensor, cache: torch.Tensor) -> torch.Tensor:
-    """x [b, s, n_h, h_d]; rotates interleaved pairs, fp32 math."""
-    if _fused(x) and x.shape[-1] % 8 == 0:
+    """x [b, s, n_h, h_d]; rotates interleaved pairs, fp32 math.  cache [s, h_d / 2, 2], or [b, s, h_d / 2, 2] for each sequence."""
+    if _fused(x) and x.shape[-1] % 8 == 0 and cache.dim() == 3:
         return layer_ops.apply_rope(x, cache)
     xs = x.float().reshape(*x.shape[:-1], -1, 2)
-    c = cache.view(1, xs.size(1), 1, xs.size(3), 2)
+    c = cache.view(-1, xs.size(1), 1, xs.size(3), 2)
     out = torch.stack(
         [xs[..., 0] * c[..., 0] - xs[..., 1] * c[..., 1], xs[..., 1] * c[..., 0] + xs[..., 0] * c[..., 1]], dim=-1
     )
@@ -167,8 +170,28 @@ class Attention(nn.Module):
         self.k_proj = _linear(s.dim, s.n_kv_heads * s.head_dim, rank, alpha, quantize_base)
         self.v_proj = _linear(s.dim, s.n_kv_heads * s.head_dim, rank, alpha, quantize_base)
         self.output_proj = _linear(s.dim, s.dim, rank, alpha, quantize_base)
+        self.sections = s.rope_sections
+        # torchtune/modules/attention.py:234-290: q_norm and k_norm, where the builder gives them
+        self.q_norm, self.k_norm = (RMSNorm(s.head_dim, s.norm_eps), RMSNorm(s.head_dim, s.norm_eps)) if s.qk_norm else (None, None)
 
-    def forward(self, x: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
+    def _norm_and_rotate(self, q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions: Optional[torch.Tensor]):
+        """Norm of the heads and rotation at given positions: one pass per direction where the fused kernels apply."""
+        if _fused(q) and self.head_dim % 16 == 0 and (self.q_norm is None or self.q_norm.scale.dtype == q.dtype):
+            scales = (None, None) if self.q_norm is None else (self.q_norm.scale, self.k_norm.scale)
+            eps = 0.0 if self.q_norm is None else self.q_norm.eps
+            return layer_ops.qk_norm_rope(q, k, rope, *scales, eps=eps, positions=positions, sections=self.sections)
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
+        if positions is None:
+            table = rope[: q.shape[1]]
+        elif self.sections is None:
+            table = rope[positions]
+        else:
+            axis = torch.repeat_interleave(torch.arange(len(self.sections), device=q.device), torch.tensor(self.sections, device=q.device))
+            table = rope[positions[axis].permute(1, 2, 0), torch.arange(axis.numel(), device=q.device)]
+        return apply_rope(q, table), apply_rope(k, table)
+
+    def forward(self, x: torch.Tensor, rope: torch.Tensor, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         b, sl, _ = x.shape
         # the three projections read the same tensor (torchtune/modules/attention.py:234,262-263): one group
         q, k, v = _shared_input(x, (self.q_proj, self.k_proj, self.v_proj)) if GROUP_SHARED_INPUT else (
@@ -176,13 +199,13 @@ class Attention(nn.Module):
         q = q.view(b, sl, self.n_heads, self.head_dim)
         k = k.view(b, sl, self.n_kv, self.head_dim)
         v = v.view(b, sl, self.n_kv, self.head_dim)
-        if FUSED_QKV_POST and self.n_kv != self.n_heads and _fused(q) and self.head_dim % 8 == 0:
+        plain = self.q_norm is None and positions is None
+        if plain and FUSED_QKV_POST and self.n_kv != self.n_heads and _fused(q) and self.head_dim % 8 == 0:
             # rotary embedding of q and k and the expansion of the k / v heads: one launch per direction
             q, k, v = layer_ops.qkv_rope_repeat(q, k, v, rope)
             o = _sdpa(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
             return self.output_proj(o.transpose(1, 2).reshape(b, sl, -1))
-        q = apply_rope(q, rope)
-        k = apply_rope(k, rope)
+        q, k = (apply_rope(q, rope), apply_rope(k, rope)) if plain else self._norm_and_rotate(q, k, rope, positions)
         if self.n_kv != self.n_heads:  # expand kv heads to query heads, as the reference does before SDPA
             rep = self.n_heads // self.n_kv
             if _fused(k) and self.head_dim % 8 == 0:
@@ -234,13 +257,13 @@ class DecoderLayer(nn.Module):
         self.mlp_norm = RMSNorm(s.dim, s.norm_eps)
         self.mlp = FeedForward(s, rank, alpha, quantize_base)
 
-    def forward(self, x: torch.Tensor, delta: Optional[torch.Tensor], rope: torch.Tensor):
+    def forward(self, x: torch.Tensor, delta: Optional[torch.Tensor], rope: torch.Tensor, positions: Optional[torch.Tensor] = None):
         """``x``: the residual stream before the previous layer's feed-forward output ``delta`` is added (``None`` for the
         first layer).  Returns the stream after the attention sub-block and this layer's feed-forward output, not yet
         added: every addition of the stream (``torchtune/modules/transformer.py:129-141``) is followed by an RMSNorm and
         runs in that norm's pass (``_add_norm``)."""
         h, n = (x, self.sa_norm(x)) if delta is None else _add_norm(x, delta, self.sa_norm)
-        h, n = _add_norm(h, self.attn(n, rope), self.mlp_norm)
+        h, n = _add_norm(h, self.attn(n, rope, positions), self.mlp_norm)
         return h, self.mlp(n)
 
 
@@ -267,16 +290,35 @@ class Decoder(nn.Module):
             self._rope = (seq_len, device, rope_cache(seq_len, self.shape.head_dim, self.shape.rope_base, device))
         return self._rope[2]
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        rope = self._rope_cache(tokens.shape[1], tokens.device)
+    def forward(self, tokens: torch.Tensor, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``positions``: of each token, [b, s], or [axes, b, s] for a shape with sections; below the shape's ``max_positions``."""
+        if positions is None and self.shape.rope_sections is not None:
+            positions = torch.arange(tokens.shape[1], device=tokens.device).expand(len(self.shape.rope_sections), *tokens.shape)
+        rope = self._rope_cache(tokens.shape[1] if positions is None else self.shape.max_positions, tokens.device)
         h = self.tok_embeddings(tokens)
         delta = None
         for layer in self.layers:
             if self.ac and torch.is_grad_enabled():
-                h, delta = checkpoint(layer, h, delta, rope, use_reentrant=False)
+                h, delta = checkpoint(layer, h, delta, rope, positions, use_reentrant=False)
             else:
-                h, delta = layer(h, delta, rope)
+                h, delta = layer(h, delta, rope, positions)
         return _add_norm(h, delta, self.norm)[1]
+
+    def token_logprobs(self, tokens: torch.Tensor, targets: torch.Tensor, *, positions: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                       entropy: bool = False, top: int = 0, ignore_index: int = -100) -> layer_ops.TokenLogprobs:
+        """Log probabilities of ``targets`` ([b, s], or [b, s, n] for several) after each token, with the entropy and the most likely
+        alternatives if asked for: what preference, policy and distillation losses read.  The vocabulary projection runs chunk by
+        chunk over the tokens, as in :meth:`loss`; a chunk's logits are kept for the backward."""
+        h = self.forward(tokens, positions)
+        hidden, several = h.reshape(-1, h.shape[-1]), targets.reshape(tokens.numel(), -1)
+        parts = []
+        for hc, tc in zip(hidden.chunk(self.loss_chunks), several.chunk(self.loss_chunks)):
+            logits = self.output(hc)
+            parts.append(layer_ops.token_logprobs(logits, tc, temperature=temperature, entropy=entropy, top=top, ignore_index=ignore_index))
+        joined = [None if p[0] is None else torch.cat(p) for p in zip(*parts)]
+        lead = tokens.shape
+        return layer_ops.TokenLogprobs(joined[0].view(targets.shape), None if joined[1] is None else joined[1].view(lead),
+                                       *(None if t is None else t.view(*lead, top) for t in joined[2:]))
 
     def loss(self, tokens: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         """Mean next-token cross entropy; the vocabulary projection is applied chunk by chunk over the sequence."""
@@ -371,4 +413,21 @@ def train_step(model: Decoder, tokens: torch.Tensor, labels: torch.Tensor) -> to
     """One forward + backward; returns the detached loss."""
     loss = model.loss(tokens, labels)
     loss.backward()
+    return loss.detach()
+
+
+def policy_step(model: Decoder, tokens: torch.Tensor, targets: torch.Tensor, advantages: torch.Tensor, optimizer: torch.optim.Optimizer, *,
+                positions: Optional[torch.Tensor] = None, temperature: float = 1.0, entropy_weight: float = 0.0,
+                ignore_index: int = -100) -> torch.Tensor:
+    """One step on ``-mean(advantage * log p(target)) - entropy_weight * mean(entropy)`` over the tokens whose target is not
+    ``ignore_index``: forward, backward, optimizer.  Returns the detached loss."""
+    r = model.token_logprobs(tokens, targets, positions=positions, temperature=temperature, entropy=entropy_weight != 0.0, ignore_index=ignore_index)
+    counted = (targets != ignore_index).float()
+    n = counted.sum().clamp(min=1.0)
+    loss = -(advantages * r.logprobs).sum() / n
+    if r.entropy is not None:
+        loss = loss - entropy_weight * (r.entropy * counted).sum() / n
+    loss.backward()
+    optimizer.step()
+    optimizer.zero_grad(set_to_none=True)
     return loss.detach()

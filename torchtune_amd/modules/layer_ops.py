@@ -181,8 +181,8 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, entropy: bool = False, top: int = 0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """Log probabilities of given tokens under ``softmax(logits / temperature)``, with the entropy and the most likely
-    alternatives: what preference and policy losses and distillation are made of (the reference's ``logits_to_logprobs``,
-    ``torchtune/rlhf/utils.py``, is an eager log softmax and a gather) and what a sampler reports.  The logits are read once
+    alternatives: what preference and policy losses and distillation are made of (in the reference, ``torchtune/rlhf/``, an eager
+    log softmax and a gather) and what a sampler reports.  The logits are read once
     forward, and once more backward; no tensor of their size is kept beside them.
 
     Args:
