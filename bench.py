@@ -591,12 +591,24 @@ def optimizer_leg(model, tokens, labels, train_step, qat: bool, steps: int, toke
     """fwd + bwd + optimizer step, with the optimizer of the reference's configs: ``torch.optim.AdamW(fused=True)``,
     lr 3e-4 / weight decay 0.01 for QLoRA (``recipes/configs/llama3_1/8B_qlora_single_device.yaml:60-64``), lr 2e-5
     for QAT (``recipes/configs/llama3_1/8B_qat_full.yaml:66-69``).  The reference's own ``tokens_per_second_per_gpu``
-    includes the optimizer (``recipes/lora_finetune_single_device.py:666-671``); the headline metric does not."""
+    includes the optimizer (``recipes/lora_finetune_single_device.py:666-671``); the headline metric does not.  Beside it the same
+    with this package's ``AdamW`` (QAT: 8-bit moments), and the step of either alone."""
     if steps <= 0:
         return None
     params = [p for p in model.parameters() if p.requires_grad]
-    opt = (torch.optim.AdamW(params, lr=2e-5, fused=True) if qat
-           else torch.optim.AdamW(params, lr=3e-4, weight_decay=0.01, fused=True))
+    group = dict(lr=2e-5) if qat else dict(lr=3e-4, weight_decay=0.01)
+    out = _optimizer_leg(model, tokens, labels, train_step, steps, tokens_per_step, params, lambda: torch.optim.AdamW(params, fused=True, **group),
+                         "torch.optim.AdamW(fused=True)")
+    from torchtune_amd import AdamW
+
+    bits = 8 if qat else 32
+    out["own"] = _optimizer_leg(model, tokens, labels, train_step, steps, tokens_per_step, params, lambda: AdamW(params, state_bits=bits, **group),
+                                "torchtune_amd.AdamW(state_bits=%d)" % bits)
+    return out
+
+
+def _optimizer_leg(model, tokens, labels, train_step, steps, tokens_per_step, params, make, name):
+    opt = make()
 
     def opt_step():
         loss = train_step(model, tokens, labels)
@@ -611,13 +623,21 @@ def optimizer_leg(model, tokens, labels, train_step, qat: bool, steps: int, toke
         loss = opt_step()
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
+    train_step(model, tokens, labels)  # gradients for the optimizer's step alone
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    for _ in range(10):
+        opt.step()
+    torch.cuda.synchronize()
+    alone = (time.perf_counter() - t0) / 10
+    opt.zero_grad(set_to_none=True)
     out = {
         "value": round(tokens_per_step * steps / dt, 1),
         "unit": "tokens/s",
         "ms_per_step": round(1e3 * dt / steps, 2),
+        "optimizer_ms": round(1e3 * alone, 3),
         "steps": steps,
-        "optimizer": "torch.optim.AdamW(fused=True) over %d tensors / %.1f M trainable parameters" % (
-            len(params), sum(p.numel() for p in params) / 1e6),
+        "optimizer": "%s over %d tensors / %.1f M trainable parameters" % (name, len(params), sum(p.numel() for p in params) / 1e6),
         "loss_after": float(loss),
     }
     del opt
