@@ -875,14 +875,15 @@ int ttamd_token_logprobs_bwd(const ttamd_logits* logits, const int64_t* tokens, 
  * eps counts as at least 1.1e-19, the root of the smallest normal number.
  *
  * chunks: device array, a description of each TTAMD_ADAMW_CHUNK consecutive elements of a tensor, tensors one after another, each
- * beginning a chunk (an empty tensor has none).  It depends on the sizes only.  The call covers tensors first .. first + n - 1
- * (n at most TTAMD_ADAMW_TENSORS), whose chunks are first_chunk .. first_chunk + n_chunks - 1.  params and grads are host
- * arrays of n device pointers.
+ * beginning a chunk (an empty tensor has none).  The call covers tensors first .. first + n - 1 (n at most
+ * TTAMD_ADAMW_TENSORS), whose chunks are first_chunk .. first_chunk + n_chunks - 1.  grads: host array of n device pointers,
+ * which unlike the parameters' may change from step to step.
  */
 #define TTAMD_ADAMW_BLOCK 128
 #define TTAMD_ADAMW_CHUNK 4096
-#define TTAMD_ADAMW_TENSORS 240
+#define TTAMD_ADAMW_TENSORS 480
 typedef struct ttamd_adamw_chunk {
+  void* param;           /* the tensor's first element */
   int64_t start;         /* its first element in the tensor */
   int64_t numel;         /* of the tensor */
   int64_t offset, block; /* of the tensor */
@@ -904,8 +905,8 @@ typedef struct ttamd_adamw_scalars {
 } ttamd_adamw_scalars;
 uint32_t ttamd_adamw_key(int64_t seed, int64_t step, uint32_t tensor);
 uint32_t ttamd_adamw_number(uint32_t key, int64_t element);
-int ttamd_adamw_step(void* const* params, const void* const* grads, int n, int dtype, const ttamd_adamw_states* states, uint32_t first,
-                     uint32_t first_chunk, uint32_t n_chunks, const ttamd_adamw_scalars* scalars, void* stream);
+int ttamd_adamw_step(const void* const* grads, int n, int dtype, const ttamd_adamw_states* states, uint32_t first, uint32_t first_chunk,
+                     uint32_t n_chunks, const ttamd_adamw_scalars* scalars, void* stream);
 /* The 8-bit moments of all chunks as bf16 numbers (nothing is lost), tensor i from element `offset` of both outputs on. */
 int ttamd_adamw_moments_bf16(const ttamd_adamw_states* states, uint32_t n_chunks, void* exp_avg, void* exp_avg_sq, void* stream);
 

@@ -181,6 +181,25 @@ def test_views_and_other_orders_in_memory(dtype, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_whose_memory_moves(bits):
+    """``p.data = ..`` between steps, as offloading and resharding do: the new memory is stepped, the old left alone."""
+    results = []
+    for move in (False, True):
+        params = _tensors([(300,), (4096,), (5000,)], torch.bfloat16)
+        opt = AdamW(params, lr=1e-2, state_bits=bits)
+        opt.step()
+        old = params[1].data
+        kept = old.clone()
+        if move:
+            params[1].data = old.clone()
+        for _ in range(2):
+            opt.step()
+        assert not move or torch.equal(old, kept)
+        results.append([p.detach().clone() for p in params] + list(opt.moments()))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_gradients_of_zero_tiny_and_huge_size(bits):
     n = 8 * BLOCK
     p = torch.nn.Parameter(torch.randn(n, device=DEV))
@@ -357,6 +376,10 @@ def test_refusals():
     half.grad = torch.zeros_like(half)
     with pytest.raises(TypeError, match="not supported"):
         AdamW([half]).step()
+    wide = torch.nn.Parameter(torch.zeros(1, device=DEV).expand(10))
+    wide.grad = torch.ones(10, device=DEV)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        AdamW([wide]).step()
     q = torch.nn.Parameter(torch.zeros(10, device=DEV))
     q.grad = torch.ones_like(q)
     opt = AdamW([q], lr=0.5)

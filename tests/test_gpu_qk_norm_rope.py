@@ -7,6 +7,7 @@ output, whose sum ``size`` is computed beside it; backward, a second row sum and
 scales' gradients add at most 512 such terms one after another."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from torchtune_amd.modules import layer_ops
 
@@ -263,6 +264,11 @@ def test_second_derivatives_and_tangents_are_refused():
     out, _ = layer_ops.qk_norm_rope(q, k, _table(2, 32).to(DEV), w1, w2)
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         torch.autograd.grad(out.sum(), q, create_graph=True)
+    cache = _table(2, 32).to(DEV)
+    with pytest.raises(RuntimeError, match="cache"):
+        layer_ops.qk_norm_rope(q, k, cache.clone().requires_grad_(), w1, w2)
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+        layer_ops.qk_norm_rope(fwAD.make_dual(k, k), k, cache)
 
 
 def test_a_trace_keeps_the_gradients():

@@ -9,6 +9,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from torchtune_amd.modules import layer_ops
 
@@ -285,6 +286,8 @@ def test_second_derivatives_are_refused_and_written_logits_noticed():
     assert not r.top_logprobs.requires_grad
     with pytest.raises(RuntimeError, match="cannot be differentiated"):
         torch.autograd.grad(r.logprobs.sum(), logits, create_graph=True)
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+        layer_ops.token_logprobs(fwAD.make_dual(logits.detach(), logits.detach()), tokens)
     r = layer_ops.token_logprobs(logits, tokens)
     with torch.no_grad():
         logits.mul_(2)

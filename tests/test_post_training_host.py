@@ -71,6 +71,8 @@ def test_adamw_refuses():
                         (ValueError, dict(lr=float("nan")))):
         with pytest.raises(error):
             AdamW([p], **more)
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="twice"):
+        AdamW([p, p]).step()
     opt = AdamW([p])
     opt.step()  # no gradient, nothing to do
     assert not opt.state
@@ -109,7 +111,9 @@ def test_the_c_entries_check_their_arguments():
     at.n_axes = 1
     heads[1].heads, heads[1].x, heads[1].out, heads[1].scale = 1, p, p, p
     assert rope()[0] == -1 and "neither" in rope()[1]
-    heads[0].scale = p
+    heads[0].scale, heads[1].x = p, p + 1
+    assert rope()[0] == -1 and "misaligned" in rope()[1]
+    heads[1].x = p
     heads[0].gy = heads[1].gy = heads[0].gscale = p
     assert rope(bwd=True)[0] == -1 and "workspace" in rope(bwd=True)[1]
     assert rope(bwd=True, ws=64)[0] == -3
@@ -128,6 +132,9 @@ def test_the_c_entries_check_their_arguments():
     logits.V = 100000
     need = lib.ttamd_token_logprobs_workspace_bytes(2, 100000, 5)
     assert need > 0 and logprobs(top=5)[0] == -1 and logprobs(top=5, ws=need - 1)[0] == -3
+    logits.data = p + 2
+    assert logprobs()[0] == -1 and "misaligned" in logprobs()[1]
+    logits.data = p
     logits.dtype = 3
     assert logprobs()[0] == -1
     assert lib.ttamd_token_logprobs_workspace_bytes(0, 5, 1) == 0 and lib.ttamd_token_logprobs_workspace_bytes(5, 5, 65) == 0
@@ -141,10 +148,10 @@ def test_the_c_entries_check_their_arguments():
     ptrs = (ctypes.c_void_p * 1)(p)
 
     def adamw(n=1, dtype=1, chunks=1):
-        rc = lib.ttamd_adamw_step(ptrs, ptrs, n, dtype, ctypes.byref(states), 0, 0, chunks, ctypes.byref(scalars), None)
+        rc = lib.ttamd_adamw_step(ptrs, n, dtype, ctypes.byref(states), 0, 0, chunks, ctypes.byref(scalars), None)
         return rc, lib.ttamd_last_error().decode()
 
-    assert adamw(n=0)[0] == -1 and adamw(n=241)[0] == -1 and adamw(dtype=4)[0] == -1 and adamw(chunks=0)[0] == -1
+    assert adamw(n=0)[0] == -1 and adamw(n=481)[0] == -1 and adamw(dtype=4)[0] == -1 and adamw(chunks=0)[0] == -1
     for name, value in (("step", 0), ("beta1", 1.0), ("beta2", -0.5), ("eps", -1.0), ("stochastic", 1)):
         keep = getattr(scalars, name)
         setattr(scalars, name, value)
@@ -155,8 +162,9 @@ def test_the_c_entries_check_their_arguments():
     states.state_bits = 16
     assert adamw()[0] == -1 and "bits" in adamw()[1]
     states.state_bits = 32
-    ptrs[0] = None
-    assert adamw()[0] == -1
+    for bad in (None, p + 2):
+        ptrs[0] = bad
+        assert adamw()[0] == -1 and "pointer" in adamw()[1]
     assert lib.ttamd_adamw_moments_bf16(ctypes.byref(states), 1, p, p, None) == -1
 
 

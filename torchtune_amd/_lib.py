@@ -225,7 +225,7 @@ SIGNATURES = {
         _int, [_c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "ttamd_adamw_key": (_u32, [_i64, _i64, _u32]),
     "ttamd_adamw_number": (_u32, [_u32, _i64]),
-    "ttamd_adamw_step": (_int, [_c_void_p, _c_void_p, _int, _int, _c_void_p, _u32, _u32, _u32, _c_void_p, _c_void_p]),
+    "ttamd_adamw_step": (_int, [_c_void_p, _int, _int, _c_void_p, _u32, _u32, _u32, _c_void_p, _c_void_p]),
     "ttamd_adamw_moments_bf16": (_int, [_c_void_p, _u32, _c_void_p, _c_void_p, _c_void_p]),
     "ttamd_swiglu_bwd_bf16": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
 }

@@ -6,9 +6,9 @@
 // in fp32, every product and sum rounded by itself.  Bound: HBM, 22 bytes an element of a bf16 parameter with 32-bit states and 10
 // with 8-bit ones.
 //
-// One launch covers up to 240 tensors: their addresses travel in the kernel's arguments (they may change from step to step),
-// their sizes and places in the state buffers stand in a table on the GPU (they do not).  A workgroup takes 4096 elements of one
-// tensor; all that it has to know of them is one entry of that table.
+// One launch covers up to 480 tensors: the gradients' addresses travel in the kernel's arguments (they may change from step to
+// step), the parameters', their sizes and their places in the state buffers stand in a table on the GPU.  A workgroup takes 4096
+// elements of one tensor; all that it has to know of them is one entry of that table.
 //
 // 8 bits: 128 elements, 16 lanes of 8, share an exponent, so that finding it takes four moves within a row of lanes.  A code is
 // the top of the fp32 number itself, exponent and 3 (m) or 4 (v) bits of mantissa, relative to the block's exponent: writing and
@@ -41,12 +41,9 @@ struct StepArgs {
   ttamd_adamw_states st;
   Scalars c;
   uint64_t seed_step;  // of the keys, see key_of
-  uint32_t first;        // tensor of t[0]
+  uint32_t first;        // tensor of g[0]
   uint32_t first_chunk;  // of workgroup 0
-  struct {
-    void* p;
-    const void* g;
-  } t[TTAMD_ADAMW_TENSORS];
+  const void* g[TTAMD_ADAMW_TENSORS];
 };
 static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
 
@@ -220,8 +217,8 @@ template <class T, bool EIGHT, bool ROUND>
 __global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
   typedef typename T::elem E;
   const ttamd_adamw_chunk c = a.st.chunks[a.first_chunk + blockIdx.x];
-  E* p = reinterpret_cast<E*>(a.t[c.tensor - a.first].p);
-  const E* g = reinterpret_cast<const E*>(a.t[c.tensor - a.first].g);
+  E* p = reinterpret_cast<E*>(c.param);
+  const E* g = reinterpret_cast<const E*>(a.g[c.tensor - a.first]);
   uint32_t key = 0;
   if constexpr (EIGHT || ROUND) key = key_of(a.seed_step, c.number);
   const int64_t at = c.start + 8 * threadIdx.x;
@@ -293,9 +290,9 @@ using namespace ttamd;
 extern "C" uint32_t ttamd_adamw_key(int64_t seed, int64_t step, uint32_t tensor) { return key_of(key_base(seed, step), tensor); }
 extern "C" uint32_t ttamd_adamw_number(uint32_t key, int64_t element) { return number_of(key, element); }
 
-extern "C" int ttamd_adamw_step(void* const* params, const void* const* grads, int n, int dtype, const ttamd_adamw_states* states,
-                                uint32_t first, uint32_t first_chunk, uint32_t n_chunks, const ttamd_adamw_scalars* s, void* stream) {
-  TT_REQUIRE(params && grads && s, "adamw_step: null pointer argument");
+extern "C" int ttamd_adamw_step(const void* const* grads, int n, int dtype, const ttamd_adamw_states* states, uint32_t first,
+                                uint32_t first_chunk, uint32_t n_chunks, const ttamd_adamw_scalars* s, void* stream) {
+  TT_REQUIRE(grads && s, "adamw_step: null pointer argument");
   if (int rc = check_states("adamw_step", states)) return rc;
   TT_REQUIRE(dtype == TTAMD_BF16 || dtype == TTAMD_F32, "adamw_step: unknown dtype code %d", dtype);
   TT_REQUIRE(n > 0 && n <= TTAMD_ADAMW_TENSORS, "adamw_step: %d tensors (1 to %d)", n, TTAMD_ADAMW_TENSORS);
@@ -309,12 +306,12 @@ extern "C" int ttamd_adamw_step(void* const* params, const void* const* grads, i
   a.seed_step = key_base(s->seed, s->step);
   a.first = first;
   a.first_chunk = first_chunk;
+  const uintptr_t element = dtype == TTAMD_BF16 ? 2 : 4;
   for (int i = 0; i < n; ++i) {
-    TT_REQUIRE(params[i] && grads[i], "adamw_step: null pointer argument");
-    a.t[i].p = params[i];
-    a.t[i].g = grads[i];
+    TT_REQUIRE(grads[i] && reinterpret_cast<uintptr_t>(grads[i]) % element == 0, "adamw_step: null or misaligned pointer argument");
+    a.g[i] = grads[i];
   }
-  for (int i = n; i < TTAMD_ADAMW_TENSORS; ++i) a.t[i] = {nullptr, nullptr};
+  for (int i = n; i < TTAMD_ADAMW_TENSORS; ++i) a.g[i] = nullptr;
   a.c = {(float)s->beta1, (float)(1 - s->beta1), (float)s->beta2, (float)(1 - s->beta2), (float)(1 - s->lr * s->weight_decay),
          (float)(s->lr / (1 - __builtin_pow(s->beta1, (double)s->step))), (float)(1 / __builtin_sqrt(1 - __builtin_pow(s->beta2, (double)s->step))),
          // the hardware's root takes what lies below the smallest normal number for 0: the roots of those are below this

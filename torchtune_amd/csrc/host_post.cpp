@@ -4,6 +4,7 @@
 // Checks of shapes and types come before those of the device, so that they hold without one.
 #include "host_common.h"
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -198,6 +199,7 @@ std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const T
   }
   same_device(k, q, kRope, "k");
   same_device(cache, q, kRope, "the cache");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && cache.requires_grad()), kRope, ": there is no gradient with respect to the cache");
   need_gpu(q, kRope);
   const Tensor w1 = q_scale ? *q_scale : Tensor(), w2 = k_scale ? *k_scale : Tensor();
   if (wants_grad({&q, &k, &w1, &w2})) {
@@ -342,11 +344,15 @@ void check_param(const Tensor& p) {
   TORCH_CHECK(!p.key_set().has(c10::DispatchKey::Python) && p.layout() == at::kStrided, kAdamW, ": parameters must be plain dense tensors");
   type_code(p, kAdamW);
   need_gpu(p, kAdamW);
+  at::assert_no_internal_overlap(p);
 }
 
 // Parameters of one type on one device with the buffers that hold their moments.
 struct Block {
   std::vector<Tensor> params;
+  std::vector<int64_t> numbers;
+  std::vector<Tensor> shadow;  // of parameters that do not lie densely
+  std::vector<void*> address;  // that the table holds
   struct Place {
     int64_t offset, numel, block;
   };
@@ -357,8 +363,8 @@ struct Block {
   at::ScalarType type;         // of the parameters
   c10::hip::HIPStream stream;  // that the buffers were made on
 
-  Block(std::vector<Tensor> ps, const std::vector<int64_t>& numbers, int bits_)
-      : params(std::move(ps)), bits(bits_), type(params[0].scalar_type()), stream(c10::hip::getCurrentHIPStream(params[0].get_device())) {
+  Block(std::vector<Tensor> ps, std::vector<int64_t> numbers_, int bits_)
+      : params(std::move(ps)), numbers(std::move(numbers_)), bits(bits_), type(params[0].scalar_type()), stream(c10::hip::getCurrentHIPStream(params[0].get_device())) {
     const c10::DeviceGuard guard(params[0].device());
     int64_t n = 0, blocks = 0;
     uint64_t chunk = 0;
@@ -380,12 +386,32 @@ struct Block {
       exp_avg_sq_exponent = at::full_like(exp_avg_exponent, 16);
     }
     steps = at::zeros({(int64_t)params.size()}, at::kLong);
-    const Tensor host = at::empty({(int64_t)(std::max<uint64_t>(chunk, 1) * sizeof(ttamd_adamw_chunk))}, at::kByte);
+    shadow.resize(params.size());
+    address.resize(params.size());
+  }
+
+  // Where the kernel finds tensor i: the parameter, or a copy of one with gaps, which lives as long as the states.
+  void* find(size_t i) {
+    if (params[i].is_non_overlapping_and_dense()) return params[i].data_ptr();
+    if (!shadow[i].defined()) shadow[i] = at::empty(params[i].sizes(), params[i].options());
+    return shadow[i].data_ptr();
+  }
+
+  // The table of chunks, made again when a parameter's memory has moved.
+  void point() {
+    bool same = table.defined();
+    for (size_t i = 0; i < params.size(); ++i) {
+      void* now = find(i);
+      same = same && now == address[i];
+      address[i] = now;
+    }
+    if (same) return;
+    const Tensor host = at::empty({(int64_t)(std::max<uint32_t>(chunks.back(), 1) * sizeof(ttamd_adamw_chunk))}, at::kByte);
     ttamd_adamw_chunk* to = (ttamd_adamw_chunk*)host.data_ptr();
     for (size_t i = 0; i < params.size(); ++i)
       for (uint32_t j = chunks[i]; j < chunks[i + 1]; ++j)
-        to[j] = {(int64_t)(j - chunks[i]) * TTAMD_ADAMW_CHUNK, places[i].numel, places[i].offset, places[i].block, (uint32_t)i, (uint32_t)numbers[i]};
-    table = host.to(params[0].device());
+        to[j] = {address[i], (int64_t)(j - chunks[i]) * TTAMD_ADAMW_CHUNK, places[i].numel, places[i].offset, places[i].block, (uint32_t)i, (uint32_t)numbers[i]};
+    table = host.to(exp_avg.device());
   }
 
   ttamd_adamw_states states() const {
@@ -406,6 +432,8 @@ struct Block {
     if (now == stream) return;
     for (const Tensor* t : {&table, &exp_avg, &exp_avg_sq, &exp_avg_exponent, &exp_avg_sq_exponent})
       if (t->defined()) c10::hip::HIPCachingAllocator::recordStream(t->storage().data_ptr(), now);
+    for (const Tensor& t : shadow)
+      if (t.defined()) c10::hip::HIPCachingAllocator::recordStream(t.storage().data_ptr(), now);
   }
 
   // a flat buffer's part of tensor i, laid out as the parameter is
@@ -418,11 +446,12 @@ struct Block {
     return flat.narrow(0, places[i].block, (places[i].numel + TTAMD_ADAMW_BLOCK - 1) / TTAMD_ADAMW_BLOCK);
   }
 
-  std::pair<Tensor, Tensor> moments() const {
+  std::pair<Tensor, Tensor> moments() {
     if (bits == 32) return {exp_avg, exp_avg_sq};
     const c10::DeviceGuard guard(exp_avg.device());
     Tensor m = at::empty(exp_avg.sizes(), exp_avg.options().dtype(at::kBFloat16)), v = at::empty_like(m);
     if (chunks.back() == 0) return {m, v};
+    point();
     used_on(c10::hip::getCurrentHIPStream(exp_avg.get_device()));
     const ttamd_adamw_states s = states();
     check(ttamd_adamw_moments_bf16(&s, chunks.back(), m.data_ptr(), v.data_ptr(), stream_of(m)), kAdamW);
@@ -448,11 +477,11 @@ struct Block {
       TORCH_CHECK(p.numel() == places[i].numel && g.sizes() == p.sizes() && p.scalar_type() == type, kAdamW,
                   ": a parameter's size or type has changed");
     }
+    point();
     used_on(now);
     const ttamd_adamw_states s = states();
     const int dtype = type == at::kBFloat16 ? TTAMD_BF16 : TTAMD_F32;
     int64_t* count = steps.data_ptr<int64_t>();
-    void* p[TTAMD_ADAMW_TENSORS];
     const void* g[TTAMD_ADAMW_TENSORS];
     for (size_t first = 0; first < n;) {
       if (!grads[first]) {
@@ -461,17 +490,14 @@ struct Block {
       }
       // neighbours that have taken as many steps
       std::vector<Tensor> hold;
-      std::vector<std::pair<Tensor, Tensor>> back;
+      std::vector<size_t> back;
       size_t end = first;
       for (; end < n && end - first < TTAMD_ADAMW_TENSORS && grads[end] && count[end] == count[first]; ++end) {
         const Tensor &t = params[end], &grad = *grads[end];
         const bool dense = t.is_non_overlapping_and_dense();
-        if (dense) {
-          p[end - first] = t.data_ptr();
-        } else {
-          const Tensor plain = t.detach();
-          back.push_back({plain, plain.contiguous()});
-          p[end - first] = back.back().second.data_ptr();
+        if (!dense) {
+          shadow[end].copy_(t);
+          back.push_back(end);
         }
         if (dense && grad.strides() == t.strides()) {
           g[end - first] = grad.data_ptr();
@@ -481,13 +507,13 @@ struct Block {
           g[end - first] = hold.back().data_ptr();
         }
         // an empty tensor has no address; nothing reads it
-        if (t.numel() == 0) g[end - first] = p[end - first] = exp_avg.data_ptr();
+        if (t.numel() == 0) g[end - first] = table.data_ptr();
       }
       ttamd_adamw_scalars c = scalars;
       c.step = count[first] + 1;
       if (chunks[end] > chunks[first])
-        check(ttamd_adamw_step(p, g, (int)(end - first), dtype, &s, (uint32_t)first, chunks[first], chunks[end] - chunks[first], &c, now.stream()), kAdamW);
-      for (auto& [to, from] : back) to.copy_(from);
+        check(ttamd_adamw_step(g, (int)(end - first), dtype, &s, (uint32_t)first, chunks[first], chunks[end] - chunks[first], &c, now.stream()), kAdamW);
+      for (size_t i : back) params[i].detach().copy_(shadow[i]);
       for (size_t i = first; i < end; ++i) {
         ++count[i];
         if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
@@ -572,12 +598,12 @@ struct AdamWGroup {
   }
 
   // the flat moments, where one block holds all parameters in their order
-  std::optional<std::pair<Tensor, Tensor>> whole() const {
+  std::optional<std::pair<Tensor, Tensor>> whole() {
     if (blocks.size() != 1 || blocks[0]->params.size() != params.size()) return std::nullopt;
     return blocks[0]->moments();
   }
   // else those of each parameter that has them, in their order
-  std::vector<std::pair<Tensor, Tensor>> moments() const {
+  std::vector<std::pair<Tensor, Tensor>> moments() {
     std::vector<std::pair<Tensor, Tensor>> all, out;
     for (const auto& b : blocks) all.push_back(b->moments());
     for (const auto& [b, at] : where)

@@ -309,6 +309,8 @@ int prepare(const char* who, RopeArgs& a, const ttamd_rope_heads* parts, const t
     TT_REQUIRE(backward ? (p.gy && (p.x || !norm) && (p.out || p.gscale)) : (p.x && p.out), "%s: null pointer argument", who);
     TT_REQUIRE(!norm || p.scale, "%s: scales for the queries and for the keys, or for neither", who);
     TT_REQUIRE(!p.gscale || norm, "%s: the gradient of a scale that is not there", who);
+    for (const void* ptr : {p.x, p.scale, p.gy, (const void*)p.out, (const void*)p.gscale})
+      TT_REQUIRE(reinterpret_cast<uintptr_t>(ptr) % (dtype == TTAMD_BF16 ? 2 : 4) == 0, "%s: misaligned pointer argument", who);
     q.x = p.x;
     q.scale = p.scale;
     q.gy = p.gy;

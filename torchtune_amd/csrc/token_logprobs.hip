@@ -24,7 +24,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kTopMax = 64;        // most alternatives
-constexpr int kCandidates = 1024;  // found in a workgroup before the exact search takes over
 constexpr int kSegmentsMax = 64;   // of a row
 
 struct LogitArgs {
@@ -168,17 +167,19 @@ __device__ __forceinline__ uint32_t kth_bound(const uint32_t (&mine)[N], int k) 
 
 constexpr int kRankAhead = 8;
 
+template <int NT>
 struct TopScratch {
+  static constexpr int kCandidates = 4 * NT;  // found in a workgroup before the exact search takes over
   uint64_t found[kCandidates + kRankAhead];
   uint64_t best[kTopMax];
-  uint32_t keys[1024];
+  uint32_t keys[NT];
   uint32_t count, bound;
-  uint64_t wave_best[16];
+  uint64_t wave_best[NT / kWave];
 };
 
 // found[0 .. n) -> the k largest, in order, in best (0 where there are fewer)
 template <int NT>
-__device__ __forceinline__ void rank(TopScratch& t, int n, int k) {
+__device__ __forceinline__ void rank(TopScratch<NT>& t, int n, int k) {
   for (int i = threadIdx.x; i < k; i += NT) t.best[i] = 0;
   if (threadIdx.x < kRankAhead) t.found[n + threadIdx.x] = 0;
   __syncthreads();
@@ -197,7 +198,7 @@ __device__ __forceinline__ void rank(TopScratch& t, int n, int k) {
 // The k largest elements of [lo, hi) of a row, in t.best.  mine: the largest of the elements this thread has seen, which are
 // the pieces of eight lo + 8 (threadIdx.x + NT i); largest: that of all threads.
 template <class T, int NT>
-__device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, uint32_t hi, float mine, float largest, int k) {
+__device__ void find_top(TopScratch<NT>& t, const typename T::elem* x, uint32_t lo, uint32_t hi, float mine, float largest, int k) {
   const uint32_t key = ordered(mine);
   if (threadIdx.x == 0) t.count = 0;
   uint32_t bound = ordered(largest);
@@ -235,7 +236,7 @@ __device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (!(v[i] >= least && at + i < hi)) continue;
-      if (slot < kCandidates) t.found[slot] = candidate(v[i], at + i);
+      if (slot < t.kCandidates) t.found[slot] = candidate(v[i], at + i);
       ++slot;
     }
   };
@@ -294,7 +295,7 @@ __device__ void find_top(TopScratch& t, const typename T::elem* x, uint32_t lo, 
   }
   __syncthreads();
   const uint32_t n = t.count;
-  if (n <= kCandidates) {  // uniform
+  if (n <= t.kCandidates) {  // uniform
     rank<NT>(t, (int)n, k);
     return;
   }
@@ -345,7 +346,7 @@ struct Given {
 
 // What is written for a row from its maximum and sums; every thread has them.
 template <class T, int NT, bool ENT>
-__device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem* x, Running r, Given<T> given, const TopScratch* t, float (*lds)[3]) {
+__device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem* x, Running r, Given<T> given, const TopScratch<NT>* t, float (*lds)[3]) {
   float s, u;
   if (__builtin_fabsf(r.max) < __builtin_inff() && !(r.s > 0.f && r.s < __builtin_inff())) {
     // c x overflows (a row masked with the lowest value of its type): the differences do not.
@@ -414,8 +415,8 @@ template <class T, int NT, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const LogitArgs a) {
   typedef typename T::elem E;
   __shared__ float lds[NT / 64][3];
-  __shared__ char scratch[TOP ? sizeof(TopScratch) : 8] __attribute__((aligned(8)));
-  TopScratch* top = reinterpret_cast<TopScratch*>(scratch);
+  __shared__ char scratch[TOP ? sizeof(TopScratch<NT>) : 8] __attribute__((aligned(8)));
+  TopScratch<NT>* top = reinterpret_cast<TopScratch<NT>*>(scratch);
   const uint32_t row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
   const E* x = row_of<T>(a, row);
   const uint32_t lo = seg * a.segment, hi = min(lo + a.segment, a.V);
@@ -458,8 +459,8 @@ __global__ __launch_bounds__(NT) void token_logprobs_fwd_kernel(const LogitArgs 
 template <class T, bool ENT, bool TOP>
 __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArgs a) {
   __shared__ float lds[4][3];
-  __shared__ char scratch[TOP ? sizeof(TopScratch) : 8] __attribute__((aligned(8)));
-  TopScratch* top = reinterpret_cast<TopScratch*>(scratch);
+  __shared__ char scratch[TOP ? sizeof(TopScratch<256>) : 8] __attribute__((aligned(8)));
+  TopScratch<256>* top = reinterpret_cast<TopScratch<256>*>(scratch);
   const uint32_t row = blockIdx.x;
   const typename T::elem* x = row_of<T>(a, row);
   const float* p = a.part + 4 * (int64_t)row * a.segments;
@@ -482,7 +483,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
     const int k = a.top, n = (int)a.segments;
     const int i = (k + n - 1) / n, need = (k + i - 1) / i;
     const uint64_t* f = a.part_top + (int64_t)row * n * k;
-    TopScratch& t = top[0];
+    TopScratch<256>& t = top[0];
     static_assert(kSegmentsMax <= kWave, "a lane for each segment");
     if (threadIdx.x == 0) t.count = 0;
     const uint32_t reached[1] = {lane < n ? (uint32_t)(f[lane * k + i - 1] >> 32) : 0u};
@@ -492,10 +493,10 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
       const uint64_t one = f[q];
       if (one == 0 || (uint32_t)(one >> 32) < bound) continue;
       const uint32_t slot = atomicAdd(&t.count, 1u);
-      if (slot < kCandidates) t.found[slot] = one;
+      if (slot < t.kCandidates) t.found[slot] = one;
     }
     __syncthreads();
-    if (t.count <= kCandidates) {  // uniform
+    if (t.count <= t.kCandidates) {  // uniform
       rank<256>(t, (int)t.count, k);
     } else {
       // equal values: each segment's are in order, and the segments too, so that a place in the result is a count over them all
@@ -612,6 +613,7 @@ int prepare(const char* who, LogitArgs& a, const ttamd_logits* l, const int64_t*
             float temperature) {
   TT_REQUIRE(l && l->data && (tokens || n_tokens == 0), "%s: null pointer argument", who);
   TT_REQUIRE(l->dtype == TTAMD_BF16 || l->dtype == TTAMD_F32, "%s: unknown dtype code %d", who, l->dtype);
+  TT_REQUIRE(reinterpret_cast<uintptr_t>(l->data) % (l->dtype == TTAMD_BF16 ? 2 : 4) == 0, "%s: misaligned pointer argument", who);
   TT_REQUIRE(l->rows > 0 && l->rows < (int64_t(1) << 31) && l->V > 0 && l->V < (int64_t(1) << 30) && l->n_inner > 0 && l->n_inner <= l->rows,
              "%s: bad shape rows=%lld V=%lld", who, (long long)l->rows, (long long)l->V);
   TT_REQUIRE(n_tokens >= 0 && n_tokens <= 65536, "%s: %lld tokens for a row", who, (long long)n_tokens);

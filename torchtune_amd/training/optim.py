@@ -66,6 +66,8 @@ class AdamW(torch.optim.Optimizer):
         known = self._plans.get(index)
         if known is not None and known[1] is params and known[2] == len(params):
             return known[0]
+        if len({id(p) for p in params}) != len(params):
+            raise ValueError("AdamW: a parameter occurs twice in a group")
         first = sum(len(g["params"]) for g in self.param_groups[:index])
         plan = _host.load().AdamWGroup(params, first, self.defaults["state_bits"])
         given = [i for i, p in enumerate(params) if self.state.get(p)]
