@@ -65,6 +65,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {  // of sixteen lanes
 }
 
 typedef uint32_t u32x2_at1_t __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2_t __attribute__((ext_vector_type(2)));
 
 // Eight elements from element `at` of n (n > 0).  FULL: all of them are there; else each for itself, those behind the end from the last one
 // (what they become is never stored).
@@ -106,6 +108,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int64_t at, int64_t n, c
   }
 }
 
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
 template <bool FIRST>
 struct Code {  // FIRST: a sign and three bits of mantissa; else four
   static constexpr int mantissa = FIRST ? 3 : 4, drop = 23 - mantissa;
@@ -115,18 +119,32 @@ struct Code {  // FIRST: a sign and three bits of mantissa; else four
     const uint32_t bits = size ? (size + base) << drop : 0u;
     return bits_f32(FIRST ? (bits & 0x7fffffffu) | (high & 0x80000000u) : bits);
   }
-  // the number's top bits after 16 bits of r (FIRST: the low ones) have decided which way they are rounded
-  static __device__ __forceinline__ uint32_t top(float x, uint32_t r) {
-    const uint32_t size = min(FIRST ? f32_bits(x) & 0x7fffffffu : f32_bits(x), 0x7f800000u);
-    const uint32_t half = 1u << (drop - 17), more = FIRST ? (r << (drop - 16)) & (0xffffu << (drop - 16)) : (r >> (32 - drop)) & (0xffffu << (drop - 16));
-    return (size + (more | half)) >> drop;
+  // the number after 16 bits of r (FIRST: the low ones) have decided which way its top bits are rounded; a NaN as infinity
+  static __device__ __forceinline__ uint32_t rounded(float x, uint32_t r) {
+    const uint32_t size = f32_bits(__builtin_fminf(__builtin_fabsf(x), __builtin_inff()));
+    return size + ((FIRST ? r & 0xffffu : r >> 16) << (drop - 16)) + (1u << (drop - 17));
+  }
+  // the top bits of two such numbers side by side, in 16 bits each
+  static __device__ __forceinline__ u16x2_t tops(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(u16x2_t, upper_halves(a, b)) >> (uint16_t)(drop - 16);
   }
   static __device__ __forceinline__ uint32_t base(uint32_t exponent) { return (exponent - 15u) << mantissa; }
   static __device__ __forceinline__ uint32_t exponent(uint32_t largest_top) { return max(largest_top >> mantissa, 16u); }
-  static __device__ __forceinline__ uint32_t code(uint32_t top, float x, uint32_t base) {
-    const int c = (int)top - (int)base;
-    if (FIRST) return c < 1 ? 0u : (uint32_t)c | ((f32_bits(x) >> 24) & 128u);
-    return (uint32_t)max(c, (int)min(f32_bits(x), 1u));  // never 0 unless x is: x is not negative
+  // codes of x and y from their top bits, in 16 bits each
+  static __device__ __forceinline__ u16x2_t codes(u16x2_t top, float x, float y, uint32_t base) {
+    const u16x2_t one = {1, 1}, b = {(uint16_t)base, (uint16_t)base};
+    const i16x2_t none = {0, 0}, c = __builtin_bit_cast(i16x2_t, top - b);
+    if (FIRST) {
+      const u16x2_t size = __builtin_bit_cast(u16x2_t, __builtin_elementwise_max(c, none));
+      const u16x2_t sign = __builtin_bit_cast(u16x2_t, upper_halves(f32_bits(x), f32_bits(y))) >> (uint16_t)15;
+      return size | (sign & __builtin_elementwise_min(size, one)) << (uint16_t)7;
+    }
+    // never 0 unless the number is, which is not negative
+    const i16x2_t least = {(int16_t)min(f32_bits(x), 1u), (int16_t)min(f32_bits(y), 1u)};
+    return __builtin_bit_cast(u16x2_t, __builtin_elementwise_max(c, least));
+  }
+  static __device__ __forceinline__ uint32_t bytes(u16x2_t a, u16x2_t b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x06040200u);
   }
 };
 
@@ -177,29 +195,51 @@ struct Piece {
       v[i] = v[i] * a.c.b2 + (g[i] * g[i]) * a.c.c2;
       const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[i]), a.c.root, a.c.eps);
       p[i] = __builtin_fmaf(m[i] * a.c.rate, -__builtin_amdgcn_rcpf(d), p[i] * a.c.keep);
-      // infinity stays one: its mantissa has no bits to carry from
-      if constexpr (ROUND) p[i] = p[i] != p[i] ? p[i] : bits_f32((f32_bits(p[i]) + (r[i] & 0xffffu)) & 0xffff0000u);
+      // Infinity stays one: its mantissa has no bits to carry from.  A NaN comes with whatever bits a 32-bit moment brought; those of bf16
+      // and of the 8-bit form have none in the lower half, and so nothing to carry either.
+      if constexpr (ROUND) {
+        const float rounded = bits_f32(f32_bits(p[i]) + (r[i] & 0xffffu));
+        p[i] = !EIGHT && p[i] != p[i] ? p[i] : rounded;
+      }
     }
-    store8<T, FULL>(params, at, c.numel, p);
+    if constexpr (ROUND) {  // bf16: the upper halves
+      typename T::Raw raw;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = upper_halves(f32_bits(p[2 * i]), f32_bits(p[2 * i + 1]));
+      if constexpr (FULL) {
+        T::store(params + at, raw);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (at + i < c.numel) params[at + i] = (uint16_t)(raw[i >> 1] >> (16 * (i & 1)));
+      }
+    } else {
+      store8<T, FULL>(params, at, c.numel, p);
+    }
     if constexpr (EIGHT) {
-      uint32_t mt[8], vt[8], mm = 0, vm = 0;
+      u16x2_t mt[4], vt[4], mm = {0, 0}, vm = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mt[i] = Code<true>::top(m[i], r[i]);
-        vt[i] = Code<false>::top(v[i], r[i]);
-        if (FULL || at + i < c.numel) {
-          mm = max(mm, mt[i]);
-          vm = max(vm, vt[i]);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (!FULL) {  // what lies behind the end does not count for the exponent
+#pragma unroll
+          for (int e = 2 * i; e < 2 * i + 2; ++e) m[e] = at + e < c.numel ? m[e] : 0.f, v[e] = at + e < c.numel ? v[e] : 0.f;
         }
+        mt[i] = Code<true>::tops(Code<true>::rounded(m[2 * i], r[2 * i]), Code<true>::rounded(m[2 * i + 1], r[2 * i + 1]));
+        vt[i] = Code<false>::tops(Code<false>::rounded(v[2 * i], r[2 * i]), Code<false>::rounded(v[2 * i + 1], r[2 * i + 1]));
+        mm = __builtin_elementwise_max(mm, mt[i]);
+        vm = __builtin_elementwise_max(vm, vt[i]);
       }
-      const uint32_t em1 = Code<true>::exponent(row_max(mm)), ev1 = Code<false>::exponent(row_max(vm));
+      const uint32_t em1 = Code<true>::exponent(row_max(max((uint32_t)mm.x, (uint32_t)mm.y)));
+      const uint32_t ev1 = Code<false>::exponent(row_max(max((uint32_t)vm.x, (uint32_t)vm.y)));
       const uint32_t bm = Code<true>::base(em1), bv = Code<false>::base(ev1);
-      u32x2_at1_t mo = {0, 0}, vo = {0, 0};
+      u16x2_t ms[4], vs[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mo[i >> 2] |= Code<true>::code(mt[i], m[i], bm) << (8 * (i & 3));
-        vo[i >> 2] |= Code<false>::code(vt[i], v[i], bv) << (8 * (i & 3));
+      for (int i = 0; i < 4; ++i) {
+        ms[i] = Code<true>::codes(mt[i], m[2 * i], m[2 * i + 1], bm);
+        vs[i] = Code<false>::codes(vt[i], v[2 * i], v[2 * i + 1], bv);
       }
+      const u32x2_at1_t mo = {Code<true>::bytes(ms[0], ms[1]), Code<true>::bytes(ms[2], ms[3])};
+      const u32x2_at1_t vo = {Code<false>::bytes(vs[0], vs[1]), Code<false>::bytes(vs[2], vs[3])};
       store_codes<FULL>(reinterpret_cast<uint8_t*>(a.st.exp_avg) + c.offset, at, c.numel, mo);
       store_codes<FULL>(reinterpret_cast<uint8_t*>(a.st.exp_avg_sq) + c.offset, at, c.numel, vo);
       if ((threadIdx.x & 15) == 0 && (FULL || at < c.numel)) {
