@@ -129,6 +129,28 @@ def test_rows_without_a_difference(dtype, rows):
             assert float(g.abs().max()) < 4 * SUM * (1 + 2 * want) / V / temperature
 
 
+@pytest.mark.parametrize("rows,V", [(2, 9000), (600, 5000), (40, 1000)])
+@pytest.mark.parametrize("size", [1e6, 3e8, 1.2e9, 1.9e9, 4e9, 1e12, -2e9])
+def test_logits_of_enormous_size(rows, V, size):
+    """fp32 logits whose neighbours are up to 65536 apart: the row's distribution is even over its largest ones, apart from differences
+    of one where the numbers are that fine.  The difference from the largest is exact; then the sums' error."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    logits = (size + torch.randint(-40, 40, (rows, V), generator=g, device=DEV).double() * max(1.0, abs(size) * 2.0 ** -24)).float()
+    z = logits.double()
+    lp = torch.log_softmax(z - z.amax(-1, keepdim=True), -1)
+    ent = -(lp.exp() * lp).sum(-1)
+    tokens = z.argmax(-1)
+    leaf = logits.clone().requires_grad_()
+    r = layer_ops.token_logprobs(leaf, tokens, entropy=True, top=40)
+    assert float((r.logprobs.double() - lp.gather(1, tokens[:, None])[:, 0]).abs().max()) < SUM + 8 * U * math.log(V)
+    assert float((r.entropy.double() - ent).abs().max()) < 2 * SUM * (1 + math.log(V))
+    order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :40]
+    assert torch.equal(r.top_tokens, order)
+    (grad,) = torch.autograd.grad(r.logprobs.sum(), leaf)
+    want = torch.zeros_like(lp).scatter_(1, tokens[:, None], 1.0) - lp.exp()
+    assert float((grad.double() - want).abs().max()) < 4 * SUM
+
+
 @pytest.mark.parametrize("rows", [1, 600])
 def test_a_row_of_nothing(rows):
     logits = _logits(rows, 6000, torch.bfloat16)

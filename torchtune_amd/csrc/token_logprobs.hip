@@ -149,13 +149,14 @@ __device__ __forceinline__ void fetch(const typename T::elem* x, uint32_t at, ui
   for (int i = 0; i < 8; ++i) v[i] = at + i < end ? T::get(x + at + i) : -__builtin_inff();
 }
 
-// A bound that k of the wave's numbers, N a lane, reach (the k-th largest, cut to 16 bits), by halving.  The wave counts with its lane
-// masks.
-template <int N>
+// A bound that k of the wave's numbers, N a lane, reach: the k-th largest, by halving, of as many bits as a T has.  The wave counts
+// with its lane masks.
+template <class T, int N>
 __device__ __forceinline__ uint32_t kth_bound(const uint32_t (&mine)[N], int k) {
+  constexpr uint32_t kLast = sizeof(typename T::elem) == 2 ? 1u << 16 : 1u;
   uint32_t bound = 0;
 #pragma unroll 1
-  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+  for (uint32_t bit = 1u << 31; bit >= kLast; bit >>= 1) {
     const uint32_t trial = bound | bit;
     int count = 0;
 #pragma unroll
@@ -215,7 +216,7 @@ __device__ void find_top(TopScratch<NT>& t, const typename T::elem* x, uint32_t 
         maxima[w] = t.keys[threadIdx.x + kWave * w];
         group[0] = max(group[0], maxima[w]);
       }
-      const uint32_t b = k <= 24 ? kth_bound(group, k) : kth_bound(maxima, k);
+      const uint32_t b = k <= 24 ? kth_bound<T>(group, k) : kth_bound<T>(maxima, k);
       if (threadIdx.x == 0) t.bound = b;
     }
     __syncthreads();
@@ -348,8 +349,10 @@ struct Given {
 template <class T, int NT, bool ENT>
 __device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem* x, Running r, Given<T> given, const TopScratch<NT>* t, float (*lds)[3]) {
   float s, u;
-  if (__builtin_fabsf(r.max) < __builtin_inff() && !(r.s > 0.f && r.s < __builtin_inff())) {
-    // c x overflows (a row masked with the lowest value of its type): the differences do not.
+  const float rest = r.s > 0.f ? __builtin_fmaf(r.max, a.c, -r.M) : 0.f;  // what M's rounding left of the largest exponent
+  const bool whole = r.s > 0.f && r.s < __builtin_inff() && __builtin_fabsf(r.u) < __builtin_inff() && __builtin_fabsf(rest) < 64.f;
+  if (__builtin_fabsf(r.max) < __builtin_inff() && !whole) {
+    // c x overflows or is too coarse (a row masked with the lowest value of its type, logits beyond 1e9): the differences are not.
     float ps = 0.f, pu = 0.f;
     for (uint32_t j = threadIdx.x; j < a.V; j += NT) {
       const float y = (T::get(x + j) - r.max) * a.c, e = __builtin_amdgcn_exp2f(y);
@@ -371,7 +374,7 @@ __device__ void finish(const LogitArgs& a, uint32_t row, const typename T::elem*
     }
   } else {
     // from M to c m: y' = y - rest, so e' = e 2^-rest
-    const float rest = r.s > 0.f ? __builtin_fmaf(r.max, a.c, -r.M) : 0.f, f = __builtin_amdgcn_exp2f(-rest);
+    const float f = __builtin_amdgcn_exp2f(-rest);
     s = r.s * f;
     u = f * (r.u - rest * r.s);
   }
@@ -487,7 +490,7 @@ __global__ __launch_bounds__(256) void token_logprobs_join_kernel(const LogitArg
     static_assert(kSegmentsMax <= kWave, "a lane for each segment");
     if (threadIdx.x == 0) t.count = 0;
     const uint32_t reached[1] = {lane < n ? (uint32_t)(f[lane * k + i - 1] >> 32) : 0u};
-    const uint32_t bound = kth_bound(reached, need);  // in every wave
+    const uint32_t bound = kth_bound<T>(reached, need);  // in every wave
     __syncthreads();
     for (int q = threadIdx.x; q < n * k; q += 256) {
       const uint64_t one = f[q];
