@@ -859,8 +859,9 @@ int ttamd_token_logprobs_bwd(const ttamd_logits* logits, const int64_t* tokens, 
  * One AdamW step over many tensors (torch.optim.AdamW's update, as the reference's recipes configure it), fp32 math:
  *   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2;
  *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m' / (sqrt(v') / sqrt(1 - beta2^step) + eps)
- * every product and sum rounded by itself.  Parameters and gradients of `dtype`, any alignment of an element; the moments of
- * all tensors lie in two buffers, tensor i's from element `offset` (fp32, state_bits 32) on.
+ * the moments with every product and sum rounded by itself, the parameter's change to a few units of its last place.  Parameters
+ * and gradients of `dtype`, any alignment of an element; the moments of all tensors lie in two buffers, tensor i's from element
+ * `offset` (fp32, state_bits 32) on.
  *
  * state_bits 8: a moment is one byte, and TTAMD_ADAMW_BLOCK consecutive elements of a tensor share a byte of exponent (the
  * tensor's blocks from `block` on in the exponent buffers).  With E the block's exponent byte,

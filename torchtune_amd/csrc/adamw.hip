@@ -3,8 +3,11 @@
 //   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g g;  p' = p (1 - lr wd) - rate (m' / (sqrt(v') root + eps))
 //   rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t), formed on the host in 64 bits
 //
-// in fp32, every product and sum rounded by itself.  Bound: HBM, 22 bytes an element of a bf16 parameter with 32-bit states and 10
-// with 8-bit ones.
+// in fp32, every product and sum rounded by itself (the moments; the parameter's change takes the hardware's root and reciprocal).
+// Bound: HBM, 22 bytes an element of a bf16 parameter with 32-bit states and 10 with 8-bit ones, where the vector ALU is as busy: some
+// 80 lane operations an element, a sixth of them for the numbers that round.  448 tensors of 42 M elements: 172 us (5.4 TB/s) and 76 us (5.5);
+// 218 M elements with 8-bit states and stochastic rounding 390 us (5.6 TB/s);
+// with IEEE division and root, bounds checks on every access and bytes handled one by one 548.
 //
 // One launch covers up to 480 tensors: the gradients' addresses travel in the kernel's arguments (they may change from step to
 // step), the parameters', their sizes and their places in the state buffers stand in a table on the GPU.  A workgroup takes 4096
@@ -68,26 +71,48 @@ typedef uint32_t u32x2_at1_t __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 typedef int16_t i16x2_t __attribute__((ext_vector_type(2)));
 
-// Eight elements from element `at` of n (n > 0).  FULL: all of them are there; else each for itself, those behind the end from the last one
+// A lane's eight elements of a piece of 2048: 8 t .. 8 t + 7, or (SPLIT) 4 t .. 4 t + 3 of its first half and of its second, so that
+// the waves write whole lines of fp32.
+template <bool SPLIT>
+struct Place {
+  static __device__ __forceinline__ int first(int thread) { return SPLIT ? 4 * thread : 8 * thread; }
+  static constexpr int offset(int e) { return SPLIT ? (e & 3) + (e >> 2) * 1024 : e; }
+};
+
+// The eight from element `at` of n (n > 0).  FULL: all of them are there; else each for itself, those behind the end from the last one
 // (what they become is never stored).
-template <class T, bool FULL>
+template <class T, bool SPLIT, bool FULL>
 __device__ __forceinline__ void load8(const typename T::elem* p, int64_t at, int64_t n, float (&v)[8]) {
-  if constexpr (FULL) {
+  if constexpr (FULL && SPLIT) {
+    T::unpack(T::join(T::load4_once(p + at), T::load4_once(p + at + 1024)), v);
+  } else if constexpr (FULL) {
     T::unpack(T::load_once(p + at), v);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = T::get(p + (at + i < n ? at + i : n - 1));
+    for (int i = 0; i < 8; ++i) {
+      const int64_t j = at + Place<SPLIT>::offset(i);
+      v[i] = T::get(p + (j < n ? j : n - 1));
+    }
   }
 }
-template <class T, bool FULL>
-__device__ __forceinline__ void store8(typename T::elem* p, int64_t at, int64_t n, const float (&v)[8]) {
-  if constexpr (FULL) {
-    T::store(p + at, T::pack(v));
+template <class T, bool SPLIT, bool FULL>
+__device__ __forceinline__ void store_raw(typename T::elem* p, int64_t at, int64_t n, const typename T::Raw& r) {
+  if constexpr (FULL && SPLIT) {
+    T::store4(p + at, T::low(r));
+    T::store4(p + at + 1024, T::high(r));
+  } else if constexpr (FULL) {
+    T::store(p + at, r);
   } else {
+    float v[8];
+    T::unpack(r, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (at + i < n) T::put(p + at + i, v[i]);
+      if (at + Place<SPLIT>::offset(i) < n) T::put(p + at + Place<SPLIT>::offset(i), v[i]);
   }
+}
+template <class T, bool SPLIT, bool FULL>
+__device__ __forceinline__ void store8(typename T::elem* p, int64_t at, int64_t n, const float (&v)[8]) {
+  store_raw<T, SPLIT, FULL>(p, at, n, T::pack(v));
 }
 template <bool FULL>
 __device__ __forceinline__ u32x2_at1_t load_codes(const uint8_t* p, int64_t at, int64_t n) {
@@ -152,13 +177,14 @@ struct Code {  // FIRST: a sign and three bits of mantissa; else four
 template <class T, bool EIGHT, bool FULL>
 struct Piece {
   typedef typename T::elem E;
+  static constexpr bool split = !EIGHT;
   float p[8], g[8], m[8], v[8];
   u32x2_at1_t mc, vc;
   uint32_t em, ev;
 
   __device__ __forceinline__ void load(const StepArgs& a, const ttamd_adamw_chunk& c, const E* params, const E* grads, int64_t at) {
-    load8<T, FULL>(params, at, c.numel, p);
-    load8<T, FULL>(grads, at, c.numel, g);
+    load8<T, split, FULL>(params, at, c.numel, p);
+    load8<T, split, FULL>(grads, at, c.numel, g);
     if constexpr (EIGHT) {
       mc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(a.st.exp_avg) + c.offset, at, c.numel);
       vc = load_codes<FULL>(reinterpret_cast<const uint8_t*>(a.st.exp_avg_sq) + c.offset, at, c.numel);
@@ -166,8 +192,8 @@ struct Piece {
       em = a.st.exp_avg_exponent[block];
       ev = a.st.exp_avg_sq_exponent[block];
     } else {
-      load8<F32, FULL>(reinterpret_cast<const float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
-      load8<F32, FULL>(reinterpret_cast<const float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
+      load8<F32, split, FULL>(reinterpret_cast<const float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
+      load8<F32, split, FULL>(reinterpret_cast<const float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
     }
   }
 
@@ -187,7 +213,7 @@ struct Piece {
     if constexpr (EIGHT || ROUND) {
       const uint32_t x0 = (uint32_t)at * kStep + key + (uint32_t)((uint64_t)at >> 32) * 0x85EBCA6Bu;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = spread(x0 + i * kStep);
+      for (int i = 0; i < 8; ++i) r[i] = spread(x0 + Place<split>::offset(i) * kStep);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -206,15 +232,9 @@ struct Piece {
       typename T::Raw raw;
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[i] = upper_halves(f32_bits(p[2 * i]), f32_bits(p[2 * i + 1]));
-      if constexpr (FULL) {
-        T::store(params + at, raw);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (at + i < c.numel) params[at + i] = (uint16_t)(raw[i >> 1] >> (16 * (i & 1)));
-      }
+      store_raw<T, split, FULL>(params, at, c.numel, raw);
     } else {
-      store8<T, FULL>(params, at, c.numel, p);
+      store8<T, split, FULL>(params, at, c.numel, p);
     }
     if constexpr (EIGHT) {
       u16x2_t mt[4], vt[4], mm = {0, 0}, vm = {0, 0};
@@ -247,8 +267,8 @@ struct Piece {
         a.st.exp_avg_sq_exponent[c.block + at / kBlock] = (uint8_t)ev1;
       }
     } else {
-      store8<F32, FULL>(reinterpret_cast<float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
-      store8<F32, FULL>(reinterpret_cast<float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
+      store8<F32, split, FULL>(reinterpret_cast<float*>(a.st.exp_avg) + c.offset, at, c.numel, m);
+      store8<F32, split, FULL>(reinterpret_cast<float*>(a.st.exp_avg_sq) + c.offset, at, c.numel, v);
     }
   }
 };
@@ -261,7 +281,7 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
   const E* g = reinterpret_cast<const E*>(a.g[c.tensor - a.first]);
   uint32_t key = 0;
   if constexpr (EIGHT || ROUND) key = key_of(a.seed_step, c.number);
-  const int64_t at = c.start + 8 * threadIdx.x;
+  const int64_t at = c.start + Place<!EIGHT>::first(threadIdx.x);
   if (c.start + kChunk <= c.numel) {  // uniform
     Piece<T, EIGHT, true> x[kPieces];
 #pragma unroll
@@ -272,16 +292,17 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const StepArgs a) {
   }
 #pragma unroll 1
   for (int i = 0; i < kPieces; ++i) {
-    const int64_t here = at + 2048 * i, wave = here - 8 * (threadIdx.x & 63);
-    if (wave >= c.numel) return;  // whole waves: the rows' maxima need all their lanes
-    if (wave + 512 <= c.numel) {
+    // whole waves (8 bits; the rows' maxima need all their lanes) or whole pieces at a time
+    const int64_t piece = c.start + 2048 * i, begin = EIGHT ? piece + 8 * (threadIdx.x & ~63) : piece;
+    if (begin >= c.numel) return;
+    if (begin + (EIGHT ? 512 : 2048) <= c.numel) {
       Piece<T, EIGHT, true> x;
-      x.load(a, c, p, g, here);
-      x.template step_and_store<ROUND>(a, c, p, here, key);
+      x.load(a, c, p, g, at + 2048 * i);
+      x.template step_and_store<ROUND>(a, c, p, at + 2048 * i, key);
     } else {
       Piece<T, EIGHT, false> x;
-      x.load(a, c, p, g, here);
-      x.template step_and_store<ROUND>(a, c, p, here, key);
+      x.load(a, c, p, g, at + 2048 * i);
+      x.template step_and_store<ROUND>(a, c, p, at + 2048 * i, key);
     }
   }
 }
@@ -298,10 +319,11 @@ __device__ __forceinline__ void read_out(const ttamd_adamw_states& st, const tta
     m[i] = Code<true>::value(mc[i >> 2], i & 3, bm);
     v[i] = Code<false>::value(vc[i >> 2], i & 3, bv);
   }
-  store8<BF16, FULL>(exp_avg + c.offset, at, c.numel, m);
-  store8<BF16, FULL>(exp_avg_sq + c.offset, at, c.numel, v);
+  store8<BF16, false, FULL>(exp_avg + c.offset, at, c.numel, m);
+  store8<BF16, false, FULL>(exp_avg_sq + c.offset, at, c.numel, v);
 }
 
+// 218 M elements in 214 us (6.1 TB/s)
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ttamd_adamw_states st, uint16_t* __restrict__ exp_avg,
                                                             uint16_t* __restrict__ exp_avg_sq) {
   const ttamd_adamw_chunk c = st.chunks[blockIdx.x];
