@@ -72,9 +72,10 @@ struct F32 {
     return Raw{f32x4_at4_t{v[0], v[1], v[2], v[3]}, f32x4_at4_t{v[4], v[5], v[6], v[7]}};
   }
   static __device__ __forceinline__ void store(elem* p, const Raw& r) {
+    // two halves of 32 bytes: the cache has to put neighbouring lanes' together
     f32x4_at4_t* q = reinterpret_cast<f32x4_at4_t*>(p);
-    __builtin_nontemporal_store(r.a, q);
-    __builtin_nontemporal_store(r.b, q + 1);
+    q[0] = r.a;
+    q[1] = r.b;
   }
   typedef f32x4_at4_t Raw4;
   static __device__ __forceinline__ Raw4 load4_once(const elem* p) { return __builtin_nontemporal_load(reinterpret_cast<const Raw4*>(p)); }
