@@ -6,6 +6,7 @@ parameter is scaled and rounded to its type: half a step, or with stochastic rou
 import copy
 import io
 import math
+import threading
 
 import pytest
 import torch
@@ -364,6 +365,67 @@ def test_states_of_the_other_width_are_refused_and_nothing_changes():
     with pytest.raises(ValueError, match="elements"):
         wide.load_state_dict(short)
     assert torch.equal(wide.state[params[0]]["exp_avg"], kept)
+
+
+def test_moments_of_transposed_parameters_are_in_the_order_of_their_memory():
+    """Also where not all parameters have states yet."""
+    p = torch.nn.Parameter(torch.randn(6, 5, device=DEV).t())
+    late = torch.nn.Parameter(torch.randn(7, device=DEV))
+    q = torch.nn.Parameter(torch.randn(3, device=DEV))
+    opt = AdamW([p, late, q], betas=(0.0, 0.0))
+    p.grad, q.grad = torch.randn(5, 6, device=DEV), torch.randn(3, device=DEV)
+    opt.step()
+    m, _ = opt.moments()
+    assert torch.equal(m, torch.cat([p.grad.t().reshape(-1), q.grad]))
+    late.grad = torch.randn(7, device=DEV)
+    opt.step()
+    m, _ = opt.moments()
+    assert torch.equal(m, torch.cat([p.grad.t().reshape(-1), late.grad, q.grad]))
+    alone = AdamW([p], betas=(0.0, 0.0))
+    alone.step()
+    assert torch.equal(alone.moments()[0], p.grad.t().reshape(-1)) and torch.equal(alone.state[p]["exp_avg"], p.grad)
+    p.data = p.data.contiguous()
+    with pytest.raises(RuntimeError, match="order"):
+        alone.step()
+    assert int(alone.state[p]["step"]) == 1
+
+
+def test_a_refused_step_leaves_its_states_visible_and_uncounted():
+    a, b = (torch.nn.Parameter(torch.ones(4, device=DEV)) for _ in range(2))
+    opt = AdamW([a, b], lr=0.1)
+    a.grad, b.grad = torch.ones(4, device=DEV), torch.ones(4, device=DEV)
+    opt.param_groups[0]["betas"] = (1.5, 0.9)
+    with pytest.raises(ValueError, match="beta"):
+        opt.step()
+    assert len(opt.state) == 2 and int(opt.state[a]["step"]) == 0 and bool((a == 1).all())
+    opt.param_groups[0]["betas"] = (0.9, 0.9)
+    opt.step()
+    assert int(opt.state[b]["step"]) == 1 and bool((b != 1).all())
+
+
+def test_threads_may_step_their_own_and_the_same_optimizer():
+    """Ten steps from each of four threads: as many steps as asked for, of one constant gradient in whatever order."""
+    p = torch.nn.Parameter(torch.ones(5000, device=DEV))
+    mine = [torch.nn.Parameter(torch.ones(5000, device=DEV)) for _ in range(4)]
+    shared, own = AdamW([p], lr=1e-3, state_bits=8), [AdamW([x], lr=1e-3, state_bits=8) for x in mine]
+    p.grad = torch.ones_like(p)
+    shared.step()
+    torch.cuda.synchronize()
+
+    def work(x, opt):
+        x.grad = torch.ones_like(x)
+        for _ in range(10):
+            opt.step()
+            shared.step()
+
+    threads = [threading.Thread(target=work, args=args) for args in zip(mine, own)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert int(shared.state[p]["step"]) == 41 and all(int(o.state[x]["step"]) == 10 for o, x in zip(own, mine))
+    assert all(torch.equal(mine[0], x) for x in mine[1:])
 
 
 def test_refusals():

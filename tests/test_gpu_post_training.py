@@ -149,6 +149,13 @@ def test_default_positions_are_the_sequence():
     assert torch.equal(a.logprobs, b.logprobs) and torch.equal(a.logprobs, c.logprobs)
 
 
+def test_a_sequence_longer_than_the_table():
+    model = harness.build_qlora_decoder(dataclasses.replace(SHAPE, max_positions=16), rank=8, alpha=16.0, device=DEV, seed=0)
+    tokens, targets, *_ = _batch(8)
+    with torch.no_grad():
+        assert torch.equal(model.token_logprobs(tokens, targets).logprobs, _model().token_logprobs(tokens, targets).logprobs)
+
+
 def test_a_full_training_step_with_the_optimizer():
     """QAT: every weight trained, bf16, 8-bit states; the ordinary training step's own gradients."""
     model = harness.build_qat_decoder("tiny", groupsize=32, device=DEV, seed=0)

@@ -8,6 +8,8 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <mutex>
+
 namespace {
 
 using at::Tensor;
@@ -347,10 +349,20 @@ void check_param(const Tensor& p) {
   at::assert_no_internal_overlap(p);
 }
 
+// The order of a dense tensor's elements in its states, as it lies in memory.  (One with gaps: row by row.)  Strides of single
+// elements say nothing.
+std::vector<int64_t> order_of(const Tensor& p) {
+  std::vector<int64_t> s = p.strides().vec();
+  for (int64_t d = 0; d < p.dim(); ++d)
+    if (p.size(d) <= 1) s[d] = 0;
+  return s;
+}
+
 // Parameters of one type on one device with the buffers that hold their moments.
 struct Block {
   std::vector<Tensor> params;
   std::vector<int64_t> numbers;
+  std::vector<std::vector<int64_t>> order;  // empty: row by row
   std::vector<Tensor> shadow;  // of parameters that do not lie densely
   std::vector<void*> address;  // that the table holds
   struct Place {
@@ -372,6 +384,7 @@ struct Block {
       const int64_t m = params[i].numel();
       places.push_back({n, m, blocks});
       chunks.push_back((uint32_t)chunk);
+      order.push_back(params[i].is_contiguous() || !params[i].is_non_overlapping_and_dense() ? std::vector<int64_t>() : order_of(params[i]));
       n += m;
       blocks += (m + TTAMD_ADAMW_BLOCK - 1) / TTAMD_ADAMW_BLOCK;
       chunk += (m + TTAMD_ADAMW_CHUNK - 1) / TTAMD_ADAMW_CHUNK;
@@ -427,13 +440,15 @@ struct Block {
     return s;
   }
 
-  // The buffers outlive what another stream does with them.
+  // The buffers outlive what another stream does with them (the later ones were made on whatever stream was current).
   void used_on(const c10::hip::HIPStream& now) const {
-    if (now == stream) return;
-    for (const Tensor* t : {&table, &exp_avg, &exp_avg_sq, &exp_avg_exponent, &exp_avg_sq_exponent})
-      if (t->defined()) c10::hip::HIPCachingAllocator::recordStream(t->storage().data_ptr(), now);
-    for (const Tensor& t : shadow)
+    auto record = [&](const Tensor& t) {
       if (t.defined()) c10::hip::HIPCachingAllocator::recordStream(t.storage().data_ptr(), now);
+    };
+    record(table);
+    for (const Tensor& t : shadow) record(t);
+    if (now == stream) return;
+    for (const Tensor* t : {&exp_avg, &exp_avg_sq, &exp_avg_exponent, &exp_avg_sq_exponent}) record(*t);
   }
 
   // a flat buffer's part of tensor i, laid out as the parameter is
@@ -465,17 +480,19 @@ struct Block {
                 ": a step cannot be recorded into a graph (its count, and with it the bias corrections, would stand still)");
     // everything is checked before anything is changed
     const size_t n = params.size();
-    std::vector<const Tensor*> grads(n);  // null: none
+    std::vector<Tensor> grads(n);  // undefined: none
     for (size_t i = 0; i < n; ++i) {
-      const Tensor &p = params[i], &g = p.grad();
+      const Tensor& p = params[i];
+      const Tensor& g = grads[i] = p.grad();
       if (!g.defined()) continue;
-      grads[i] = &g;
       check_param(p);
       TORCH_CHECK(g.layout() == at::kStrided && !g.key_set().has(c10::DispatchKey::Python), kAdamW, ": gradients must be plain dense tensors");
       TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), kAdamW, ": a gradient is ", g.scalar_type(), ", its parameter ", p.scalar_type());
       TORCH_CHECK(g.device() == p.device() && p.device() == exp_avg.device(), kAdamW, ": a parameter or its gradient has left ", exp_avg.device().str());
       TORCH_CHECK(p.numel() == places[i].numel && g.sizes() == p.sizes() && p.scalar_type() == type, kAdamW,
                   ": a parameter's size or type has changed");
+      TORCH_CHECK(order[i].empty() ? p.is_contiguous() || !p.is_non_overlapping_and_dense() : order_of(p) == order[i], kAdamW,
+                  ": the order of a parameter's elements in memory has changed");
     }
     point();
     used_on(now);
@@ -484,7 +501,7 @@ struct Block {
     int64_t* count = steps.data_ptr<int64_t>();
     const void* g[TTAMD_ADAMW_TENSORS];
     for (size_t first = 0; first < n;) {
-      if (!grads[first]) {
+      if (!grads[first].defined()) {
         ++first;
         continue;
       }
@@ -492,8 +509,8 @@ struct Block {
       std::vector<Tensor> hold;
       std::vector<size_t> back;
       size_t end = first;
-      for (; end < n && end - first < TTAMD_ADAMW_TENSORS && grads[end] && count[end] == count[first]; ++end) {
-        const Tensor &t = params[end], &grad = *grads[end];
+      for (; end < n && end - first < TTAMD_ADAMW_TENSORS && grads[end].defined() && count[end] == count[first]; ++end) {
+        const Tensor &t = params[end], &grad = grads[end];
         const bool dense = t.is_non_overlapping_and_dense();
         if (!dense) {
           shadow[end].copy_(t);
@@ -530,12 +547,15 @@ struct AdamWGroup {
   std::vector<std::unique_ptr<Block>> blocks;
   int64_t number;
   int bits;
+  std::mutex mutex;  // calls run without the interpreter's lock
 
   AdamWGroup(std::vector<Tensor> ps, int64_t first_number, int64_t bits_)
       : params(std::move(ps)), where(params.size(), {-1, -1}), number(first_number), bits((int)bits_) {}
 
   // states for these parameters, a block for each device and type; what has them already keeps them
   void make(const std::vector<int64_t>& of) {
+    const std::lock_guard<std::mutex> lock(mutex);
+    const at::NoGradGuard no_grad;
     std::vector<int64_t> left;
     for (int64_t i : of)
       if (where.at(i).first < 0) left.push_back(i);
@@ -549,11 +569,12 @@ struct AdamWGroup {
           other.push_back(i);
           continue;
         }
-        where[i] = {(int)blocks.size(), (int)ps.size()};
         ps.push_back(params[i]);
         numbers.push_back(number + i);
       }
+      const int block = (int)blocks.size();
       blocks.push_back(std::make_unique<Block>(std::move(ps), numbers, bits));
+      for (size_t k = 0; k < numbers.size(); ++k) where[numbers[k] - number] = {block, (int)k};
       left = std::move(other);
     }
   }
@@ -570,19 +591,23 @@ struct AdamWGroup {
     return s;
   }
 
-  // the places of parameters that got their states in this step
-  std::vector<int64_t> step(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, bool stochastic) {
-    const at::NoGradGuard no_grad;
-    std::vector<int64_t> fresh;
+  // the places of parameters that have a gradient and no states yet
+  std::vector<int64_t> fresh() const {
+    std::vector<int64_t> found;
     for (size_t i = 0; i < params.size(); ++i) {
       if (where[i].first >= 0 || !params[i].grad().defined()) continue;
-      const Tensor& g = params[i].grad();
+      const Tensor g = params[i].grad();
       check_param(params[i]);
       TORCH_CHECK(g.layout() == at::kStrided, kAdamW, ": gradients must be plain dense tensors");
       TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, kAdamW, ": a step cannot be recorded into a graph");
-      fresh.push_back((int64_t)i);
+      found.push_back((int64_t)i);
     }
-    if (!fresh.empty()) make(fresh);
+    return found;
+  }
+
+  void step(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, bool stochastic) {
+    const std::lock_guard<std::mutex> lock(mutex);
+    const at::NoGradGuard no_grad;
     ttamd_adamw_scalars c = {};
     c.lr = lr;
     c.beta1 = beta1;
@@ -594,20 +619,24 @@ struct AdamWGroup {
       c.stochastic = stochastic && b->params[0].scalar_type() == at::kBFloat16;
       b->step(c);
     }
-    return fresh;
   }
 
   // the flat moments, where one block holds all parameters in their order
   std::optional<std::pair<Tensor, Tensor>> whole() {
     if (blocks.size() != 1 || blocks[0]->params.size() != params.size()) return std::nullopt;
+    const std::lock_guard<std::mutex> lock(mutex);
     return blocks[0]->moments();
   }
   // else those of each parameter that has them, in their order
   std::vector<std::pair<Tensor, Tensor>> moments() {
+    const std::lock_guard<std::mutex> lock(mutex);
     std::vector<std::pair<Tensor, Tensor>> all, out;
     for (const auto& b : blocks) all.push_back(b->moments());
-    for (const auto& [b, at] : where)
-      if (b >= 0) out.push_back({blocks[b]->like(all[b].first, at), blocks[b]->like(all[b].second, at)});
+    for (const auto& [b, at] : where) {
+      if (b < 0) continue;
+      const Block::Place& p = blocks[b]->places[at];
+      out.push_back({all[b].first.narrow(0, p.offset, p.numel), all[b].second.narrow(0, p.offset, p.numel)});
+    }
     return out;
   }
 };
@@ -622,6 +651,7 @@ void bind_post(py::module_& m) {
       .def(py::init<std::vector<Tensor>, int64_t, int64_t>())
       .def("make", &AdamWGroup::make, unlocked)
       .def("state", &AdamWGroup::state)
+      .def("fresh", &AdamWGroup::fresh)
       .def("step", &AdamWGroup::step, unlocked)
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);

@@ -294,7 +294,7 @@ class Decoder(nn.Module):
         """``positions``: of each token, [b, s], or [axes, b, s] for a shape with sections; below the shape's ``max_positions``."""
         if positions is None and self.shape.rope_sections is not None:
             positions = torch.arange(tokens.shape[1], device=tokens.device).expand(len(self.shape.rope_sections), *tokens.shape)
-        rope = self._rope_cache(tokens.shape[1] if positions is None else self.shape.max_positions, tokens.device)
+        rope = self._rope_cache(tokens.shape[1] if positions is None else max(tokens.shape[1], self.shape.max_positions), tokens.device)
         h = self.tok_embeddings(tokens)
         delta = None
         for layer in self.layers:

@@ -38,7 +38,7 @@ class AdamW(torch.optim.Optimizer):
 
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
-    other tensors in their place.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  A step cannot be recorded into a
+    other tensors in their place.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  A step cannot be recorded into a
     graph.
     """
 
@@ -99,20 +99,24 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: amsgrad and maximize are not supported")
             plan, params = self._plan(index), group["params"]
             beta1, beta2 = group["betas"]
-            for i in plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], d["seed"], d["stochastic_rounding"]):
-                self._show(plan, params, i)
+            fresh = plan.fresh()
+            if fresh:
+                plan.make(fresh)
+                for i in fresh:
+                    self._show(plan, params, i)
+            plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], d["seed"], d["stochastic_rounding"])
         return loss
 
     def moments(self):
-        """``(exp_avg, exp_avg_sq)`` of all parameters that have states, one after another in their order, as two flat tensors of
-        numbers: the fp32 states themselves where they lie that way already, bfloat16 (exact) for 8-bit states."""
+        """``(exp_avg, exp_avg_sq)`` of all parameters that have states, one after another in their order (a parameter's elements as
+        they lie in memory), as two flat tensors of numbers: the fp32 states themselves where they lie that way already, bfloat16 (exact) for 8-bit states."""
         firsts, seconds = [], []
         for index in range(len(self.param_groups)):
             plan = self._plan(index)
             whole = plan.whole()
             for m, v in plan.moments() if whole is None else [whole]:
-                firsts.append(m.reshape(-1))
-                seconds.append(v.reshape(-1))
+                firsts.append(m)
+                seconds.append(v)
         if not firsts:
             raise RuntimeError("AdamW.moments: no parameter has taken a step yet")
         return (firsts[0], seconds[0]) if len(firsts) == 1 else (torch.cat(firsts), torch.cat(seconds))
