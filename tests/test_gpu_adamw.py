@@ -428,6 +428,37 @@ def test_threads_may_step_their_own_and_the_same_optimizer():
     assert all(torch.equal(mine[0], x) for x in mine[1:])
 
 
+def test_more_than_2_to_the_31_elements():
+    """The first, the middle and the last of a parameter of 2^31 + 5000 elements: the steps of a small one."""
+    n = 2 ** 31 + 5000
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV, dtype=torch.bfloat16))
+    p.grad = torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    small = []
+    for at in (0, 2 ** 31 - 2048, n - 2048):
+        part = slice(at, at + 2048)
+        p.data[part] = torch.randn(2048, generator=g, device=DEV).to(torch.bfloat16)
+        p.grad[part] = torch.randn(2048, generator=g, device=DEV).to(torch.bfloat16)
+        small.append((part, torch.nn.Parameter(p.detach()[part].clone())))
+        small[-1][1].grad = p.grad[part].clone()
+    opt = AdamW([p], lr=1e-2)
+    others = AdamW([q for _, q in small], lr=1e-2)
+    for _ in range(2):
+        opt.step()
+        others.step()
+    for part, q in small:
+        assert torch.equal(p.detach()[part], q.detach()) and torch.equal(opt.state[p]["exp_avg_sq"][part], others.state[q]["exp_avg_sq"])
+    assert not bool(p.detach()[4096:2 ** 31 - 4096].any())
+    del opt, others
+    opt = AdamW([p], lr=0.0, betas=(0.0, 0.0), state_bits=8)  # the moments are the gradient and its square, rounded
+    opt.step()
+    m, v = opt.moments()
+    for part, q in small:
+        assert bool(((m[part].float() - q.grad.float()).abs() <= q.grad.float().abs() / 8 + 2.0 ** -14 * q.grad.float().abs().max()).all())
+        assert bool(((v[part].float() - q.grad.float() ** 2).abs() <= q.grad.float() ** 2 / 16 + 2.0 ** -14 * q.grad.float().abs().max() ** 2).all())
+    assert not bool(m[4096:2 ** 31 - 4096].any()) and not bool(v[4096:2 ** 31 - 4096].any())
+
+
 def test_refusals():
     p = torch.nn.Parameter(torch.zeros(10, device=DEV))
     opt = AdamW([p])

@@ -229,6 +229,25 @@ def test_agrees_with_the_separate_rotation():
     assert torch.equal(a, layer_ops.apply_rope(q, cache)) and torch.equal(b, layer_ops.apply_rope(k, cache))
 
 
+def test_more_than_2_to_the_31_elements():
+    """The last tokens of 2^31 and more elements: what they give by themselves, and their gradients."""
+    s, nh, d = 2 ** 19 + 7, 32, 128
+    q = torch.zeros(1, s, nh, d, device=DEV, dtype=torch.bfloat16)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q[:, -9:] = torch.randn(1, 9, nh, d, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(d, generator=g, device=DEV).to(torch.bfloat16)
+    cache, positions = _table(50, d).to(DEV), torch.randint(0, 50, (1, s), generator=g, device=DEV)
+    q.requires_grad_()
+    empty = q.detach()[:, :, :0]
+    out, _ = layer_ops.qk_norm_rope(q, empty, cache, w, w, positions=positions)
+    (gx,) = torch.autograd.grad(out, q, out.detach())
+    few = q.detach()[:, -9:].clone().requires_grad_()
+    want, _ = layer_ops.qk_norm_rope(few, empty[:, -9:], cache, w, w, positions=positions[:, -9:])
+    (gw,) = torch.autograd.grad(want, few, want.detach())
+    assert torch.equal(out[:, -9:], want) and torch.equal(gx[:, -9:], gw)
+    assert not bool(out[:, :-9].any()) and not bool(gx[:, :-9].any())
+
+
 def test_recorded_into_a_graph():
     xs, ws, gys = _inputs(2, 50, 8, 2, 64, torch.bfloat16, True, "joined")
     cache, positions = _table(100, 64).to(DEV), torch.randint(0, 100, (2, 50), device=DEV)

@@ -260,6 +260,24 @@ def test_gradient_against_differences():
     assert abs(float(slope - (grad * way).sum())) < size * (h * h + SUM / h)
 
 
+def test_more_than_2_to_the_31_logits():
+    """The last rows of 2^31 and more logits: what they give by themselves."""
+    rows, V = 2 ** 14 + 40, 2 ** 17
+    logits = torch.zeros(rows, V, device=DEV, dtype=torch.bfloat16)
+    logits[-30:] = _logits(30, V, torch.bfloat16)
+    tokens = _tokens(rows, V)
+    logits.requires_grad_()
+    r = layer_ops.token_logprobs(logits, tokens, entropy=True, top=3)
+    (g,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), logits)
+    few = torch.cat([logits.detach()[-30:]] * 40).requires_grad_()  # as many rows as are not cut into segments
+    q = layer_ops.token_logprobs(few, tokens[-30:].repeat(40), entropy=True, top=3)
+    (h,) = torch.autograd.grad(q.logprobs.sum() + q.entropy.sum(), few)
+    for a, b in zip(r, q):
+        assert torch.equal(a[-30:], b[-30:])
+    assert torch.equal(g[-30:], h[-30:])
+    assert float((r.logprobs.detach()[:-30] + math.log(V)).abs().max()) < SUM + 8 * U * math.log(V)
+
+
 def test_agrees_with_the_chunk_loss():
     logits, tokens = _logits(40, 4096, torch.bfloat16), _tokens(40, 4096)
     tokens[3] = -100

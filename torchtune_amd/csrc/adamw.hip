@@ -5,7 +5,7 @@
 //
 // in fp32, every product and sum rounded by itself (the moments; the parameter's change takes the hardware's root and reciprocal).
 // Bound: HBM, 22 bytes an element of a bf16 parameter with 32-bit states and 10 with 8-bit ones, where the vector ALU is as busy: some
-// 80 lane operations an element, a sixth of them for the numbers that round.  448 tensors of 42 M elements: 172 us (5.4 TB/s) and 76 us (5.5);
+// 80 lane operations an element, a sixth of them for the numbers that round.  448 tensors of 42 M elements: 156 us (5.9 TB/s) and 76 us (5.5);
 // 218 M elements with 8-bit states and stochastic rounding 390 us (5.6 TB/s);
 // with IEEE division and root, bounds checks on every access and bytes handled one by one 548.
 //

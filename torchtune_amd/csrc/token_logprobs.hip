@@ -11,7 +11,7 @@
 //
 // Bound: HBM, closely followed by the vector ALU in the forward over bf16: at 6 TB/s a compute unit takes about 5 elements a
 // cycle, which leaves twelve lane operations for each, and exp2 alone takes four.  2048 x 128256 in bf16 with the entropy: forward
-// 95 us (525 MB, 5.5 TB/s), backward 163 us (1.05 GB, 6.4 TB/s); 700 x 50257 in fp32, rows at odd places: 24 and 56 us (6.0 and 5.1).
+// 95 us (525 MB, 5.5 TB/s), backward 163 us (1.05 GB, 6.4 TB/s); 700 x 50257 in fp32, rows at odd places: 24 and 47 us (5.9 and 6.0).
 //
 // The largest elements come from the same pass: a number that k maxima of disjoint sets of elements reach is no larger than the k-th
 // largest element, so that only threads whose maximum reaches it (a few more than k) look at their elements again; what they find is
