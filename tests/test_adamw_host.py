@@ -1,0 +1,59 @@
+"""What ``training.AdamW`` refuses and keeps before any kernel is launched (all on the CPU, where a step ends at the parameters' device)."""
+import pytest
+import torch
+
+from torchtune_amd import AdamW
+
+
+def _saved(p, strides, seed=0):
+    """8-bit states of a parameter that lies with these strides"""
+    g = torch.Generator().manual_seed(seed)
+    code = lambda: torch.randint(0, 128, (p.numel(),), dtype=torch.uint8, generator=g).as_strided(p.shape, strides)
+    exponents = torch.randint(90, 120, (-(-p.numel() // 128),), dtype=torch.uint8, generator=g)
+    return {"step": 3, "exp_avg": code(), "exp_avg_sq": code(), "exp_avg_exponent": exponents, "exp_avg_sq_exponent": exponents.clone()}
+
+
+_ROWS, _COLUMNS = (48, 1), (1, 64)
+
+
+def _parameter(layout):
+    return torch.nn.Parameter({"rows": lambda: torch.zeros(64, 48), "columns": lambda: torch.zeros(48, 64).t(),
+                               "gaps": lambda: torch.zeros(64, 50)[:, 1:49], "gaps in columns": lambda: torch.zeros(48, 70).t()[3:67],
+                               "one row": lambda: torch.zeros(64, 48)[:1], "3d": lambda: torch.zeros(48, 4, 16).permute(1, 2, 0)}[layout]())
+
+
+@pytest.mark.parametrize("layout,strides,fits", [
+    ("rows", _ROWS, True), ("rows", _COLUMNS, False), ("columns", _COLUMNS, True), ("columns", _ROWS, False),
+    # a parameter with gaps is copied row by row
+    ("gaps", _ROWS, True), ("gaps", _COLUMNS, False), ("gaps in columns", _ROWS, True), ("gaps in columns", _COLUMNS, False),
+    ("one row", (48, 1), True), ("one row", (1, 1), True), ("3d", (16, 1, 64), True), ("3d", (768, 48, 1), False),
+])
+def test_eight_bit_states_of_another_order_in_memory(layout, strides, fits):
+    """Their exponents belong to neighbours in memory: refused where those would be others, before anything changes."""
+    p = _parameter(layout)
+    opt = AdamW([p], state_bits=8)
+    saved = {"state": {0: _saved(p, strides)}, "param_groups": opt.state_dict()["param_groups"]}
+    with pytest.raises(RuntimeError if fits else ValueError, match="AMD GPU" if fits else "another order"):
+        opt.load_state_dict(saved)
+    assert fits or not opt.state
+
+
+def test_flat_eight_bit_states():
+    """One after another: right for a parameter whose rows lie that way, and for no other."""
+    for layout, fits in (("rows", True), ("gaps", True), ("columns", False)):
+        p = _parameter(layout)
+        opt = AdamW([p], state_bits=8)
+        saved = {"state": {0: {name: t.reshape(-1) if name in ("exp_avg", "exp_avg_sq") else t for name, t in _saved(p, _ROWS).items()}},
+                 "param_groups": opt.state_dict()["param_groups"]}
+        with pytest.raises(RuntimeError if fits else ValueError, match="AMD GPU" if fits else "another order"):
+            opt.load_state_dict(saved)
+
+
+def test_states_in_32_bits_follow_their_elements():
+    """No block, no order: the check lets them through."""
+    p = _parameter("rows")
+    opt = AdamW([p])
+    m = torch.zeros(48, 64).t()
+    saved = {"state": {0: {"step": 1, "exp_avg": m, "exp_avg_sq": m}}, "param_groups": opt.state_dict()["param_groups"]}
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        opt.load_state_dict(saved)

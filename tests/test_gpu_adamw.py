@@ -539,3 +539,34 @@ def test_on_another_stream():
         results.append(torch.cat([p.detach() for p in params]))
         del junk
     assert torch.equal(*results)
+
+
+def test_eight_bit_states_are_not_loaded_into_another_order():
+    """A block's exponent is that of neighbours in memory.  Rows of very different sizes, so that another block's exponent would show."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    grad = torch.randn(64, 64, generator=g, device=DEV) * torch.exp(4 * torch.randn(64, 1, generator=g, device=DEV))
+    p = torch.nn.Parameter(torch.zeros(64, 64, device=DEV).t())
+    p.grad = grad
+    opt = AdamW([p], state_bits=8)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    moments = [x.clone() for x in opt.moments()]
+    rows = torch.nn.Parameter(p.detach().contiguous())
+    with pytest.raises(ValueError, match="another order"):
+        AdamW([rows], state_bits=8).load_state_dict(saved)
+    again = AdamW([torch.nn.Parameter(torch.zeros(64, 64, device=DEV).t())], state_bits=8)
+    again.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(again.moments(), moments))
+    # the same parameter, laid out anew: its own states are refused, by a load and by a group that has grown, and are still there
+    p.data = p.data.contiguous()
+    with pytest.raises(ValueError, match="another order"):
+        opt.load_state_dict(saved)
+    late = torch.nn.Parameter(torch.zeros(5, device=DEV))
+    late.grad = torch.ones(5, device=DEV)
+    opt.param_groups[0]["params"].append(late)
+    with pytest.raises(ValueError, match="another order"):
+        opt.step()
+    assert int(opt.state[p]["step"]) == 1 and torch.equal(opt.state[p]["exp_avg"], saved["state"][0]["exp_avg"]) and bool((late == 0).all())
+    p.data = p.data.t().contiguous().t()
+    opt.step()
+    assert int(opt.state[p]["step"]) == 2 and int(opt.state[late]["step"]) == 1

@@ -6,11 +6,26 @@ or, to save memory, an optimizer of a third package with 8-bit states.  :class:`
 from __future__ import annotations
 
 from itertools import chain
-from typing import Dict, Tuple
+from typing import Dict, List, Tuple
 
 import torch
 
 from .. import _host
+
+
+def _order(t: torch.Tensor) -> List[int]:
+    """The dimensions of more than one element, from the slowest to the fastest in memory."""
+    return sorted((d for d in range(t.dim()) if t.shape[d] > 1), key=lambda d: -t.stride(d))
+
+
+def _order_of_states(p: torch.Tensor) -> List[int]:
+    """That of a parameter's states: as it lies itself, or row by row if it has gaps."""
+    order, step = _order(p), 1
+    for d in reversed(order):
+        if p.stride(d) != step:
+            return sorted(order)
+        step *= p.shape[d]
+    return order
 
 
 class AdamW(torch.optim.Optimizer):
@@ -71,6 +86,9 @@ class AdamW(torch.optim.Optimizer):
         first = sum(len(g["params"]) for g in self.param_groups[:index])
         plan = _host.load().AdamWGroup(params, first, self.defaults["state_bits"])
         given = [i for i, p in enumerate(params) if self.state.get(p)]
+        if self.defaults["state_bits"] == 8:
+            for i in given:
+                self._check_order(self.state[params[i]], params[i])
         plan.make(given)
         for i in given:
             held = self.state[params[i]]
@@ -124,7 +142,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """What :meth:`state_dict` gave, of an optimizer with as many bits."""
+        """What :meth:`state_dict` gave, of an optimizer with as many bits.  With 8 bits the parameters have to lie in memory in the order in
+        which those of the saved states lay (of dense ones the states have the strides), since neighbours there share exponents."""
         saved, eight = state_dict["state"], self.defaults["state_bits"] == 8
         ids = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
         params = list(chain.from_iterable(g["params"] for g in self.param_groups))
@@ -153,3 +172,17 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW.load_state_dict: {name} is {t.dtype}, the states of this optimizer have {8 if eight else 32} bits")
             if t.numel() != (blocks if name.endswith("exponent") else p.numel()):
                 raise ValueError(f"AdamW.load_state_dict: {name} has {t.numel()} elements, the parameter {p.numel()}")
+        if eight:
+            AdamW._check_order(held, p)
+
+    @staticmethod
+    def _check_order(held, p) -> None:
+        """8 bits: the exponents are those of neighbours in memory, so codes in another order would meet others' exponents."""
+        want = _order_of_states(p)
+        for name in ("exp_avg", "exp_avg_sq"):
+            t = held[name]
+            have = _order(t)
+            same = have == want if t.shape == p.shape else have == sorted(have) and want == sorted(want)
+            if p.numel() and not same:
+                raise ValueError(f"AdamW: the 8-bit {name} {tuple(t.shape)} of strides {t.stride()} lies in another order than its parameter "
+                                 f"{tuple(p.shape)} of strides {p.stride()}")
