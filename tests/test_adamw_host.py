@@ -57,3 +57,39 @@ def test_states_in_32_bits_follow_their_elements():
     saved = {"state": {0: {"step": 1, "exp_avg": m, "exp_avg_sq": m}}, "param_groups": opt.state_dict()["param_groups"]}
     with pytest.raises(RuntimeError, match="AMD GPU"):
         opt.load_state_dict(saved)
+
+
+def test_options_of_a_group_are_checked_and_taken():
+    p = lambda: torch.nn.Parameter(torch.zeros(200))
+    with pytest.raises(ValueError, match="state_bits"):
+        AdamW([{"params": [p()], "state_bits": 16}])
+    opt = AdamW([p()])
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.add_param_group({"params": [p()], "state_bits": 16})
+    assert len(opt.param_groups) == 1
+    # a group with 8 bits beside one with 32: states of its own width get as far as the device, the other's are refused
+    opt = AdamW([{"params": [p()]}, {"params": [p()], "state_bits": 8}])
+    eight = _saved(opt.param_groups[1]["params"][0], (1,))
+    wide = {"step": 1, "exp_avg": torch.zeros(200), "exp_avg_sq": torch.zeros(200)}
+    groups = opt.state_dict()["param_groups"]
+    for states, error, match in (({1: eight}, RuntimeError, "AMD GPU"), ({0: wide}, RuntimeError, "AMD GPU"), ({0: eight}, ValueError, "bits"),
+                                 ({1: wide}, ValueError, "expected")):
+        with pytest.raises(error, match=match):
+            opt.load_state_dict({"state": states, "param_groups": groups})
+
+
+def test_options_of_a_state_dict():
+    p = torch.nn.Parameter(torch.zeros(200))
+    saved = AdamW([p], lr=0.5, seed=9, stochastic_rounding=True).state_dict()
+    opt = AdamW([p], seed=1)
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["seed"] == 9 and opt.param_groups[0]["stochastic_rounding"] and opt.param_groups[0]["lr"] == 0.5
+    eight = AdamW([p], state_bits=8)
+    eight.load_state_dict(saved)  # no states, nothing to refuse
+    assert eight.param_groups[0]["state_bits"] == 8
+    # torch's groups know nothing of them
+    opt.load_state_dict(torch.optim.AdamW([p], lr=0.25).state_dict())
+    assert opt.param_groups[0]["seed"] == 9 and opt.param_groups[0]["stochastic_rounding"] and opt.param_groups[0]["lr"] == 0.25
+    assert opt.param_groups[0]["state_bits"] == 32
+    with pytest.raises(ValueError):
+        opt.load_state_dict({"state": {}, "param_groups": saved["param_groups"] * 2})

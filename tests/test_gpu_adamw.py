@@ -570,3 +570,48 @@ def test_eight_bit_states_are_not_loaded_into_another_order():
     p.data = p.data.t().contiguous().t()
     opt.step()
     assert int(opt.state[p]["step"]) == 2 and int(opt.state[late]["step"]) == 1
+
+
+def test_a_run_continued_by_an_optimizer_built_with_another_seed():
+    params = _tensors([(3000,), (200,)], torch.bfloat16)
+    opt = AdamW(params, lr=1e-3, state_bits=8, stochastic_rounding=True, seed=9)
+    opt.step()
+    other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = AdamW(other, lr=1.0, state_bits=8, seed=1)
+    again.load_state_dict(opt.state_dict())
+    for p, q in zip(params, other):
+        q.grad = p.grad.clone()
+    for _ in range(2):
+        opt.step()
+        again.step()
+    for p, q in zip(params, other):
+        assert torch.equal(p.detach(), q.detach()) and all(torch.equal(opt.state[p][name], again.state[q][name]) for name in opt.state[p])
+
+
+def test_options_of_the_groups_own():
+    """Width, seed and rounding of each group, as an optimizer of its own would have them."""
+    def groups(params):
+        return [{"params": params[:2], "state_bits": 8, "seed": 5}, {"params": params[2:4], "seed": 6, "stochastic_rounding": True},
+                {"params": params[4:], "state_bits": 8, "seed": 7, "stochastic_rounding": True}]
+
+    shapes = [(300,), (129,)] * 3
+    params = _tensors(shapes, torch.bfloat16)
+    opt = AdamW(groups(params), lr=1e-2)
+    scalars = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2)
+    refs = [_Reference(p, i, (8, 32, 8)[i // 2], 5 + i // 2, **scalars) for i, p in enumerate(params)]
+    for _ in range(2):
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for i, (p, b, r) in enumerate(zip(params, before, refs)):
+            r.take(b, p.grad)
+            r.check(p, opt.state[p], whole_step=i >= 2)
+    m, v = opt.moments()
+    assert torch.equal(m.float().cpu(), torch.cat([r.m for r in refs])) and torch.equal(v.float().cpu(), torch.cat([r.v for r in refs]))
+    # stochastic rounding shows: some parameters are not the nearest to what they should be
+    off = torch.cat([(p.detach().cpu().double() - r.want).abs() / (r.want.abs() * torch.finfo(p.dtype).eps / 2 + 16 * U * r.size) for p, r in zip(params[2:], refs[2:])])
+    assert bool((off > 1).any())
+    # the width of states that are there does not change
+    opt.param_groups[0]["state_bits"] = 32
+    with pytest.raises(ValueError, match="bits"):
+        opt.step()
+    assert all(int(opt.state[p]["step"]) == 2 for p in params)

@@ -51,6 +51,9 @@ class AdamW(torch.optim.Optimizer):
             then kept on average, as they would be with a float32 copy. Default: False
         seed (int): of the stochastic rounding. Default: 0
 
+    Every option may be a group's own.  Loading a state dict takes its options over, as for any optimizer, ``seed`` and
+    ``stochastic_rounding`` among them, so that a run goes on with the numbers that it would have had; ``state_bits`` stays, and states of the other width are refused.
+
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
     other tensors in their place.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and
@@ -65,11 +68,15 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
         if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
             raise ValueError(f"AdamW: betas must be two numbers in [0, 1), got {betas}")
-        if state_bits not in (8, 32):
-            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
         self._plans: Dict[int, tuple] = {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
+
+    def add_param_group(self, param_group) -> None:
+        bits = param_group.get("state_bits", self.defaults["state_bits"])
+        if bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {bits}")
+        super().add_param_group(param_group)
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
@@ -77,18 +84,18 @@ class AdamW(torch.optim.Optimizer):
 
     def _plan(self, index: int):
         """The group's native side; it takes over the states that are there already."""
-        params = self.param_groups[index]["params"]
+        group = self.param_groups[index]
+        params, bits = group["params"], group["state_bits"]
         known = self._plans.get(index)
-        if known is not None and known[1] is params and known[2] == len(params):
+        if known is not None and known[1] is params and known[2:] == (len(params), bits):
             return known[0]
         if len({id(p) for p in params}) != len(params):
             raise ValueError("AdamW: a parameter occurs twice in a group")
         first = sum(len(g["params"]) for g in self.param_groups[:index])
-        plan = _host.load().AdamWGroup(params, first, self.defaults["state_bits"])
+        plan = _host.load().AdamWGroup(params, first, bits)
         given = [i for i, p in enumerate(params) if self.state.get(p)]
-        if self.defaults["state_bits"] == 8:
-            for i in given:
-                self._check_order(self.state[params[i]], params[i])
+        for i in given:
+            self._check_states(self.state[params[i]], params[i], bits)
         plan.make(given)
         for i in given:
             held = self.state[params[i]]
@@ -98,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
                     tensor.fill_(int(held[name]))
                 else:
                     tensor.copy_(held[name].reshape(tensor.shape))
-        self._plans[index] = (plan, params, len(params))
+        self._plans[index] = (plan, params, len(params), bits)
         return plan
 
     def _show(self, plan, params, i: int) -> None:
@@ -111,7 +118,6 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        d = self.defaults
         for index, group in enumerate(self.param_groups):
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("AdamW: amsgrad and maximize are not supported")
@@ -122,7 +128,8 @@ class AdamW(torch.optim.Optimizer):
                 plan.make(fresh)
                 for i in fresh:
                     self._show(plan, params, i)
-            plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], d["seed"], d["stochastic_rounding"])
+            plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]),
+                      bool(group["stochastic_rounding"]))
         return loss
 
     def moments(self):
@@ -144,15 +151,19 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """What :meth:`state_dict` gave, of an optimizer with as many bits.  With 8 bits the parameters have to lie in memory in the order in
         which those of the saved states lay (of dense ones the states have the strides), since neighbours there share exponents."""
-        saved, eight = state_dict["state"], self.defaults["state_bits"] == 8
-        ids = list(chain.from_iterable(g["params"] for g in state_dict["param_groups"]))
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # else the base class refuses it
+            for theirs, ours in zip(groups, self.param_groups):
+                for key, p in zip(theirs["params"], ours["params"]):
+                    if key in saved:
+                        self._check_states(saved[key], p, ours["state_bits"])
+            # the width stays; another AdamW's groups have no such options
+            groups = [{"stochastic_rounding": ours["stochastic_rounding"], "seed": ours["seed"], **theirs, "state_bits": ours["state_bits"]}
+                      for theirs, ours in zip(groups, self.param_groups)]
+        ids = list(chain.from_iterable(g["params"] for g in groups))
         params = list(chain.from_iterable(g["params"] for g in self.param_groups))
-        if len(ids) == len(params):  # else the base class refuses it
-            for key, p in zip(ids, params):
-                if key in saved:
-                    self._check_saved(saved[key], p, eight)
         # the states pass the base class by: it would cast them to the parameters' type
-        super().load_state_dict({**state_dict, "state": {}})
+        super().load_state_dict({**state_dict, "state": {}, "param_groups": groups})
         for key, p in zip(ids, params):
             if key in saved:
                 self.state[p] = dict(saved[key])
@@ -161,17 +172,18 @@ class AdamW(torch.optim.Optimizer):
             self._plan(index)
 
     @staticmethod
-    def _check_saved(held, p, eight: bool) -> None:
+    def _check_states(held, p, bits: int) -> None:
+        eight = bits == 8
         names = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_exponent", "exp_avg_sq_exponent"} if eight else set())
         if not names <= set(held):
-            raise ValueError(f"AdamW.load_state_dict: a state holds {sorted(held)}, expected {sorted(names)}")
+            raise ValueError(f"AdamW: a state holds {sorted(held)}, expected {sorted(names)}")
         blocks = -(-p.numel() // 128)
         for name in names - {"step"}:
             t = held[name]
             if (t.dtype == torch.uint8) != eight:
-                raise ValueError(f"AdamW.load_state_dict: {name} is {t.dtype}, the states of this optimizer have {8 if eight else 32} bits")
+                raise ValueError(f"AdamW: {name} is {t.dtype}, the states of this optimizer have {bits} bits")
             if t.numel() != (blocks if name.endswith("exponent") else p.numel()):
-                raise ValueError(f"AdamW.load_state_dict: {name} has {t.numel()} elements, the parameter {p.numel()}")
+                raise ValueError(f"AdamW: {name} has {t.numel()} elements, the parameter {p.numel()}")
         if eight:
             AdamW._check_order(held, p)
 
