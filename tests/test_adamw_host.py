@@ -93,3 +93,23 @@ def test_options_of_a_state_dict():
     assert opt.param_groups[0]["state_bits"] == 32
     with pytest.raises(ValueError):
         opt.load_state_dict({"state": {}, "param_groups": saved["param_groups"] * 2})
+
+
+def test_a_parameter_replaced_in_its_group():
+    """The list is the same and as long, the parameter is another: the native side is made anew."""
+    old, new, kept = (torch.nn.Parameter(torch.zeros(4)) for _ in range(3))
+    opt = AdamW([old, kept])
+    first = opt._plan(0)
+    assert opt._plan(0) is first
+    opt.param_groups[0]["params"][0] = new
+    new.grad = torch.ones(4)
+    assert opt._plan(0) is not first
+    with pytest.raises(RuntimeError, match="AMD GPU"):  # it is asked for a step
+        opt.step()
+    opt.param_groups[0]["params"] = [kept]
+    opt.step()  # no gradient
+    assert opt._plan(0).holds([kept]) and not opt._plan(0).holds([new]) and not opt._plan(0).holds([kept, new]) and not opt._plan(0).holds([None])
+    with pytest.warns(UserWarning):
+        twice = AdamW([old, old])
+    with pytest.raises(ValueError, match="twice"):
+        twice.step()

@@ -615,3 +615,33 @@ def test_options_of_the_groups_own():
     with pytest.raises(ValueError, match="bits"):
         opt.step()
     assert all(int(opt.state[p]["step"]) == 2 for p in params)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("with_states", [False, True])
+def test_a_parameter_replaced_in_its_group(bits, with_states):
+    """``param_groups[0]["params"][i] = other``, as resizing and pruning do: the new one is stepped, from states given for it, and the old
+    one is left alone; the neighbours go on."""
+    params = _tensors([(300,), (129,), (40,)], torch.float32)
+    group = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
+    opt = AdamW(params, **group, state_bits=bits, seed=4)
+    refs = [_Reference(p, i, bits, 4, **group) for i, p in enumerate(params)]
+
+    def step(used):
+        before = [p.detach().clone() for p in used]
+        opt.step()
+        for p, b, r in zip(used, before, refs):
+            r.take(b, p.grad)
+            r.check(p, opt.state[p])
+
+    step(params)
+    old, new = params[1], _tensors([(129,) if with_states else (200,)], torch.float32, 7)[0]
+    kept = old.detach().clone()
+    opt.param_groups[0]["params"][1] = new
+    if with_states:
+        opt.state[new] = {name: t.clone() for name, t in opt.state.pop(old).items()}
+    else:
+        refs[1] = _Reference(new, 1, bits, 4, **group)
+    for _ in range(2):
+        step([params[0], new, params[2]])
+    assert torch.equal(old.detach(), kept) and int(opt.state[new]["step"]) == (3 if with_states else 2)

@@ -6,6 +6,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPCachingAllocator.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <mutex>
@@ -552,6 +553,18 @@ struct AdamWGroup {
   AdamWGroup(std::vector<Tensor> ps, int64_t first_number, int64_t bits_)
       : params(std::move(ps)), where(params.size(), {-1, -1}), number(first_number), bits((int)bits_) {}
 
+  // whether a list still holds these parameters (the tensors themselves: an element may have been replaced)
+  bool holds(const py::handle& list) const {
+    const py::object items = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), "expected a list of parameters"));
+    if (!items) throw py::error_already_set();
+    if (PySequence_Fast_GET_SIZE(items.ptr()) != (Py_ssize_t)params.size()) return false;
+    for (size_t i = 0; i < params.size(); ++i) {
+      PyObject* p = PySequence_Fast_GET_ITEM(items.ptr(), (Py_ssize_t)i);
+      if (!THPVariable_Check(p) || THPVariable_Unpack(p).unsafeGetTensorImpl() != params[i].unsafeGetTensorImpl()) return false;
+    }
+    return true;
+  }
+
   // states for these parameters, a block for each device and type; what has them already keeps them
   void make(const std::vector<int64_t>& of) {
     const std::lock_guard<std::mutex> lock(mutex);
@@ -649,6 +662,7 @@ void bind_post(py::module_& m) {
   m.def("token_logprobs", &token_logprobs, unlocked);
   py::class_<AdamWGroup>(m, "AdamWGroup")
       .def(py::init<std::vector<Tensor>, int64_t, int64_t>())
+      .def("holds", &AdamWGroup::holds)
       .def("make", &AdamWGroup::make, unlocked)
       .def("state", &AdamWGroup::state)
       .def("fresh", &AdamWGroup::fresh)

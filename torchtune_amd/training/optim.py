@@ -87,7 +87,7 @@ class AdamW(torch.optim.Optimizer):
         group = self.param_groups[index]
         params, bits = group["params"], group["state_bits"]
         known = self._plans.get(index)
-        if known is not None and known[1] is params and known[2:] == (len(params), bits):
+        if known is not None and known[1] == bits and known[0].holds(params):
             return known[0]
         if len({id(p) for p in params}) != len(params):
             raise ValueError("AdamW: a parameter occurs twice in a group")
@@ -105,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
                     tensor.fill_(int(held[name]))
                 else:
                     tensor.copy_(held[name].reshape(tensor.shape))
-        self._plans[index] = (plan, params, len(params), bits)
+        self._plans[index] = (plan, bits)
         return plan
 
     def _show(self, plan, params, i: int) -> None:
