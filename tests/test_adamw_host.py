@@ -113,3 +113,16 @@ def test_a_parameter_replaced_in_its_group():
         twice = AdamW([old, old])
     with pytest.raises(ValueError, match="twice"):
         twice.step()
+
+
+def test_states_taken_out_of_the_dictionary():
+    """What the native side holds for them is given up."""
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([p])
+    first = opt._plan(0)
+    assert opt._plan(0) is first
+    opt.state = type(opt.state)(dict)
+    second = opt._plan(0)
+    assert second is not first and opt._plan(0) is second
+    opt.state[torch.nn.Parameter(torch.zeros(1))] = {}
+    assert opt._plan(0) is not second

@@ -3,6 +3,7 @@ hold of them), and in 64 bits for the parameters.
 
 Tolerances.  A parameter's change is a product of a quotient: five roundings and the scalars' own, less than 16 * 2^-24 of its size; the
 parameter is scaled and rounded to its type: half a step, or with stochastic rounding a whole one."""
+import collections
 import copy
 import io
 import math
@@ -645,3 +646,28 @@ def test_a_parameter_replaced_in_its_group(bits, with_states):
     for _ in range(2):
         step([params[0], new, params[2]])
     assert torch.equal(old.detach(), kept) and int(opt.state[new]["step"]) == (3 if with_states else 2)
+
+
+@pytest.mark.parametrize("how", ["clear", "replace", "pop"])
+def test_states_taken_out_begin_anew(how):
+    """As an optimizer made at that point would go on, for the parameters whose states are gone."""
+    params = _tensors([(300,), (129,)], torch.float32)
+    group = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
+    opt = AdamW([{"params": params[:1]}, {"params": params[1:]}], **group, state_bits=8, seed=4)
+    refs = [_Reference(p, i, 8, 4, **group) for i, p in enumerate(params)]
+    for step in range(4):
+        if step == 2:
+            if how == "clear":
+                opt.state.clear()
+            elif how == "replace":
+                opt.state = collections.defaultdict(dict)
+            else:
+                opt.state.pop(params[0])
+            for i, p in enumerate(params[:1 if how == "pop" else 2]):
+                refs[i] = _Reference(p, i, 8, 4, **group)
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for p, b, r in zip(params, before, refs):
+            r.take(b, p.grad)
+            r.check(p, opt.state[p])
+    assert len(opt.state_dict()["state"]) == 2

@@ -56,7 +56,7 @@ class AdamW(torch.optim.Optimizer):
 
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
-    other tensors in their place.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and
+    other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and
     order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  A step cannot be recorded into a graph.
     """
 
@@ -68,7 +68,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
         if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
             raise ValueError(f"AdamW: betas must be two numbers in [0, 1), got {betas}")
-        self._plans: Dict[int, tuple] = {}
+        self._forget()
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
 
@@ -80,10 +80,16 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
-        self._plans = {}
+        self._forget()
+
+    def _forget(self) -> None:
+        self._plans: Dict[int, tuple] = {}
+        self._seen = (None, 0)  # the dictionary of states and its length when the plans were right
 
     def _plan(self, index: int):
         """The group's native side; it takes over the states that are there already."""
+        if self._seen[0] is not self.state or self._seen[1] != len(self.state):  # states were taken out, or put in
+            self._forget()
         group = self.param_groups[index]
         params, bits = group["params"], group["state_bits"]
         known = self._plans.get(index)
@@ -106,6 +112,7 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     tensor.copy_(held[name].reshape(tensor.shape))
         self._plans[index] = (plan, bits)
+        self._seen = (self.state, len(self.state))
         return plan
 
     def _show(self, plan, params, i: int) -> None:
@@ -128,6 +135,7 @@ class AdamW(torch.optim.Optimizer):
                 plan.make(fresh)
                 for i in fresh:
                     self._show(plan, params, i)
+                self._seen = (self.state, len(self.state))
             plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]),
                       bool(group["stochastic_rounding"]))
         return loss
@@ -167,7 +175,7 @@ class AdamW(torch.optim.Optimizer):
         for key, p in zip(ids, params):
             if key in saved:
                 self.state[p] = dict(saved[key])
-        self._plans = {}
+        self._forget()
         for index in range(len(self.param_groups)):
             self._plan(index)
 
