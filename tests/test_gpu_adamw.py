@@ -671,3 +671,53 @@ def test_states_taken_out_begin_anew(how):
             r.take(b, p.grad)
             r.check(p, opt.state[p])
     assert len(opt.state_dict()["state"]) == 2
+
+
+def _blocks_of_all_kinds():
+    """Two groups; the first with two types and a parameter that joined later: four blocks in all."""
+    params = _tensors([(300,), (8, 16)], torch.float32) + _tensors([(129,)], torch.bfloat16, 1) + _tensors([(9, 16)], torch.float32, 2) + _tensors([(70,), (6, 5)], torch.float32, 3)
+    opt = AdamW([{"params": params[:4]}, {"params": params[4:]}], lr=1e-2)
+    late, params[3].grad = params[3].grad, None
+    opt.step()
+    params[3].grad = late
+    opt.step()
+    return params, opt
+
+
+@pytest.mark.parametrize("which", [1, 3, 5])
+@pytest.mark.parametrize("why", ["order", "size", "gone"])
+def test_a_step_refused_for_one_parameter_moves_none(which, why):
+    params, opt = _blocks_of_all_kinds()
+    before, counts = [p.detach().clone() for p in params], [int(opt.state[p]["step"]) for p in params]
+    moments = [x.clone() for x in opt.moments()]
+    p, kept = params[which], params[which].data
+    if why == "order":
+        p.data = kept.t().contiguous().t()
+    elif why == "size":
+        p.grad = None
+        p.data = torch.zeros(3, device=DEV)
+        p.grad = torch.ones(3, device=DEV)
+    else:
+        g = p.grad
+        p.grad = None
+        p.data = kept.cpu()
+        p.grad = g.cpu()
+    with pytest.raises(RuntimeError, match="order" if why == "order" else "size" if why == "size" else "AMD GPU"):
+        opt.step()
+    p.data = kept
+    assert all(torch.equal(q.detach(), b) for q, b in zip(params, before)) and [int(opt.state[q]["step"]) for q in params] == counts
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), moments))
+
+
+@pytest.mark.parametrize("name,bad", [("betas", (0.9, 1.5)), ("betas", (math.nan, 0.9)), ("eps", -1.0), ("eps", math.nan), ("amsgrad", True), ("maximize", True)])
+def test_a_step_refused_for_one_group_moves_none(name, bad):
+    params, opt = _blocks_of_all_kinds()
+    before, counts = [p.detach().clone() for p in params], [int(opt.state[p]["step"]) for p in params]
+    kept = opt.param_groups[1].get(name)
+    opt.param_groups[1][name] = bad
+    with pytest.raises(ValueError, match="eps|amsgrad"):
+        opt.step()
+    assert all(torch.equal(q.detach(), b) for q, b in zip(params, before)) and [int(opt.state[q]["step"]) for q in params] == counts
+    opt.param_groups[1][name] = kept
+    opt.step()
+    assert [int(opt.state[q]["step"]) for q in params] == [n + 1 for n in counts]

@@ -474,14 +474,13 @@ struct Block {
     return {m, v};
   }
 
-  void step(const ttamd_adamw_scalars& scalars) {
+  // The gradients (undefined: none) of a step that can be taken; nothing is changed here.
+  std::vector<Tensor> gradients() const {
     const c10::DeviceGuard guard(params[0].device());
-    const auto now = c10::hip::getCurrentHIPStream(params[0].get_device());
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, kAdamW,
                 ": a step cannot be recorded into a graph (its count, and with it the bias corrections, would stand still)");
-    // everything is checked before anything is changed
     const size_t n = params.size();
-    std::vector<Tensor> grads(n);  // undefined: none
+    std::vector<Tensor> grads(n);
     for (size_t i = 0; i < n; ++i) {
       const Tensor& p = params[i];
       const Tensor& g = grads[i] = p.grad();
@@ -495,7 +494,14 @@ struct Block {
       TORCH_CHECK(order[i].empty() ? p.is_contiguous() || !p.is_non_overlapping_and_dense() : order_of(p) == order[i], kAdamW,
                   ": the order of a parameter's elements in memory has changed");
     }
-    point();
+    return grads;
+  }
+
+  // grads: what gradients() gave, and point() has been called since
+  void step(const std::vector<Tensor>& grads, const ttamd_adamw_scalars& scalars) {
+    const c10::DeviceGuard guard(params[0].device());
+    const auto now = c10::hip::getCurrentHIPStream(params[0].get_device());
+    const size_t n = params.size();
     used_on(now);
     const ttamd_adamw_states s = states();
     const int dtype = type == at::kBFloat16 ? TTAMD_BF16 : TTAMD_F32;
@@ -618,22 +624,6 @@ struct AdamWGroup {
     return found;
   }
 
-  void step(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, bool stochastic) {
-    const std::lock_guard<std::mutex> lock(mutex);
-    const at::NoGradGuard no_grad;
-    ttamd_adamw_scalars c = {};
-    c.lr = lr;
-    c.beta1 = beta1;
-    c.beta2 = beta2;
-    c.eps = eps;
-    c.weight_decay = weight_decay;
-    c.seed = seed;
-    for (auto& b : blocks) {
-      c.stochastic = stochastic && b->params[0].scalar_type() == at::kBFloat16;
-      b->step(c);
-    }
-  }
-
   // the flat moments, where one block holds all parameters in their order
   std::optional<std::pair<Tensor, Tensor>> whole() {
     if (blocks.size() != 1 || blocks[0]->params.size() != params.size()) return std::nullopt;
@@ -654,6 +644,43 @@ struct AdamWGroup {
   }
 };
 
+// group, lr, beta1, beta2, eps, weight_decay, seed, stochastic
+typedef std::tuple<AdamWGroup*, double, double, double, double, double, int64_t, bool> GroupStep;
+
+// One step of several groups: everything is checked, in all of them, before anything is changed.
+void adamw_step(const std::vector<GroupStep>& groups) {
+  const at::NoGradGuard no_grad;
+  std::vector<std::unique_lock<std::mutex>> locks;
+  struct Ready {
+    Block* block;
+    std::vector<Tensor> grads;
+    ttamd_adamw_scalars scalars;
+  };
+  std::vector<Ready> ready;
+  for (const auto& [group, lr, beta1, beta2, eps, weight_decay, seed, stochastic] : groups) {
+    locks.emplace_back(group->mutex);
+    ttamd_adamw_scalars c = {};
+    c.lr = lr;
+    c.beta1 = beta1;
+    c.beta2 = beta2;
+    c.eps = eps;
+    c.weight_decay = weight_decay;
+    c.seed = seed;
+    for (auto& b : group->blocks) {
+      c.stochastic = stochastic && b->type == at::kBFloat16;
+      std::vector<Tensor> grads = b->gradients();
+      if (std::none_of(grads.begin(), grads.end(), [](const Tensor& g) { return g.defined(); })) continue;
+      TORCH_CHECK_VALUE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0, kAdamW, ": betas ", beta1, ", ", beta2, " and eps ", eps);
+      ready.push_back({b.get(), std::move(grads), c});
+    }
+  }
+  for (Ready& r : ready) {
+    const c10::DeviceGuard guard(r.block->params[0].device());
+    r.block->point();
+  }
+  for (Ready& r : ready) r.block->step(r.grads, r.scalars);
+}
+
 }  // namespace
 
 void bind_post(py::module_& m) {
@@ -666,7 +693,7 @@ void bind_post(py::module_& m) {
       .def("make", &AdamWGroup::make, unlocked)
       .def("state", &AdamWGroup::state)
       .def("fresh", &AdamWGroup::fresh)
-      .def("step", &AdamWGroup::step, unlocked)
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);
+  m.def("adamw_step", &adamw_step, unlocked);
 }

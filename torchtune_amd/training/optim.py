@@ -120,14 +120,16 @@ class AdamW(torch.optim.Optimizer):
         self.state[params[i]] = dict(zip(names, plan.state(i)))
 
     def step(self, closure=None):
-        """One step; with ``closure``, which computes the loss again, its value is returned."""
+        """One step; with ``closure``, which computes the loss again, its value is returned.  A step that is refused for one
+        parameter or group changes none."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if any(group.get("amsgrad") or group.get("maximize") for group in self.param_groups):
+            raise ValueError("AdamW: amsgrad and maximize are not supported")
+        steps = []
         for index, group in enumerate(self.param_groups):
-            if group.get("amsgrad") or group.get("maximize"):
-                raise ValueError("AdamW: amsgrad and maximize are not supported")
             plan, params = self._plan(index), group["params"]
             beta1, beta2 = group["betas"]
             fresh = plan.fresh()
@@ -136,8 +138,8 @@ class AdamW(torch.optim.Optimizer):
                 for i in fresh:
                     self._show(plan, params, i)
                 self._seen = (self.state, len(self.state))
-            plan.step(float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]),
-                      bool(group["stochastic_rounding"]))
+            steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]), bool(group["stochastic_rounding"])))
+        _host.load().adamw_step(steps)
         return loss
 
     def moments(self):
