@@ -721,3 +721,23 @@ def test_a_step_refused_for_one_group_moves_none(name, bad):
     opt.param_groups[1][name] = kept
     opt.step()
     assert [int(opt.state[q]["step"]) for q in params] == [n + 1 for n in counts]
+
+
+def test_a_parameter_with_gaps_whose_memory_and_shape_change():
+    """As many elements in the same order, laid out with other gaps."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    wide, other = torch.randn(12, 10, generator=g, device=DEV), torch.zeros(8, 30, device=DEV)
+    group = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01)
+    p = torch.nn.Parameter(wide[:, 1:9])
+    opt, r = AdamW([p], **group), _Reference(p, 0, 32, 0, **group)
+    for shape in ((12, 8), (8, 12), (8, 12)):
+        if tuple(p.shape) != shape:
+            other[:, 3:15] = p.detach().reshape(8, 12)
+            p.grad = None
+            p.data = other[:, 3:15]
+        p.grad = torch.randn(shape, generator=g, device=DEV)
+        before = p.detach().clone()
+        opt.step()
+        r.take(before, p.grad)
+        r.check(p, opt.state[p])
+    assert bool((other[:, :3] == 0).all()) and bool((other[:, 15:] == 0).all())

@@ -407,7 +407,7 @@ struct Block {
   // Where the kernel finds tensor i: the parameter, or a copy of one with gaps, which lives as long as the states.
   void* find(size_t i) {
     if (params[i].is_non_overlapping_and_dense()) return params[i].data_ptr();
-    if (!shadow[i].defined()) shadow[i] = at::empty(params[i].sizes(), params[i].options());
+    if (!shadow[i].defined() || shadow[i].sizes() != params[i].sizes()) shadow[i] = at::empty(params[i].sizes(), params[i].options());
     return shadow[i].data_ptr();
   }
 
