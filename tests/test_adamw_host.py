@@ -126,3 +126,22 @@ def test_states_taken_out_of_the_dictionary():
     assert second is not first and opt._plan(0) is second
     opt.state[torch.nn.Parameter(torch.zeros(1))] = {}
     assert opt._plan(0) is not second
+
+
+@pytest.mark.parametrize("what", ["parameter", "gradient"])
+@pytest.mark.parametrize("elements", [0, 99])
+def test_memory_that_has_been_given_up(what, elements):
+    """A storage resized under a tensor: refused, before the device is looked at; one that is whole gets that far."""
+    p = torch.nn.Parameter(torch.zeros(120)[20:].view(10, 10))
+    p.grad = torch.ones(10, 11)[:, 1:]
+    opt = AdamW([p])
+    t = p if what == "parameter" else p.grad
+    whole = t.untyped_storage().nbytes()
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        opt.step()
+    t.untyped_storage().resize_(elements * 4)
+    with pytest.raises(RuntimeError, match=f"memory of a {what}"):
+        opt.step()
+    t.untyped_storage().resize_(whole)
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        opt.step()

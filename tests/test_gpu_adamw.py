@@ -741,3 +741,22 @@ def test_a_parameter_with_gaps_whose_memory_and_shape_change():
         r.take(before, p.grad)
         r.check(p, opt.state[p])
     assert bool((other[:, :3] == 0).all()) and bool((other[:, 15:] == 0).all())
+
+
+@pytest.mark.parametrize("what", ["parameter", "gradient"])
+def test_memory_that_was_given_up_and_came_back(what):
+    """After the first step, so that the table of addresses is there: refused while it is away, and nothing moves."""
+    params = _tensors([(300,), (129,)], torch.float32)
+    opt = AdamW(params, lr=1e-2)
+    opt.step()
+    t = params[1] if what == "parameter" else params[1].grad
+    kept, first, size = t.detach().clone(), params[0].detach().clone(), t.untyped_storage().nbytes()
+    torch.cuda.synchronize()
+    t.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match=f"memory of a {what}"):
+        opt.step()
+    t.untyped_storage().resize_(size)
+    t.detach().copy_(kept)
+    assert torch.equal(params[0].detach(), first) and [int(opt.state[p]["step"]) for p in params] == [1, 1]
+    opt.step()
+    assert bool((params[0].detach() != first).any()) and [int(opt.state[p]["step"]) for p in params] == [2, 2]

@@ -343,11 +343,30 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
 // ---------------------------------------------------------------------------------------------------
 constexpr const char* kAdamW = "AdamW";
 
+// From the first byte of a tensor's elements to behind the last (of one that has any).
+int64_t span_bytes(const Tensor& t) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return (last + 1) * (int64_t)t.itemsize();
+}
+
+// A tensor's memory may have been given up under it (sharding and offloading resize storages).
+void check_memory(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 0 || (int64_t)t.storage().nbytes() >= t.storage_offset() * (int64_t)t.itemsize() + span_bytes(t), kAdamW, ": the memory of ",
+              name, " ", t.sizes(), " is not there, its storage has ", t.storage().nbytes(), " bytes");
+}
+
 void check_param(const Tensor& p) {
   TORCH_CHECK(!p.key_set().has(c10::DispatchKey::Python) && p.layout() == at::kStrided, kAdamW, ": parameters must be plain dense tensors");
   type_code(p, kAdamW);
+  check_memory(p, "a parameter");
   need_gpu(p, kAdamW);
   at::assert_no_internal_overlap(p);
+}
+
+void check_gradient(const Tensor& g) {
+  TORCH_CHECK(g.layout() == at::kStrided && !g.key_set().has(c10::DispatchKey::Python), kAdamW, ": gradients must be plain dense tensors");
+  check_memory(g, "a gradient");
 }
 
 // The order of a dense tensor's elements in its states, as it lies in memory.  (One with gaps: row by row.)  Strides of single
@@ -485,8 +504,8 @@ struct Block {
       const Tensor& p = params[i];
       const Tensor& g = grads[i] = p.grad();
       if (!g.defined()) continue;
+      check_gradient(g);
       check_param(p);
-      TORCH_CHECK(g.layout() == at::kStrided && !g.key_set().has(c10::DispatchKey::Python), kAdamW, ": gradients must be plain dense tensors");
       TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), kAdamW, ": a gradient is ", g.scalar_type(), ", its parameter ", p.scalar_type());
       TORCH_CHECK(g.device() == p.device() && p.device() == exp_avg.device(), kAdamW, ": a parameter or its gradient has left ", exp_avg.device().str());
       TORCH_CHECK(p.numel() == places[i].numel && g.sizes() == p.sizes() && p.scalar_type() == type, kAdamW,
@@ -616,8 +635,8 @@ struct AdamWGroup {
     for (size_t i = 0; i < params.size(); ++i) {
       if (where[i].first >= 0 || !params[i].grad().defined()) continue;
       const Tensor g = params[i].grad();
+      check_gradient(g);
       check_param(params[i]);
-      TORCH_CHECK(g.layout() == at::kStrided, kAdamW, ": gradients must be plain dense tensors");
       TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, kAdamW, ": a step cannot be recorded into a graph");
       found.push_back((int64_t)i);
     }
