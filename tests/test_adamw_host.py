@@ -145,3 +145,46 @@ def test_memory_that_has_been_given_up(what, elements):
     t.untyped_storage().resize_(whole)
     with pytest.raises(RuntimeError, match="AMD GPU"):
         opt.step()
+
+
+def _views(base, *places):
+    return [torch.nn.Parameter(base.as_strided(size, stride, offset)) for size, stride, offset in places]
+
+
+@pytest.mark.parametrize("places,shared", [
+    # one after another, an empty one among them; the same twice; by one element; a part of a larger one
+    ([((10,), (1,), 0), ((0,), (1,), 5), ((10,), (1,), 10), ((4, 5), (5, 1), 20)], None),
+    ([((10,), (1,), 30), ((10,), (1,), 0), ((10,), (1,), 30)], (0, 2)),
+    ([((10,), (1,), 9), ((10,), (1,), 0)], (0, 1)),
+    ([((100,), (1,), 0), ((4, 5), (5, 1), 20), ((1,), (1,), 200)], (0, 1)),
+    # columns of one matrix of pitch 20, that begin anywhere; by one column; the last columns with the first of the next row
+    ([((10, 5), (20, 1), 7), ((10, 8), (20, 1), 12), ((10, 7), (20, 1), 0)], None),
+    ([((10, 5), (20, 1), 7), ((10, 8), (20, 1), 11)], (0, 1)),
+    ([((10, 5), (20, 1), 18), ((10, 8), (20, 1), 3)], None),
+    ([((10, 6), (20, 1), 18), ((10, 8), (20, 1), 3)], (0, 1)),
+    # transposed columns, single columns, interleaved elements, columns of one matrix in three dimensions
+    ([((5, 10), (1, 20), 0), ((8, 10), (1, 20), 5)], None),
+    ([((10,), (20,), 3), ((10,), (20,), 4), ((10, 3), (20, 1), 5)], None),
+    ([((50,), (2,), 0), ((50,), (2,), 1)], None),
+    ([((50,), (2,), 0), ((50,), (2,), 2)], (0, 1)),
+    ([((4, 5, 3), (100, 20, 1), 0), ((4, 5, 17), (100, 20, 1), 3)], None),
+    ([((4, 2, 20), (100, 20, 1), 0), ((4, 3, 20), (100, 20, 1), 40)], None),
+    # rows in between, in the same columns: the same places modulo the pitch of a row, others modulo that of two
+    ([((5, 8), (40, 1), 0), ((5, 8), (40, 1), 20)], None),
+    # elements of the one are in the gaps of the other, but along no dimension: not seen
+    ([((5,), (4,), 0), ((5,), (6,), 1)], (0, 1)),
+])
+def test_parameters_that_share_memory(places, shared):
+    from torchtune_amd import _host
+
+    params = _views(torch.zeros(400), *places)
+    assert _host.load().overlapping(params) == shared
+    assert _host.load().overlapping(params[::-1]) == (None if shared is None else tuple(sorted(len(params) - 1 - i for i in shared)))
+    # by the elements themselves
+    marks = [torch.zeros(400, dtype=torch.bool) for _ in places]
+    for m, (size, stride, offset) in zip(marks, places):
+        m.as_strided(size, stride, offset).fill_(True)
+    if shared is None:
+        assert int(sum(m.int() for m in marks).max()) <= 1
+    elif places[0][1] != (4,):
+        assert bool((marks[shared[0]] & marks[shared[1]]).any())

@@ -760,3 +760,33 @@ def test_memory_that_was_given_up_and_came_back(what):
     assert torch.equal(params[0].detach(), first) and [int(opt.state[p]["step"]) for p in params] == [1, 1]
     opt.step()
     assert bool((params[0].detach() != first).any()) and [int(opt.state[p]["step"]) for p in params] == [2, 2]
+
+
+def test_parameters_that_share_memory_are_refused():
+    """In one launch they would be stepped at the same time.  Columns of one matrix share none; one of two that share may go alone."""
+    base = torch.ones(40, 50, device=DEV)
+    a, b, c = (torch.nn.Parameter(t) for t in (base[:, 3:20], base[:, 20:33], base[4:6, 10:25]))
+    opt = AdamW([a, b, c], lr=0.1)
+    for p in (a, b, c):
+        p.grad = torch.ones(p.shape, device=DEV)
+    with pytest.raises(RuntimeError, match="parameters 0 and 2.* share memory"):
+        opt.step()
+    assert bool((base == 1).all()) and all(int(opt.state[p]["step"]) == 0 for p in (a, b, c))
+    c.grad = None
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in (a, b, c)] == [1, 1, 0]
+    assert bool((base[:, 3:33] != 1).all()) and bool((base[:, :3] == 1).all()) and bool((base[:, 33:] == 1).all())
+    # memory that moves into a neighbour's
+    x, y = (torch.nn.Parameter(torch.ones(100, device=DEV)) for _ in range(2))
+    x.grad, y.grad = torch.ones(100, device=DEV), torch.ones(100, device=DEV)
+    opt = AdamW([x, y], lr=0.1)
+    opt.step()
+    after = x.detach().clone()
+    kept, both = y.data, torch.ones(150, device=DEV)
+    x.data, y.data = both[:100], both[50:]
+    with pytest.raises(RuntimeError, match="share memory"):
+        opt.step()
+    assert bool((both == 1).all())
+    x.data, y.data = after, kept
+    opt.step()
+    assert int(opt.state[x]["step"]) == 2

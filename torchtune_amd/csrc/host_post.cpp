@@ -369,6 +369,50 @@ void check_gradient(const Tensor& g) {
   check_memory(g, "a gradient");
 }
 
+// Whether two tensors are seen to share no byte: their elements' places modulo the pitch of one of their dimensions lie in
+// intervals that do not meet, as those of columns of one matrix.
+bool apart(const Tensor& a, const Tensor& b) {
+  const auto place = [](const Tensor& t) { return (uint64_t)reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  const auto width = [](const Tensor& t, int64_t pitch) {  // of the interval
+    int64_t w = (int64_t)t.itemsize();
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1 && t.stride(d) * (int64_t)t.itemsize() % pitch) w += (t.size(d) - 1) * t.stride(d) * (int64_t)t.itemsize();
+    return w;
+  };
+  for (const Tensor* t : {&a, &b}) {
+    for (int64_t d = 0; d < t->dim(); ++d) {
+      const int64_t pitch = t->stride(d) * (int64_t)t->itemsize();
+      if (t->size(d) < 2 || pitch <= 0) continue;
+      const int64_t shift = (int64_t)((place(b) % pitch + pitch - place(a) % pitch) % pitch);
+      if (width(a, pitch) <= shift && shift + width(b, pitch) <= pitch) return true;
+    }
+  }
+  return false;
+}
+
+// Two of these tensors that share memory or cannot be seen not to.  Those that lie densely, one after another, cost a sort.
+std::optional<std::pair<int64_t, int64_t>> overlapping(const std::vector<Tensor>& tensors) {
+  struct Span {
+    uintptr_t begin, end;
+    int64_t of;
+  };
+  std::vector<Span> spans, open;
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const Tensor& t = tensors[i];
+    if (!t.defined() || t.numel() == 0) continue;
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+    spans.push_back({begin, begin + (uintptr_t)span_bytes(t), (int64_t)i});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (const Span& s : spans) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span& o) { return o.end <= s.begin; }), open.end());
+    for (const Span& o : open)
+      if (!apart(tensors[o.of], tensors[s.of])) return std::make_pair(std::min(o.of, s.of), std::max(o.of, s.of));
+    open.push_back(s);
+  }
+  return std::nullopt;
+}
+
 // The order of a dense tensor's elements in its states, as it lies in memory.  (One with gaps: row by row.)  Strides of single
 // elements say nothing.
 std::vector<int64_t> order_of(const Tensor& p) {
@@ -390,6 +434,7 @@ struct Block {
   };
   std::vector<Place> places;
   std::vector<uint32_t> chunks;  // first chunk of each tensor, and the end
+  bool shared = false;          // some of the addresses may be in several parameters
   Tensor table, exp_avg, exp_avg_sq, exp_avg_exponent, exp_avg_sq_exponent, steps;
   int bits;
   at::ScalarType type;         // of the parameters
@@ -439,6 +484,7 @@ struct Block {
       address[i] = now;
     }
     if (same) return;
+    shared = overlapping(params).has_value();
     const Tensor host = at::empty({(int64_t)(std::max<uint32_t>(chunks.back(), 1) * sizeof(ttamd_adamw_chunk))}, at::kByte);
     ttamd_adamw_chunk* to = (ttamd_adamw_chunk*)host.data_ptr();
     for (size_t i = 0; i < params.size(); ++i)
@@ -514,6 +560,17 @@ struct Block {
                   ": the order of a parameter's elements in memory has changed");
     }
     return grads;
+  }
+
+  // One launch steps many parameters at a time, so that none may be part of another.
+  void check_apart(const std::vector<Tensor>& grads) const {
+    if (!shared) return;
+    std::vector<Tensor> stepped(params.size());
+    for (size_t i = 0; i < params.size(); ++i)
+      if (grads[i].defined()) stepped[i] = params[i];
+    const auto two = overlapping(stepped);
+    TORCH_CHECK(!two, kAdamW, ": parameters ", numbers[two->first], " and ", numbers[two->second], ", ", stepped[two->first].sizes(), " and ",
+                stepped[two->second].sizes(), ", share memory");
   }
 
   // grads: what gradients() gave, and point() has been called since
@@ -696,6 +753,7 @@ void adamw_step(const std::vector<GroupStep>& groups) {
   for (Ready& r : ready) {
     const c10::DeviceGuard guard(r.block->params[0].device());
     r.block->point();
+    r.block->check_apart(r.grads);
   }
   for (Ready& r : ready) r.block->step(r.grads, r.scalars);
 }
@@ -715,4 +773,5 @@ void bind_post(py::module_& m) {
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);
   m.def("adamw_step", &adamw_step, unlocked);
+  m.def("overlapping", &overlapping);
 }

@@ -57,7 +57,8 @@ class AdamW(torch.optim.Optimizer):
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
     other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and
-    order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  A step cannot be recorded into a graph.
+    order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused.  A step
+    cannot be recorded into a graph.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
