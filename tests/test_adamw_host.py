@@ -1,8 +1,15 @@
 """What ``training.AdamW`` refuses and keeps before any kernel is launched (all on the CPU, where a step ends at the parameters' device)."""
+import copy
+import io
+import threading
+import time
+import types
+
 import pytest
 import torch
 
 from torchtune_amd import AdamW
+from torchtune_amd.training import optim
 
 
 def _saved(p, strides, seed=0):
@@ -188,3 +195,48 @@ def test_parameters_that_share_memory(places, shared):
         assert int(sum(m.int() for m in marks).max()) <= 1
     elif places[0][1] != (4,):
         assert bool((marks[shared[0]] & marks[shared[1]]).any())
+
+
+@pytest.mark.parametrize("call", ["step", "moments", "state_dict"])
+def test_threads_make_one_native_side(call, monkeypatch):
+    """The first calls of several threads, while making it takes its time."""
+    real, made = optim._host.load(), []
+
+    def slowly(*args):
+        made.append(threading.get_ident())
+        time.sleep(0.05)
+        return real.AdamWGroup(*args)
+
+    monkeypatch.setattr(optim._host, "load", lambda: types.SimpleNamespace(AdamWGroup=slowly, adamw_step=real.adamw_step))
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4))])
+    start = threading.Barrier(4)
+
+    def work(i):
+        start.wait()
+        if call == "step" or i % 2:
+            opt.step()
+        elif call == "state_dict":
+            opt.state_dict()
+        else:
+            with pytest.raises(RuntimeError, match="no parameter"):
+                opt.moments()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1
+
+
+def test_a_copy_has_a_lock_of_its_own():
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4))])
+    f = io.BytesIO()
+    torch.save(opt, f)
+    f.seek(0)
+    for other in (copy.deepcopy(opt), torch.load(f, weights_only=False)):  # written three lines above
+        other.step()
+        assert other._lock is not opt._lock
+    lock = opt._lock
+    opt.load_state_dict(opt.state_dict())
+    assert opt._lock is lock

@@ -790,3 +790,35 @@ def test_parameters_that_share_memory_are_refused():
     x.data, y.data = after, kept
     opt.step()
     assert int(opt.state[x]["step"]) == 2
+
+
+def test_threads_take_the_first_step_of_one_optimizer():
+    """Four threads at once, no states before: as many steps as asked for, in one set of states, which another thread reads meanwhile."""
+    for _ in range(5):
+        params = _tensors([(5000,)] * 20, torch.float32)
+        opt, alone = AdamW(params, lr=1e-3, state_bits=8), None
+        torch.cuda.synchronize()
+        start = threading.Barrier(5)
+
+        def work():
+            start.wait()
+            for _ in range(5):
+                opt.step()
+
+        def read():
+            start.wait()
+            for _ in range(20):
+                opt.state_dict()
+
+        threads = [threading.Thread(target=work) for _ in range(4)] + [threading.Thread(target=read)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        other = _tensors([(5000,)] * 20, torch.float32)
+        alone = AdamW(other, lr=1e-3, state_bits=8)
+        for _ in range(20):
+            alone.step()
+        for p, q in zip(params, other):
+            assert int(opt.state[p]["step"]) == 20 and torch.equal(p.detach(), q.detach())
+            assert all(torch.equal(opt.state[p][name], alone.state[q][name]) for name in opt.state[p])

@@ -675,7 +675,8 @@ struct AdamWGroup {
   }
 
   // (step, exp_avg, exp_avg_sq[, exponents of both]) of a parameter
-  std::vector<Tensor> state(int64_t i) const {
+  std::vector<Tensor> state(int64_t i) {
+    const std::lock_guard<std::mutex> lock(mutex);
     const Block& b = *blocks.at(where.at(i).first);
     const size_t at = where[i].second;
     std::vector<Tensor> s = {b.steps.select(0, at), b.like(b.exp_avg, at), b.like(b.exp_avg_sq, at)};
@@ -687,7 +688,8 @@ struct AdamWGroup {
   }
 
   // the places of parameters that have a gradient and no states yet
-  std::vector<int64_t> fresh() const {
+  std::vector<int64_t> fresh() {
+    const std::lock_guard<std::mutex> lock(mutex);
     std::vector<int64_t> found;
     for (size_t i = 0; i < params.size(); ++i) {
       if (where[i].first >= 0 || !params[i].grad().defined()) continue;
@@ -702,8 +704,8 @@ struct AdamWGroup {
 
   // the flat moments, where one block holds all parameters in their order
   std::optional<std::pair<Tensor, Tensor>> whole() {
-    if (blocks.size() != 1 || blocks[0]->params.size() != params.size()) return std::nullopt;
     const std::lock_guard<std::mutex> lock(mutex);
+    if (blocks.size() != 1 || blocks[0]->params.size() != params.size()) return std::nullopt;
     return blocks[0]->moments();
   }
   // else those of each parameter that has them, in their order
@@ -768,8 +770,8 @@ void bind_post(py::module_& m) {
       .def(py::init<std::vector<Tensor>, int64_t, int64_t>())
       .def("holds", &AdamWGroup::holds)
       .def("make", &AdamWGroup::make, unlocked)
-      .def("state", &AdamWGroup::state)
-      .def("fresh", &AdamWGroup::fresh)
+      .def("state", &AdamWGroup::state, unlocked)
+      .def("fresh", &AdamWGroup::fresh, unlocked)
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);
   m.def("adamw_step", &adamw_step, unlocked);

@@ -5,6 +5,7 @@ or, to save memory, an optimizer of a third package with 8-bit states.  :class:`
 """
 from __future__ import annotations
 
+import threading
 from itertools import chain
 from typing import Dict, List, Tuple
 
@@ -56,9 +57,9 @@ class AdamW(torch.optim.Optimizer):
 
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
-    other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory may be replaced (``p.data = ..``) by one of the same size, type and
-    order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused.  A step
-    cannot be recorded into a graph.
+    other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory
+    may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused.  Calls of
+    several threads wait for each other.  A step cannot be recorded into a graph.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -69,6 +70,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
         if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
             raise ValueError(f"AdamW: betas must be two numbers in [0, 1), got {betas}")
+        self._lock = threading.RLock()  # of the plans and the states' dictionary: calls of several threads wait for each other
         self._forget()
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
@@ -77,10 +79,13 @@ class AdamW(torch.optim.Optimizer):
         bits = param_group.get("state_bits", self.defaults["state_bits"])
         if bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32, got {bits}")
-        super().add_param_group(param_group)
+        with self._lock:
+            super().add_param_group(param_group)
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
+        if "_lock" not in self.__dict__:  # unpickled or copied
+            self._lock = threading.RLock()
         self._forget()
 
     def _forget(self) -> None:
@@ -127,6 +132,11 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        with self._lock:
+            self._step()
+        return loss
+
+    def _step(self) -> None:
         if any(group.get("amsgrad") or group.get("maximize") for group in self.param_groups):
             raise ValueError("AdamW: amsgrad and maximize are not supported")
         steps = []
@@ -141,27 +151,35 @@ class AdamW(torch.optim.Optimizer):
                 self._seen = (self.state, len(self.state))
             steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]), bool(group["stochastic_rounding"])))
         _host.load().adamw_step(steps)
-        return loss
 
     def moments(self):
         """``(exp_avg, exp_avg_sq)`` of all parameters that have states, one after another in their order (a parameter's elements as
         they lie in memory), as two flat tensors of numbers: the fp32 states themselves where they lie that way already, bfloat16
         (exact) for 8-bit states."""
         firsts, seconds = [], []
-        for index in range(len(self.param_groups)):
-            plan = self._plan(index)
-            whole = plan.whole()
-            for m, v in plan.moments() if whole is None else [whole]:
-                firsts.append(m)
-                seconds.append(v)
+        with self._lock:
+            for index in range(len(self.param_groups)):
+                plan = self._plan(index)
+                whole = plan.whole()
+                for m, v in plan.moments() if whole is None else [whole]:
+                    firsts.append(m)
+                    seconds.append(v)
         if not firsts:
             raise RuntimeError("AdamW.moments: no parameter has taken a step yet")
         return (firsts[0], seconds[0]) if len(firsts) == 1 else (torch.cat(firsts), torch.cat(seconds))
+
+    def state_dict(self):
+        with self._lock:
+            return super().state_dict()
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """What :meth:`state_dict` gave, of an optimizer with as many bits.  With 8 bits the parameters have to lie in memory in the order in
         which those of the saved states lay (of dense ones the states have the strides), since neighbours there share exponents."""
+        with self._lock:
+            self._load(state_dict)
+
+    def _load(self, state_dict) -> None:
         saved, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # else the base class refuses it
             for theirs, ours in zip(groups, self.param_groups):
