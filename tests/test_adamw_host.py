@@ -240,3 +240,34 @@ def test_a_copy_has_a_lock_of_its_own():
     lock = opt._lock
     opt.load_state_dict(opt.state_dict())
     assert opt._lock is lock
+
+
+def test_hooks_of_a_load():
+    """Hooks before it see the states and may change them; what is checked is what they leave."""
+    p = torch.nn.Parameter(torch.zeros(200))
+    saved = {"state": {0: {"step": 1, "exp_avg": torch.zeros(200), "exp_avg_sq": torch.zeros(200)}}, "param_groups": AdamW([p]).state_dict()["param_groups"]}
+    opt, seen = AdamW([p]), []
+
+    def look(o, d):
+        seen.append(sorted(d["state"]))
+
+    def drop(o, d):
+        return {**d, "state": {}}
+
+    def spoil(o, d):
+        return {**d, "state": {0: {"step": 1}}}
+
+    opt.register_load_state_dict_pre_hook(look)
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        opt.load_state_dict(saved)
+    handle = opt.register_load_state_dict_pre_hook(spoil)
+    with pytest.raises(ValueError, match="expected"):
+        opt.load_state_dict(saved)
+    handle.remove()
+    opt.register_load_state_dict_pre_hook(drop)
+    opt.register_load_state_dict_pre_hook(look)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append("after"))
+    opt.load_state_dict(saved)
+    assert seen == [[0], [0], [0], [], "after"] and sorted(saved["state"]) == [0]
+    opt.load_state_dict(saved)
+    assert len(seen) == 8 and not opt.state

@@ -822,3 +822,35 @@ def test_threads_take_the_first_step_of_one_optimizer():
         for p, q in zip(params, other):
             assert int(opt.state[p]["step"]) == 20 and torch.equal(p.detach(), q.detach())
             assert all(torch.equal(opt.state[p][name], alone.state[q][name]) for name in opt.state[p])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hooks_of_a_load(bits):
+    """Hooks before it may change the states; hooks after it find them in place, and what they write there counts."""
+    params = _tensors([(300,), (33, 7)], torch.bfloat16)
+    opt = AdamW(params, lr=1e-2, state_bits=bits)
+    for _ in range(2):
+        opt.step()
+    saved = opt.state_dict()
+    kept = copy.deepcopy(saved["state"])
+    other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = AdamW(other, lr=1e-2, state_bits=bits)
+
+    def count_from_seven(o, d):
+        return {**d, "state": {k: {**s, "step": torch.tensor(7)} for k, s in d["state"].items()}}
+
+    def after(o):
+        for i, q in enumerate(other):
+            assert int(o.state[q]["step"]) == 7 and o.state[q]["exp_avg"].data_ptr() != saved["state"][i]["exp_avg"].data_ptr()
+            assert all(torch.equal(o.state[q][name], kept[i][name]) for name in kept[i] if name != "step")
+        o.state[other[0]]["exp_avg"].zero_()
+
+    again.register_load_state_dict_pre_hook(count_from_seven)
+    again.register_load_state_dict_post_hook(after)
+    again.load_state_dict(saved)
+    assert bool((again.state[other[0]]["exp_avg"] == 0).all()) and torch.equal(again.state[other[1]]["exp_avg"], kept[1]["exp_avg"])
+    assert all(torch.equal(saved["state"][i][name], kept[i][name]) for i in kept for name in kept[i])  # what was loaded is not touched
+    for q in other:
+        q.grad = torch.zeros_like(q)
+    again.step()
+    assert bool((again.state[other[0]]["exp_avg"] == 0).all()) and [int(again.state[q]["step"]) for q in other] == [8, 8]

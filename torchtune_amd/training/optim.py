@@ -6,7 +6,6 @@ or, to save memory, an optimizer of a third package with 8-bit states.  :class:`
 from __future__ import annotations
 
 import threading
-from itertools import chain
 from typing import Dict, List, Tuple
 
 import torch
@@ -71,6 +70,7 @@ class AdamW(torch.optim.Optimizer):
         if not all(0.0 <= b < 1.0 for b in betas) or len(betas) != 2:
             raise ValueError(f"AdamW: betas must be two numbers in [0, 1), got {betas}")
         self._lock = threading.RLock()  # of the plans and the states' dictionary: calls of several threads wait for each other
+        self._taken = None  # states on their way from a state dict
         self._forget()
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
@@ -86,7 +86,12 @@ class AdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         if "_lock" not in self.__dict__:  # unpickled or copied
             self._lock = threading.RLock()
+            self._taken = None
         self._forget()
+        if self._taken is not None:  # a state dict is being loaded
+            self.state.update(self._taken)
+            for index in range(len(self.param_groups)):
+                self._plan(index)
 
     def _forget(self) -> None:
         self._plans: Dict[int, tuple] = {}
@@ -177,28 +182,28 @@ class AdamW(torch.optim.Optimizer):
         """What :meth:`state_dict` gave, of an optimizer with as many bits.  With 8 bits the parameters have to lie in memory in the order in
         which those of the saved states lay (of dense ones the states have the strides), since neighbours there share exponents."""
         with self._lock:
-            self._load(state_dict)
+            # last of the hooks that see the dictionary before it is loaded
+            hook = self.register_load_state_dict_pre_hook(AdamW._take)
+            try:
+                super().load_state_dict(state_dict)
+            finally:
+                hook.remove()
+                self._taken = None
 
-    def _load(self, state_dict) -> None:
+    def _take(self, state_dict):
+        """The states, checked; the base class, which would cast them to the parameters' type, gets the groups alone."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
+        self._taken = {}
         if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:  # else the base class refuses it
             for theirs, ours in zip(groups, self.param_groups):
                 for key, p in zip(theirs["params"], ours["params"]):
                     if key in saved:
                         self._check_states(saved[key], p, ours["state_bits"])
+                        self._taken[p] = dict(saved[key])
             # the width stays; another AdamW's groups have no such options
             groups = [{"stochastic_rounding": ours["stochastic_rounding"], "seed": ours["seed"], **theirs, "state_bits": ours["state_bits"]}
                       for theirs, ours in zip(groups, self.param_groups)]
-        ids = list(chain.from_iterable(g["params"] for g in groups))
-        params = list(chain.from_iterable(g["params"] for g in self.param_groups))
-        # the states pass the base class by: it would cast them to the parameters' type
-        super().load_state_dict({**state_dict, "state": {}, "param_groups": groups})
-        for key, p in zip(ids, params):
-            if key in saved:
-                self.state[p] = dict(saved[key])
-        self._forget()
-        for index in range(len(self.param_groups)):
-            self._plan(index)
+        return {**state_dict, "state": {}, "param_groups": groups}
 
     @staticmethod
     def _check_states(held, p, bits: int) -> None:
