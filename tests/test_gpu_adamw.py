@@ -854,3 +854,19 @@ def test_hooks_of_a_load(bits):
         q.grad = torch.zeros_like(q)
     again.step()
     assert bool((again.state[other[0]]["exp_avg"] == 0).all()) and [int(again.state[q]["step"]) for q in other] == [8, 8]
+
+
+def test_a_group_that_cannot_take_over_its_states_keeps_them():
+    """A group that has grown, one of whose states has been spoilt: an error, and no other state is lost."""
+    params = _tensors([(300,), (129,)], torch.float32)
+    opt = AdamW(params, lr=1e-2)
+    opt.step()
+    kept = [opt.state[p]["exp_avg"].clone() for p in params]
+    opt.state[params[1]] = {**opt.state[params[1]], "step": "seven"}
+    opt.param_groups[0]["params"].append(torch.nn.Parameter(torch.zeros(5, device=DEV)))
+    with pytest.raises(ValueError, match="seven"):
+        opt.step()
+    assert int(opt.state[params[0]]["step"]) == 1 and all(torch.equal(opt.state[p]["exp_avg"], k) for p, k in zip(params, kept))
+    opt.state[params[1]]["step"] = 1
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in params] == [2, 2]

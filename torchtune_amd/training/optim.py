@@ -114,21 +114,23 @@ class AdamW(torch.optim.Optimizer):
         for i in given:
             self._check_states(self.state[params[i]], params[i], bits)
         plan.make(given)
+        states = {}
         for i in given:
-            held = self.state[params[i]]
-            self._show(plan, params, i)
-            for name, tensor in self.state[params[i]].items():
+            held, own = self.state[params[i]], self._shown(plan, i)
+            for name, tensor in own.items():
                 if name == "step":
                     tensor.fill_(int(held[name]))
                 else:
                     tensor.copy_(held[name].reshape(tensor.shape))
+            states[params[i]] = own
+        self.state.update(states)  # all of them or, after an error, none
         self._plans[index] = (plan, bits)
         self._seen = (self.state, len(self.state))
         return plan
 
-    def _show(self, plan, params, i: int) -> None:
-        names = ("step", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent")
-        self.state[params[i]] = dict(zip(names, plan.state(i)))
+    @staticmethod
+    def _shown(plan, i: int) -> dict:
+        return dict(zip(("step", "exp_avg", "exp_avg_sq", "exp_avg_exponent", "exp_avg_sq_exponent"), plan.state(i)))
 
     def step(self, closure=None):
         """One step; with ``closure``, which computes the loss again, its value is returned.  A step that is refused for one
@@ -152,7 +154,7 @@ class AdamW(torch.optim.Optimizer):
             if fresh:
                 plan.make(fresh)
                 for i in fresh:
-                    self._show(plan, params, i)
+                    self.state[params[i]] = self._shown(plan, i)
                 self._seen = (self.state, len(self.state))
             steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]), bool(group["stochastic_rounding"])))
         _host.load().adamw_step(steps)
