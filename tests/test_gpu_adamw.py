@@ -870,3 +870,93 @@ def test_a_group_that_cannot_take_over_its_states_keeps_them():
     opt.state[params[1]]["step"] = 1
     opt.step()
     assert [int(opt.state[p]["step"]) for p in params] == [2, 2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_one_launch_holds_all_with_gradients(bits):
+    """700 of one group in a step: a launch that is full, and the rest in another."""
+    params = _tensors([(5 + i % 97,) for i in range(1000)], torch.float32)
+    scalars = dict(lr=1e-2, betas=(0.8, 0.9), eps=1e-8, weight_decay=0.01)
+    opt = AdamW([{"params": params[:700]}, {"params": params[700:]}], **scalars, state_bits=bits, seed=3)
+    refs = [_Reference(p, i, bits, 3, **scalars) for i, p in enumerate(params)]
+    for _ in range(2):
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for p, b, r in zip(params, before, refs):
+            r.take(b, p.grad)
+            r.check(p, opt.state[p])
+
+
+@pytest.mark.parametrize("b2", [0.95, 0.999])
+def test_a_run_with_eight_bits_beside_one_with_32(b2):
+    """200 steps on the same gradients, which change: blocks of different scale, a drift with noise half as large.
+
+    An error of a held moment is ``b`` times the one before, plus that of the holding: ``e' = b e + d``.  ``d`` is 0 on average and within a step
+    ``u`` of the number that is held, so that its variance is at most u^2 / 4; beside it a bias of at most 2^-16 u (numbers of 16 bits), the
+    smallest code where the range ends (0 or that code is held), and four roundings of either run.  Variances of the elements add up; the sum
+    of all errors, each over its block's scale, stays within six standard deviations and the bias.
+    The change of a parameter is linear in the first moment.  In the second, of relative variance V <= 2^-10 min(steps, 1 / (1 - b2^2)), it
+    is larger by 3/8 V on average, to second order; twice that is allowed, and 1 % for the first order over 65536 elements."""
+    n, steps, b1 = 1 << 16, 200, 0.9
+    g = torch.Generator(device=DEV).manual_seed(11)
+    scale = torch.exp(3 * torch.randn(n // BLOCK, generator=g, device=DEV)).repeat_interleave(BLOCK)
+    params = [torch.nn.Parameter(torch.zeros(n, device=DEV)) for _ in range(2)]
+    opts = [AdamW([p], lr=1e-3, betas=(b1, b2), weight_decay=0.0, state_bits=bits, seed=2) for p, bits in zip(params, (8, 32))]
+    variance, bias = [torch.zeros(n, dtype=torch.float64, device=DEV) for _ in range(2)], [torch.zeros(n, dtype=torch.float64, device=DEV) for _ in range(2)]
+    for _ in range(steps):
+        grad = scale * (1 + 0.5 * torch.randn(n, generator=g, device=DEV))
+        for p, opt in zip(params, opts):
+            p.grad = grad
+            opt.step()
+        held, exact = ([x.double() for x in opt.moments()] for opt in opts)
+        for k, (b, mantissa, name) in enumerate(((b1, 3, "exp_avg_exponent"), (b2, 4, "exp_avg_sq_exponent"))):
+            field = opts[0].state[params[0]][name].double().repeat_interleave(BLOCK)
+            least = torch.exp2(field - 142) * (1 + 2.0 ** -mantissa)
+            h = held[k].abs()
+            u = torch.where(h == 0, least, torch.exp2(torch.floor(torch.log2(h.clamp(min=1e-300)))) * 2.0 ** -mantissa)
+            variance[k] = b * b * variance[k] + u * u / 4
+            bias[k] = b * bias[k] + 2.0 ** -16 * u + torch.where(h <= least, least, 0.0) + 4 * U * (h + u + exact[k].abs())
+    for k, unit in enumerate((scale.double(), scale.double() ** 2)):
+        off = float(((held[k] - exact[k]) / unit).sum())
+        bound = 6 * math.sqrt(float((variance[k] / unit ** 2).sum())) + float((bias[k] / unit).sum())
+        assert abs(off) <= bound, (k, off, bound)
+        assert bound < 0.05 * float((exact[k] / unit).sum().abs())  # a bound that says something
+    far, wide = (float(p.detach().double().mean()) for p in params)
+    tolerance = 0.75 * 2.0 ** -10 * min(steps, 1 / (1 - b2 * b2)) + 0.01
+    assert wide < 0 and abs(far / wide - 1) <= tolerance, (far, wide, tolerance)
+
+
+def test_small_elements_beside_a_large_one_in_eight_bits():
+    """What a block's range of 2^15 leaves of them, as the format is described: first moments 0, second moments the smallest code, and so
+    smaller changes than with 32 bits from the second step on (the first one's moments have not been held before they are used).  The next block
+    is not touched by it.
+
+    Of a gradient g = 1e-6: step 1 changes it by lr g / (g + eps).  In steps 2 and 3 the first moment is 0.1 g, over 1 - 0.9^t at most
+    5.3e-7; the second at least 2^-16 of the large one's, 0.9e-3, so that its root over that of 1 - 0.999^3 is at least 2.1e-3: each changes
+    it by at most 2.6e-4 lr."""
+    p = torch.nn.Parameter(torch.zeros(2 * BLOCK, device=DEV))
+    p.grad = torch.full((2 * BLOCK,), 1e-6, device=DEV)
+    p.grad[0] = 1.0
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=8)
+    for _ in range(3):
+        opt.step()
+    m, v = (x.float() for x in opt.moments())
+    field = opt.state[p]["exp_avg_sq_exponent"].double()
+    assert bool((m[1:BLOCK] == 0).all()) and bool((v[1:BLOCK].double() == 2.0 ** (float(field[0]) - 142) * 17 / 16).all())
+    assert float(v[1]) > 2.0 ** -16 * float(v[0]) and bool((m[BLOCK:] > 0).all()) and bool((v[BLOCK:] < 1e-11).all())
+    change, first = -p.detach().double(), 1e-2 * 1e-6 / (1e-6 + 1e-8)
+    assert bool((change[1:BLOCK] > first * (1 - 16 * U)).all()) and bool((change[1:BLOCK] < first * (1 + 16 * U) + 2 * 2.6e-4 * 1e-2).all())
+    assert float(change[BLOCK:].min()) > 2e-2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_eps_and_no_gradient(bits):
+    """0 / 0 where eps is 0: such an element keeps its place, but for the decay."""
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    p.grad = torch.zeros(300, device=DEV)
+    p.grad[7] = 1.0
+    opt = AdamW([p], lr=0.5, eps=0.0, weight_decay=0.25, state_bits=bits)
+    opt.step()
+    idle = torch.ones(300, dtype=torch.bool, device=DEV)
+    idle[7] = False
+    assert bool((p.detach()[idle] == 0.875).all()) and abs(float(p.detach()[7]) - 0.375) < 16 * U

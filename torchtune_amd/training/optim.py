@@ -38,7 +38,10 @@ class AdamW(torch.optim.Optimizer):
     They are rounded stochastically, since a change of ``1 - b2`` in a step is smaller than what rounding to the nearest would
     let through; the numbers are a function of ``seed``, the step, the parameter's place and the element's, so that a run can be
     repeated and continued.  A gradient that is not finite makes its element NaN for good, as in 32 bits; with 8 bits the 127
-    others of its block lose their moments and stand still.
+    others of its block lose their moments and stand still.  In 8 bits a block spans about 2^15: a first moment below that of its block's largest
+    is held as 0 and a second one as 2^-15 of the largest, so that an element whose gradients are that much smaller than its neighbours'
+    (the second moment: than their squares) moves less than with 32 bits.  ``eps`` counts as at least 1.1e-19, so that with ``eps=0`` an
+    element that never had a gradient stands still.
 
     Args:
         params: parameters or groups, as for any ``torch.optim.Optimizer``
