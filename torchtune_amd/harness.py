@@ -309,8 +309,11 @@ class Decoder(nn.Module):
         """Log probabilities of ``targets`` ([b, s], or [b, s, n] for several) after each token, with the entropy and the most likely
         alternatives if asked for: what preference, policy and distillation losses read.  The vocabulary projection runs chunk by
         chunk over the tokens, as in :meth:`loss`; a chunk's logits are kept for the backward."""
+        per = targets.shape[tokens.dim():]
+        if targets.shape[: tokens.dim()] != tokens.shape or len(per) > 1:
+            raise ValueError(f"token_logprobs: targets {tuple(targets.shape)} do not fit tokens {tuple(tokens.shape)}")
         h = self.forward(tokens, positions)
-        hidden, several = h.reshape(-1, h.shape[-1]), targets.reshape(tokens.numel(), -1)
+        hidden, several = h.reshape(-1, h.shape[-1]), targets.reshape(tokens.numel(), per[0] if per else 1)
         parts = []
         for hc, tc in zip(hidden.chunk(self.loss_chunks), several.chunk(self.loss_chunks)):
             logits = self.output(hc)
