@@ -352,8 +352,9 @@ int64_t span_bytes(const Tensor& t) {
 
 // A tensor's memory may have been given up under it (sharding and offloading resize storages).
 void check_memory(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.numel() == 0 || (int64_t)t.storage().nbytes() >= t.storage_offset() * (int64_t)t.itemsize() + span_bytes(t), kAdamW, ": the memory of ",
-              name, " ", t.sizes(), " is not there, its storage has ", t.storage().nbytes(), " bytes");
+  const int64_t there = (int64_t)t.storage().nbytes(), size = (int64_t)t.itemsize(), from = t.storage_offset() * size;
+  TORCH_CHECK(t.numel() == 0 || there >= from + (t.is_non_overlapping_and_dense() ? t.numel() * size : span_bytes(t)), kAdamW, ": the memory of ", name,
+              " ", t.sizes(), " is not there, its storage has ", there, " bytes");
 }
 
 void check_param(const Tensor& p) {
@@ -361,7 +362,7 @@ void check_param(const Tensor& p) {
   type_code(p, kAdamW);
   check_memory(p, "a parameter");
   need_gpu(p, kAdamW);
-  at::assert_no_internal_overlap(p);
+  if (!p.is_non_overlapping_and_dense()) at::assert_no_internal_overlap(p);
 }
 
 void check_gradient(const Tensor& g) {
@@ -687,8 +688,10 @@ struct AdamWGroup {
     return s;
   }
 
-  // the places of parameters that have a gradient and no states yet
-  std::vector<int64_t> fresh() {
+  // the places of parameters that have a gradient and no states yet; none if the list holds other parameters than these
+  std::optional<std::vector<int64_t>> fresh(const py::handle& list) {
+    if (!holds(list)) return std::nullopt;
+    const py::gil_scoped_release unlocked;
     const std::lock_guard<std::mutex> lock(mutex);
     std::vector<int64_t> found;
     for (size_t i = 0; i < params.size(); ++i) {
@@ -771,7 +774,7 @@ void bind_post(py::module_& m) {
       .def("holds", &AdamWGroup::holds)
       .def("make", &AdamWGroup::make, unlocked)
       .def("state", &AdamWGroup::state, unlocked)
-      .def("fresh", &AdamWGroup::fresh, unlocked)
+      .def("fresh", &AdamWGroup::fresh)
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);
   m.def("adamw_step", &adamw_step, unlocked);

@@ -100,10 +100,14 @@ class AdamW(torch.optim.Optimizer):
         self._plans: Dict[int, tuple] = {}
         self._seen = (None, 0)  # the dictionary of states and its length when the plans were right
 
-    def _plan(self, index: int):
-        """The group's native side; it takes over the states that are there already."""
-        if self._seen[0] is not self.state or self._seen[1] != len(self.state):  # states were taken out, or put in
+    def _look(self) -> None:
+        state, length = self._seen
+        if state is not self.state or length != len(state):  # states were taken out, or put in
             self._forget()
+
+    def _plan(self, index: int):
+        """The group's native side; a new one takes over the states that are there already."""
+        self._look()
         group = self.param_groups[index]
         params, bits = group["params"], group["state_bits"]
         known = self._plans.get(index)
@@ -147,19 +151,24 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _step(self) -> None:
-        if any(group.get("amsgrad") or group.get("maximize") for group in self.param_groups):
-            raise ValueError("AdamW: amsgrad and maximize are not supported")
+        self._look()
         steps = []
         for index, group in enumerate(self.param_groups):
-            plan, params = self._plan(index), group["params"]
-            beta1, beta2 = group["betas"]
-            fresh = plan.fresh()
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW: amsgrad and maximize are not supported")
+            params = group["params"]
+            plan, bits = self._plans.get(index, (None, 0))
+            fresh = plan.fresh(params) if bits == group["state_bits"] else None
+            if fresh is None:  # no native side for these parameters and options
+                plan = self._plan(index)
+                fresh = plan.fresh(params)
             if fresh:
                 plan.make(fresh)
                 for i in fresh:
                     self.state[params[i]] = self._shown(plan, i)
                 self._seen = (self.state, len(self.state))
-            steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], int(group["seed"]), bool(group["stochastic_rounding"])))
+            beta1, beta2 = group["betas"]
+            steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], group["seed"], group["stochastic_rounding"]))
         _host.load().adamw_step(steps)
 
     def moments(self):
