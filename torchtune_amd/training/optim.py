@@ -94,7 +94,7 @@ class AdamW(torch.optim.Optimizer):
         if self._taken is not None:  # a state dict is being loaded
             self.state.update(self._taken)
             for index in range(len(self.param_groups)):
-                self._plan(index)
+                self._plan(index, checked=True)
 
     def _forget(self) -> None:
         self._plans: Dict[int, tuple] = {}
@@ -105,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
         if state is not self.state or length != len(state):  # states were taken out, or put in
             self._forget()
 
-    def _plan(self, index: int):
+    def _plan(self, index: int, checked: bool = False):
         """The group's native side; a new one takes over the states that are there already."""
         self._look()
         group = self.param_groups[index]
@@ -118,8 +118,9 @@ class AdamW(torch.optim.Optimizer):
         first = sum(len(g["params"]) for g in self.param_groups[:index])
         plan = _host.load().AdamWGroup(params, first, bits)
         given = [i for i, p in enumerate(params) if self.state.get(p)]
-        for i in given:
-            self._check_states(self.state[params[i]], params[i], bits)
+        if not checked:
+            for i in given:
+                self._check_states(self.state[params[i]], params[i], bits)
         plan.make(given)
         states = {}
         for i in given:
@@ -232,7 +233,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: {name} is {t.dtype}, the states of this optimizer have {bits} bits")
             if t.numel() != (blocks if name.endswith("exponent") else p.numel()):
                 raise ValueError(f"AdamW: {name} has {t.numel()} elements, the parameter {p.numel()}")
-        if eight:
+        if eight and not (p.is_contiguous() and held["exp_avg"].is_contiguous() and held["exp_avg_sq"].is_contiguous()):
             AdamW._check_order(held, p)
 
     @staticmethod
