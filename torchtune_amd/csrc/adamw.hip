@@ -5,8 +5,8 @@
 //
 // in fp32, every product and sum rounded by itself (the moments; the parameter's change takes the hardware's root and reciprocal).
 // Bound: HBM, 22 bytes an element of a bf16 parameter with 32-bit states and 10 with 8-bit ones, where the vector ALU is as busy: some
-// 80 lane operations an element, a sixth of them for the numbers that round.  448 tensors of 42 M elements: 156 us (5.9 TB/s) and 76 us (5.5);
-// 218 M elements with 8-bit states and stochastic rounding 390 us (5.6 TB/s);
+// 80 lane operations an element, a sixth of them for the numbers that round.  448 tensors of 42 M elements: 157 us (5.9 TB/s) and 71 - 78 us
+// (5.4 - 5.9); 218 M elements with 8-bit states and stochastic rounding 353 us (6.2 TB/s), or 390 on another card of the kind;
 // with IEEE division and root, bounds checks on every access and bytes handled one by one 548.
 //
 // One launch covers up to 480 tensors: the gradients' addresses travel in the kernel's arguments (they may change from step to
@@ -323,7 +323,7 @@ __device__ __forceinline__ void read_out(const ttamd_adamw_states& st, const tta
   store8<BF16, false, FULL>(exp_avg_sq + c.offset, at, c.numel, v);
 }
 
-// 218 M elements in 214 us (6.1 TB/s)
+// 218 M elements in 225 us (5.8 TB/s)
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const ttamd_adamw_states st, uint16_t* __restrict__ exp_avg,
                                                             uint16_t* __restrict__ exp_avg_sq) {
   const ttamd_adamw_chunk c = st.chunks[blockIdx.x];

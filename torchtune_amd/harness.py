@@ -171,7 +171,7 @@ class Attention(nn.Module):
         self.v_proj = _linear(s.dim, s.n_kv_heads * s.head_dim, rank, alpha, quantize_base)
         self.output_proj = _linear(s.dim, s.dim, rank, alpha, quantize_base)
         self.sections = s.rope_sections
-        # torchtune/modules/attention.py:234-290: q_norm and k_norm, where the builder gives them
+        # norms of the heads, before the rotation, for models that have them there
         self.q_norm, self.k_norm = (RMSNorm(s.head_dim, s.norm_eps), RMSNorm(s.head_dim, s.norm_eps)) if s.qk_norm else (None, None)
 
     def _norm_and_rotate(self, q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions: Optional[torch.Tensor]):

@@ -73,8 +73,9 @@ def qkv_rope_repeat(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: to
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cache: torch.Tensor, q_scale: Optional[torch.Tensor] = None,
                  k_scale: Optional[torch.Tensor] = None, *, eps: float = 1e-6, positions: Optional[torch.Tensor] = None,
                  sections: Optional[Sequence[int]] = None, interleaved: bool = True):
-    """Norm of every query and key head and its rotation, one pass forward and one backward: the ``q_norm`` / ``k_norm`` and
-    ``pos_embeddings`` of the reference's attention (``torchtune/modules/attention.py:234-290``), in fp32 and rounded once.
+    """Norm of every query and key head, then its rotation, one pass forward and one backward, in fp32 and rounded once: for models that
+    norm before they rotate.  (With a scale that differs within a pair the other order is another function; rotate with
+    :func:`apply_rope` and norm after it for models of that kind.)
 
     Args:
         q, k (torch.Tensor): ``[b, s, n_h, h_d]`` and ``[b, s, n_kv, h_d]``, bfloat16 or float32, ``h_d`` a multiple of 16 up to 512.
@@ -187,11 +188,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
 
     Args:
         logits (torch.Tensor): ``[.., V]``, bfloat16 or float32; a shifted view such as ``logits[:, :-1]`` is read where it is
-        tokens (torch.Tensor): int64, a token for each row ``[..]`` or several ``[.., n]``; the same one may occur twice
+        tokens (torch.Tensor): int64, a token for each row ``[..]`` or several ``[.., n]``; the same one may occur twice.  The
+            backward compares a row's tokens with each other: 256 of them cost little, thousands their square
         temperature (float): between 1e-6 and 1e6. Default: 1
         entropy (bool): also return ``-sum p log p`` of each row
         top (int): also return that many largest log probabilities, at most 64, with their tokens; of equal logits the lower
-            token comes first
+            token comes first.  Of a row with fewer than ``top`` tokens above ``-inf``, or with thousands of equal largest ones, each
+            alternative costs about one more pass over the row
         ignore_index (int): a token that stands for none: its log probability is 0 and has no gradient.  Any other token
             outside the vocabulary gives NaN.
 
