@@ -271,3 +271,15 @@ def test_hooks_of_a_load():
     assert seen == [[0], [0], [0], [], "after"] and sorted(saved["state"]) == [0]
     opt.load_state_dict(saved)
     assert len(seen) == 8 and not opt.state
+
+
+def test_a_width_written_into_a_group():
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([p])
+    opt.param_groups[0]["state_bits"] = 16
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.step()
+    opt.param_groups[0]["state_bits"] = 8  # no states yet
+    opt.step()
+    with pytest.raises(TypeError):
+        opt.add_param_group([p])

@@ -60,8 +60,8 @@ class AdamW(torch.optim.Optimizer):
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
     other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory
-    may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused.  Calls of
-    several threads wait for each other.  A step cannot be recorded into a graph.
+    may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused where
+    one launch would step both.  Calls of several threads wait for each other.  A step cannot be recorded into a graph.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -79,11 +79,15 @@ class AdamW(torch.optim.Optimizer):
                                       stochastic_rounding=bool(stochastic_rounding), seed=int(seed)))
 
     def add_param_group(self, param_group) -> None:
-        bits = param_group.get("state_bits", self.defaults["state_bits"])
-        if bits not in (8, 32):
-            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {bits}")
+        if isinstance(param_group, dict):  # else the base class refuses it
+            self._check_bits(param_group.get("state_bits", self.defaults["state_bits"]))
         with self._lock:
             super().add_param_group(param_group)
+
+    @staticmethod
+    def _check_bits(bits) -> None:
+        if bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {bits}")
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
@@ -113,6 +117,7 @@ class AdamW(torch.optim.Optimizer):
         known = self._plans.get(index)
         if known is not None and known[1] == bits and known[0].holds(params):
             return known[0]
+        self._check_bits(bits)
         if len({id(p) for p in params}) != len(params):
             raise ValueError("AdamW: a parameter occurs twice in a group")
         first = sum(len(g["params"]) for g in self.param_groups[:index])
