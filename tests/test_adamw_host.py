@@ -126,12 +126,12 @@ def test_states_taken_out_of_the_dictionary():
     """What the native side holds for them is given up."""
     p = torch.nn.Parameter(torch.zeros(4))
     opt = AdamW([p])
-    first = opt._plan(0)
-    assert opt._plan(0) is first
-    opt.state = type(opt.state)(dict)
     second = opt._plan(0)
-    assert second is not first and opt._plan(0) is second
-    opt.state[torch.nn.Parameter(torch.zeros(1))] = {}
+    opt.state = type(opt.state)(dict)  # as empty as the one before
+    assert opt._plan(0) is second
+    assert not opt.state[torch.nn.Parameter(torch.zeros(1))]  # an entry made by looking for one
+    assert len(opt.state) == 1 and opt._plan(0) is second
+    opt.state[torch.nn.Parameter(torch.zeros(1))] = {"step": 1}
     assert opt._plan(0) is not second
 
 

@@ -5,6 +5,7 @@ Tolerances.  A parameter's change is a product of a quotient: five roundings and
 parameter is scaled and rounded to its type: half a step, or with stochastic rounding a whole one."""
 import collections
 import copy
+import gc
 import io
 import math
 import threading
@@ -960,3 +961,44 @@ def test_no_eps_and_no_gradient(bits):
     idle = torch.ones(300, dtype=torch.bool, device=DEV)
     idle[7] = False
     assert bool((p.detach()[idle] == 0.875).all()) and abs(float(p.detach()[7]) - 0.375) < 16 * U
+
+
+def test_looking_for_states_moves_none():
+    """An empty entry, made by asking for one that is not there, is no reason to make the states anew; one that is put in is."""
+    params = _tensors([(300,), (129,), (40,)], torch.float32)
+    params[1].grad, params[2].grad, kept = None, None, params[1].grad
+    opt = AdamW(params, lr=1e-2)
+    opt.step()
+    at = opt.state[params[0]]["exp_avg"].data_ptr()
+    assert not opt.state[params[1]]
+    opt.step()
+    assert opt.state[params[0]]["exp_avg"].data_ptr() == at and int(opt.state[params[0]]["step"]) == 2
+    params[1].grad = kept
+    opt.step()
+    assert opt.state[params[0]]["exp_avg"].data_ptr() == at and [int(opt.state[p]["step"]) for p in params[:2]] == [3, 1]
+    # given states for one that has none yet
+    opt.state[params[2]] = {"step": 6, "exp_avg": torch.ones(40, device=DEV), "exp_avg_sq": torch.ones(40, device=DEV)}
+    params[2].grad = torch.zeros(40, device=DEV)
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in params] == [4, 2, 7] and bool((opt.state[params[2]]["exp_avg"] - 0.9).abs().max() < 4 * U)
+
+
+def test_memory_of_states_that_were_replaced():
+    """New native sides do not keep the buffers of those before them."""
+    params = _tensors([(1 << 20,), (1 << 20,)], torch.float32)
+    opt = AdamW(params, lr=1e-2)
+    opt.step()
+    torch.cuda.synchronize()
+    gc.collect()
+    before = torch.cuda.memory_allocated()
+    for seed in range(4):
+        new = _tensors([(1 << 20,)], torch.float32, seed)[0]
+        opt.state[new] = {name: t.clone() for name, t in opt.state.pop(params[0]).items()}
+        opt.param_groups[0]["params"][0] = params[0] = new
+        opt.step()
+        opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+        opt.step()
+    del new
+    torch.cuda.synchronize()
+    gc.collect()
+    assert torch.cuda.memory_allocated() < before + (1 << 20) and int(opt.state[params[0]]["step"]) == 9

@@ -102,12 +102,17 @@ class AdamW(torch.optim.Optimizer):
 
     def _forget(self) -> None:
         self._plans: Dict[int, tuple] = {}
-        self._seen = (None, 0)  # the dictionary of states and its length when the plans were right
+        self._owned: Dict[torch.Tensor, dict] = {}  # the entries of the dictionary of states that show theirs
+        self._seen = (None, 0)  # that dictionary and its length when the plans were right
 
     def _look(self) -> None:
         state, length = self._seen
-        if state is not self.state or length != len(state):  # states were taken out, or put in
-            self._forget()
+        if state is self.state and length == len(state):
+            return
+        state, owned = self.state, self._owned
+        if any(state.get(p) is not own for p, own in owned.items()) or any(held and p not in owned for p, held in state.items()):
+            self._forget()  # states were taken out, or put in
+        self._seen = (state, len(state))
 
     def _plan(self, index: int, checked: bool = False):
         """The group's native side; a new one takes over the states that are there already."""
@@ -137,6 +142,7 @@ class AdamW(torch.optim.Optimizer):
                     tensor.copy_(held[name].reshape(tensor.shape))
             states[params[i]] = own
         self.state.update(states)  # all of them or, after an error, none
+        self._owned = {p: own for p, own in {**self._owned, **states}.items() if self.state.get(p) is own}
         self._plans[index] = (plan, bits)
         self._seen = (self.state, len(self.state))
         return plan
@@ -171,7 +177,7 @@ class AdamW(torch.optim.Optimizer):
             if fresh:
                 plan.make(fresh)
                 for i in fresh:
-                    self.state[params[i]] = self._shown(plan, i)
+                    self.state[params[i]] = self._owned[params[i]] = self._shown(plan, i)
                 self._seen = (self.state, len(self.state))
             beta1, beta2 = group["betas"]
             steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], group["seed"], group["stochastic_rounding"]))
