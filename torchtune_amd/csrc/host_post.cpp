@@ -777,6 +777,12 @@ void bind_post(py::module_& m) {
       .def("fresh", &AdamWGroup::fresh)
       .def("whole", &AdamWGroup::whole, unlocked)
       .def("moments", &AdamWGroup::moments, unlocked);
+  // one group, as most optimizers have, without the list: half a microsecond
+  m.def("adamw_step",
+        [](AdamWGroup& group, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, bool stochastic) {
+          adamw_step({GroupStep(&group, lr, beta1, beta2, eps, weight_decay, seed, stochastic)});
+        },
+        unlocked);
   m.def("adamw_step", &adamw_step, unlocked);
   m.def("overlapping", &overlapping);
 }

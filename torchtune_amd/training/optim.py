@@ -142,7 +142,9 @@ class AdamW(torch.optim.Optimizer):
                     tensor.copy_(held[name].reshape(tensor.shape))
             states[params[i]] = own
         self.state.update(states)  # all of them or, after an error, none
-        self._owned = {p: own for p, own in {**self._owned, **states}.items() if self.state.get(p) is own}
+        if index in self._plans:  # entries that were its own and are gone keep nothing alive
+            self._owned = {p: own for p, own in self._owned.items() if self.state.get(p) is own}
+        self._owned.update(states)
         self._plans[index] = (plan, bits)
         self._seen = (self.state, len(self.state))
         return plan
@@ -181,7 +183,8 @@ class AdamW(torch.optim.Optimizer):
                 self._seen = (self.state, len(self.state))
             beta1, beta2 = group["betas"]
             steps.append((plan, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"], group["seed"], group["stochastic_rounding"]))
-        _host.load().adamw_step(steps)
+        native = _host.load().adamw_step
+        native(*steps[0]) if len(steps) == 1 else native(steps)
 
     def moments(self):
         """``(exp_avg, exp_avg_sq)`` of all parameters that have states, one after another in their order (a parameter's elements as
