@@ -38,9 +38,9 @@ class AdamW(torch.optim.Optimizer):
     They are rounded stochastically, since a change of ``1 - b2`` in a step is smaller than what rounding to the nearest would
     let through; the numbers are a function of ``seed``, the step, the parameter's place and the element's, so that a run can be
     repeated and continued.  A gradient that is not finite makes its element NaN for good, as in 32 bits; with 8 bits the 127
-    others of its block lose their moments and stand still.  In 8 bits a block spans about 2^15: a first moment below that of its block's largest
-    is held as 0 and a second one as 2^-15 of the largest, so that an element whose gradients are that much smaller than its neighbours'
-    (the second moment: than their squares) moves less than with 32 bits.  ``eps`` counts as at least 1.1e-19, so that with ``eps=0`` an
+    others of its block lose their moments and stand still.  In 8 bits a block spans about 2^15: below that part of its block's largest a
+    first moment is held as 0 and a second one, which goes with the gradients' squares, as that part, so that an element with so much
+    smaller gradients than its neighbours' moves less than with 32 bits.  ``eps`` counts as at least 1.1e-19, so that with ``eps=0`` an
     element that never had a gradient stands still.
 
     Args:
@@ -55,13 +55,15 @@ class AdamW(torch.optim.Optimizer):
         seed (int): of the stochastic rounding. Default: 0
 
     Every option may be a group's own.  Loading a state dict takes its options over, as for any optimizer, ``seed`` and
-    ``stochastic_rounding`` among them, so that a run goes on with the numbers that it would have had; ``state_bits`` stays, and states of the other width are refused.
+    ``stochastic_rounding`` among them, so that a run goes on with the numbers that it would have had; ``state_bits`` stays, and states
+    of the other width are refused.
 
     ``state[p]`` holds ``step``, ``exp_avg``, ``exp_avg_sq`` (and ``exp_avg_exponent``, ``exp_avg_sq_exponent`` with 8 bits), made when ``p``
     first has a gradient; they are parts of buffers that all parameters share, so write into them, or load a state dict, but do not put
     other tensors in their place.  A parameter whose entry is taken out of ``state`` begins anew.  A parameter's memory
-    may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded with 32 bits.  Parameters that share memory are refused where
-    one launch would step both.  Calls of several threads wait for each other.  A step cannot be recorded into a graph.
+    may be replaced (``p.data = ..``) by one of the same size, type and order.  A state dict of ``torch.optim.AdamW`` can be loaded
+    with 32 bits.  Parameters that share memory are refused where one launch would step both.  Calls of several threads wait for each
+    other.  A step cannot be recorded into a graph.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
